@@ -1,0 +1,129 @@
+/*
+ * mxfp4_few.hip - products of MXFP4 operands (mxfp4.h), one workgroup per 16 rows of weights, its waves along K.
+ *
+ *   Y[t, r] = sum_k X[t, k] W[r, k]          or, of two tensors, silu(X . gate) * (X . up)
+ *
+ * v_mfma_scale_f32_16x16x128_f8f6f4 multiplies 16 rows by 16 tokens over 128 columns and applies both blocks' powers of two: the
+ * products of codes are exact, the sums are fp32. Every load is a whole kilobyte of an operand in the instruction's own lane order,
+ * from memory to registers. A wave takes 512 columns at a time (four instructions per row group and token group share one dword of
+ * exponents per lane), wave w the 512-column pieces w, w + waves, ...; the waves' sums meet in LDS and are added in the waves' order.
+ */
+#include "mxfp4.h"
+
+namespace qlin {
+using namespace mxfp4;
+
+namespace {
+
+/* the first `left` of four results to consecutive elements, at any element address */
+__device__ __forceinline__ void store4(float *y, f32x4 a, int left) {
+    typedef f32x4 anywhere __attribute__((aligned(4)));
+    if (left > 3) {
+        *reinterpret_cast<anywhere *>(y) = a;
+    } else {
+        for (int v = 0; v < 3; v++)
+            if (v < left) y[v] = a[v];
+    }
+}
+__device__ __forceinline__ void store4(__bf16 *y, f32x4 a, int left) {
+    typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+    typedef bf16x4 anywhere __attribute__((aligned(2)));
+    const bf16x4 b = {(__bf16)a[0], (__bf16)a[1], (__bf16)a[2], (__bf16)a[3]}; /* nearest even, the one rounding of a result */
+    if (left > 3) {
+        *reinterpret_cast<anywhere *>(y) = b;
+    } else {
+        for (int v = 0; v < 3; v++)
+            if (v < left) y[v] = b[v];
+    }
+}
+
+/* MATS 2: gate and up; NT: token groups of 16 per workgroup */
+template <int MATS, int NT, int WAVES, class OUT>
+__global__ void __launch_bounds__(64 * WAVES)
+few_kernel(const uint8_t *__restrict__ W, const uint8_t *__restrict__ up, const uint8_t *__restrict__ X, OUT *__restrict__ Y, int n_rows, int n_tok, Shape w,
+           Shape x, size_t ldy) {
+    __shared__ f32x4 sums[WAVES][MATS * NT][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int token_blocks = (x.groups + NT - 1) / NT;
+    const int group = blockIdx.x / (unsigned)token_blocks, t0 = (blockIdx.x - group * token_blocks) * NT;
+    f32x4 acc[MATS][NT] = {};
+    for (int q = wave; q < w.quads; q += WAVES) {
+        u32x4 a[MATS][4], b[NT][4];
+        int sa[MATS], sb[NT];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int tile = min(4 * q + i, w.tiles - 1);
+#pragma unroll
+            for (int m = 0; m < MATS; m++)
+                a[m][i] = *reinterpret_cast<const u32x4 *>((m ? up : W) + ((size_t)group * w.tiles + tile) * kTileBytes + lane * 16);
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+                b[n][i] = *reinterpret_cast<const u32x4 *>(X + ((size_t)min(t0 + n, x.groups - 1) * x.tiles + tile) * kTileBytes + lane * 16);
+        }
+#pragma unroll
+        for (int m = 0; m < MATS; m++)
+            sa[m] = *reinterpret_cast<const int *>((m ? up : W) + w.code_bytes() + ((size_t)group * w.quads + q) * kScaleBytes + lane * 4);
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+            sb[n] = *reinterpret_cast<const int *>(X + x.code_bytes() + ((size_t)min(t0 + n, x.groups - 1) * x.quads + q) * kScaleBytes + lane * 4);
+        const int tiles = w.tiles - 4 * q; /* of these four, those that are there */
+        auto step = [&](auto at) {
+            constexpr int i = decltype(at)::value;
+            if (i < tiles) {
+#pragma unroll
+                for (int m = 0; m < MATS; m++)
+#pragma unroll
+                    for (int n = 0; n < NT; n++)
+                        acc[m][n] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(widened(a[m][i]), widened(b[n][i]), acc[m][n], 4, 4, i, sa[m], i, sb[n]);
+            }
+        };
+        step(std::integral_constant<int, 0>{});
+        step(std::integral_constant<int, 1>{});
+        step(std::integral_constant<int, 2>{});
+        step(std::integral_constant<int, 3>{});
+    }
+#pragma unroll
+    for (int m = 0; m < MATS; m++)
+#pragma unroll
+        for (int n = 0; n < NT; n++) sums[wave][m * NT + n][lane] = acc[m][n];
+    __syncthreads();
+    /* lane l of the result holds rows 4 (l / 16) .. + 3 of token l % 16 */
+    for (int i = threadIdx.x; i < NT * 64; i += 64 * WAVES) {
+        const int n = i >> 6, l = i & 63, t = (t0 + n) * 16 + (l & 15), r = group * 16 + (l >> 4) * 4;
+        f32x4 s[MATS];
+#pragma unroll
+        for (int m = 0; m < MATS; m++) {
+            s[m] = sums[0][m * NT + n][l];
+#pragma unroll
+            for (int v = 1; v < WAVES; v++) s[m] += sums[v][m * NT + n][l];
+        }
+        if constexpr (MATS == 2)
+            for (int v = 0; v < 4; v++) s[0][v] = silu_mul(s[0][v], s[1][v]);
+        if (t < n_tok && r < n_rows) store4(Y + (size_t)t * ldy + r, s[0], n_rows - r);
+    }
+}
+
+template <int MATS, int NT, class OUT> hipError_t few(const Mxfp4Product &p) {
+    constexpr int kWaves = 8;
+    const Shape w = shape_of(p.n_rows, p.n_cols), x = shape_of(p.n_tok, p.n_cols);
+    const dim3 grid((unsigned)w.groups * (unsigned)((x.groups + NT - 1) / NT));
+    few_kernel<MATS, NT, kWaves, OUT><<<grid, 64 * kWaves, 0, p.stream>>>(p.W, p.up, p.X, static_cast<OUT *>(p.Y), p.n_rows, p.n_tok, w, x, (size_t)p.ldy);
+    return hipGetLastError();
+}
+template <int MATS, class OUT> hipError_t few_tokens(const Mxfp4Product &p) {
+    const int groups = (p.n_tok + 15) / 16;
+    if (groups == 1) return few<MATS, 1, OUT>(p);
+    if (groups == 2) return few<MATS, 2, OUT>(p);
+    if (groups == 3) return few<MATS, 3, OUT>(p);
+    return few<MATS, 4, OUT>(p);
+}
+
+}  // namespace
+
+hipError_t launch_mxfp4_few(const Mxfp4Product &p, int n_cu) {
+    (void)n_cu;
+    if (p.up) return p.bf16_out ? few_tokens<2, __bf16>(p) : few_tokens<2, float>(p);
+    return p.bf16_out ? few_tokens<1, __bf16>(p) : few_tokens<1, float>(p);
+}
+
+}  // namespace qlin

@@ -1,0 +1,228 @@
+/*
+ * mxfp4_pack.hip - float rows to MXFP4, as GGML blocks or as an operand of the matrix instructions (mxfp4.h), and GGML blocks to
+ * an operand.
+ *
+ * A block of 32 elements x shares the power of two 2^p that puts its largest magnitude into [4, 8): p = floor(log2 max|x|) - 2, at
+ * least -127, stored as p + 127. A code is the e2m1 number (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign) nearest to x / 2^p, on a tie the
+ * one with the even code, and 6 beyond 6: what v_cvt_scalef32_pk_fp4_f32 computes. Magnitudes of (6, 8) of a block's largest binade
+ * so become 6; the larger power of two would halve the resolution of all others. A block that holds an infinity or a NaN gets
+ * exponent 255, NaN of the E8M0 format - every product with it is NaN - and codes of magnitude 6, which the decoders of this library
+ * turn into infinities.
+ *
+ * Four lanes share a block, 8 consecutive elements each, so that a wave reads 512 consecutive elements of a row, 16 bytes per lane
+ * and load in 16-bit types. The 4 KB of codes that a workgroup makes pass LDS once: out of the lanes they would go to memory in
+ * pieces of 4 bytes. Bound by memory for many rows and by the launch for few.
+ */
+#include "mxfp4.h"
+
+namespace qlin {
+using namespace mxfp4;
+
+namespace {
+
+struct Bf16 { uint16_t bits; };
+
+template <class T> struct alignas(16) Eight { T v[8]; };
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(_Float16 v) { return (float)v; }
+__device__ __forceinline__ float to_f32(Bf16 v) { return __uint_as_float((uint32_t)v.bits << 16); }
+
+/* elements p[0..7], those at `left` and behind as zeros; VEC: p is on 16 bytes and `left` a multiple of 8 */
+template <class T, bool VEC> __device__ __forceinline__ void load8(const T *p, int left, float (&x)[8]) {
+    if constexpr (VEC) {
+        Eight<T> e = {};
+        if (left > 0) e = *reinterpret_cast<const Eight<T> *>(p);
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = to_f32(e.v[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            x[i] = 0.0f;
+            if (i < left) x[i] = to_f32(p[i]);
+        }
+    }
+}
+
+template <int CTRL> __device__ __forceinline__ uint32_t quad_perm(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xf, 0xf, true);
+}
+constexpr int kXor1 = 0xB1, kXor2 = 0x4E; /* lane q of four takes lane q ^ 1, q ^ 2 */
+
+/* four codes in 16 bits to a byte each */
+__device__ __forceinline__ uint32_t spread(uint32_t v) {
+    v = (v | v << 8) & 0x00FF00FFu;
+    return (v | v << 4) & 0x0F0F0F0Fu;
+}
+
+/* the four lanes of a block, 8 elements each in order: its exponent (in all four) and this lane's dword of its 16 code bytes, whose
+ * place is dword_of(q) */
+struct Packed { uint32_t exponent, codes; };
+__device__ __forceinline__ int dword_of(int q) { return (q & 1) * 2 + (q >> 1); }
+__device__ __forceinline__ Packed pack8(const float (&x)[8], int q) {
+    uint32_t m = 0, negative = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const uint32_t b = __float_as_uint(x[i]);
+        m = max(m, b & 0x7FFFFFFFu);
+        negative |= (b >> 31) << (4 * i + 3);
+    }
+    m = max(m, quad_perm<kXor1>(m));
+    m = max(m, quad_perm<kXor2>(m));
+    const bool not_finite = m >= 0x7F800000u;
+    const uint32_t e = not_finite ? 255u : (uint32_t)max((int)(m >> 23) - 2, 0);
+    const float power = __uint_as_float(e == 0 ? 0x00400000u : e << 23);
+    uint32_t own = 0;
+    own = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(own, x[0], x[1], power, 0);
+    own = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(own, x[2], x[3], power, 1);
+    own = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(own, x[4], x[5], power, 2);
+    own = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(own, x[6], x[7], power, 3);
+    if (not_finite) own = negative | 0x77777777u;
+    /* byte j = element j | element j + 16: lanes 0 and 2 (1 and 3) make bytes 0..7 (8..15) together, the lower one the first four */
+    const uint32_t other = quad_perm<kXor2>(own);
+    const uint32_t low = q < 2 ? own : other >> 16, high = q < 2 ? other : own >> 16;
+    return {e, spread(low & 0xFFFFu) | spread(high & 0xFFFFu) << 4};
+}
+
+/* one workgroup: a row group's 512 columns */
+template <class T, bool VEC>
+__global__ void __launch_bounds__(256) operand_kernel(const T *__restrict__ X, uint8_t *__restrict__ op, int n_rows, int n_cols, size_t ldx, Shape s) {
+    constexpr int kRun = 16 * 4 + 4; /* dwords from one block of a tile to the next: 16 rows, and 4 against bank conflicts */
+    __shared__ __attribute__((aligned(16))) uint32_t codes[16 * kRun];
+    __shared__ __attribute__((aligned(16))) uint8_t scales[kScaleBytes];
+    const int group = blockIdx.x / (unsigned)s.quads, quad = blockIdx.x - group * s.quads;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int block = lane >> 2, q = lane & 3; /* of the 512 columns' 16 */
+    const int col = quad * 512 + lane * 8;
+    float x[4][8];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int row = group * 16 + 4 * wave + i;
+        load8<T, VEC>(X + (size_t)row * ldx + col, row < n_rows ? n_cols - col : 0, x[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int r = 4 * wave + i;
+        const Packed p = pack8(x[i], q);
+        codes[block * kRun + r * 4 + dword_of(q)] = p.codes;
+        if (q == 0) scales[((block & 3) * 16 + r) * 4 + (block >> 2)] = (uint8_t)p.exponent;
+    }
+    __syncthreads();
+    const int tile = quad * 4 + wave;
+    if (tile < s.tiles)
+        *reinterpret_cast<uint4 *>(op + ((size_t)group * s.tiles + tile) * kTileBytes + lane * 16) =
+            *reinterpret_cast<const uint4 *>(codes + (4 * wave + (lane >> 4)) * kRun + (lane & 15) * 4);
+    if (threadIdx.x < 16)
+        *reinterpret_cast<uint4 *>(op + s.code_bytes() + ((size_t)group * s.quads + quad) * kScaleBytes + threadIdx.x * 16) =
+            *reinterpret_cast<const uint4 *>(scales + threadIdx.x * 16);
+}
+
+/* the same from GGML blocks: codes and exponents are moved, not changed */
+__global__ void __launch_bounds__(256) operand_of_blocks_kernel(const uint8_t *__restrict__ W, uint8_t *__restrict__ op, int n_rows, int n_blocks, Shape s) {
+    constexpr int kRow = 16 * kBlockBytes;
+    __shared__ uint8_t raw[16 * kRow];
+    __shared__ __attribute__((aligned(16))) uint8_t scales[kScaleBytes];
+    const int group = blockIdx.x / (unsigned)s.quads, quad = blockIdx.x - group * s.quads;
+    const int here = min(16, n_blocks - quad * 16) * kBlockBytes; /* bytes of a row */
+    for (int i = threadIdx.x; i < 16 * kRow; i += 256) {
+        const int r = i / kRow, at = i - r * kRow, row = group * 16 + r;
+        uint8_t v = 0;
+        if (row < n_rows && at < here) v = W[((size_t)row * n_blocks + quad * 16) * kBlockBytes + at];
+        raw[i] = v;
+    }
+    __syncthreads();
+    const int r = threadIdx.x & 15, block = threadIdx.x >> 4, tile = quad * 4 + (block >> 2);
+    const uint8_t *b = raw + r * kRow + block * kBlockBytes;
+    u32x4 v;
+    __builtin_memcpy(&v, b + 1, 16);
+    if (tile < s.tiles)
+        *reinterpret_cast<u32x4 *>(op + ((size_t)group * s.tiles + tile) * kTileBytes + ((block & 3) * 16 + r) * 16) = v;
+    scales[((block & 3) * 16 + r) * 4 + (block >> 2)] = b[0];
+    __syncthreads();
+    if (threadIdx.x < 16)
+        *reinterpret_cast<uint4 *>(op + s.code_bytes() + ((size_t)group * s.quads + quad) * kScaleBytes + threadIdx.x * 16) =
+            *reinterpret_cast<const uint4 *>(scales + threadIdx.x * 16);
+}
+
+/* one workgroup: 256 consecutive blocks of the rows end to end, 4352 bytes of the result */
+template <class T, bool VEC>
+__global__ void __launch_bounds__(256) blocks_kernel(const T *__restrict__ X, uint8_t *__restrict__ W, size_t n_blocks, int per_row, size_t ldx, bool wide) {
+    constexpr int kBytes = 256 * kBlockBytes;
+    __shared__ __attribute__((aligned(16))) uint8_t out[kBytes];
+    const size_t first = (size_t)blockIdx.x * 256;
+    const size_t row0 = first / (unsigned)per_row; /* (per_row > 0: a kernel is launched for whole blocks only) */
+    const unsigned block0 = (unsigned)(first - row0 * per_row);
+    const int q = threadIdx.x & 3;
+    float x[4][8];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const unsigned n = block0 + 64 * i + (threadIdx.x >> 2), down = n / (unsigned)per_row;
+        const size_t row = row0 + down, col = (size_t)(n - down * per_row) * kBlock + 8 * q;
+        const bool there = first + 64 * i + (threadIdx.x >> 2) < n_blocks;
+        load8<T, VEC>(X + (there ? row * ldx + col : 0), there ? 8 : 0, x[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        uint8_t *b = out + (64 * i + (threadIdx.x >> 2)) * kBlockBytes;
+        const Packed p = pack8(x[i], q);
+        if (q == 0) b[0] = (uint8_t)p.exponent;
+        __builtin_memcpy(b + 1 + 4 * dword_of(q), &p.codes, 4);
+    }
+    __syncthreads();
+    uint8_t *to = W + first * kBlockBytes;
+    const int bytes = (int)min((size_t)256, n_blocks - first) * kBlockBytes;
+    if (wide) {
+        for (int i = threadIdx.x; i < bytes / 16; i += 256) reinterpret_cast<uint4 *>(to)[i] = reinterpret_cast<const uint4 *>(out)[i];
+        const int done = bytes & ~15;
+        if ((int)threadIdx.x < bytes - done) to[done + threadIdx.x] = out[done + threadIdx.x];
+    } else {
+        for (int i = threadIdx.x; i < bytes; i += 256) to[i] = out[i];
+    }
+}
+
+/* rows that can be read in 16-byte loads */
+template <class T> bool reads_wide(const void *X, int n_cols, int ldx) {
+    return (reinterpret_cast<uintptr_t>(X) & 15) == 0 && n_cols % 8 == 0 && (size_t)ldx * sizeof(T) % 16 == 0;
+}
+
+template <class T> hipError_t operand_of(const void *X, void *op, int n_rows, int n_cols, int ldx, hipStream_t stream) {
+    const Shape s = shape_of(n_rows, n_cols);
+    const dim3 grid((unsigned)s.groups * (unsigned)s.quads);
+    const T *x = static_cast<const T *>(X);
+    uint8_t *o = static_cast<uint8_t *>(op);
+    if (reads_wide<T>(X, n_cols, ldx)) operand_kernel<T, true><<<grid, 256, 0, stream>>>(x, o, n_rows, n_cols, (size_t)ldx, s);
+    else operand_kernel<T, false><<<grid, 256, 0, stream>>>(x, o, n_rows, n_cols, (size_t)ldx, s);
+    return hipGetLastError();
+}
+
+template <class T> hipError_t blocks_of(const void *X, void *W, int n_rows, int n_cols, int ldx, hipStream_t stream) {
+    const int per_row = n_cols / kBlock;
+    const size_t n_blocks = (size_t)n_rows * per_row;
+    const dim3 grid((unsigned)((n_blocks + 255) / 256));
+    const bool wide = (reinterpret_cast<uintptr_t>(W) & 15) == 0;
+    const T *x = static_cast<const T *>(X);
+    uint8_t *w = static_cast<uint8_t *>(W);
+    if (reads_wide<T>(X, n_cols, ldx)) blocks_kernel<T, true><<<grid, 256, 0, stream>>>(x, w, n_blocks, per_row, (size_t)ldx, wide);
+    else blocks_kernel<T, false><<<grid, 256, 0, stream>>>(x, w, n_blocks, per_row, (size_t)ldx, wide);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_mxfp4_operand(uint32_t type, const void *X, void *op, int n_rows, int n_cols, int ldx, hipStream_t stream) {
+    if (type == T_F32) return operand_of<float>(X, op, n_rows, n_cols, ldx, stream);
+    if (type == T_F16) return operand_of<_Float16>(X, op, n_rows, n_cols, ldx, stream);
+    if (type == T_BF16) return operand_of<Bf16>(X, op, n_rows, n_cols, ldx, stream);
+    const Shape s = shape_of(n_rows, n_cols);
+    operand_of_blocks_kernel<<<dim3((unsigned)s.groups * (unsigned)s.quads), 256, 0, stream>>>(
+        static_cast<const uint8_t *>(X), static_cast<uint8_t *>(op), n_rows, n_cols / kBlock, s);
+    return hipGetLastError();
+}
+
+hipError_t launch_mxfp4_blocks(uint32_t type, const void *X, void *W, int n_rows, int n_cols, int ldx, hipStream_t stream) {
+    if (type == T_F32) return blocks_of<float>(X, W, n_rows, n_cols, ldx, stream);
+    if (type == T_F16) return blocks_of<_Float16>(X, W, n_rows, n_cols, ldx, stream);
+    return blocks_of<Bf16>(X, W, n_rows, n_cols, ldx, stream);
+}
+
+}  // namespace qlin

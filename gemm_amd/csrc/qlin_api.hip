@@ -24,6 +24,7 @@
 #include <mutex>
 #include <string>
 
+#include "mxfp4.h"
 #include "qlin_device.h"
 #include "qlin_internal.h"
 
@@ -1433,6 +1434,116 @@ int qlin_moe_ffn_dev(uint32_t type, const void *gate_exps, const void *up_exps, 
                      int n_tok, int top_k, int n_embd, int n_ff, int n_expert, void *workspace, void *stream) {
     return qlin_moe_ffn_types_dev(type, type, type, gate_exps, up_exps, down_exps, X, expert_idx, expert_w, out, n_tok,
                                   top_k, n_embd, n_ff, n_expert, workspace, stream);
+}
+
+/* ------------------------------------------------------------------ 4-bit operands */
+
+namespace {
+size_t float_bytes(uint32_t type) { return type == T_F32 ? 4 : type == T_F16 || type == T_BF16 ? 2 : 0; }
+/* the rows of a float matrix: 0 or an error */
+int check_float_rows(const char *what, uint32_t type, const void *X, int n_rows, int n_cols, int ldx) {
+    if (n_rows < 0 || n_cols < 0 || ldx < n_cols) return fail(QLIN_ERR_ARG, "%s: negative size or a row pitch below the row", what);
+    if (n_rows == 0 || n_cols == 0) return QLIN_OK;
+    if (!X) return fail(QLIN_ERR_ARG, "%s: null pointer", what);
+    if (!aligned(X, float_bytes(type))) return fail(QLIN_ERR_ARG, "%s: misaligned pointer", what);
+    return QLIN_OK;
+}
+/* sizes that the kernels of an operand can number */
+constexpr int kMaxOperandCols = (1 << 24) - 1;
+bool operand_fits(int n_rows, int n_cols) {
+    const mxfp4::Shape s = mxfp4::shape_of(n_rows, n_cols);
+    return n_cols <= kMaxOperandCols && (size_t)s.groups * s.quads <= INT_MAX;
+}
+}  // namespace
+
+int qlin_quantize_mxfp4_dev(uint32_t x_type, const void *X, void *W, int n_rows, int n_cols, int ldx, void *stream) {
+    if (!float_bytes(x_type)) return fail(QLIN_ERR_TYPE, "only F32, F16 and BF16 rows are quantised (got type %u)", x_type);
+    if (n_cols % mxfp4::kBlock) return fail(QLIN_ERR_ARG, "n_cols %d is not a whole number of 32-element blocks", n_cols);
+    if (int rc = check_float_rows("X", x_type, X, n_rows, n_cols, ldx)) return rc;
+    if (n_rows == 0 || n_cols == 0) return QLIN_OK;
+    if (!W) return fail(QLIN_ERR_ARG, "null pointer");
+    if ((size_t)n_rows * (n_cols / mxfp4::kBlock) > (size_t)INT_MAX * 256) return fail(QLIN_ERR_ARG, "%d x %d elements in one call", n_rows, n_cols);
+    if (int rc = init_once()) return rc;
+    HIP_TRY(launch_mxfp4_blocks(x_type, X, W, n_rows, n_cols, ldx, (hipStream_t)stream));
+    return QLIN_OK;
+}
+
+size_t qlin_mxfp4_operand_bytes(int n_rows, int n_cols) {
+    if (n_rows <= 0 || n_cols <= 0) return 0;
+    return mxfp4::shape_of(n_rows, n_cols).bytes();
+}
+
+int qlin_mxfp4_operand_dev(uint32_t type, const void *X, void *operand, int n_rows, int n_cols, int ldx, void *stream) {
+    if (type == T_MXFP4) {
+        if (n_rows < 0 || n_cols < 0 || n_cols % mxfp4::kBlock) return fail(QLIN_ERR_ARG, "n_cols %d is not a whole number of 32-element blocks", n_cols);
+        if (ldx != n_cols) return fail(QLIN_ERR_ARG, "rows of blocks follow each other (ldx %d, n_cols %d)", ldx, n_cols);
+        if (n_rows && n_cols && !X) return fail(QLIN_ERR_ARG, "null pointer");
+    } else {
+        if (!float_bytes(type)) return fail(QLIN_ERR_TYPE, "an operand is made of F32, F16, BF16 or MXFP4 rows (got type %u)", type);
+        if (int rc = check_float_rows("X", type, X, n_rows, n_cols, ldx)) return rc;
+    }
+    if (n_rows == 0 || n_cols == 0) return QLIN_OK;
+    if (!operand || !aligned(operand, 16)) return fail(QLIN_ERR_ARG, "the operand needs 16-byte aligned memory");
+    if (!operand_fits(n_rows, n_cols)) return fail(QLIN_ERR_ARG, "an operand of %d x %d is too large", n_rows, n_cols);
+    if (int rc = init_once()) return rc;
+    HIP_TRY(launch_mxfp4_operand(type, X, operand, n_rows, n_cols, ldx, (hipStream_t)stream));
+    return QLIN_OK;
+}
+
+size_t qlin_mxfp4_gemm_workspace_bytes(int n_cols, int n_tok) { return qlin_mxfp4_operand_bytes(n_tok, n_cols); }
+
+static int mxfp4_gemm(const void *W, const void *up, bool pair, uint32_t x_type, const void *X, uint32_t y_type, void *Y, int n_rows, int n_cols,
+                      int n_tok, int ldx, int ldy, void *workspace, size_t workspace_bytes, void *stream) {
+    if (x_type != T_MXFP4 && !float_bytes(x_type)) return fail(QLIN_ERR_TYPE, "activations are an MXFP4 operand, F32, F16 or BF16 (got type %u)", x_type);
+    if (y_type != T_F32 && y_type != T_BF16) return fail(QLIN_ERR_TYPE, "results are F32 or BF16 (got type %u)", y_type);
+    if (n_rows < 0 || n_cols <= 0 || n_tok < 0 || ldy < n_rows) return fail(QLIN_ERR_ARG, "negative size, no columns, or a row pitch below the row");
+    if (x_type != T_MXFP4)
+        if (int rc = check_float_rows("X", x_type, X, n_tok, n_cols, ldx)) return rc;
+    if (n_rows == 0 || n_tok == 0) return QLIN_OK;
+    if (!W || (pair && !up) || !X || !Y) return fail(QLIN_ERR_ARG, "null pointer");
+    if (!aligned(W, 16) || !aligned(up, 16) || (x_type == T_MXFP4 && !aligned(X, 16)) || !aligned(Y, float_bytes(y_type)))
+        return fail(QLIN_ERR_ARG, "operands need 16-byte alignment, Y an element's");
+    if (!operand_fits(n_rows, n_cols) || !operand_fits(n_tok, n_cols) || (size_t)((n_rows + 15ll) / 16) * ((n_tok + 15ll) / 16) > INT_MAX)
+        return fail(QLIN_ERR_ARG, "a product of %d x %d x %d is too large", n_rows, n_cols, n_tok);
+    if (x_type != T_MXFP4 && (!workspace || !aligned(workspace, 16) || workspace_bytes < qlin_mxfp4_gemm_workspace_bytes(n_cols, n_tok)))
+        return fail(QLIN_ERR_ARG, "the workspace needs %zu bytes, 16-byte aligned", qlin_mxfp4_gemm_workspace_bytes(n_cols, n_tok));
+    if (int rc = init_once()) return rc;
+    if (x_type != T_MXFP4) HIP_TRY(launch_mxfp4_operand(x_type, X, workspace, n_tok, n_cols, ldx, (hipStream_t)stream));
+    const Mxfp4Product p = {static_cast<const uint8_t *>(W), static_cast<const uint8_t *>(up), static_cast<const uint8_t *>(x_type == T_MXFP4 ? X : workspace), Y,
+                            n_rows, n_cols, n_tok, ldy, y_type == T_BF16, (hipStream_t)stream};
+    HIP_TRY(launch_mxfp4_few(p, g.n_cu));
+    return QLIN_OK;
+}
+
+int qlin_mxfp4_gemm_dev(const void *W, uint32_t x_type, const void *X, uint32_t y_type, void *Y, int n_rows, int n_cols, int n_tok, int ldx, int ldy,
+                        void *workspace, size_t workspace_bytes, void *stream) {
+    return mxfp4_gemm(W, nullptr, false, x_type, X, y_type, Y, n_rows, n_cols, n_tok, ldx, ldy, workspace, workspace_bytes, stream);
+}
+
+int qlin_mxfp4_gemm_silu_mul_dev(const void *Wgate, const void *Wup, uint32_t x_type, const void *X, uint32_t y_type, void *Y, int n_rows, int n_cols,
+                                 int n_tok, int ldx, int ldy, void *workspace, size_t workspace_bytes, void *stream) {
+    return mxfp4_gemm(Wgate, Wup, true, x_type, X, y_type, Y, n_rows, n_cols, n_tok, ldx, ldy, workspace, workspace_bytes, stream);
+}
+
+/* ------------------------------------------------------------------ sampling */
+
+size_t qlin_sample_workspace_bytes(int n_seq, int n_vocab) { return n_seq > 0 && n_vocab > 0 ? sample_workspace_bytes(n_seq, n_vocab) : 0; }
+
+int qlin_sample_dev(uint32_t type, const void *logits, int n_seq, int n_vocab, int ld, const float *temperature, const int32_t *top_k, const float *top_p,
+                    const float *min_p, const float *u, int32_t *ids, float *probs, void *workspace, size_t workspace_bytes, void *stream) {
+    if (!float_bytes(type)) return fail(QLIN_ERR_TYPE, "logits are F32, F16 or BF16 (got type %u)", type);
+    if (int rc = check_float_rows("logits", type, logits, n_seq, n_vocab, ld)) return rc;
+    if (n_seq == 0) return QLIN_OK;
+    if (n_vocab == 0) return fail(QLIN_ERR_ARG, "sampling from no tokens");
+    if (!u || !ids) return fail(QLIN_ERR_ARG, "null pointer");
+    for (const void *p : {(const void *)temperature, (const void *)top_k, (const void *)top_p, (const void *)min_p, (const void *)u, (const void *)ids, (const void *)probs})
+        if (!aligned(p, 4)) return fail(QLIN_ERR_ARG, "misaligned pointer");
+    const size_t need = qlin_sample_workspace_bytes(n_seq, n_vocab);
+    if (need && (!workspace || !aligned(workspace, 256) || workspace_bytes < need)) return fail(QLIN_ERR_ARG, "the workspace needs %zu bytes, 256-byte aligned", need);
+    if (int rc = init_once()) return rc;
+    const SampleCall c = {logits, n_seq, n_vocab, ld, temperature, top_k, top_p, min_p, u, ids, probs, workspace, (hipStream_t)stream};
+    HIP_TRY(launch_sample(type, c));
+    return QLIN_OK;
 }
 
 int qlin_probe_mfma_bf16(int iters, void *stream, double *flops) {

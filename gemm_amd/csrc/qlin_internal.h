@@ -269,6 +269,20 @@ hipError_t launch_silu_mul(float *h, const float *gate, const float *up, int n, 
  * loop `if (v[j] > v[best]) best = j` (server/server_llm.c:224-228). result holds
  * QLIN_ARGMAX_RESULT_BYTES bytes: the rest is scratch for the first stage. */
 hipError_t launch_argmax(const float *v, int n, float *result, hipStream_t stream);
+/* the next token of each sequence from its logits (sample.hip); null temperature, top_k, top_p, min_p: 1, 0, 1, 0; probs may be null */
+struct SampleCall {
+    const void *logits;
+    int n_seq, n_vocab, ld;
+    const float *temperature;
+    const int32_t *top_k;
+    const float *top_p, *min_p, *u;
+    int32_t *ids;
+    float *probs;
+    void *workspace;
+    hipStream_t stream;
+};
+size_t sample_workspace_bytes(int n_seq, int n_vocab);
+hipError_t launch_sample(uint32_t type, const SampleCall &c);
 /* measurement probes (probe.hip): a register-only MFMA loop (flops issued come back in *flops) with the
  * cycle and 100 MHz counters around it, and a streaming read of a device buffer */
 hipError_t launch_probe_mfma(int iters, int n_cu, hipStream_t stream, double *flops);

@@ -88,6 +88,15 @@ SIGNATURES = {
                                          C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, _vp, _vp]),
     "qlin_moe_ffn_static_dev": (C.c_int, [C.c_uint32, C.c_uint32, C.c_uint32, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
                                           C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, _vp]),
+    "qlin_quantize_mxfp4_dev": (C.c_int, [C.c_uint32, _vp, _vp, C.c_int, C.c_int, C.c_int, _vp]),
+    "qlin_mxfp4_operand_bytes": (C.c_size_t, [C.c_int, C.c_int]),
+    "qlin_mxfp4_operand_dev": (C.c_int, [C.c_uint32, _vp, _vp, C.c_int, C.c_int, C.c_int, _vp]),
+    "qlin_mxfp4_gemm_workspace_bytes": (C.c_size_t, [C.c_int, C.c_int]),
+    "qlin_mxfp4_gemm_dev": (C.c_int, [_vp, C.c_uint32, _vp, C.c_uint32, _vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, _vp, C.c_size_t, _vp]),
+    "qlin_mxfp4_gemm_silu_mul_dev": (C.c_int, [_vp, _vp, C.c_uint32, _vp, C.c_uint32, _vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, _vp,
+                                               C.c_size_t, _vp]),
+    "qlin_sample_workspace_bytes": (C.c_size_t, [C.c_int, C.c_int]),
+    "qlin_sample_dev": (C.c_int, [C.c_uint32, _vp, C.c_int, C.c_int, C.c_int, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, C.c_size_t, _vp]),
     "qlin_gguf_open": (C.c_int, [C.c_char_p, _vp]),
     "qlin_gguf_close": (None, [_vp]),
     "qlin_gguf_version": (C.c_uint32, [_vp]),
@@ -371,6 +380,43 @@ def moe_ffn_types_dev(types, dgate, dup, ddown, dX, didx, dw, dout, n_tok, top_k
 def moe_ffn_static_dev(types, dgate, dup, ddown, dX, didx, dw, dout, n_tok, top_k, n_embd, n_ff, n_expert, stream=None):
     check(load().qlin_moe_ffn_static_dev(types[0], types[1], types[2], dgate.ptr, dup.ptr, ddown.ptr, dX.ptr, didx.ptr,
                                          dw.ptr, dout.ptr, n_tok, top_k, n_embd, n_ff, n_expert, stream))
+
+
+def quantize_mxfp4_dev(x_type, dX, dW, n_rows, n_cols, ldx, stream=None):
+    check(load().qlin_quantize_mxfp4_dev(x_type, dX.ptr, dW.ptr, n_rows, n_cols, ldx, stream))
+
+
+def mxfp4_operand_bytes(n_rows, n_cols):
+    return load().qlin_mxfp4_operand_bytes(n_rows, n_cols)
+
+
+def mxfp4_operand_dev(type_id, dX, doperand, n_rows, n_cols, ldx, stream=None):
+    check(load().qlin_mxfp4_operand_dev(type_id, dX.ptr, doperand.ptr, n_rows, n_cols, ldx, stream))
+
+
+def mxfp4_gemm_workspace_bytes(n_cols, n_tok):
+    return load().qlin_mxfp4_gemm_workspace_bytes(n_cols, n_tok)
+
+
+def mxfp4_gemm_dev(dW, x_type, dX, y_type, dY, n_rows, n_cols, n_tok, ldx, ldy, dws, stream=None):
+    check(load().qlin_mxfp4_gemm_dev(dW.ptr, x_type, dX.ptr, y_type, dY.ptr, n_rows, n_cols, n_tok, ldx, ldy,
+                                     dws.ptr if dws is not None else None, dws.nbytes if dws is not None else 0, stream))
+
+
+def mxfp4_gemm_silu_mul_dev(dWgate, dWup, x_type, dX, y_type, dY, n_rows, n_cols, n_tok, ldx, ldy, dws, stream=None):
+    check(load().qlin_mxfp4_gemm_silu_mul_dev(dWgate.ptr, dWup.ptr, x_type, dX.ptr, y_type, dY.ptr, n_rows, n_cols, n_tok, ldx, ldy,
+                                              dws.ptr if dws is not None else None, dws.nbytes if dws is not None else 0, stream))
+
+
+def sample_workspace_bytes(n_seq, n_vocab):
+    return load().qlin_sample_workspace_bytes(n_seq, n_vocab)
+
+
+def sample_dev(logits_type, dlogits, n_seq, n_vocab, ld, dtemperature, dtop_k, dtop_p, dmin_p, du, dids, dprobs, dws, stream=None):
+    """dtemperature, dtop_k, dtop_p, dmin_p and dprobs may be None"""
+    opt = [b.ptr if b is not None else None for b in (dtemperature, dtop_k, dtop_p, dmin_p)]
+    check(load().qlin_sample_dev(logits_type, dlogits.ptr, n_seq, n_vocab, ld, *opt, du.ptr, dids.ptr, dprobs.ptr if dprobs is not None else None,
+                                 dws.ptr if dws is not None else None, dws.nbytes if dws is not None else 0, stream))
 
 
 def sync(stream=None):

@@ -339,6 +339,66 @@ int qlin_moe_ffn_static_dev(uint32_t type_gate, uint32_t type_up, uint32_t type_
                             const int32_t *expert_idx, const float *expert_w, float *out, int n_tok, int top_k,
                             int n_embd, int n_ff, int n_expert, void *stream);
 
+/* ------------------------------------------------------------------ 4-bit operands
+ * Products whose both factors are MXFP4, on the scaled 4-bit matrix instructions: 32 elements share a power of two and hold an
+ * e2m1 number each (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign). No counterpart in the reference, which decodes MXFP4 weights
+ * (common/ggml_dequant.h:2818-2830) and multiplies in fp32; what these calls round and the others do not are the activations.
+ * Pointers and stream belong to the current device, as in the group above.
+ *
+ * Quantisation: a block's power of two is that of its largest magnitude, divided by four (exponent byte floor(log2 max|x|) + 125, at
+ * least 0); its codes are the nearest e2m1 numbers, on a tie the one with the even code, 6 beyond 6. A block with an infinity or a
+ * NaN gets exponent byte 255, which every product takes as NaN (the token's or the row's results are NaN, the others are not
+ * touched), and codes of magnitude 6, which qlin_dequant_dev decodes to infinities. */
+
+/* W = the MXFP4 blocks (17 bytes each, as in a GGUF file) of float rows: the inverse of qlin_dequant_dev for type 39. X F32, F16 or
+ * BF16 with row pitch ldx elements, n_cols a multiple of 32; no alignment beyond an element's (16-byte rows are read faster). X and
+ * W must not overlap. */
+int qlin_quantize_mxfp4_dev(uint32_t x_type, const void *X, void *W, int n_rows, int n_cols, int ldx, void *stream);
+/* The layout that the products take, made of MXFP4 blocks (type 39: weights, once after loading; n_cols a multiple of 32, ldx ==
+ * n_cols) or of F32, F16 or BF16 rows (quantised as above, any n_cols, row pitch ldx). operand: device memory, 16-byte aligned,
+ * qlin_mxfp4_operand_bytes(n_rows, n_cols) bytes (17/32 byte per element, rows rounded up to 16 and columns to 128; 0 for sizes that
+ * are negative), written whole. Tensors that take the same activations make one operand where their rows stand behind each
+ * other. */
+size_t qlin_mxfp4_operand_bytes(int n_rows, int n_cols);
+int qlin_mxfp4_operand_dev(uint32_t ggml_type, const void *X, void *operand, int n_rows, int n_cols, int ldx, void *stream);
+/* Y[t*ldy + r] = sum_k X[t, k] W[r, k] for r < n_rows, t < n_tok. W: an operand of n_rows x n_cols. X: an operand of n_tok x n_cols
+ * (x_type 39; ldx and workspace are not looked at, qlin_mxfp4_operand_dev makes one for several products) or F32, F16 or BF16
+ * rows of pitch ldx, which are quantised into the workspace first: device memory, 16-byte aligned,
+ * qlin_mxfp4_gemm_workspace_bytes(n_cols, n_tok) bytes; calls that share one must be ordered on one stream, and graphs that share
+ * one must not run at the same time. Y F32 or BF16 (y_type), any pitch >= n_rows and any element alignment. The products of codes are
+ * exact and their sums fp32 (relative L2 ~1e-7 for F32 results against a double-precision product of the same operands); BF16
+ * results are rounded once. The same call gives the same bits. n_cols below 2^24. */
+size_t qlin_mxfp4_gemm_workspace_bytes(int n_cols, int n_tok);
+int qlin_mxfp4_gemm_dev(const void *W, uint32_t x_type, const void *X, uint32_t y_type, void *Y, int n_rows, int n_cols, int n_tok, int ldx,
+                        int ldy, void *workspace, size_t workspace_bytes, void *stream);
+/* Y[t*ldy + r] = silu(X . Wgate) * (X . Wup), silu(g) = g / (1 + exp(-g)): qlin_gemv_silu_mul_dev for these operands and any number of
+ * tokens, the activation applied to the fp32 sums. Wgate and Wup are operands of n_rows x n_cols each. */
+int qlin_mxfp4_gemm_silu_mul_dev(const void *Wgate, const void *Wup, uint32_t x_type, const void *X, uint32_t y_type, void *Y, int n_rows,
+                                 int n_cols, int n_tok, int ldx, int ldy, void *workspace, size_t workspace_bytes, void *stream);
+
+/* ------------------------------------------------------------------ sampling
+ * ids[s] = the next token of sequence s from its logits (F32, F16 or BF16, row pitch ld elements), where the greedy pick of
+ * qlin_gemv_argmax_dev (server/server_llm.c:224-228) always takes the largest. The tokens of a sequence stand in the order of
+ * their logits, largest first and equal ones by index; those that hold NaN or -infinity are not there (tokens that the caller rules
+ * out). A token weighs exp((logit - largest logit) / temperature). Of them are kept
+ *   top_k   the first so many (0 or less: all)
+ *   top_p   of those the shortest run from the first whose weights reach top_p times their sum, at least one (1 or more: all)
+ *   min_p   of those the ones whose weight is at least min_p times the first one's (0 or less: all; above 1 as 1)
+ * and the pick is the first at which the running sum of weights exceeds u times the sum of the kept, the last one with a weight if
+ * there is none. Temperature 0 or less picks the first of the order. A sequence of which no token is there gets id -1.
+ * probs (may be NULL): the pick's weight divided by the sum of the kept; 1 for the first of the order, 0 for id -1.
+ * temperature, top_k, top_p, min_p and u are device arrays of n_seq elements, u of numbers in [0, 1) (a smaller one or NaN counts as
+ * 0); each of the first four may be NULL, which is 1, 0, 1 and 0 for every sequence (so is a NaN among top_p and min_p; NaN as a
+ * temperature is 0). Several +infinities share the weight among them. Weights are 64-bit exponentials and their sums integers of at
+ * most 2^-44 (up to 262144 tokens) of the largest weight: the same call gives the same token, and a token below half a unit is never
+ * picked.
+ * workspace: device memory, 256-byte aligned, qlin_sample_workspace_bytes(n_seq, n_vocab) bytes (0: it may be NULL), which holds
+ * nothing between calls; calls that share one must be ordered on one stream. */
+size_t qlin_sample_workspace_bytes(int n_seq, int n_vocab);
+int qlin_sample_dev(uint32_t logits_type, const void *logits, int n_seq, int n_vocab, int ld, const float *temperature, const int32_t *top_k,
+                    const float *top_p, const float *min_p, const float *u, int32_t *ids, float *probs, void *workspace,
+                    size_t workspace_bytes, void *stream);
+
 /* ------------------------------------------------------------------ GGUF file -> HBM
  * The tensor table and key/value pairs of a GGUF model file (versions 2 and 3, as read by
  * gguf_open, common/gguf_loader.h:343-411) and its tensor bytes in device memory.
