@@ -7,14 +7,21 @@
  * reach p times their sum, min-p of those the tokens with w >= m (the largest has 1). The pick is the first kept token at which the
  * running sum of weights exceeds u times the sum of the kept.
  *
- * Nothing is sorted. A cut ("the k-th", "where the sum reaches s") is found by its value: floats map to unsigned keys of the same
- * order, and of the keys' 11 + 11 + 10 bits each pass over the row fixes the next by a histogram of counts and weights. Tokens
- * that share the value at a cut weigh the same, so how many of them stay is a division, and which one is picked a count by index.
+ * A row is not sorted. Its tokens fall into 2048 bins by their distance from the largest logit, in bins of 1/64 of the temperature (of
+ * 1/2040 of the row's range where that is finer); what is further away than 2047 bins weighs less than 1.3e-14 and is not counted.
+ * Sums over the bins say in which bin a cut lies - the k-th token, p times the sum, the smallest weight, u times the sum - or, as
+ * long as an earlier cut inside a bin leaves a sum open, in which few of them. Only the tokens of those bins are listed and sorted (a
+ * few hundred of 150000), and the cuts are made exactly on the list. With top_k of 1 to 1024 all kept tokens fit the list, and the
+ * bins hold counts instead of weights.
+ *   One pass over the row finds the largest and smallest logit, one fills the bins, one lists; the second and third read from the
+ * caches what the first brought.
  *
- * Weights are exp in 64 bits, as 64-bit integers of 2^-shift with shift such that a row of the largest weight does not overflow
- * (2^-45 at 152k tokens): borders between tokens lie closer to each other than fp32 sums resolve, and integer sums do not depend on
- * their order, so the same call gives the same token. A token below half a unit has no weight and is never picked, as one of 10^5 such
- * tokens would be once in 10^8 calls.
+ * Weights and sums are 64-bit: the borders between tokens lie closer to each other than fp32 sums resolve, and the token is to be the
+ * one that the definition gives. A bin's weight is exp(centre) times the sum of exp(offset from the centre), offsets below 1/128, so
+ * that a token costs a polynomial of degree 5 (3e-16) instead of an exponential; the sum is of integers of 2^-40, which do not depend on
+ * the order of the additions: the same call gives the same token.
+ *   A list that overflows (a bin of more than 2048 tokens: rows of equal logits) leaves the row to sample_by_value, which takes
+ * several passes for each cut.
  */
 #include "qlin_device.h"
 #include "qlin_internal.h"
@@ -40,6 +47,31 @@ __device__ __forceinline__ uint32_t key_of(float v) {
 }
 __device__ __forceinline__ float value_of(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k); }
 
+
+/* a sequence's settings */
+struct Settings {
+    float t, p, m, u;
+    int k;
+};
+__device__ __forceinline__ Settings settings_of(const SampleCall &c, int seq) {
+    Settings s;
+    s.t = c.temperature ? c.temperature[seq] : 1.0f;
+    s.k = c.top_k ? c.top_k[seq] : 0;
+    s.p = c.top_p ? c.top_p[seq] : 1.0f;
+    s.m = c.min_p && c.min_p[seq] > 0.0f ? fminf(c.min_p[seq], 1.0f) : 0.0f;
+    const float u = c.u[seq];
+    s.u = u > 0.0f ? u : 0.0f;
+    return s;
+}
+__device__ __forceinline__ bool takes_first(const Settings &s) { return !(s.t > 0.0f) || s.k == 1; }
+
+__device__ __forceinline__ uint64_t shfl_u64(uint64_t v, int from) {
+    return (uint64_t)__shfl((uint32_t)(v >> 32), from, 64) << 32 | __shfl((uint32_t)v, from, 64);
+}
+__device__ __forceinline__ double shfl_up_f64(double v, int by) { return __shfl_up(v, by, 64); }
+
+/* ------------------------------------------------------------------ a row by the bits of its values */
+
 struct Weights {
     float max;
     double per_t; /* 1 / T */
@@ -55,30 +87,28 @@ struct Weights {
 struct Sum { uint32_t count; uint64_t weight; };
 __device__ __forceinline__ Sum operator+(Sum a, Sum b) { return {a.count + b.count, a.weight + b.weight}; }
 
-__device__ __forceinline__ uint64_t shfl_u64(uint64_t v, int from) {
-    return (uint64_t)__shfl((uint32_t)(v >> 32), from, 64) << 32 | __shfl((uint32_t)v, from, 64);
-}
+constexpr int kBins = 2048, kListed = 2048, kTopList = 1024; /* bins; tokens of a list; top_k up to which a list holds all kept */
 
 struct Shared {
-    uint32_t count[2048];
-    uint64_t weight[2048];
+    union {
+        uint64_t weight[kBins]; /* sums of 2^-bits exp(offset); afterwards, as doubles, running sums of weights */
+        double upto[kBins];
+    };
+    uint32_t count[kBins]; /* afterwards running sums */
+    uint64_t list[kListed];
+    union {
+        double run[kListed];     /* running sums of the list's weights */
+        uint64_t sorted[kListed];
+    };
     Sum wave[kWaves];
-    float wave_max[kWaves];
-    uint32_t digit;
+    double wave_f64[kWaves];
+    uint32_t wave_u32[kWaves];
+    float wave_max[kWaves], wave_min[kWaves];
+    uint32_t digit, n_list, best, found[4];
     Sum above;
     int picked;
+    bool last;
 };
-
-__device__ float max_of_workgroup(float v, Shared &s) {
-    for (int off = 32; off; off >>= 1) v = fmaxf(v, __shfl_xor(v, off, 64));
-    if ((threadIdx.x & 63) == 0) s.wave_max[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = s.wave_max[0];
-    for (int w = 1; w < kWaves; w++) v = fmaxf(v, s.wave_max[w]);
-    __syncthreads();
-    return v;
-}
-
 /* sum of all threads' v, in every thread; `before`: of the threads before this one */
 __device__ Sum sum_of_workgroup(Sum v, Shared &s, Sum *before) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -161,44 +191,11 @@ template <class T> __device__ int nth_of_value(const T *x, int n, uint32_t k, ui
     return s.picked;
 }
 
-template <class T>
-__global__ void __launch_bounds__(kThreads)
-sample_kernel(const T *__restrict__ logits, int n, size_t ld, const float *__restrict__ temperature, const int32_t *__restrict__ top_k,
-              const float *__restrict__ top_p, const float *__restrict__ min_p, const float *__restrict__ u, int32_t *__restrict__ ids,
-              float *__restrict__ probs, int shift) {
-    __shared__ Shared s;
-    const int seq = blockIdx.x;
-    const T *x = logits + (size_t)seq * ld;
-    const float t = temperature ? temperature[seq] : 1.0f;
-    const int k = top_k ? top_k[seq] : 0;
-    const float p = top_p ? top_p[seq] : 1.0f;
-    const float m = min_p && min_p[seq] > 0.0f ? fminf(min_p[seq], 1.0f) : 0.0f;
-
-    float best = kMinusInf;
-    for (int i = threadIdx.x; i < n; i += kThreads) {
-        const float v = to_f32(x[i]);
-        if (is_there(v)) best = fmaxf(best, v);
-    }
-    Weights w;
-    w.max = max_of_workgroup(best, s);
-    if (!is_there(w.max)) {
-        if (threadIdx.x == 0) {
-            ids[seq] = -1;
-            if (probs) probs[seq] = 0.0f;
-        }
-        return;
-    }
-    if (!(t > 0.0f) || k == 1) {
-        const int at = nth_of_value(x, n, key_of(w.max), 1, s);
-        if (threadIdx.x == 0) {
-            ids[seq] = at;
-            if (probs) probs[seq] = 1.0f;
-        }
-        return;
-    }
-    w.per_t = 1.0 / (double)t;
+/* the whole row by values: for rows whose lists overflow. n tokens, of which the largest is w.max */
+template <class T> __device__ void sample_by_value(const T *x, int n, const Settings &set, Weights w, int32_t *id, float *prob, Shared &s) {
+    int shift = 62; /* n << shift stays below 2^63 */
+    while (shift > 0 && ((uint64_t)n >> (62 - shift)) > 1) shift--;
     w.unit = (double)(1ull << shift);
-
     Sum all = {0, 0};
     for (int i = threadIdx.x; i < n; i += kThreads) {
         const float v = to_f32(x[i]);
@@ -208,43 +205,470 @@ sample_kernel(const T *__restrict__ logits, int n, size_t ld, const float *__res
 
     uint32_t last = 0; /* key of the last kept token's value (0: everything is kept) */
     uint64_t total = all.weight;
-    if (k > 0 && (uint32_t)k < all.count) {
-        const Cut c = find_cut<false>(x, n, w, (uint64_t)k, s);
+    if (set.k > 0 && (uint32_t)set.k < all.count) {
+        const Cut c = find_cut<false>(x, n, w, (uint64_t)set.k, s);
         last = c.key;
-        total = c.above.weight + (k - c.above.count) * w(value_of(c.key));
+        total = c.above.weight + (set.k - c.above.count) * w(value_of(c.key));
     }
-    if (p < 1.0f) {
-        const uint64_t target = min(max((uint64_t)ceil(fmax((double)p, 0.0) * (double)total), (uint64_t)1), total);
+    if (set.p < 1.0f) {
+        const uint64_t target = min(max((uint64_t)ceil(fmax((double)set.p, 0.0) * (double)total), (uint64_t)1), total);
         const Cut c = find_cut<true>(x, n, w, target, s);
         const uint64_t each = w(value_of(c.key)); /* not 0: the sum grows here */
         last = c.key;
         total = c.above.weight + (target - c.above.weight + each - 1) / each * each;
     }
-    if (m > 0.0f && (last == 0 || w.real(value_of(last)) < (double)m)) {
+    if (set.m > 0.0f && (last == 0 || w.real(value_of(last)) < (double)set.m)) {
         Sum kept = {0, 0};
         for (int i = threadIdx.x; i < n; i += kThreads) {
             const float v = to_f32(x[i]);
-            if (is_there(v) && (v == w.max || (key_of(v) > last && w.real(v) >= (double)m))) kept = kept + Sum{1, w(v)};
+            if (is_there(v) && (v == w.max || (key_of(v) > last && w.real(v) >= (double)set.m))) kept = kept + Sum{1, w(v)};
         }
         total = sum_of_workgroup(kept, s, nullptr).weight;
     }
-    const float draw = u[seq];
-    uint64_t target = draw > 0.0f ? (uint64_t)fmin((double)draw * (double)total, 9.0e18) : 0;
+    uint64_t target = (uint64_t)fmin((double)set.u * (double)total, 9.0e18);
     target = min(target, total - 1) + 1;
     const Cut c = find_cut<true>(x, n, w, target, s);
     const uint64_t each = w(value_of(c.key));
     const int at = nth_of_value(x, n, c.key, (uint32_t)((target - c.above.weight + each - 1) / each), s);
     if (threadIdx.x == 0) {
-        ids[seq] = at;
-        if (probs) probs[seq] = (float)((double)each / (double)total);
+        *id = at;
+        if (prob) *prob = (float)((double)each / (double)total);
     }
 }
 
+/* ------------------------------------------------------------------ a row by bins */
+
+/* fn(value, index) for this thread's share of elements lo .. hi - 1 of x: 16-byte loads between the first and the last address on
+ * 16 bytes, four in flight per thread */
+template <class T, class F> __device__ __forceinline__ void for_each(const T *x, int lo, int hi, F fn) {
+    constexpr int kPer = 16 / sizeof(T);
+    struct alignas(16) Vec { T v[kPer]; };
+    const int skip = (int)(((16 - (reinterpret_cast<uintptr_t>(x + lo) & 15)) & 15) / sizeof(T));
+    const int first = min(lo + skip, hi), vecs = (hi - first) / kPer, behind = first + vecs * kPer;
+    if ((int)threadIdx.x < first - lo) fn(to_f32(x[lo + threadIdx.x]), lo + (int)threadIdx.x);
+    if ((int)threadIdx.x < hi - behind) fn(to_f32(x[behind + threadIdx.x]), behind + (int)threadIdx.x);
+    const Vec *p = reinterpret_cast<const Vec *>(x + first);
+    int i = threadIdx.x;
+    for (; i + 3 * kThreads < vecs; i += 4 * kThreads) {
+        const Vec a = p[i], b = p[i + kThreads], c = p[i + 2 * kThreads], d = p[i + 3 * kThreads];
+#pragma unroll
+        for (int j = 0; j < kPer; j++) fn(to_f32(a.v[j]), first + i * kPer + j);
+#pragma unroll
+        for (int j = 0; j < kPer; j++) fn(to_f32(b.v[j]), first + (i + kThreads) * kPer + j);
+#pragma unroll
+        for (int j = 0; j < kPer; j++) fn(to_f32(c.v[j]), first + (i + 2 * kThreads) * kPer + j);
+#pragma unroll
+        for (int j = 0; j < kPer; j++) fn(to_f32(d.v[j]), first + (i + 3 * kThreads) * kPer + j);
+    }
+    for (; i < vecs; i += kThreads) {
+        const Vec a = p[i];
+#pragma unroll
+        for (int j = 0; j < kPer; j++) fn(to_f32(a.v[j]), first + i * kPer + j);
+    }
+}
+
+struct Range { float max, min; };
+__device__ Range range_of_workgroup(Range r, Shared &s) {
+    for (int off = 32; off; off >>= 1) {
+        r.max = fmaxf(r.max, __shfl_xor(r.max, off, 64));
+        r.min = fminf(r.min, __shfl_xor(r.min, off, 64));
+    }
+    if ((threadIdx.x & 63) == 0) s.wave_max[threadIdx.x >> 6] = r.max, s.wave_min[threadIdx.x >> 6] = r.min;
+    __syncthreads();
+    for (int w = 0; w < kWaves; w++) r.max = fmaxf(r.max, s.wave_max[w]), r.min = fminf(r.min, s.wave_min[w]);
+    __syncthreads();
+    return r;
+}
+template <class T> __device__ __forceinline__ Range range_of_share(const T *x, int lo, int hi) {
+    Range r = {kMinusInf, -kMinusInf};
+    for_each(x, lo, hi, [&](float v, int) {
+        const bool there = is_there(v);
+        r.max = fmaxf(r.max, there ? v : kMinusInf);
+        r.min = fminf(r.min, there ? v : -kMinusInf);
+    });
+    return r;
+}
+
+/* the bins of a row */
+struct Grid {
+    float max;
+    double per_t;  /* 1 / T */
+    double scale;  /* bins per unit of logits */
+    double step;   /* a bin in units of the exponent: at most 1/64 */
+    double unit;   /* 2^bits: of the sums of exp(offset) */
+    __device__ Grid(const Range &r, float t, int n) : max(r.max), per_t(1.0 / (double)t) {
+        const double span = (double)r.max - (double)r.min;
+        scale = fmax(64.0 * per_t, span > 0.0 ? 2040.0 / span : 0.0);
+        if (!(scale > 0.0)) scale = 1.0;
+        step = per_t / scale;
+        int bits = 40; /* n << bits stays below 2^62 */
+        while (bits > 0 && ((uint64_t)n >> (61 - bits)) > 0) bits--;
+        unit = (double)(1ull << bits);
+    }
+    /* in bins from the largest; 2047 and more: not counted */
+    __device__ __forceinline__ double place(float v) const { return v == max ? 0.0 : ((double)max - (double)v) * scale; }
+    __device__ __forceinline__ uint64_t offset_weight(double place, int bin) const {
+        const double g = ((double)bin + 0.5 - place) * step;
+        double e = fma(g, 1.0 / 120, 1.0 / 24);
+        e = fma(e, g, 1.0 / 6);
+        e = fma(e, g, 0.5);
+        e = fma(e, g, 1.0);
+        e = fma(e, g, 1.0);
+        /* the integer nearest to e * unit is what the sum with 2^52 holds below the exponent */
+        return (uint64_t)__double_as_longlong(fma(e, unit, 4503599627370496.0)) & 0x000FFFFFFFFFFFFFull;
+    }
+    __device__ double weight(float v) const { return v == max ? 1.0 : max == -kMinusInf ? 0.0 : exp(((double)v - (double)max) * per_t); }
+};
+constexpr int kLastBin = kBins - 2;
+
+/* what a row's bins hold: counts where the list will hold all kept tokens, else weights, and both where top_k is larger than that */
+__device__ __forceinline__ bool needs_counts(const Settings &s) { return s.k > 0; }
+__device__ __forceinline__ bool needs_weights(const Settings &s) { return s.k <= 0 || s.k > kTopList; }
+
+template <class T> __device__ __forceinline__ void fill_bins(const T *x, int lo, int hi, const Grid &g, const Settings &set, Shared &s) {
+    if (!needs_weights(set)) {
+        for_each(x, lo, hi, [&](float v, int) {
+            const double at = g.place(v);
+            if (is_there(v) && at < kBins - 1) atomicAdd(&s.count[(int)at], 1u);
+        });
+    } else {
+        const bool counts = needs_counts(set);
+        for_each(x, lo, hi, [&](float v, int) {
+            const double at = g.place(v);
+            if (is_there(v) && at < kBins - 1) {
+                const int bin = (int)at;
+                atomicAdd((unsigned long long *)&s.weight[bin], (unsigned long long)g.offset_weight(at, bin));
+                if (counts) atomicAdd(&s.count[bin], 1u);
+            }
+        });
+    }
+}
+
+/* counts and weights to running sums */
+__device__ void sum_bins(const Grid &g, const Settings &set, Shared &s) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, b = 2 * threadIdx.x;
+    if (needs_weights(set)) {
+        const double a0 = (double)s.weight[b] / g.unit * exp(-((double)b + 0.5) * g.step);
+        const double a1 = b + 1 > kLastBin ? 0.0 : (double)s.weight[b + 1] / g.unit * exp(-((double)b + 1.5) * g.step);
+        double run = a0 + a1;
+        for (int off = 1; off < 64; off <<= 1) {
+            const double o = shfl_up_f64(run, off);
+            if (lane >= off) run += o;
+        }
+        if (lane == 63) s.wave_f64[wave] = run;
+        __syncthreads();
+        double before = 0.0;
+        for (int w = 0; w < wave; w++) before += s.wave_f64[w];
+        /* (a running sum must not fall from one bin to the next: both are the same sum and a1) */
+        s.upto[b + 1] = before + run;
+        s.upto[b] = before + run - a1;
+    }
+    if (needs_counts(set)) {
+        const uint32_t a0 = s.count[b], a1 = s.count[b + 1];
+        uint32_t run = a0 + a1;
+        for (int off = 1; off < 64; off <<= 1) {
+            const uint32_t o = __shfl_up(run, off, 64);
+            if (lane >= off) run += o;
+        }
+        if (lane == 63) s.wave_u32[wave] = run;
+        __syncthreads();
+        uint32_t before = 0;
+        for (int w = 0; w < wave; w++) before += s.wave_u32[w];
+        s.count[b] = before + run - a1;
+        s.count[b + 1] = before + run;
+    }
+    __syncthreads();
+}
+
+/* first bin whose running sum fulfils `reached`, kLastBin + 1 if none does */
+template <class F> __device__ int first_bin(F reached) {
+    int lo = 0, hi = kLastBin + 1;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (reached(mid)) hi = mid;
+        else lo = mid + 1;
+    }
+    return lo;
+}
+
+/* the bins to list, as up to four runs in order, and which of them hold which cut */
+struct Run { int lo, hi; };
+struct Wanted {
+    Run k, p, m, u; /* the bins in which each cut may lie; empty (hi < lo): it does not cut */
+    Run run[4];     /* their union */
+    int n;
+    bool all;       /* the list holds every kept token (run[0] from bin 0) */
+};
+__device__ void add_run(Wanted &w, Run r) {
+    if (r.hi < r.lo) return;
+    int i = 0;
+    while (i < w.n && w.run[i].hi + 1 < r.lo) i++;
+    if (i == w.n || r.hi + 1 < w.run[i].lo) { /* apart from all */
+        for (int j = w.n; j > i; j--) w.run[j] = w.run[j - 1];
+        w.run[i] = r;
+        w.n++;
+        return;
+    }
+    w.run[i].lo = min(w.run[i].lo, r.lo);
+    w.run[i].hi = max(w.run[i].hi, r.hi);
+    while (i + 1 < w.n && w.run[i + 1].lo <= w.run[i].hi + 1) {
+        w.run[i].hi = max(w.run[i].hi, w.run[i + 1].hi);
+        for (int j = i + 1; j + 1 < w.n; j++) w.run[j] = w.run[j + 1];
+        w.n--;
+    }
+}
+__device__ Wanted wanted_bins(const Grid &g, const Settings &set, const Shared &s) {
+    constexpr double kSlack = 1e-11; /* of the sums' rounding */
+    const Run none = {0, -1};
+    Wanted w = {none, none, none, none, {none, none, none, none}, 0, !needs_weights(set)};
+    if (w.all) {
+        w.run[0] = {0, min(first_bin([&](int b) { return s.count[b] >= (uint32_t)set.k; }), kLastBin)};
+        w.n = 1;
+        return w;
+    }
+    auto before = [&](int b) { return b > 0 ? s.upto[b - 1] : 0.0; };
+    double lo = s.upto[kLastBin], hi = lo; /* between which the sum of the kept lies */
+    if (set.k > 0) {
+        const int b = first_bin([&](int i) { return s.count[i] >= (uint32_t)set.k; });
+        if (b <= kLastBin) w.k = {b, b}, lo = before(b), hi = s.upto[b];
+    }
+    if (set.p < 1.0f) {
+        const double p = fmax((double)set.p, 0.0);
+        w.p.lo = min(first_bin([&](int i) { return s.upto[i] >= p * lo * (1.0 - kSlack); }), kLastBin);
+        w.p.hi = min(first_bin([&](int i) { return s.upto[i] >= p * hi * (1.0 + kSlack); }), kLastBin);
+        lo = fmin(lo, before(w.p.lo));
+        hi = fmin(hi, s.upto[w.p.hi]);
+    }
+    if (set.m > 0.0f) {
+        const double at = -log((double)set.m) / g.step;
+        if (at < kBins) {
+            w.m = {max((int)at - 1, 0), min((int)at + 1, kLastBin)};
+            lo = fmin(lo, before(w.m.lo));
+            hi = fmin(hi, s.upto[w.m.hi]);
+        }
+    }
+    const double u = fmin((double)set.u, 1.0);
+    w.u.lo = min(first_bin([&](int i) { return s.upto[i] > u * lo * (1.0 - kSlack); }), kLastBin);
+    w.u.hi = min(first_bin([&](int i) { return s.upto[i] > u * hi * (1.0 + kSlack); }), kLastBin);
+    if (w.u.hi == kLastBin && u * hi * (1.0 + kSlack) >= s.upto[kLastBin]) /* the last bin that weighs anything */
+        w.u.hi = min(first_bin([&](int i) { return s.upto[i] >= s.upto[kLastBin] * (1.0 - kSlack); }), kLastBin);
+    w.u.hi = max(w.u.hi, w.u.lo);
+    add_run(w, w.k);
+    add_run(w, w.p);
+    add_run(w, w.m);
+    add_run(w, w.u);
+    return w;
+}
+
+/* ascending order of these is the order of the tokens */
+__device__ __forceinline__ uint64_t entry_of(float v, int i) { return (uint64_t)(~key_of(v)) << 32 | (uint32_t)i; }
+__device__ __forceinline__ float entry_value(uint64_t e) { return value_of(~(uint32_t)(e >> 32)); }
+
+/* fn(entry) for the tokens of the wanted bins */
+template <class T, class F> __device__ __forceinline__ void for_each_wanted(const T *x, int lo, int hi, const Grid &g, const Wanted &w, F fn) {
+    for_each(x, lo, hi, [&](float v, int i) {
+        const double at = g.place(v);
+        if (!is_there(v) || !(at < kBins - 1)) return;
+        const int b = (int)at;
+        bool in = false;
+#pragma unroll
+        for (int r = 0; r < 4; r++) in = in || (b >= w.run[r].lo && b <= w.run[r].hi);
+        if (in) fn(entry_of(v, i));
+    });
+}
+
+/* s.list[0 .. n) into order (n <= kListed) */
+__device__ void sort_list(int n, Shared &s) {
+    if (n <= 256) { /* by the number of smaller ones: 4 (16 for up to 64) threads count for each */
+        const int each = n <= 64 ? 16 : 4, i = threadIdx.x / each, part = threadIdx.x % each;
+        uint64_t mine = 0;
+        uint32_t rank = 0;
+        if (i < n) {
+            mine = s.list[i];
+            for (int j = part; j < n; j += each) rank += s.list[j] < mine;
+        }
+        for (int off = 1; off < each; off <<= 1) rank += __shfl_xor(rank, off, 64);
+        if (i < n && part == 0) s.sorted[rank] = mine;
+        __syncthreads();
+        if ((int)threadIdx.x < n) s.list[threadIdx.x] = s.sorted[threadIdx.x];
+        __syncthreads();
+        return;
+    }
+    int size = 512;
+    while (size < n) size <<= 1;
+    for (int i = n + threadIdx.x; i < size; i += kThreads) s.list[i] = ~0ull;
+    __syncthreads();
+    for (int k = 2; k <= size; k <<= 1)
+        for (int j = k >> 1; j; j >>= 1) {
+            const int t = threadIdx.x, i = 2 * t - (t & (j - 1)); /* the lower of the pair */
+            if (t < size / 2) {
+                const uint64_t a = s.list[i], b = s.list[i + j];
+                if ((a > b) == ((i & k) == 0)) s.list[i] = b, s.list[i + j] = a;
+            }
+            __syncthreads();
+        }
+}
+
+/* the cuts on the sorted list */
+template <class G> __device__ void pick_from_list(int n, const G &g, const Settings &set, const Wanted &w, int32_t *id, float *prob, Shared &s) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i0 = 2 * threadIdx.x;
+    if (threadIdx.x < 4) s.found[threadIdx.x] = (uint32_t)n;
+    double wt[2];
+    int bin[2];
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+        const bool there = i0 + e < n;
+        const float v = there ? entry_value(s.list[i0 + e]) : 0.0f;
+        wt[e] = there ? g.weight(v) : 0.0;
+        bin[e] = there ? (int)g.place(v) : kBins;
+    }
+    double run = wt[0] + wt[1];
+    for (int off = 1; off < 64; off <<= 1) {
+        const double o = shfl_up_f64(run, off);
+        if (lane >= off) run += o;
+    }
+    if (lane == 63) s.wave_f64[wave] = run;
+    __syncthreads();
+    double ahead = 0.0;
+    for (int v = 0; v < wave; v++) ahead += s.wave_f64[v];
+    s.run[i0 + 1] = ahead + run;
+    s.run[i0] = ahead + run - wt[1];
+    /* where the runs of bins begin in the list */
+#pragma unroll
+    for (int r = 0; r < 4; r++)
+#pragma unroll
+        for (int e = 1; e >= 0; e--)
+            if (r < w.n && bin[e] >= w.run[r].lo) atomicMin(&s.found[r], (uint32_t)(i0 + e));
+    __syncthreads();
+    double base[4]; /* running sum over the row minus running sum over the list, by run */
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+        base[r] = 0.0;
+        if (!w.all && r < w.n) {
+            const uint32_t at = s.found[r];
+            base[r] = (w.run[r].lo > 0 ? s.upto[w.run[r].lo - 1] : 0.0) - (at > 0 ? s.run[at - 1] : 0.0);
+        }
+    }
+    auto sum_to = [&](int i, int b) { /* running sum at entry i, of bin b */
+        double off = base[0];
+#pragma unroll
+        for (int r = 1; r < 4; r++)
+            if (r < w.n && b >= w.run[r].lo) off = base[r];
+        return s.run[i] + off;
+    };
+    double sums[2];
+#pragma unroll
+    for (int e = 0; e < 2; e++) sums[e] = i0 + e < n ? sum_to(i0 + e, bin[e]) : 0.0;
+    auto bin_at = [&](int i) { return (int)g.place(entry_value(s.list[i])); };
+    /* first entry within `where` for which the test holds, n if there is none */
+    auto first = [&](Run where, auto test) {
+        __syncthreads();
+        if (threadIdx.x == 0) s.best = (uint32_t)n;
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < 2; e++)
+            if (i0 + e < n && bin[e] >= where.lo && bin[e] <= where.hi && test(i0 + e, wt[e], sums[e])) {
+                atomicMin(&s.best, (uint32_t)(i0 + e));
+                break;
+            }
+        __syncthreads();
+        return (int)s.best;
+    };
+    const Run everywhere = {0, kBins};
+    int kept = n; /* list entries from here on are cut off (those between the runs lie on the right side by construction) */
+    double total = w.all ? s.run[n - 1] : s.upto[kLastBin];
+    if (w.all) {
+        kept = min(set.k, n);
+        total = s.run[kept - 1];
+    } else if (w.k.hi >= w.k.lo) {
+        const uint32_t at = (uint32_t)set.k - (w.k.lo > 0 ? s.count[w.k.lo - 1] : 0u); /* of the bin's tokens, from 1 */
+        const int start = first(w.k, [](int, double, double) { return true; });
+        kept = min(start + (int)at, n);
+        total = sum_to(kept - 1, w.k.lo);
+    }
+    if (set.p < 1.0f) {
+        const double target = fmax((double)set.p, 0.0) * total;
+        const int i = first(w.all ? everywhere : w.p, [&](int, double, double sum) { return sum >= target; });
+        if (i < kept) {
+            kept = i + 1;
+            total = sum_to(i, bin_at(i));
+        }
+    }
+    if (w.all ? set.m > 0.0f : w.m.hi >= w.m.lo) {
+        const int i = first(w.all ? everywhere : w.m, [&](int, double weight, double) { return weight < (double)set.m; });
+        const int from = i < n || w.all ? i : first(Run{w.m.hi + 1, kBins}, [](int, double, double) { return true; });
+        kept = min(kept, from); /* (what lies behind the bins of this cut is lighter) */
+        if (i < n) total = fmin(total, sum_to(i, bin_at(i)) - g.weight(entry_value(s.list[i])));
+        else if (!w.all) total = fmin(total, s.upto[w.m.hi]);
+    }
+    const double target = (double)set.u * total;
+    int i = first(w.all ? everywhere : w.u, [&](int at, double weight, double sum) { return at < kept && weight > 0.0 && sum > target; });
+    if (i >= n) { /* u of 1, or the last border rounded away: the last kept token that weighs anything */
+        __syncthreads();
+        if (threadIdx.x == 0) s.best = 0;
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < 2; e++)
+            if (i0 + e < kept && wt[e] > 0.0) atomicMax(&s.best, (uint32_t)(i0 + e));
+        __syncthreads();
+        i = (int)s.best;
+    }
+    if (threadIdx.x == 0) {
+        *id = (int32_t)(uint32_t)s.list[i];
+        if (prob) *prob = (float)(g.weight(entry_value(s.list[i])) / total);
+    }
+}
+
+__device__ __forceinline__ void nothing_there(int32_t *id, float *prob) {
+    if (threadIdx.x == 0) {
+        *id = -1;
+        if (prob) *prob = 0.0f;
+    }
+}
+
+/* one workgroup per sequence */
+template <class T> __global__ void __launch_bounds__(kThreads) sample_row_kernel(const T *__restrict__ logits, SampleCall c) {
+    __shared__ Shared s;
+    const int seq = blockIdx.x, n = c.n_vocab;
+    const T *x = logits + (size_t)seq * c.ld;
+    int32_t *id = c.ids + seq;
+    float *prob = c.probs ? c.probs + seq : nullptr;
+    const Settings set = settings_of(c, seq);
+    const Range r = range_of_workgroup(range_of_share(x, 0, n), s);
+    if (!is_there(r.max)) return nothing_there(id, prob);
+    if (threadIdx.x == 0) s.best = (uint32_t)n, s.n_list = 0;
+    if (takes_first(set)) {
+        __syncthreads();
+        for_each(x, 0, n, [&](float v, int i) {
+            if (v == r.max) atomicMin(&s.best, (uint32_t)i);
+        });
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            *id = (int32_t)s.best;
+            if (prob) *prob = 1.0f;
+        }
+        return;
+    }
+    const Grid g(r, set.t, n);
+    for (int i = threadIdx.x; i < kBins; i += kThreads) s.weight[i] = 0, s.count[i] = 0;
+    __syncthreads();
+    fill_bins(x, 0, n, g, set, s);
+    __syncthreads();
+    sum_bins(g, set, s);
+    const Wanted w = wanted_bins(g, set, s);
+    for_each_wanted(x, 0, n, g, w, [&](uint64_t e) {
+        const uint32_t at = atomicAdd(&s.n_list, 1u);
+        if (at < kListed) s.list[at] = e;
+    });
+    __syncthreads();
+    const uint32_t listed = s.n_list;
+    if (listed > kListed) return sample_by_value(x, n, set, Weights{r.max, g.per_t, 0.0}, id, prob, s);
+    sort_list((int)listed, s);
+    pick_from_list((int)listed, g, set, w, id, prob, s);
+}
+
 template <class T> hipError_t sample(const SampleCall &c) {
-    int shift = 62; /* n << shift stays below 2^63 */
-    while (shift > 0 && ((uint64_t)c.n_vocab >> (62 - shift)) > 1) shift--;
-    sample_kernel<T><<<c.n_seq, kThreads, 0, c.stream>>>(static_cast<const T *>(c.logits), c.n_vocab, (size_t)c.ld, c.temperature, c.top_k, c.top_p, c.min_p, c.u,
-                                                        c.ids, c.probs, shift);
+    sample_row_kernel<T><<<c.n_seq, kThreads, 0, c.stream>>>(static_cast<const T *>(c.logits), c);
     return hipGetLastError();
 }
 
