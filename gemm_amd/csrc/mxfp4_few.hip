@@ -120,10 +120,14 @@ template <int MATS, class OUT> hipError_t few_tokens(const Mxfp4Product &p) {
 
 }  // namespace
 
-hipError_t launch_mxfp4_few(const Mxfp4Product &p, int n_cu) {
-    (void)n_cu;
+hipError_t launch_mxfp4_few(const Mxfp4Product &p) {
     if (p.up) return p.bf16_out ? few_tokens<2, __bf16>(p) : few_tokens<2, float>(p);
     return p.bf16_out ? few_tokens<1, __bf16>(p) : few_tokens<1, float>(p);
+}
+
+hipError_t launch_mxfp4_product(const Mxfp4Product &p, int n_cu) {
+    (void)n_cu;
+    return launch_mxfp4_few(p);
 }
 
 }  // namespace qlin

@@ -1,0 +1,284 @@
+/*
+ * mxfp4_tile.hip - products of MXFP4 operands (mxfp4.h) for many tokens: tiles of 64 MB rows x 64 NB tokens on four waves, two by two.
+ *
+ *   Y[t, r] = sum_k X[t, k] W[r, k]          or, of two tensors, silu(X . gate) * (X . up)
+ *
+ * v_mfma_scale_f32_32x32x64_f8f6f4 on 4-bit operands (9.6 PFLOP/s from registers on this part; the 16x16x128 form 6.9), fp32 sums.
+ * A wave holds 32 MB rows x 32 NB tokens as sums in registers. Both operands go from memory to LDS by load-to-LDS requests of 1 KB, an
+ * operand tile each, three column tiles ahead of their use in four stages; a fragment is one ds_read_b128 without bank conflicts,
+ * fetched half a column tile (64 columns) ahead into the second of two register sets. The exponents of 512 columns come the same
+ * way, a dword per lane, row and block, one byte for each of four column tiles. One barrier per column tile, in its middle: from there
+ * on fragments come from the next stage.
+ *   Of two tensors, the first MB / 2 row blocks of a wave are gate rows and the others the same rows of up: both sums of a result are in
+ * one lane.
+ */
+#include "mxfp4.h"
+#include "gemm_kq_formats.h"
+
+namespace qlin {
+using namespace mxfp4;
+
+namespace {
+
+using kq::dma16;
+
+template <int VM> QLIN_INL void wait_vmcnt_lds() { /* vmcnt(VM) and lgkmcnt(0) */
+    __builtin_amdgcn_s_waitcnt((VM & 15) | ((VM >> 4) << 14) | (7 << 4));
+}
+
+/* the stages are objects of their own: a fetch from one never waits for a request into another */
+template <int MB, int NB, int ST> QLIN_INL uint8_t *stage_of() {
+    __shared__ __attribute__((aligned(1024))) uint8_t stage[(4 * MB + 4 * NB) * kTileBytes];
+    return stage;
+}
+template <int MB, int NB> QLIN_INL uint8_t *exponents_of() {
+    __shared__ __attribute__((aligned(1024))) uint8_t exponents[(4 * MB + 4 * NB) * kScaleBytes];
+    return exponents;
+}
+
+template <int MB_, int NB_, bool PAIR_> struct Ctx {
+    static constexpr int MB = MB_, NB = NB_, kReq = MB + NB, kExpReq = (MB + NB + 3) / 4, kSlots = MB * NB;
+    static constexpr bool PAIR = PAIR_;
+    f32x16 acc[MB][NB];
+    u32x4 a[2][MB], b[2][NB];     /* fragments, [half column tile] */
+    int ea[2][MB], eb[2][NB];     /* exponents of these 512 columns */
+    int na[2][MB], nb[2][NB];     /* and of the next */
+    __amdgpu_buffer_rsrc_t w_rsrc, x_rsrc, e_rsrc[kExpReq];
+    uint32_t w_off[MB], x_off[NB]; /* of this wave's row groups, in scalar registers */
+    uint32_t e_off[kExpReq];
+    int e_to[kExpReq];
+    uint32_t lane16, a_at, b_at, ea_at, eb_at;
+    int wave, tiles, quads;
+    /* byte offset of row block m in a stage, for wave row 0 */
+    static constexpr int block(int m) { return PAIR && m >= MB / 2 ? (2 * MB + 2 * (m - MB / 2)) : 2 * m; }
+};
+
+constexpr int first_of(int t, int n, int slots) { return t >= slots ? n : (t * n + slots - 1) / slots; }
+
+template <int ST, int I, class C> QLIN_INL void request(C &c, int tile) { /* requests 0 .. kReq - 1 of this wave for a column tile */
+    const uint32_t at = (uint32_t)min(tile, c.tiles - 1) * kTileBytes; /* past the last tile: a harmless repetition */
+    uint8_t *st = stage_of<C::MB, C::NB, ST>();
+    if constexpr (I < C::MB) dma16(c.w_rsrc, st + (C::MB * c.wave + I) * kTileBytes, c.lane16, c.w_off[I] + at);
+    else dma16(c.x_rsrc, st + (4 * C::MB + C::NB * c.wave + I - C::MB) * kTileBytes, c.lane16, c.x_off[I - C::MB] + at);
+}
+template <int I, class C> QLIN_INL void request_exponents(C &c, int quad) {
+    dma16(c.e_rsrc[I], exponents_of<C::MB, C::NB>() + c.e_to[I], c.e_off[I], (uint32_t)min(quad, c.quads - 1) * kScaleBytes);
+}
+/* fragment I of half H of stage ST: a 0, b 0 .. NB - 1, a 1 .. */
+template <int ST, int H, int I, class C> QLIN_INL void fetch(C &c) {
+    const uint8_t *st = stage_of<C::MB, C::NB, ST>();
+    if constexpr (I >= 1 && I <= C::NB)
+        c.b[H][I - 1] = *reinterpret_cast<const u32x4 *>(st + c.b_at + 2 * (I - 1) * kTileBytes + H * 512);
+    else
+        c.a[H][I ? I - C::NB : 0] = *reinterpret_cast<const u32x4 *>(st + c.a_at + C::block(I ? I - C::NB : 0) * kTileBytes + H * 512);
+}
+template <int I, class C> QLIN_INL void fetch_exponent(C &c) { /* of the next 512 columns, 0 .. 2 kReq - 1 */
+    const uint8_t *e = exponents_of<C::MB, C::NB>();
+    constexpr int h = I & 1, i = I >> 1;
+    if constexpr (i < C::MB) c.na[h][i] = *reinterpret_cast<const int *>(e + c.ea_at + C::block(i) * kScaleBytes + h * 128);
+    else c.nb[h][i - C::MB] = *reinterpret_cast<const int *>(e + c.eb_at + 2 * (i - C::MB) * kScaleBytes + h * 128);
+}
+
+template <int LO, int HI, class F> QLIN_INL void each(F fn) {
+    if constexpr (LO < HI) {
+        fn(std::integral_constant<int, LO>{});
+        each<LO + 1, HI>(fn);
+    }
+}
+
+/* slot T of half H of column tile `tile`, which is number U of its four */
+template <int U, int H, int T, class C> QLIN_INL void slot(C &c, int tile) {
+    constexpr int S = C::kSlots, m = T / C::NB, n = T % C::NB, g = H * S + T;
+    if constexpr (H == 1 && T == 0) {
+        /* The next tile's requests of this wave have landed: younger are those of the tile after it (with the exponents', which
+         * tile 0 of a quad requests after this point) and those of the one behind so far. The fragments of this tile are in
+         * registers, so that after the barrier its stage may be written. */
+        constexpr int so_far = first_of(S, C::kReq, 2 * S);
+        wait_vmcnt_lds<C::kReq + so_far + (U == 1 ? C::kExpReq : 0)>();
+        __builtin_amdgcn_s_barrier();
+    }
+    c.acc[m][n] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(widened(c.b[H][n]), widened(c.a[H][m]), c.acc[m][n], 4, 4, U, c.eb[H][n], U, c.ea[H][m]);
+    constexpr int early = S > 4 ? S * 3 / 4 : S; /* fragments are there before they are used */
+    each<first_of(T, C::kReq, early), first_of(T + 1, C::kReq, early)>([&](auto i) {
+        if constexpr (H == 0) fetch<U, 1, decltype(i)::value>(c);
+        else fetch<(U + 1) & 3, 0, decltype(i)::value>(c);
+    });
+    if constexpr (U == 0 && H == 1 && T == 0) each<0, C::kExpReq>([&](auto i) { request_exponents<decltype(i)::value>(c, (tile >> 2) + 1); });
+    if constexpr (U == 3) each<first_of(g, 2 * C::kReq, 2 * S), first_of(g + 1, 2 * C::kReq, 2 * S)>([&](auto i) { fetch_exponent<decltype(i)::value>(c); });
+    each<first_of(g, C::kReq, 2 * S), first_of(g + 1, C::kReq, 2 * S)>([&](auto i) { request<(U + 3) & 3, decltype(i)::value>(c, tile + 3); });
+    __builtin_amdgcn_sched_barrier(0);
+}
+template <int U, class C> QLIN_INL void run_tile(C &c, int tile) {
+    each<0, C::kSlots>([&](auto t) { slot<U, 0, decltype(t)::value>(c, tile); });
+    each<0, C::kSlots>([&](auto t) { slot<U, 1, decltype(t)::value>(c, tile); });
+}
+template <class C> QLIN_INL void take_exponents(C &c) {
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+#pragma unroll
+        for (int m = 0; m < C::MB; m++) c.ea[h][m] = c.na[h][m];
+#pragma unroll
+        for (int n = 0; n < C::NB; n++) c.eb[h][n] = c.nb[h][n];
+    }
+}
+
+/* Two results of this lane's row, of tokens t and t + 1, of which those below `tokens` are there; to = the row's place in token t. 32 lanes
+ * hold 32 consecutive rows: a store instruction writes two runs of 128 bytes of F32, or after an exchange between neighbouring lanes
+ * four of 64 bytes of BF16. */
+QLIN_INL void put2(float *to, size_t ldy, float a, float b, int tokens, int rows_left) {
+    if (rows_left <= 0) return;
+    if (tokens > 0) to[0] = a;
+    if (tokens > 1) to[ldy] = b;
+}
+QLIN_INL void put2(__bf16 *to, size_t ldy, float a, float b, int tokens, int rows_left) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    typedef bf16x2 anywhere __attribute__((aligned(2)));
+    const bool odd = threadIdx.x & 1; /* even lanes store token t of both rows, odd ones token t + 1 */
+    const float other = __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(odd ? a : b), 0xB1, 0xf, 0xf, true));
+    const bf16x2 v = {(__bf16)(odd ? other : a), (__bf16)(odd ? b : other)}; /* nearest even, the one rounding of a result */
+    to += odd ? (ptrdiff_t)ldy - 1 : 0;
+    rows_left += odd;
+    if (tokens <= (int)odd) return;
+    if (rows_left > 1) *reinterpret_cast<anywhere *>(to) = v;
+    else if (rows_left == 1) to[0] = v[0];
+}
+
+/* the bytes of an operand from row group `from` of a part with `pitch` bytes per group, as a buffer descriptor counts them */
+QLIN_INL uint32_t bytes_from(int groups, int from, uint32_t pitch) {
+    const size_t n = (size_t)(groups - from) * pitch;
+    return n > 0xFFFFFFFFu ? 0xFFFFFFFFu : (uint32_t)n;
+}
+
+template <int MB, int NB, bool PAIR, class OUT>
+__global__ void __launch_bounds__(256, MB + NB > 4 ? 1 : 2)
+tile_kernel(const uint8_t *__restrict__ W, const uint8_t *__restrict__ up, const uint8_t *__restrict__ X, OUT *__restrict__ Y, int n_rows, int n_tok, Shape w,
+            Shape x, size_t ldy, int row_tiles, int tok_tiles) {
+    /* consecutive workgroups go to different dies, each with an L2 of its own; the token tiles that share a row tile meet in one */
+    const int die = blockIdx.x & 7, at = blockIdx.x >> 3;
+    const int tok_tile = at % tok_tiles, row_tile = (at / tok_tiles) * 8 + die;
+    if (row_tile >= row_tiles) return;
+    constexpr int kRowGroups = PAIR ? 2 * MB : 4 * MB; /* row groups of a tensor per tile */
+    const int lane = threadIdx.x & 63;
+    Ctx<MB, NB, PAIR> c;
+    using C = Ctx<MB, NB, PAIR>;
+    c.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    c.tiles = w.tiles;
+    c.quads = w.quads;
+    c.lane16 = lane * 16;
+    const int wm = c.wave >> 1, wn = c.wave & 1;
+    const uint32_t code_pitch = (uint32_t)w.tiles * kTileBytes, exp_pitch = (uint32_t)w.quads * kScaleBytes;
+    const int g0 = row_tile * kRowGroups, x0 = tok_tile * 4 * NB;
+    /* codes: this wave requests MB row groups of the 4 MB (of two tensors, waves 0 and 1 gate's and 2 and 3 up's) and NB token groups;
+     * groups past the end repeat the last one */
+    const bool of_up = PAIR && c.wave >= 2;
+    c.w_rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(of_up ? up : W) + (size_t)g0 * code_pitch, 0, bytes_from(w.groups, g0, code_pitch), 0x00020000);
+    c.x_rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(X) + (size_t)x0 * code_pitch, 0, bytes_from(x.groups, x0, code_pitch), 0x00020000);
+#pragma unroll
+    for (int i = 0; i < MB; i++) c.w_off[i] = (uint32_t)min(MB * (of_up ? c.wave - 2 : c.wave) + i, w.groups - 1 - g0) * code_pitch;
+#pragma unroll
+    for (int i = 0; i < NB; i++) c.x_off[i] = (uint32_t)min(NB * c.wave + i, x.groups - 1 - x0) * code_pitch;
+    /* exponents: request id holds four groups' 256 bytes, ids below MB those of the rows */
+#pragma unroll
+    for (int i = 0; i < C::kExpReq; i++) {
+        const int id = min(c.wave + 4 * i, MB + NB - 1);
+        const bool rows = id < MB, second = PAIR && rows && 2 * id >= MB;
+        const uint8_t *part = rows ? (second ? up : W) + w.code_bytes() + (size_t)g0 * exp_pitch : X + x.code_bytes() + (size_t)x0 * exp_pitch;
+        const int last = rows ? w.groups - 1 - g0 : x.groups - 1 - x0;
+        const int group = (rows ? 4 * id - (second ? 2 * MB : 0) : 4 * (id - MB)) + (lane >> 4);
+        c.e_rsrc[i] = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(part), 0, bytes_from(last + 1, 0, exp_pitch), 0x00020000);
+        c.e_off[i] = (uint32_t)min(group, last) * exp_pitch + (lane & 15) * 16;
+        c.e_to[i] = id * 4 * kScaleBytes;
+    }
+    /* a lane's block of a 32-row fragment: row l % 32, that is group (l / 16) % 2, and block l / 32 of a half's two */
+    const uint32_t in_pair = (lane >> 4) & 1, in_half = lane >> 5, in_group = lane & 15;
+    constexpr int kWaveGroups = PAIR ? MB : 2 * MB;
+    c.a_at = (wm * kWaveGroups + in_pair) * kTileBytes + in_half * 256 + in_group * 16;
+    c.b_at = (4 * MB + wn * 2 * NB + in_pair) * kTileBytes + in_half * 256 + in_group * 16;
+    c.ea_at = (wm * kWaveGroups + in_pair) * kScaleBytes + in_half * 64 + in_group * 4;
+    c.eb_at = (4 * MB + wn * 2 * NB + in_pair) * kScaleBytes + in_half * 64 + in_group * 4;
+#pragma unroll
+    for (int m = 0; m < MB; m++)
+#pragma unroll
+        for (int n = 0; n < NB; n++)
+#pragma unroll
+            for (int v = 0; v < 16; v++) c.acc[m][n][v] = 0.0f;
+
+    /* The last columns' one to three tiles of a quad: a chain of tiles behind the loop, or where its registers would spill (16 blocks) a
+     * whole quad, whose missing tiles multiply repeated codes by 2^-127 twice: their exponent bytes are 0 on both sides, and 2^-254
+     * times any sum of codes is 0 in fp32. */
+    constexpr bool kChain = MB * NB <= 8;
+    each<0, C::kExpReq>([&](auto i) { request_exponents<decltype(i)::value>(c, 0); });
+    each<0, C::kReq>([&](auto i) { request<0, decltype(i)::value>(c, 0); });
+    each<0, C::kReq>([&](auto i) { request<1, decltype(i)::value>(c, 1); });
+    each<0, C::kReq>([&](auto i) { request<2, decltype(i)::value>(c, 2); });
+    wait_vmcnt_lds<2 * C::kReq>();
+    __builtin_amdgcn_s_barrier();
+    each<0, 2 * C::kReq>([&](auto i) { fetch_exponent<decltype(i)::value>(c); });
+    take_exponents(c);
+    each<0, C::kReq>([&](auto i) { fetch<0, 0, decltype(i)::value>(c); });
+#pragma unroll 1
+    for (int tile = 0; tile < c.tiles - (kChain ? 3 : 0); tile += 4) {
+        run_tile<0>(c, tile);
+        run_tile<1>(c, tile + 1);
+        run_tile<2>(c, tile + 2);
+        run_tile<3>(c, tile + 3);
+        take_exponents(c);
+    }
+    if constexpr (kChain) {
+        const int full = c.tiles & ~3;
+        if (c.tiles & 3) run_tile<0>(c, full);
+        if (c.tiles & 2) run_tile<1>(c, full + 1);
+        if ((c.tiles & 3) == 3) run_tile<2>(c, full + 2);
+    }
+    wait_vmcnt_lds<0>(); /* requests past the last tile are still on their way into LDS */
+
+    /* register v of lane l: token 8 (v / 4) + 4 (l / 32) + v % 4, row l % 32 */
+    constexpr int kOut = PAIR ? MB / 2 : MB;
+    const int t0 = (tok_tile * 2 + wn) * 32 * NB + 4 * (lane >> 5), r0 = (row_tile * 2 + wm) * 32 * kOut + (lane & 31);
+#pragma unroll
+    for (int n = 0; n < NB; n++)
+#pragma unroll
+        for (int v = 0; v < 16; v += 2) {
+            const int t = t0 + 32 * n + 8 * (v / 4) + v % 4;
+            OUT *y = Y + (size_t)t * ldy + r0;
+#pragma unroll
+            for (int m = 0; m < kOut; m++) {
+                float a = c.acc[m][n][v], b = c.acc[m][n][v + 1];
+                if constexpr (PAIR) a = silu_mul(a, c.acc[m + MB / 2][n][v]), b = silu_mul(b, c.acc[m + MB / 2][n][v + 1]);
+                put2(y + 32 * m, ldy, a, b, n_tok - t, n_rows - r0 - 32 * m);
+            }
+        }
+}
+
+template <int MB, int NB, bool PAIR, class OUT> hipError_t tiles(const Mxfp4Product &p) {
+    const Shape w = shape_of(p.n_rows, p.n_cols), x = shape_of(p.n_tok, p.n_cols);
+    constexpr int kRows = (PAIR ? 32 : 64) * MB, kTok = 64 * NB;
+    const int row_tiles = (p.n_rows + kRows - 1) / kRows, tok_tiles = (p.n_tok + kTok - 1) / kTok;
+    const dim3 grid((unsigned)((row_tiles + 7) / 8 * 8) * (unsigned)tok_tiles);
+    tile_kernel<MB, NB, PAIR, OUT><<<grid, 256, 0, p.stream>>>(p.W, p.up, p.X, static_cast<OUT *>(p.Y), p.n_rows, p.n_tok, w, x, (size_t)p.ldy, row_tiles, tok_tiles);
+    return hipGetLastError();
+}
+template <int MB, int NB> hipError_t tiles_for(const Mxfp4Product &p) {
+    if (p.up) {
+        if constexpr (MB % 2 == 0) return p.bf16_out ? tiles<MB, NB, true, __bf16>(p) : tiles<MB, NB, true, float>(p);
+        else return hipErrorInvalidValue;
+    }
+    return p.bf16_out ? tiles<MB, NB, false, __bf16>(p) : tiles<MB, NB, false, float>(p);
+}
+
+}  // namespace
+
+hipError_t launch_mxfp4_tiles(int mb, int nb, const Mxfp4Product &p) {
+    switch (10 * mb + nb) {
+    case 44: return tiles_for<4, 4>(p);
+    case 42: return tiles_for<4, 2>(p);
+    case 24: return tiles_for<2, 4>(p);
+    case 22: return tiles_for<2, 2>(p);
+    case 41: return tiles_for<4, 1>(p);
+    case 21: return tiles_for<2, 1>(p);
+    case 11: return tiles_for<1, 1>(p);
+    default: return hipErrorInvalidValue;
+    }
+}
+
+}  // namespace qlin

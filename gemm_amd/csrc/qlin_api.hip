@@ -1511,7 +1511,7 @@ static int mxfp4_gemm(const void *W, const void *up, bool pair, uint32_t x_type,
     if (x_type != T_MXFP4) HIP_TRY(launch_mxfp4_operand(x_type, X, workspace, n_tok, n_cols, ldx, (hipStream_t)stream));
     const Mxfp4Product p = {static_cast<const uint8_t *>(W), static_cast<const uint8_t *>(up), static_cast<const uint8_t *>(x_type == T_MXFP4 ? X : workspace), Y,
                             n_rows, n_cols, n_tok, ldy, y_type == T_BF16, (hipStream_t)stream};
-    HIP_TRY(launch_mxfp4_few(p, g.n_cu));
+    HIP_TRY(launch_mxfp4_product(p, g.n_cu));
     return QLIN_OK;
 }
 
@@ -1622,6 +1622,18 @@ int qlin_probe_gemm_tile(int tile, uint32_t type, const void *W, const uint16_t 
     if (int rc = init_once()) return rc;
     if (tile == 1) HIP_TRY(launch_gemm_kq_bf16_wave4s_multi(type, 1, &W, X, &Y, &n_rows, n_cols, n_tok, ldx, &ldy, (hipStream_t)stream));
     else HIP_TRY(launch_gemm_kq_bf16_wave4_multi(type, tile ? tile : 8, 1, &W, X, &Y, &n_rows, n_cols, n_tok, ldx, &ldy, (hipStream_t)stream));
+    return QLIN_OK;
+}
+
+int qlin_probe_mxfp4_gemm(int kernel, const void *W, const void *up, const void *X, uint32_t y_type, void *Y, int n_rows, int n_cols, int n_tok, int ldy,
+                          void *stream) {
+    if (y_type != T_F32 && y_type != T_BF16) return fail(QLIN_ERR_TYPE, "results are F32 or BF16 (got type %u)", y_type);
+    if (kernel < 0 || n_rows <= 0 || n_cols <= 0 || n_tok <= 0 || ldy < n_rows || !operand_fits(n_rows, n_cols) || !operand_fits(n_tok, n_cols)) return fail(QLIN_ERR_ARG, "bad kernel or size");
+    if (!W || !X || !Y || !aligned(W, 16) || !aligned(up, 16) || !aligned(X, 16) || !aligned(Y, float_bytes(y_type))) return fail(QLIN_ERR_ARG, "null or misaligned pointer");
+    if (int rc = init_once()) return rc;
+    const Mxfp4Product p = {static_cast<const uint8_t *>(W), static_cast<const uint8_t *>(up), static_cast<const uint8_t *>(X), Y, n_rows, n_cols, n_tok, ldy, y_type == T_BF16, (hipStream_t)stream};
+    if (kernel == 0) HIP_TRY(launch_mxfp4_few(p));
+    else HIP_TRY(launch_mxfp4_tiles(kernel / 10, kernel % 10, p));
     return QLIN_OK;
 }
 

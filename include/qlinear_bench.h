@@ -30,6 +30,11 @@ int qlin_probe_hbm_read(const void *buf, size_t n_bytes, void *stream);
  * other and for the parity tests of each on small shapes. */
 int qlin_probe_gemm_tile(int tile, uint32_t ggml_type, const void *W, const uint16_t *X, float *Y, int n_rows, int n_cols,
                          int n_tok, int ldx, int ldy, void *stream);
+/* One kernel of the 4-bit products by name, whatever the choice of qlin_mxfp4_gemm_dev would be: 0 = 16 rows per workgroup, its waves
+ * along K; 10 a + b = tiles of 64 a rows x 64 b tokens (44, 42, 24, 22, 41, 21, 11; not 11 with `up`). W, up (NULL: one tensor) and X are
+ * operands. */
+int qlin_probe_mxfp4_gemm(int kernel, const void *W, const void *up, const void *X, uint32_t y_type, void *Y, int n_rows, int n_cols, int n_tok,
+                          int ldy, void *stream);
 /* what qlin_gemm_bf16_any_dev does with a shape: 1 and 2 = a tile kernel, of the class of 256 x 128 or of 128 x 64 tiles (tensors of
  * one class share a launch; which tiles it takes says qlin_probe_gemm_blocks), 3 = the few-token kernel, 0 = none of them (a matvec
  * per token, or decode to bf16 + dense product) */

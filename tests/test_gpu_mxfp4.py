@@ -192,6 +192,15 @@ def test_product(rows, cols, tok):
         check(got, xq @ w.T, f.product_bound(xq, w), y_type)
 
 
+def gated(xq, g, u):
+    """results in 64 bits and how far they may be off: the slope of silu is at most 1.1; expf, the sum, the quotient and the product take
+    at most 8 half steps; a quotient below fp32's normal numbers may be lost"""
+    a, b = xq @ g.T, xq @ u.T
+    ea, eb = f.product_bound(xq, g), f.product_bound(xq, u)
+    want = f.silu_mul(a, b)
+    return want, 1.1 * ea * (np.abs(b) + eb) + np.abs(f.silu_mul(a, 1.0)) * eb + 8 * 2.0 ** -24 * np.abs(want) + 2.0 ** -126 * (1 + np.abs(b))
+
+
 @pytest.mark.parametrize("rows,cols,tok", SHAPES)
 def test_gate_and_up(rows, cols, tok):
     (G, g_type, g), (U, _, u) = weights(rows, cols, rows + tok), weights(rows, cols, rows + tok + 1)
@@ -200,13 +209,38 @@ def test_gate_and_up(rows, cols, tok):
         a, x = as_type(activations(tok, cols, cols + tok) * 0.5, x_type)
         xq = f.values_of(f.quantized(f.padded(x)))
         got = multiply(ops, x_type, upload_rows(a, cols + pad), y_type, rows, cols, tok, pad, cols + pad)
-        a, b = xq @ g.T, xq @ u.T
-        ea, eb = f.product_bound(xq, g), f.product_bound(xq, u)
-        want = f.silu_mul(a, b)
-        # the slope of silu is at most 1.1; expf, the sum, the quotient and the product take at most 8 half steps; a quotient below fp32's
-        # normal numbers may be lost
-        bound = 1.1 * ea * (np.abs(b) + eb) + np.abs(f.silu_mul(a, 1.0)) * eb + 8 * 2.0 ** -24 * np.abs(want) + 2.0 ** -126 * (1 + np.abs(b))
+        want, bound = gated(xq, g, u)
         check(got, want, bound, y_type)
+
+
+KERNELS = [0, 11, 21, 41, 22, 24, 42, 44]
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("rows,cols,tok", [(1, 1, 1), (100, 128, 70), (130, 384, 33), (65, 640, 130), (300, 1000, 129), (513, 1056, 255), (257, 2080, 257), (640, 512, 300)])
+def test_every_kernel(kernel, rows, cols, tok):
+    """each kernel on small shapes, whatever the choice between them: rows, tokens and columns inside a tile, over several, one to
+    five column tiles past a whole quad"""
+    (G, g_type, g), (U, _, u) = weights(rows, cols, rows), weights(rows, cols, rows + 1)
+    ops = [operand(g_type, W, rows, cols)[0] for W in (G, U)]
+    a, x = as_type(activations(tok, cols, cols), F32)
+    xq = f.values_of(f.quantized(f.padded(x)))
+    x_op, _ = operand(F32, a, tok, cols)
+    for up in (None,) if kernel == 11 else (None, ops[1]):
+        for y_type, size, pad in ((F32, 4, 3), (BF16, 2, 0)):
+            ldy = rows + pad
+            out = filled(tok * ldy * size + 64)
+            qlinear.check(qlinear.load().qlin_probe_mxfp4_gemm(kernel, ops[0].ptr, up.ptr if up else None, x_op.ptr, y_type, out.ptr, rows, cols, tok, ldy, None))
+            qlinear.sync()
+            raw = out.to_numpy(np.uint8, (out.nbytes,))
+            body = raw[:-64].reshape(tok, ldy * size)
+            assert (raw[-64:] == FILL).all() and (body[:, rows * size:] == FILL).all()
+            y = np.ascontiguousarray(body[:, :rows * size])
+            got = y.view(np.float32).astype(np.float64) if y_type == F32 else synth.bf16_bits_to_f32(y.view(np.uint16)).astype(np.float64)
+            want, bound = xq @ g.T, f.product_bound(xq, g)
+            if up:
+                want, bound = gated(xq, g, u)
+            check(got, want, bound, y_type)
 
 
 @pytest.mark.parametrize("tok", [1, 5, 40, 100, 300])
