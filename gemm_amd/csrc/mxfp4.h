@@ -68,18 +68,23 @@ hipError_t launch_mxfp4_operand(uint32_t type, const void *X, void *op, int n_ro
 /* float rows to GGML blocks, n_cols a multiple of 32 */
 hipError_t launch_mxfp4_blocks(uint32_t type, const void *X, void *W, int n_rows, int n_cols, int ldx, hipStream_t stream);
 
-/* Y[t * ldy + r] = sum over k of X[t][k] W[r][k] of two operands, or with `up` silu(X . W) * (X . up); Y F32 or BF16 */
+/* Y[t * ldy + r] = sum over k of X[t][k] W[r][k], or with `up` silu(X . W) * (X . up); W and up operands, X an operand (x_type MXFP4) or
+ * floats where mxfp4_quantises_in_product; Y F32 or BF16 */
 struct Mxfp4Product {
-    const uint8_t *W, *up, *X;
+    const uint8_t *W, *up;
+    uint32_t x_type;
+    const void *X;
     void *Y;
-    int n_rows, n_cols, n_tok, ldy;
+    int n_rows, n_cols, n_tok, ldx, ldy;
     bool bf16_out;
     hipStream_t stream;
 };
+bool mxfp4_quantises_in_product(const Mxfp4Product &p);
 hipError_t launch_mxfp4_few(const Mxfp4Product &p);
-/* in tiles of 64 mb rows (32 mb of each of two tensors) x 64 nb tokens; mb and nb of 1, 2 and 4 (mxfp4_tile.hip says which) */
+/* in tiles of 64 mb rows (32 mb of each of two tensors) x 64 nb tokens; (mb, nb) = (4, 4), (2, 2), (2, 1), (1, 1) */
 hipError_t launch_mxfp4_tiles(int mb, int nb, const Mxfp4Product &p);
-/* whichever suits the sizes */
+/* the kernel for a product: 0 = launch_mxfp4_few, 10 mb + nb = tiles */
+int mxfp4_choice(const Mxfp4Product &p, int n_cu);
 hipError_t launch_mxfp4_product(const Mxfp4Product &p, int n_cu);
 
 }  // namespace qlin

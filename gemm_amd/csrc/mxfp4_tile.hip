@@ -13,6 +13,9 @@
  * one lane.
  */
 #include "mxfp4.h"
+
+#include <cmath>
+
 #include "gemm_kq_formats.h"
 
 namespace qlin {
@@ -122,15 +125,22 @@ template <class C> QLIN_INL void take_exponents(C &c) {
     }
 }
 
+template <bool STREAM> QLIN_INL void put(float *to, float v) {
+    if constexpr (STREAM) __builtin_nontemporal_store(v, to);
+    else *to = v;
+}
 /* Two results of this lane's row, of tokens t and t + 1, of which those below `tokens` are there; to = the row's place in token t. 32 lanes
  * hold 32 consecutive rows: a store instruction writes two runs of 128 bytes of F32, or after an exchange between neighbouring lanes
- * four of 64 bytes of BF16. */
-QLIN_INL void put2(float *to, size_t ldy, float a, float b, int tokens, int rows_left) {
+ * four of 64 bytes of BF16. STREAM marks them as not read again soon: what would wait in the L2 for the end of the kernel goes to
+ * memory beside the next tiles' products (14336 x 4096, 1024 tokens in 128 x 128 tiles 45.6 -> 36.8 us, 4096 tokens in 256 x 256 141 -> 137),
+ * but only where rows lie on 64 bytes, so that a run is whole sectors: else they are written twice (23207 rows x 576, 1073 tokens 28 -> 58,
+ * rows on 32 bytes 26 -> 45). */
+template <bool STREAM> QLIN_INL void put2(float *to, size_t ldy, float a, float b, int tokens, int rows_left) {
     if (rows_left <= 0) return;
-    if (tokens > 0) to[0] = a;
-    if (tokens > 1) to[ldy] = b;
+    if (tokens > 0) put<STREAM>(to, a);
+    if (tokens > 1) put<STREAM>(to + ldy, b);
 }
-QLIN_INL void put2(__bf16 *to, size_t ldy, float a, float b, int tokens, int rows_left) {
+template <bool STREAM> QLIN_INL void put2(__bf16 *to, size_t ldy, float a, float b, int tokens, int rows_left) {
     typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
     typedef bf16x2 anywhere __attribute__((aligned(2)));
     const bool odd = threadIdx.x & 1; /* even lanes store token t of both rows, odd ones token t + 1 */
@@ -139,8 +149,10 @@ QLIN_INL void put2(__bf16 *to, size_t ldy, float a, float b, int tokens, int row
     to += odd ? (ptrdiff_t)ldy - 1 : 0;
     rows_left += odd;
     if (tokens <= (int)odd) return;
-    if (rows_left > 1) *reinterpret_cast<anywhere *>(to) = v;
-    else if (rows_left == 1) to[0] = v[0];
+    if (rows_left > 1) {
+        if constexpr (STREAM) __builtin_nontemporal_store(v, reinterpret_cast<anywhere *>(to));
+        else *reinterpret_cast<anywhere *>(to) = v;
+    } else if (rows_left == 1) to[0] = v[0];
 }
 
 /* the bytes of an operand from row group `from` of a part with `pitch` bytes per group, as a buffer descriptor counts them */
@@ -152,11 +164,16 @@ QLIN_INL uint32_t bytes_from(int groups, int from, uint32_t pitch) {
 template <int MB, int NB, bool PAIR, class OUT>
 __global__ void __launch_bounds__(256, MB + NB > 4 ? 1 : 2)
 tile_kernel(const uint8_t *__restrict__ W, const uint8_t *__restrict__ up, const uint8_t *__restrict__ X, OUT *__restrict__ Y, int n_rows, int n_tok, Shape w,
-            Shape x, size_t ldy, int row_tiles, int tok_tiles) {
-    /* consecutive workgroups go to different dies, each with an L2 of its own; the token tiles that share a row tile meet in one */
-    const int die = blockIdx.x & 7, at = blockIdx.x >> 3;
-    const int tok_tile = at % tok_tiles, row_tile = (at / tok_tiles) * 8 + die;
-    if (row_tile >= row_tiles) return;
+            Shape x, size_t ldy, int row_tiles, int tok_tiles, bool stream) {
+    /* Consecutive workgroups go to different dies, each with an L2 of its own: a die takes a run of the tiles, numbered through groups of
+     * kGroup row tiles, in a group the row tiles of a token tile first, so that what runs at a time on a die shares its rows and tokens. */
+    constexpr int kGroup = 8;
+    const unsigned n_tiles = (unsigned)row_tiles * (unsigned)tok_tiles, per_die = gridDim.x >> 3;
+    const unsigned id = (blockIdx.x & 7) * per_die + (blockIdx.x >> 3);
+    if (id >= n_tiles) return;
+    const unsigned of_group = (unsigned)kGroup * tok_tiles, first = id / of_group * kGroup, rest = id % of_group;
+    const unsigned height = min((unsigned)row_tiles - first, (unsigned)kGroup);
+    const int tok_tile = rest / height, row_tile = first + rest % height;
     constexpr int kRowGroups = PAIR ? 2 * MB : 4 * MB; /* row groups of a tensor per tile */
     const int lane = threadIdx.x & 63;
     Ctx<MB, NB, PAIR> c;
@@ -235,27 +252,32 @@ tile_kernel(const uint8_t *__restrict__ W, const uint8_t *__restrict__ up, const
     /* register v of lane l: token 8 (v / 4) + 4 (l / 32) + v % 4, row l % 32 */
     constexpr int kOut = PAIR ? MB / 2 : MB;
     const int t0 = (tok_tile * 2 + wn) * 32 * NB + 4 * (lane >> 5), r0 = (row_tile * 2 + wm) * 32 * kOut + (lane & 31);
+    auto store = [&](auto streams) {
 #pragma unroll
-    for (int n = 0; n < NB; n++)
+        for (int n = 0; n < NB; n++)
 #pragma unroll
-        for (int v = 0; v < 16; v += 2) {
-            const int t = t0 + 32 * n + 8 * (v / 4) + v % 4;
-            OUT *y = Y + (size_t)t * ldy + r0;
+            for (int v = 0; v < 16; v += 2) {
+                const int t = t0 + 32 * n + 8 * (v / 4) + v % 4;
+                OUT *y = Y + (size_t)t * ldy + r0;
 #pragma unroll
-            for (int m = 0; m < kOut; m++) {
-                float a = c.acc[m][n][v], b = c.acc[m][n][v + 1];
-                if constexpr (PAIR) a = silu_mul(a, c.acc[m + MB / 2][n][v]), b = silu_mul(b, c.acc[m + MB / 2][n][v + 1]);
-                put2(y + 32 * m, ldy, a, b, n_tok - t, n_rows - r0 - 32 * m);
+                for (int m = 0; m < kOut; m++) {
+                    float a = c.acc[m][n][v], b = c.acc[m][n][v + 1];
+                    if constexpr (PAIR) a = silu_mul(a, c.acc[m + MB / 2][n][v]), b = silu_mul(b, c.acc[m + MB / 2][n][v + 1]);
+                    put2<decltype(streams)::value>(y + 32 * m, ldy, a, b, n_tok - t, n_rows - r0 - 32 * m);
+                }
             }
-        }
+    };
+    if (stream) store(std::true_type{});
+    else store(std::false_type{});
 }
 
 template <int MB, int NB, bool PAIR, class OUT> hipError_t tiles(const Mxfp4Product &p) {
     const Shape w = shape_of(p.n_rows, p.n_cols), x = shape_of(p.n_tok, p.n_cols);
     constexpr int kRows = (PAIR ? 32 : 64) * MB, kTok = 64 * NB;
     const int row_tiles = (p.n_rows + kRows - 1) / kRows, tok_tiles = (p.n_tok + kTok - 1) / kTok;
-    const dim3 grid((unsigned)((row_tiles + 7) / 8 * 8) * (unsigned)tok_tiles);
-    tile_kernel<MB, NB, PAIR, OUT><<<grid, 256, 0, p.stream>>>(p.W, p.up, p.X, static_cast<OUT *>(p.Y), p.n_rows, p.n_tok, w, x, (size_t)p.ldy, row_tiles, tok_tiles);
+    const dim3 grid(((unsigned)row_tiles * (unsigned)tok_tiles + 7) / 8 * 8);
+    const bool stream = (reinterpret_cast<uintptr_t>(p.Y) & 63) == 0 && (size_t)p.ldy * sizeof(OUT) % 64 == 0;
+    tile_kernel<MB, NB, PAIR, OUT><<<grid, 256, 0, p.stream>>>(p.W, p.up, static_cast<const uint8_t *>(p.X), static_cast<OUT *>(p.Y), p.n_rows, p.n_tok, w, x, (size_t)p.ldy, row_tiles, tok_tiles, stream);
     return hipGetLastError();
 }
 template <int MB, int NB> hipError_t tiles_for(const Mxfp4Product &p) {
@@ -271,14 +293,62 @@ template <int MB, int NB> hipError_t tiles_for(const Mxfp4Product &p) {
 hipError_t launch_mxfp4_tiles(int mb, int nb, const Mxfp4Product &p) {
     switch (10 * mb + nb) {
     case 44: return tiles_for<4, 4>(p);
-    case 42: return tiles_for<4, 2>(p);
-    case 24: return tiles_for<2, 4>(p);
     case 22: return tiles_for<2, 2>(p);
-    case 41: return tiles_for<4, 1>(p);
     case 21: return tiles_for<2, 1>(p);
     case 11: return tiles_for<1, 1>(p);
     default: return hipErrorInvalidValue;
     }
+}
+
+namespace {
+
+/* What a product takes, us: `start`, then the longest of the rounds that the tiles make of the chip (`resident` workgroups per compute
+ * unit), one at a time (`wait` per column tile: the chain of requests, barriers and matrix instructions of a workgroup that has the unit to
+ * itself, `rest` per tile) or side by side (`work`: what they take of the unit from each other); the weights from memory; and the
+ * results to it, per MB. Fitted to 229 measured products of 17 to 4096 tokens, 256 to 28672 rows and 256 to 14336 columns, which
+ * the smallest estimate's kernel takes 1.6 % longer than the fastest in the mean and 28 % at most (23551 rows x 6912, 169 tokens: 39 us against
+ * 30 of a 128 x 256 tile, which was built with two more shapes and left out: together they gain 0.1 %). */
+struct TileCost { int mb, nb, resident; float start, wait, work, rest, result, weights; };
+constexpr TileCost kTileCosts[] = {{1, 1, 4, 2.888f, 0.123f, 0.097f, 0.552f, 0.108f, 0.163f},
+                                   {2, 1, 3, 3.019f, 0.105f, 0.149f, 1.114f, 0.114f, 0.167f},
+                                   {2, 2, 2, 2.368f, 0.167f, 0.202f, 2.146f, 0.155f, 0.220f},
+                                   {4, 4, 1, 0.378f, 0.493f, 0.003f, 8.793f, 0.154f, 0.326f}};
+float rounds(double n, int at_a_time) { return (float)ceil(n / at_a_time); }
+float tile_us(const TileCost &c, const Mxfp4Product &p, int n_cu) {
+    const Shape w = shape_of(p.n_rows, p.n_cols);
+    const int rows = (p.up ? 32 : 64) * c.mb, tok = 64 * c.nb;
+    const double n = ceil((double)p.n_rows / rows) * ceil((double)p.n_tok / tok);
+    const float alone = rounds(n, n_cu * c.resident) * (c.wait * w.tiles + c.rest), together = rounds(n, n_cu) * (c.work * w.tiles + c.rest / c.resident);
+    const double mb_in = (double)w.bytes() * (p.up ? 2 : 1) * 1e-6, mb_out = (double)p.n_rows * p.n_tok * (p.bf16_out ? 2 : 4) * 1e-6;
+    return c.start + fmaxf(fmaxf(alone, together), c.weights * (float)mb_in) + c.result * (float)mb_out;
+}
+/* the kernel of 16 rows per workgroup: what its workgroups read, or the weights from memory, or the 32-column-tile pieces of a wave in turn */
+float few_us(const Mxfp4Product &p) {
+    const Shape w = shape_of(p.n_rows, p.n_cols), x = shape_of(p.n_tok, p.n_cols);
+    const int mats = p.up ? 2 : 1, nt = x.groups < 4 ? x.groups : 4;
+    const double kb = (double)w.groups * ((x.groups + nt - 1) / nt) * w.tiles;
+    const double mb_in = (double)w.bytes() * mats * 1e-6, mb_out = (double)p.n_rows * p.n_tok * (p.bf16_out ? 2 : 4) * 1e-6;
+    return 3.2253f + fmaxf(fmaxf((float)(kb * 1e-3 * (0.0189 * mats + 0.0894 * nt)), 0.1766f * (float)mb_in), 1.2065f * ((w.tiles + 31) / 32)) + 0.7458f * (float)mb_out;
+}
+
+}  // namespace
+
+int mxfp4_choice(const Mxfp4Product &p, int n_cu) {
+    /* up to 16 tokens, one token group: never more than 5 % behind the tiles, and without a launch to quantise for the fewest */
+    if (p.n_tok <= 16) return 0;
+    int best = 0;
+    float least = few_us(p);
+    for (const TileCost &c : kTileCosts) {
+        if (p.up && c.mb == 1) continue; /* no row block for the second tensor */
+        const float t = tile_us(c, p, n_cu);
+        if (t < least) least = t, best = 10 * c.mb + c.nb;
+    }
+    return best;
+}
+
+hipError_t launch_mxfp4_product(const Mxfp4Product &p, int n_cu) {
+    const int k = mxfp4_choice(p, n_cu);
+    return k == 0 ? launch_mxfp4_few(p) : launch_mxfp4_tiles(k / 10, k % 10, p);
 }
 
 }  // namespace qlin

@@ -1508,9 +1508,12 @@ static int mxfp4_gemm(const void *W, const void *up, bool pair, uint32_t x_type,
     if (x_type != T_MXFP4 && (!workspace || !aligned(workspace, 16) || workspace_bytes < qlin_mxfp4_gemm_workspace_bytes(n_cols, n_tok)))
         return fail(QLIN_ERR_ARG, "the workspace needs %zu bytes, 16-byte aligned", qlin_mxfp4_gemm_workspace_bytes(n_cols, n_tok));
     if (int rc = init_once()) return rc;
-    if (x_type != T_MXFP4) HIP_TRY(launch_mxfp4_operand(x_type, X, workspace, n_tok, n_cols, ldx, (hipStream_t)stream));
-    const Mxfp4Product p = {static_cast<const uint8_t *>(W), static_cast<const uint8_t *>(up), static_cast<const uint8_t *>(x_type == T_MXFP4 ? X : workspace), Y,
-                            n_rows, n_cols, n_tok, ldy, y_type == T_BF16, (hipStream_t)stream};
+    Mxfp4Product p = {static_cast<const uint8_t *>(W), static_cast<const uint8_t *>(up), x_type, X, Y, n_rows, n_cols, n_tok, ldx, ldy, y_type == T_BF16, (hipStream_t)stream};
+    if (x_type != T_MXFP4 && !mxfp4_quantises_in_product(p)) {
+        HIP_TRY(launch_mxfp4_operand(x_type, X, workspace, n_tok, n_cols, ldx, (hipStream_t)stream));
+        p.x_type = T_MXFP4;
+        p.X = workspace;
+    }
     HIP_TRY(launch_mxfp4_product(p, g.n_cu));
     return QLIN_OK;
 }
@@ -1631,10 +1634,19 @@ int qlin_probe_mxfp4_gemm(int kernel, const void *W, const void *up, const void 
     if (kernel < 0 || n_rows <= 0 || n_cols <= 0 || n_tok <= 0 || ldy < n_rows || !operand_fits(n_rows, n_cols) || !operand_fits(n_tok, n_cols)) return fail(QLIN_ERR_ARG, "bad kernel or size");
     if (!W || !X || !Y || !aligned(W, 16) || !aligned(up, 16) || !aligned(X, 16) || !aligned(Y, float_bytes(y_type))) return fail(QLIN_ERR_ARG, "null or misaligned pointer");
     if (int rc = init_once()) return rc;
-    const Mxfp4Product p = {static_cast<const uint8_t *>(W), static_cast<const uint8_t *>(up), static_cast<const uint8_t *>(X), Y, n_rows, n_cols, n_tok, ldy, y_type == T_BF16, (hipStream_t)stream};
+    const Mxfp4Product p = {static_cast<const uint8_t *>(W), static_cast<const uint8_t *>(up), T_MXFP4, X, Y, n_rows, n_cols, n_tok, n_cols, ldy, y_type == T_BF16, (hipStream_t)stream};
     if (kernel == 0) HIP_TRY(launch_mxfp4_few(p));
     else HIP_TRY(launch_mxfp4_tiles(kernel / 10, kernel % 10, p));
     return QLIN_OK;
+}
+
+int qlin_probe_mxfp4_kernel(int pair, uint32_t y_type, int n_rows, int n_cols, int n_tok) {
+    if ((y_type != T_F32 && y_type != T_BF16) || n_rows <= 0 || n_cols <= 0 || n_tok <= 0 || !operand_fits(n_rows, n_cols) || !operand_fits(n_tok, n_cols)) return fail(QLIN_ERR_ARG, "bad type or size");
+    Mxfp4Product p = {};
+    static const uint8_t some = 0;
+    p.up = pair ? &some : nullptr;
+    p.n_rows = n_rows, p.n_cols = n_cols, p.n_tok = n_tok, p.bf16_out = y_type == T_BF16;
+    return mxfp4_choice(p, g.n_cu);
 }
 
 int qlin_probe_hbm_read(const void *buf, size_t n_bytes, void *stream) {

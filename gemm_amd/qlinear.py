@@ -136,6 +136,7 @@ SIGNATURES = {
     "qlin_probe_gemm_f32_route": (C.c_int, [C.c_uint32, C.c_int, C.c_int, C.c_int]),
     "qlin_probe_gemm_tile": (C.c_int, [C.c_int, C.c_uint32, _vp, _vp, _vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, _vp]),
     "qlin_probe_mxfp4_gemm": (C.c_int, [C.c_int, _vp, _vp, _vp, C.c_uint32, _vp, C.c_int, C.c_int, C.c_int, C.c_int, _vp]),
+    "qlin_probe_mxfp4_kernel": (C.c_int, [C.c_int, C.c_uint32, C.c_int, C.c_int, C.c_int]),
     "qlin_timer_begin": (C.c_int, [_vp]),
     "qlin_timer_end": (C.c_int, [_vp, _fp]),
 }

@@ -31,10 +31,12 @@ int qlin_probe_hbm_read(const void *buf, size_t n_bytes, void *stream);
 int qlin_probe_gemm_tile(int tile, uint32_t ggml_type, const void *W, const uint16_t *X, float *Y, int n_rows, int n_cols,
                          int n_tok, int ldx, int ldy, void *stream);
 /* One kernel of the 4-bit products by name, whatever the choice of qlin_mxfp4_gemm_dev would be: 0 = 16 rows per workgroup, its waves
- * along K; 10 a + b = tiles of 64 a rows x 64 b tokens (44, 42, 24, 22, 41, 21, 11; not 11 with `up`). W, up (NULL: one tensor) and X are
+ * along K; 10 a + b = tiles of 64 a rows x 64 b tokens (44, 22, 21, 11; not 11 with `up`). W, up (NULL: one tensor) and X are
  * operands. */
 int qlin_probe_mxfp4_gemm(int kernel, const void *W, const void *up, const void *X, uint32_t y_type, void *Y, int n_rows, int n_cols, int n_tok,
                           int ldy, void *stream);
+/* the kernel, numbered so, that qlin_mxfp4_gemm_dev (pair: qlin_mxfp4_gemm_silu_mul_dev) takes for a size */
+int qlin_probe_mxfp4_kernel(int pair, uint32_t y_type, int n_rows, int n_cols, int n_tok);
 /* what qlin_gemm_bf16_any_dev does with a shape: 1 and 2 = a tile kernel, of the class of 256 x 128 or of 128 x 64 tiles (tensors of
  * one class share a launch; which tiles it takes says qlin_probe_gemm_blocks), 3 = the few-token kernel, 0 = none of them (a matvec
  * per token, or decode to bf16 + dense product) */
