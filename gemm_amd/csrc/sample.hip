@@ -88,6 +88,7 @@ struct Sum { uint32_t count; uint64_t weight; };
 __device__ __forceinline__ Sum operator+(Sum a, Sum b) { return {a.count + b.count, a.weight + b.weight}; }
 
 constexpr int kBins = 2048, kListed = 2048, kTopList = 1024; /* bins; tokens of a list; top_k up to which a list holds all kept */
+constexpr int kFewOfThreads = 512; /* top_k up to which the threads' largest logits bound it */
 
 struct Shared {
     union {
@@ -317,6 +318,9 @@ struct Grid {
         /* the integer nearest to e * unit is what the sum with 2^52 holds below the exponent */
         return (uint64_t)__double_as_longlong(fma(e, unit, 4503599627370496.0)) & 0x000FFFFFFFFFFFFFull;
     }
+    /* floats below (above) every value of place `at` and less (and more) */
+    __device__ float value_below(int at) const { return __double2float_rd((double)max - (double)at / scale * (1.0 + 1e-9)); }
+    __device__ float value_above(int at) const { return __double2float_ru((double)max - (double)at / scale * (1.0 - 1e-9)); }
     __device__ double weight(float v) const { return v == max ? 1.0 : max == -kMinusInf ? 0.0 : exp(((double)v - (double)max) * per_t); }
 };
 constexpr int kLastBin = kBins - 2;
@@ -380,16 +384,24 @@ __device__ void sum_bins(const Grid &g, const Settings &set, Shared &s) {
     __syncthreads();
 }
 
-/* first bin whose running sum fulfils `reached`, kLastBin + 1 if none does */
-template <class F> __device__ int first_bin(F reached) {
-    int lo = 0, hi = kLastBin + 1;
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (reached(mid)) hi = mid;
-        else lo = mid + 1;
+/* The first bin of which `one` holds, and the first of which `other` holds (running sums: once true, true to the end); kLastBin + 1 if there
+ * is none. All threads of the workgroup call it. */
+struct Pair { int one, other; };
+template <class F, class G> __device__ Pair first_bins(Shared &s, F one, G other) {
+    if (threadIdx.x < 2) s.found[threadIdx.x] = kLastBin + 1;
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+        const int b = 2 * threadIdx.x + e;
+        if (b <= kLastBin && one(b) && (b == 0 || !one(b - 1))) s.found[0] = b;
+        if (b <= kLastBin && other(b) && (b == 0 || !other(b - 1))) s.found[1] = b;
     }
-    return lo;
+    __syncthreads();
+    const Pair r = {(int)s.found[0], (int)s.found[1]};
+    __syncthreads();
+    return r;
 }
+template <class F> __device__ int first_bin(Shared &s, F one) { return first_bins(s, one, [](int) { return false; }).one; }
 
 /* the bins to list, as up to four runs in order, and which of them hold which cut */
 struct Run { int lo, hi; };
@@ -417,42 +429,42 @@ __device__ void add_run(Wanted &w, Run r) {
         w.n--;
     }
 }
-__device__ Wanted wanted_bins(const Grid &g, const Settings &set, const Shared &s) {
+__device__ Wanted wanted_bins(const Grid &g, const Settings &set, Shared &s) {
     constexpr double kSlack = 1e-11; /* of the sums' rounding */
     const Run none = {0, -1};
     Wanted w = {none, none, none, none, {none, none, none, none}, 0, !needs_weights(set)};
     if (w.all) {
-        w.run[0] = {0, min(first_bin([&](int b) { return s.count[b] >= (uint32_t)set.k; }), kLastBin)};
+        w.run[0] = {0, min(first_bin(s, [&](int b) { return s.count[b] >= (uint32_t)set.k; }), kLastBin)};
         w.n = 1;
         return w;
     }
     auto before = [&](int b) { return b > 0 ? s.upto[b - 1] : 0.0; };
-    double lo = s.upto[kLastBin], hi = lo; /* between which the sum of the kept lies */
+    const double everything = s.upto[kLastBin];
+    double lo = everything, hi = lo; /* between which the sum of the kept lies */
     if (set.k > 0) {
-        const int b = first_bin([&](int i) { return s.count[i] >= (uint32_t)set.k; });
+        const int b = first_bin(s, [&](int i) { return s.count[i] >= (uint32_t)set.k; });
         if (b <= kLastBin) w.k = {b, b}, lo = before(b), hi = s.upto[b];
     }
     if (set.p < 1.0f) {
-        const double p = fmax((double)set.p, 0.0);
-        w.p.lo = min(first_bin([&](int i) { return s.upto[i] >= p * lo * (1.0 - kSlack); }), kLastBin);
-        w.p.hi = min(first_bin([&](int i) { return s.upto[i] >= p * hi * (1.0 + kSlack); }), kLastBin);
+        const double p = fmax((double)set.p, 0.0), at_least = p * lo * (1.0 - kSlack), at_most = p * hi * (1.0 + kSlack);
+        const Pair f = first_bins(s, [&](int i) { return s.upto[i] >= at_least; }, [&](int i) { return s.upto[i] >= at_most; });
+        w.p = {min(f.one, kLastBin), min(f.other, kLastBin)};
         lo = fmin(lo, before(w.p.lo));
         hi = fmin(hi, s.upto[w.p.hi]);
     }
     if (set.m > 0.0f) {
         const double at = -log((double)set.m) / g.step;
         if (at < kBins) {
-            w.m = {max((int)at - 1, 0), min((int)at + 1, kLastBin)};
+            w.m = {min(max((int)at - 1, 0), kLastBin), min((int)at + 1, kLastBin)};
             lo = fmin(lo, before(w.m.lo));
             hi = fmin(hi, s.upto[w.m.hi]);
         }
     }
-    const double u = fmin((double)set.u, 1.0);
-    w.u.lo = min(first_bin([&](int i) { return s.upto[i] > u * lo * (1.0 - kSlack); }), kLastBin);
-    w.u.hi = min(first_bin([&](int i) { return s.upto[i] > u * hi * (1.0 + kSlack); }), kLastBin);
-    if (w.u.hi == kLastBin && u * hi * (1.0 + kSlack) >= s.upto[kLastBin]) /* the last bin that weighs anything */
-        w.u.hi = min(first_bin([&](int i) { return s.upto[i] >= s.upto[kLastBin] * (1.0 - kSlack); }), kLastBin);
-    w.u.hi = max(w.u.hi, w.u.lo);
+    /* (beyond the sum of all, for a random number of 1, the last bin that weighs anything) */
+    const double u = fmin((double)set.u, 1.0), at_least = fmin(u * lo * (1.0 - kSlack), everything * (1.0 - kSlack));
+    const double at_most = fmin(u * hi * (1.0 + kSlack), everything * (1.0 - kSlack));
+    const Pair f = first_bins(s, [&](int i) { return s.upto[i] > at_least; }, [&](int i) { return s.upto[i] > at_most; });
+    w.u = {min(f.one, kLastBin), min(max(f.one, f.other), kLastBin)};
     add_run(w, w.k);
     add_run(w, w.p);
     add_run(w, w.m);
@@ -464,11 +476,16 @@ __device__ Wanted wanted_bins(const Grid &g, const Settings &set, const Shared &
 __device__ __forceinline__ uint64_t entry_of(float v, int i) { return (uint64_t)(~key_of(v)) << 32 | (uint32_t)i; }
 __device__ __forceinline__ float entry_value(uint64_t e) { return value_of(~(uint32_t)(e >> 32)); }
 
-/* fn(entry) for the tokens of the wanted bins */
+/* fn(entry) for the tokens of the wanted bins: most fail a comparison of floats with bounds a little wider than all of them */
 template <class T, class F> __device__ __forceinline__ void for_each_wanted(const T *x, int lo, int hi, const Grid &g, const Wanted &w, F fn) {
+    int last = w.run[0].hi;
+#pragma unroll
+    for (int r = 1; r < 4; r++) last = max(last, w.run[r].hi);
+    const float low = g.value_below(last + 1), high = w.run[0].lo == 0 ? g.max : g.value_above(w.run[0].lo);
     for_each(x, lo, hi, [&](float v, int i) {
+        if (!(v >= low && v <= high && is_there(v))) return;
         const double at = g.place(v);
-        if (!is_there(v) || !(at < kBins - 1)) return;
+        if (!(at < kBins - 1)) return;
         const int b = (int)at;
         bool in = false;
 #pragma unroll
@@ -626,6 +643,10 @@ __device__ __forceinline__ void nothing_there(int32_t *id, float *prob) {
     }
 }
 
+__device__ __forceinline__ void clear_bins(Shared &s) {
+    for (int i = threadIdx.x; i < kBins; i += kThreads) s.weight[i] = 0, s.count[i] = 0;
+}
+
 /* one workgroup per sequence */
 template <class T> __global__ void __launch_bounds__(kThreads) sample_row_kernel(const T *__restrict__ logits, SampleCall c) {
     __shared__ Shared s;
@@ -634,14 +655,16 @@ template <class T> __global__ void __launch_bounds__(kThreads) sample_row_kernel
     int32_t *id = c.ids + seq;
     float *prob = c.probs ? c.probs + seq : nullptr;
     const Settings set = settings_of(c, seq);
-    const Range r = range_of_workgroup(range_of_share(x, 0, n), s);
+    const Range mine = range_of_share(x, 0, n), r = range_of_workgroup(mine, s);
     if (!is_there(r.max)) return nothing_there(id, prob);
     if (threadIdx.x == 0) s.best = (uint32_t)n, s.n_list = 0;
+    clear_bins(s);
+    __syncthreads();
     if (takes_first(set)) {
-        __syncthreads();
-        for_each(x, 0, n, [&](float v, int i) {
-            if (v == r.max) atomicMin(&s.best, (uint32_t)i);
-        });
+        if (mine.max == r.max) /* few threads have it */
+            for_each(x, 0, n, [&](float v, int i) {
+                if (v == r.max) atomicMin(&s.best, (uint32_t)i);
+            });
         __syncthreads();
         if (threadIdx.x == 0) {
             *id = (int32_t)s.best;
@@ -650,11 +673,26 @@ template <class T> __global__ void __launch_bounds__(kThreads) sample_row_kernel
         return;
     }
     const Grid g(r, set.t, n);
-    for (int i = threadIdx.x; i < kBins; i += kThreads) s.weight[i] = 0, s.count[i] = 0;
-    __syncthreads();
-    fill_bins(x, 0, n, g, set, s);
-    __syncthreads();
-    sum_bins(g, set, s);
+    /* The k-th largest of the threads' own largest logits is not above the k-th of all. For a k that is small beside the threads it is close
+     * below (of 128256 logits and k = 512 some 700 are as large), and the pass that counts all tokens into bins is saved. */
+    bool counted = false;
+    if (set.k > 0 && set.k <= kFewOfThreads) {
+        if (is_there(mine.max)) {
+            const double at = g.place(mine.max);
+            if (at < kBins - 1) atomicAdd(&s.count[(int)at], 1u);
+        }
+        __syncthreads();
+        sum_bins(g, set, s);
+        counted = s.count[kLastBin] >= (uint32_t)set.k;
+        __syncthreads();
+        if (!counted) clear_bins(s);
+        __syncthreads();
+    }
+    if (!counted) {
+        fill_bins(x, 0, n, g, set, s);
+        __syncthreads();
+        sum_bins(g, set, s);
+    }
     const Wanted w = wanted_bins(g, set, s);
     for_each_wanted(x, 0, n, g, w, [&](uint64_t e) {
         const uint32_t at = atomicAdd(&s.n_list, 1u);
@@ -667,17 +705,209 @@ template <class T> __global__ void __launch_bounds__(kThreads) sample_row_kernel
     pick_from_list((int)listed, g, set, w, id, prob, s);
 }
 
+/* ------------------------------------------------------------------ few sequences: several workgroups for each, three launches */
+
+/* What a sequence keeps in the workspace. A part of the row is a workgroup's; candidates are its tokens that top_k of up to kFewOfParts
+ * can keep. */
+struct Part { float max, min; int first; uint32_t n; };
+struct Row {
+    uint64_t weight[kBins];
+    uint64_t list[kListed];
+    uint32_t count[kBins];
+    uint32_t n_list, done, unused[62];
+};
+constexpr int kCandidates = 256, kFewOfParts = 128;
+__host__ __device__ constexpr size_t row_bytes(int parts) { return sizeof(Row) + (size_t)parts * (sizeof(Part) + kCandidates * sizeof(uint64_t)); }
+static_assert(sizeof(Row) % 256 == 0 && sizeof(Part) == 16, "alignment of what follows");
+__device__ __forceinline__ Row *row_of(const SampleCall &c, int seq, int parts) { return reinterpret_cast<Row *>(static_cast<uint8_t *>(c.workspace) + (size_t)seq * row_bytes(parts)); }
+__device__ __forceinline__ Part *parts_of(Row *r) { return reinterpret_cast<Part *>(r + 1); }
+__device__ __forceinline__ uint64_t *candidates_of(Row *r, int parts) { return reinterpret_cast<uint64_t *>(parts_of(r) + parts); }
+__device__ __forceinline__ bool by_candidates(const Settings &s) { return s.k > 1 && s.k <= kFewOfParts; }
+struct Share { int lo, hi; };
+__device__ __forceinline__ Share share_of(int n, int parts, int part) {
+    const int per = ((n + parts - 1) / parts + 63) & ~63; /* (rows on 16 bytes stay so) */
+    return {min(part * per, n), min((part + 1) * per, n)};
+}
+
+/* the range of each part, its candidates, and empty bins */
+template <class T> __global__ void __launch_bounds__(kThreads) sample_parts_kernel(const T *__restrict__ logits, SampleCall c, int parts) {
+    __shared__ Shared s;
+    const int seq = blockIdx.x / (unsigned)parts, part = blockIdx.x - seq * parts;
+    const T *x = logits + (size_t)seq * c.ld;
+    Row *row = row_of(c, seq, parts);
+    const Settings set = settings_of(c, seq);
+    const Share sh = share_of(c.n_vocab, parts, part);
+    for (int i = part * kThreads + threadIdx.x; i < kBins; i += parts * kThreads) row->weight[i] = 0, row->count[i] = 0;
+    if (part == 0 && threadIdx.x == 0) row->n_list = 0, row->done = 0;
+    if (threadIdx.x == 0) s.best = (uint32_t)c.n_vocab, s.n_list = 0;
+    const Range mine = range_of_share(x, sh.lo, sh.hi), r = range_of_workgroup(mine, s);
+    if (takes_first(set)) {
+        if (is_there(r.max) && mine.max == r.max)
+            for_each(x, sh.lo, sh.hi, [&](float v, int i) {
+                if (v == r.max) atomicMin(&s.best, (uint32_t)i);
+            });
+    } else if (by_candidates(set) && is_there(r.max)) {
+        /* the k-th largest of 256 groups' largest logits (equal ones in any order): the part's first k tokens are not below it. Nor
+         * does anything weigh that the bins would not count. */
+        const float group = fmaxf(fmaxf(mine.max, __shfl_xor(mine.max, 1, 64)), fmaxf(__shfl_xor(mine.max, 2, 64), __shfl_xor(mine.max, 3, 64)));
+        float *groups = reinterpret_cast<float *>(s.count);
+        if ((threadIdx.x & 3) == 0) groups[threadIdx.x >> 2] = group;
+        if (threadIdx.x == 0) s.digit = __float_as_uint(kMinusInf);
+        __syncthreads();
+        { /* four threads count for each group */
+            const int i = threadIdx.x >> 2;
+            const float own = groups[i];
+            int rank = 0;
+            for (int j = threadIdx.x & 3; j < 256; j += 4) rank += groups[j] > own || (groups[j] == own && j < i);
+            rank += __shfl_xor(rank, 1, 64);
+            rank += __shfl_xor(rank, 2, 64);
+            if ((threadIdx.x & 3) == 0 && rank == set.k - 1) s.digit = __float_as_uint(own);
+        }
+        __syncthreads();
+        const double reach = (double)r.max - 32.0 * (double)set.t;
+        const float low = fmaxf(__uint_as_float(s.digit), __double2float_rd(reach));
+        uint64_t *to = candidates_of(row, parts) + (size_t)part * kCandidates;
+        if (mine.max >= low)
+            for_each(x, sh.lo, sh.hi, [&](float v, int i) {
+                if (v >= low && is_there(v)) {
+                    const uint32_t at = atomicAdd(&s.n_list, 1u);
+                    if (at < kCandidates) to[at] = entry_of(v, i);
+                }
+            });
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) parts_of(row)[part] = {r.max, r.min, (int)s.best, s.n_list};
+}
+
+__device__ Range range_of_parts(const Part *p, int parts) {
+    Range r = {kMinusInf, -kMinusInf};
+    for (int i = 0; i < parts; i++) r.max = fmaxf(r.max, p[i].max), r.min = fminf(r.min, p[i].min);
+    return r;
+}
+
+/* the pick where the parts already hold what it takes; else each part's tokens into the bins */
+template <class T> __global__ void __launch_bounds__(kThreads) sample_bins_kernel(const T *__restrict__ logits, SampleCall c, int parts) {
+    __shared__ Shared s;
+    const int seq = blockIdx.x / (unsigned)parts, part = blockIdx.x - seq * parts, n = c.n_vocab;
+    const T *x = logits + (size_t)seq * c.ld;
+    Row *row = row_of(c, seq, parts);
+    const Part *p = parts_of(row);
+    const Settings set = settings_of(c, seq);
+    const Range r = range_of_parts(p, parts);
+    int32_t *id = c.ids + seq;
+    float *prob = c.probs ? c.probs + seq : nullptr;
+    if (!is_there(r.max) || takes_first(set)) {
+        if (part == 0 && threadIdx.x == 0) {
+            int first = n;
+            for (int i = 0; i < parts; i++)
+                if (p[i].max == r.max) first = min(first, p[i].first);
+            *id = is_there(r.max) ? first : -1;
+            if (prob) *prob = is_there(r.max) ? 1.0f : 0.0f;
+        }
+        return;
+    }
+    const Grid g(r, set.t, n);
+    if (by_candidates(set) && part > 0) return;
+    clear_bins(s);
+    if (threadIdx.x == 0) s.n_list = 0;
+    __syncthreads();
+    if (!by_candidates(set)) {
+        const Share sh = share_of(n, parts, part);
+        fill_bins(x, sh.lo, sh.hi, g, set, s);
+        __syncthreads();
+        for (int i = threadIdx.x; i < kBins; i += kThreads) {
+            if (const uint64_t w = s.weight[i]) atomicAdd((unsigned long long *)&row->weight[i], (unsigned long long)w);
+            if (const uint32_t k = s.count[i]) atomicAdd(&row->count[i], k);
+        }
+        return;
+    }
+    const uint64_t *from = candidates_of(row, parts);
+    bool overflow = false;
+    auto each = [&](auto fn) {
+        for (int i = threadIdx.x; i < parts * kCandidates; i += kThreads)
+            if ((uint32_t)(i % kCandidates) < p[i / kCandidates].n) {
+                const uint64_t e = from[i];
+                const double at = g.place(entry_value(e));
+                if (at < kBins - 1) fn(e, (int)at);
+            }
+    };
+    for (int i = 0; i < parts; i++) overflow = overflow || (p[i].n > kCandidates && g.place(p[i].max) < kBins - 1);
+    each([&](uint64_t, int bin) { atomicAdd(&s.count[bin], 1u); });
+    __syncthreads();
+    sum_bins(g, set, s);
+    const Wanted w = wanted_bins(g, set, s);
+    each([&](uint64_t e, int bin) {
+        if (bin > w.run[0].hi) return;
+        const uint32_t at = atomicAdd(&s.n_list, 1u);
+        if (at < kListed) s.list[at] = e;
+    });
+    __syncthreads();
+    const uint32_t listed = s.n_list;
+    if (overflow || listed > kListed) return sample_by_value(x, n, set, Weights{r.max, g.per_t, 0.0}, id, prob, s);
+    sort_list((int)listed, s);
+    pick_from_list((int)listed, g, set, w, id, prob, s);
+}
+
+/* the list of the wanted bins; the part that is done last makes the pick */
+template <class T> __global__ void __launch_bounds__(kThreads) sample_pick_kernel(const T *__restrict__ logits, SampleCall c, int parts) {
+    __shared__ Shared s;
+    const int seq = blockIdx.x / (unsigned)parts, part = blockIdx.x - seq * parts, n = c.n_vocab;
+    const Settings set = settings_of(c, seq);
+    if (takes_first(set) || by_candidates(set)) return;
+    Row *row = row_of(c, seq, parts);
+    const Range r = range_of_parts(parts_of(row), parts);
+    if (!is_there(r.max)) return;
+    const T *x = logits + (size_t)seq * c.ld;
+    const Grid g(r, set.t, n);
+    for (int i = threadIdx.x; i < kBins; i += kThreads) s.weight[i] = row->weight[i], s.count[i] = row->count[i];
+    __syncthreads();
+    sum_bins(g, set, s);
+    const Wanted w = wanted_bins(g, set, s);
+    const Share sh = share_of(n, parts, part);
+    for_each_wanted(x, sh.lo, sh.hi, g, w, [&](uint64_t e) {
+        const uint32_t at = atomicAdd(&row->n_list, 1u);
+        if (at < kListed) __hip_atomic_store(&row->list[at], e, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    });
+    __threadfence(); /* this thread's entries are there before its workgroup counts as done */
+    __syncthreads();
+    if (threadIdx.x == 0) s.last = __hip_atomic_fetch_add(&row->done, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)parts - 1;
+    __syncthreads();
+    if (!s.last) return;
+    __threadfence();
+    const uint32_t listed = __hip_atomic_load(&row->n_list, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    int32_t *id = c.ids + seq;
+    float *prob = c.probs ? c.probs + seq : nullptr;
+    if (listed > kListed) return sample_by_value(x, n, set, Weights{r.max, g.per_t, 0.0}, id, prob, s);
+    for (int i = threadIdx.x; i < (int)listed; i += kThreads) s.list[i] = __hip_atomic_load(&row->list[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    sort_list((int)listed, s);
+    pick_from_list((int)listed, g, set, w, id, prob, s);
+}
+
+/* workgroups per sequence: 1 = the kernel of one, else the three launches */
+int parts_for(int n_seq, int n_vocab) {
+    if (n_seq > 64 || n_vocab < 16384) return 1;
+    return n_vocab < 65536 ? n_vocab / 4096 : 16;
+}
+
 template <class T> hipError_t sample(const SampleCall &c) {
-    sample_row_kernel<T><<<c.n_seq, kThreads, 0, c.stream>>>(static_cast<const T *>(c.logits), c);
+    const T *x = static_cast<const T *>(c.logits);
+    const int parts = parts_for(c.n_seq, c.n_vocab);
+    if (parts == 1) {
+        sample_row_kernel<T><<<c.n_seq, kThreads, 0, c.stream>>>(x, c);
+    } else {
+        sample_parts_kernel<T><<<c.n_seq * parts, kThreads, 0, c.stream>>>(x, c, parts);
+        sample_bins_kernel<T><<<c.n_seq * parts, kThreads, 0, c.stream>>>(x, c, parts);
+        sample_pick_kernel<T><<<c.n_seq * parts, kThreads, 0, c.stream>>>(x, c, parts);
+    }
     return hipGetLastError();
 }
 
 }  // namespace
 
 size_t sample_workspace_bytes(int n_seq, int n_vocab) {
-    (void)n_seq;
-    (void)n_vocab;
-    return 0;
+    const int parts = parts_for(n_seq, n_vocab);
+    return parts == 1 ? 0 : (size_t)n_seq * row_bytes(parts);
 }
 
 hipError_t launch_sample(uint32_t type, const SampleCall &c) {

@@ -84,7 +84,8 @@ def random_settings(rng, n_seq):
 
 @pytest.mark.parametrize("type_id", [F32, F16, BF16])
 @pytest.mark.parametrize("n_seq,n,pad", [(1, 1, 0), (3, 2, 1), (5, 7, 0), (9, 63, 0), (4, 64, 3), (7, 65, 0), (40, 1000, 0), (12, 1025, 7), (33, 4097, 0), (300, 500, 0), (2, 32003, 0),
-                                         (3, 32768, 64), (1, 151936, 0), (5, 128256, 8)])
+                                         (3, 32768, 64), (1, 151936, 0), (5, 128256, 8),
+                                         (64, 16384, 0), (65, 16385, 3), (20, 16383, 0), (66, 70000, 0)])
 def test_picks(type_id, n_seq, n, pad):
     rng = np.random.default_rng(n_seq * 1000 + n)
     x = np.pad(random_logits(rng, n_seq, n), ((0, 0), (0, pad)), constant_values=99.0)  # what lies behind a row is larger than all of it
@@ -93,10 +94,10 @@ def test_picks(type_id, n_seq, n, pad):
         compare(type_id, x, rng.random(n_seq), **random_settings(rng, n_seq), vocab=n)
 
 
-@pytest.mark.parametrize("name,value", [("k", 5), ("k", 40), ("k", 5000), ("p", 0.9), ("p", 0.5), ("p", 0.0), ("p", -1.0), ("m", 0.05), ("m", 1.0), ("m", 2.0), ("t", 0.0), ("t", -1.0),
+@pytest.mark.parametrize("name,value", [("k", 5), ("k", 40), ("k", 128), ("k", 129), ("k", 512), ("k", 600), ("k", 1024), ("k", 1025), ("k", 5000), ("p", 0.9), ("p", 0.5), ("p", 0.0), ("p", -1.0), ("m", 0.05), ("m", 1.0), ("m", 2.0), ("t", 0.0), ("t", -1.0),
                                         ("t", 100.0), ("t", 1e-3), ("t", np.inf), ("t", np.nan), ("p", np.nan), ("m", np.nan), ("k", -3)])
-def test_one_setting(name, value):
-    n_seq, n = 16, 5000
+@pytest.mark.parametrize("n_seq,n", [(16, 5000), (16, 20000), (70, 20000)])  # one workgroup per sequence, several, and one again
+def test_one_setting(n_seq, n, name, value):
     rng = np.random.default_rng(11)
     compare(F32, random_logits(rng, n_seq, n), rng.random(n_seq), **{name: [value] * n_seq})
 
@@ -116,10 +117,10 @@ def test_equal_logits(n):
             compare(type_id, x, u, k=rng.integers(2, n + 5, 24))
 
 
-def test_masks():
+@pytest.mark.parametrize("n", [3001, 20011])
+def test_masks(n):
     """tokens that are ruled out by -infinity or NaN, or pushed down to the type's lowest value; rows of which nothing is left"""
     rng = np.random.default_rng(5)
-    n = 3001
     x = random_logits(rng, 14, n)
     x[0] = -np.inf
     x[1] = np.nan
