@@ -95,7 +95,7 @@ struct Shared {
         uint64_t weight[kBins]; /* sums of 2^-bits exp(offset); afterwards, as doubles, running sums of weights */
         double upto[kBins];
     };
-    uint32_t count[kBins]; /* afterwards running sums */
+    __attribute__((aligned(16))) uint32_t count[kBins]; /* afterwards running sums */
     uint64_t list[kListed];
     union {
         double run[kListed];     /* running sums of the list's weights */
@@ -105,10 +105,9 @@ struct Shared {
     double wave_f64[kWaves];
     uint32_t wave_u32[kWaves];
     float wave_max[kWaves], wave_min[kWaves];
-    uint32_t digit, n_list, best, found[4];
+    uint32_t digit, n_list, best, found[2], least[10];
     Sum above;
     int picked;
-    bool last;
 };
 /* sum of all threads' v, in every thread; `before`: of the threads before this one */
 __device__ Sum sum_of_workgroup(Sum v, Shared &s, Sum *before) {
@@ -494,77 +493,124 @@ template <class T, class F> __device__ __forceinline__ void for_each_wanted(cons
     });
 }
 
-/* s.list[0 .. n) into order (n <= kListed) */
-__device__ void sort_list(int n, Shared &s) {
-    if (n <= 256) { /* by the number of smaller ones: 4 (16 for up to 64) threads count for each */
-        const int each = n <= 64 ? 16 : 4, i = threadIdx.x / each, part = threadIdx.x % each;
-        uint64_t mine = 0;
-        uint32_t rank = 0;
-        if (i < n) {
-            mine = s.list[i];
-            for (int j = part; j < n; j += each) rank += s.list[j] < mine;
-        }
-        for (int off = 1; off < each; off <<= 1) rank += __shfl_xor(rank, off, 64);
-        if (i < n && part == 0) s.sorted[rank] = mine;
-        __syncthreads();
-        if ((int)threadIdx.x < n) s.list[threadIdx.x] = s.sorted[threadIdx.x];
-        __syncthreads();
-        return;
+__device__ __forceinline__ uint64_t shfl_xor_u64(uint64_t v, int by) {
+    return (uint64_t)__shfl_xor((uint32_t)(v >> 32), by, 64) << 32 | __shfl_xor((uint32_t)v, by, 64);
+}
+/* s.list[0 .. n) into order: a bitonic network over `size` entries (a power of two, E per thread: entry e * kThreads + thread), its
+ * short exchanges between the lanes of a wave, the longer ones through LDS, alternating between two buffers, one barrier each */
+template <int E> __device__ void sort_network(int n, int size, Shared &s) {
+    const int t = threadIdx.x;
+    uint64_t v[E];
+    if (t < size) {
+#pragma unroll
+        for (int e = 0; e < E; e++) v[e] = e * kThreads + t < n ? s.list[e * kThreads + t] : ~0ull;
     }
-    int size = 512;
-    while (size < n) size <<= 1;
-    for (int i = n + threadIdx.x; i < size; i += kThreads) s.list[i] = ~0ull;
-    __syncthreads();
+    uint64_t *buffer = s.sorted;
     for (int k = 2; k <= size; k <<= 1)
         for (int j = k >> 1; j; j >>= 1) {
-            const int t = threadIdx.x, i = 2 * t - (t & (j - 1)); /* the lower of the pair */
-            if (t < size / 2) {
-                const uint64_t a = s.list[i], b = s.list[i + j];
-                if ((a > b) == ((i & k) == 0)) s.list[i] = b, s.list[i + j] = a;
+            if (E == 2 && j == kThreads) {
+                const uint64_t a = v[0], b = v[E - 1]; /* (k is the whole size: ascending) */
+                v[0] = min(a, b), v[E - 1] = max(a, b);
+                continue;
             }
-            __syncthreads();
+            uint64_t o[E];
+            if (j >= 64) {
+                if (t < size) {
+#pragma unroll
+                    for (int e = 0; e < E; e++) buffer[e * kThreads + t] = v[e];
+                }
+                __syncthreads();
+                if (t < size) {
+#pragma unroll
+                    for (int e = 0; e < E; e++) o[e] = buffer[e * kThreads + (t ^ j)];
+                }
+                buffer = buffer == s.sorted ? s.list : s.sorted;
+            } else if (t < size) {
+#pragma unroll
+                for (int e = 0; e < E; e++) o[e] = shfl_xor_u64(v[e], j);
+            }
+            if (t < size) {
+#pragma unroll
+                for (int e = 0; e < E; e++) {
+                    const bool smaller = ((t & j) == 0) == (((e * kThreads + t) & k) == 0);
+                    v[e] = smaller ? min(v[e], o[e]) : max(v[e], o[e]);
+                }
+            }
         }
+    __syncthreads();
+    if (t < size) {
+#pragma unroll
+        for (int e = 0; e < E; e++) s.list[e * kThreads + t] = v[e];
+    }
+    __syncthreads();
+}
+__device__ void sort_list(int n, Shared &s) {
+    int size = 64;
+    while (size < n) size <<= 1;
+    if (size > kThreads) sort_network<2>(n, size, s);
+    else sort_network<1>(n, size, s);
 }
 
-/* the cuts on the sorted list */
-template <class G> __device__ void pick_from_list(int n, const G &g, const Settings &set, const Wanted &w, int32_t *id, float *prob, Shared &s) {
+/* The cuts on the sorted list, two entries per thread of `WAVES` waves: one wave for up to 128, which then needs no barrier, else all. */
+constexpr int kOneWave = 128;
+template <int WAVES> __device__ void pick_with(int n, const Grid &g, const Settings &set, const Wanted &w, int32_t *id, float *prob, Shared &s) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i0 = 2 * threadIdx.x;
-    if (threadIdx.x < 4) s.found[threadIdx.x] = (uint32_t)n;
+    auto meet = [&] {
+        if constexpr (WAVES > 1) __syncthreads();
+        else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    };
+    /* the least of the waves' least entries for which a test holds, n if there is none; each call has a place of its own */
+    if (threadIdx.x < 10) s.least[threadIdx.x] = (uint32_t)n;
+    float value[2];
     double wt[2];
     int bin[2];
 #pragma unroll
     for (int e = 0; e < 2; e++) {
         const bool there = i0 + e < n;
-        const float v = there ? entry_value(s.list[i0 + e]) : 0.0f;
-        wt[e] = there ? g.weight(v) : 0.0;
-        bin[e] = there ? (int)g.place(v) : kBins;
+        value[e] = there ? entry_value(s.list[i0 + e]) : 0.0f;
+        wt[e] = there ? g.weight(value[e]) : 0.0;
+        bin[e] = there ? (int)g.place(value[e]) : kBins;
     }
     double run = wt[0] + wt[1];
     for (int off = 1; off < 64; off <<= 1) {
         const double o = shfl_up_f64(run, off);
         if (lane >= off) run += o;
     }
-    if (lane == 63) s.wave_f64[wave] = run;
-    __syncthreads();
     double ahead = 0.0;
-    for (int v = 0; v < wave; v++) ahead += s.wave_f64[v];
+    if constexpr (WAVES > 1) {
+        if (lane == 63) s.wave_f64[wave] = run;
+        meet();
+        for (int v = 0; v < wave; v++) ahead += s.wave_f64[v];
+    }
     s.run[i0 + 1] = ahead + run;
     s.run[i0] = ahead + run - wt[1];
-    /* where the runs of bins begin in the list */
+    meet();
+    int calls = 0;
+    auto first = [&](Run where, auto test) {
+        int best = n;
 #pragma unroll
-    for (int r = 0; r < 4; r++)
-#pragma unroll
-        for (int e = 1; e >= 0; e--)
-            if (r < w.n && bin[e] >= w.run[r].lo) atomicMin(&s.found[r], (uint32_t)(i0 + e));
-    __syncthreads();
-    double base[4]; /* running sum over the row minus running sum over the list, by run */
-#pragma unroll
-    for (int r = 0; r < 4; r++) {
-        base[r] = 0.0;
-        if (!w.all && r < w.n) {
-            const uint32_t at = s.found[r];
-            base[r] = (w.run[r].lo > 0 ? s.upto[w.run[r].lo - 1] : 0.0) - (at > 0 ? s.run[at - 1] : 0.0);
+        for (int e = 1; e >= 0; e--) {
+            const uint64_t holds = __ballot(i0 + e < n && bin[e] >= where.lo && bin[e] <= where.hi && test(i0 + e, wt[e], e));
+            if (holds) best = min(best, 2 * (wave * 64 + (int)__builtin_ctzll(holds)) + e);
         }
+        if constexpr (WAVES > 1) {
+            if (lane == 0 && best < n) atomicMin(&s.least[calls], (uint32_t)best);
+            meet();
+            best = (int)s.least[calls];
+        }
+        calls++;
+        return best;
+    };
+    auto any = [](int, double, int) { return true; };
+    /* running sum over the row minus running sum over the list, by run of bins */
+    double base[4] = {0.0, 0.0, 0.0, 0.0};
+    if (!w.all) {
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+            if (r < w.n) {
+                const int at = first({w.run[r].lo, kBins}, any);
+                base[r] = (w.run[r].lo > 0 ? s.upto[w.run[r].lo - 1] : 0.0) - (at > 0 ? s.run[at - 1] : 0.0);
+            }
     }
     auto sum_to = [&](int i, int b) { /* running sum at entry i, of bin b */
         double off = base[0];
@@ -576,21 +622,7 @@ template <class G> __device__ void pick_from_list(int n, const G &g, const Setti
     double sums[2];
 #pragma unroll
     for (int e = 0; e < 2; e++) sums[e] = i0 + e < n ? sum_to(i0 + e, bin[e]) : 0.0;
-    auto bin_at = [&](int i) { return (int)g.place(entry_value(s.list[i])); };
-    /* first entry within `where` for which the test holds, n if there is none */
-    auto first = [&](Run where, auto test) {
-        __syncthreads();
-        if (threadIdx.x == 0) s.best = (uint32_t)n;
-        __syncthreads();
-#pragma unroll
-        for (int e = 0; e < 2; e++)
-            if (i0 + e < n && bin[e] >= where.lo && bin[e] <= where.hi && test(i0 + e, wt[e], sums[e])) {
-                atomicMin(&s.best, (uint32_t)(i0 + e));
-                break;
-            }
-        __syncthreads();
-        return (int)s.best;
-    };
+    auto sum_at = [&](int i) { return sum_to(i, (int)g.place(entry_value(s.list[i]))); };
     const Run everywhere = {0, kBins};
     int kept = n; /* list entries from here on are cut off (those between the runs lie on the right side by construction) */
     double total = w.all ? s.run[n - 1] : s.upto[kLastBin];
@@ -599,41 +631,38 @@ template <class G> __device__ void pick_from_list(int n, const G &g, const Setti
         total = s.run[kept - 1];
     } else if (w.k.hi >= w.k.lo) {
         const uint32_t at = (uint32_t)set.k - (w.k.lo > 0 ? s.count[w.k.lo - 1] : 0u); /* of the bin's tokens, from 1 */
-        const int start = first(w.k, [](int, double, double) { return true; });
-        kept = min(start + (int)at, n);
+        kept = min(first(w.k, any) + (int)at, n);
         total = sum_to(kept - 1, w.k.lo);
     }
     if (set.p < 1.0f) {
         const double target = fmax((double)set.p, 0.0) * total;
-        const int i = first(w.all ? everywhere : w.p, [&](int, double, double sum) { return sum >= target; });
+        const int i = first(w.all ? everywhere : w.p, [&](int, double, int e) { return sums[e] >= target; });
         if (i < kept) {
             kept = i + 1;
-            total = sum_to(i, bin_at(i));
+            total = sum_at(i);
         }
     }
     if (w.all ? set.m > 0.0f : w.m.hi >= w.m.lo) {
-        const int i = first(w.all ? everywhere : w.m, [&](int, double weight, double) { return weight < (double)set.m; });
-        const int from = i < n || w.all ? i : first(Run{w.m.hi + 1, kBins}, [](int, double, double) { return true; });
+        const int i = first(w.all ? everywhere : w.m, [&](int, double weight, int) { return weight < (double)set.m; });
+        const int from = i < n || w.all ? i : first({w.m.hi + 1, kBins}, any);
+        if (i < n && i < kept) total = fmin(total, sum_at(i) - g.weight(entry_value(s.list[i])));
+        else if (i >= n && !w.all) total = fmin(total, s.upto[w.m.hi]);
         kept = min(kept, from); /* (what lies behind the bins of this cut is lighter) */
-        if (i < n) total = fmin(total, sum_to(i, bin_at(i)) - g.weight(entry_value(s.list[i])));
-        else if (!w.all) total = fmin(total, s.upto[w.m.hi]);
     }
     const double target = (double)set.u * total;
-    int i = first(w.all ? everywhere : w.u, [&](int at, double weight, double sum) { return at < kept && weight > 0.0 && sum > target; });
-    if (i >= n) { /* u of 1, or the last border rounded away: the last kept token that weighs anything */
-        __syncthreads();
-        if (threadIdx.x == 0) s.best = 0;
-        __syncthreads();
-#pragma unroll
-        for (int e = 0; e < 2; e++)
-            if (i0 + e < kept && wt[e] > 0.0) atomicMax(&s.best, (uint32_t)(i0 + e));
-        __syncthreads();
-        i = (int)s.best;
+    int i = first(w.all ? everywhere : w.u, [&](int at, double weight, int e) { return at < kept && weight > 0.0 && sums[e] > target; });
+    if (i >= n) { /* u of 1, or the last border rounded away: the last kept token that weighs anything, which is before the first that does not */
+        const int none = first(everywhere, [&](int at, double weight, int) { return at >= kept || !(weight > 0.0); });
+        i = max(none - 1, 0);
     }
     if (threadIdx.x == 0) {
         *id = (int32_t)(uint32_t)s.list[i];
         if (prob) *prob = (float)(g.weight(entry_value(s.list[i])) / total);
     }
+}
+__device__ __forceinline__ void pick_from_list(int n, const Grid &g, const Settings &set, const Wanted &w, int32_t *id, float *prob, Shared &s) {
+    if (n > kOneWave) pick_with<kWaves>(n, g, set, w, id, prob, s);
+    else if (threadIdx.x < 64) pick_with<1>(n, g, set, w, id, prob, s);
 }
 
 __device__ __forceinline__ void nothing_there(int32_t *id, float *prob) {
@@ -705,7 +734,7 @@ template <class T> __global__ void __launch_bounds__(kThreads) sample_row_kernel
     pick_from_list((int)listed, g, set, w, id, prob, s);
 }
 
-/* ------------------------------------------------------------------ few sequences: several workgroups for each, three launches */
+/* ------------------------------------------------------------------ few sequences: several workgroups for each, four launches */
 
 /* What a sequence keeps in the workspace. A part of the row is a workgroup's; candidates are its tokens that top_k of up to kFewOfParts
  * can keep. */
@@ -714,7 +743,7 @@ struct Row {
     uint64_t weight[kBins];
     uint64_t list[kListed];
     uint32_t count[kBins];
-    uint32_t n_list, done, unused[62];
+    uint32_t n_list, unused[63];
 };
 constexpr int kCandidates = 256, kFewOfParts = 128;
 __host__ __device__ constexpr size_t row_bytes(int parts) { return sizeof(Row) + (size_t)parts * (sizeof(Part) + kCandidates * sizeof(uint64_t)); }
@@ -738,7 +767,7 @@ template <class T> __global__ void __launch_bounds__(kThreads) sample_parts_kern
     const Settings set = settings_of(c, seq);
     const Share sh = share_of(c.n_vocab, parts, part);
     for (int i = part * kThreads + threadIdx.x; i < kBins; i += parts * kThreads) row->weight[i] = 0, row->count[i] = 0;
-    if (part == 0 && threadIdx.x == 0) row->n_list = 0, row->done = 0;
+    if (part == 0 && threadIdx.x == 0) row->n_list = 0;
     if (threadIdx.x == 0) s.best = (uint32_t)c.n_vocab, s.n_list = 0;
     const Range mine = range_of_share(x, sh.lo, sh.hi), r = range_of_workgroup(mine, s);
     if (takes_first(set)) {
@@ -758,7 +787,13 @@ template <class T> __global__ void __launch_bounds__(kThreads) sample_parts_kern
             const int i = threadIdx.x >> 2;
             const float own = groups[i];
             int rank = 0;
-            for (int j = threadIdx.x & 3; j < 256; j += 4) rank += groups[j] > own || (groups[j] == own && j < i);
+#pragma unroll
+            for (int b = 0; b < 16; b++) {
+                const int j = 64 * (threadIdx.x & 3) + 4 * b;
+                const float4 v = *reinterpret_cast<const float4 *>(groups + j);
+                rank += (v.x > own || (v.x == own && j < i)) + (v.y > own || (v.y == own && j + 1 < i));
+                rank += (v.z > own || (v.z == own && j + 2 < i)) + (v.w > own || (v.w == own && j + 3 < i));
+            }
             rank += __shfl_xor(rank, 1, 64);
             rank += __shfl_xor(rank, 2, 64);
             if ((threadIdx.x & 3) == 0 && rank == set.k - 1) s.digit = __float_as_uint(own);
@@ -779,9 +814,16 @@ template <class T> __global__ void __launch_bounds__(kThreads) sample_parts_kern
     if (threadIdx.x == 0) parts_of(row)[part] = {r.max, r.min, (int)s.best, s.n_list};
 }
 
+/* the row's range, in every thread: a lane loads one part's (there are at most kMaxParts) */
+constexpr int kMaxParts = 16;
 __device__ Range range_of_parts(const Part *p, int parts) {
-    Range r = {kMinusInf, -kMinusInf};
-    for (int i = 0; i < parts; i++) r.max = fmaxf(r.max, p[i].max), r.min = fminf(r.min, p[i].min);
+    const Part mine = p[min((int)threadIdx.x & (kMaxParts - 1), parts - 1)];
+    Range r = {mine.max, mine.min};
+#pragma unroll
+    for (int off = kMaxParts / 2; off; off >>= 1) {
+        r.max = fmaxf(r.max, __shfl_xor(r.max, off, 64));
+        r.min = fminf(r.min, __shfl_xor(r.min, off, 64));
+    }
     return r;
 }
 
@@ -821,26 +863,35 @@ template <class T> __global__ void __launch_bounds__(kThreads) sample_bins_kerne
         }
         return;
     }
+    /* every candidate in a register, with the bin that it falls into: one trip to memory */
+    constexpr int kEach = kMaxParts * kCandidates / kThreads;
     const uint64_t *from = candidates_of(row, parts);
+    uint64_t entry[kEach];
+    int bin[kEach];
     bool overflow = false;
-    auto each = [&](auto fn) {
-        for (int i = threadIdx.x; i < parts * kCandidates; i += kThreads)
-            if ((uint32_t)(i % kCandidates) < p[i / kCandidates].n) {
-                const uint64_t e = from[i];
-                const double at = g.place(entry_value(e));
-                if (at < kBins - 1) fn(e, (int)at);
-            }
-    };
-    for (int i = 0; i < parts; i++) overflow = overflow || (p[i].n > kCandidates && g.place(p[i].max) < kBins - 1);
-    each([&](uint64_t, int bin) { atomicAdd(&s.count[bin], 1u); });
+#pragma unroll
+    for (int j = 0; j < kEach; j++) {
+        const int i = threadIdx.x + j * kThreads, of = min(i / kCandidates, parts - 1);
+        entry[j] = from[min(i, parts * kCandidates - 1)];
+        const Part q = p[of];
+        const double at = g.place(entry_value(entry[j]));
+        const bool there = i < parts * kCandidates && (uint32_t)(i % kCandidates) < q.n && at < kBins - 1;
+        bin[j] = there ? (int)at : kBins;
+        overflow = overflow || (q.n > kCandidates && g.place(q.max) < kBins - 1);
+    }
+    overflow = __syncthreads_or(overflow);
+#pragma unroll
+    for (int j = 0; j < kEach; j++)
+        if (bin[j] < kBins) atomicAdd(&s.count[bin[j]], 1u);
     __syncthreads();
     sum_bins(g, set, s);
     const Wanted w = wanted_bins(g, set, s);
-    each([&](uint64_t e, int bin) {
-        if (bin > w.run[0].hi) return;
-        const uint32_t at = atomicAdd(&s.n_list, 1u);
-        if (at < kListed) s.list[at] = e;
-    });
+#pragma unroll
+    for (int j = 0; j < kEach; j++)
+        if (bin[j] <= w.run[0].hi) {
+            const uint32_t at = atomicAdd(&s.n_list, 1u);
+            if (at < kListed) s.list[at] = entry[j];
+        }
     __syncthreads();
     const uint32_t listed = s.n_list;
     if (overflow || listed > kListed) return sample_by_value(x, n, set, Weights{r.max, g.per_t, 0.0}, id, prob, s);
@@ -848,8 +899,8 @@ template <class T> __global__ void __launch_bounds__(kThreads) sample_bins_kerne
     pick_from_list((int)listed, g, set, w, id, prob, s);
 }
 
-/* the list of the wanted bins; the part that is done last makes the pick */
-template <class T> __global__ void __launch_bounds__(kThreads) sample_pick_kernel(const T *__restrict__ logits, SampleCall c, int parts) {
+/* the list of the wanted bins */
+template <class T> __global__ void __launch_bounds__(kThreads) sample_list_kernel(const T *__restrict__ logits, SampleCall c, int parts) {
     __shared__ Shared s;
     const int seq = blockIdx.x / (unsigned)parts, part = blockIdx.x - seq * parts, n = c.n_vocab;
     const Settings set = settings_of(c, seq);
@@ -857,37 +908,53 @@ template <class T> __global__ void __launch_bounds__(kThreads) sample_pick_kerne
     Row *row = row_of(c, seq, parts);
     const Range r = range_of_parts(parts_of(row), parts);
     if (!is_there(r.max)) return;
-    const T *x = logits + (size_t)seq * c.ld;
     const Grid g(r, set.t, n);
     for (int i = threadIdx.x; i < kBins; i += kThreads) s.weight[i] = row->weight[i], s.count[i] = row->count[i];
+    if (threadIdx.x == 0) s.n_list = 0;
     __syncthreads();
     sum_bins(g, set, s);
     const Wanted w = wanted_bins(g, set, s);
     const Share sh = share_of(n, parts, part);
-    for_each_wanted(x, sh.lo, sh.hi, g, w, [&](uint64_t e) {
-        const uint32_t at = atomicAdd(&row->n_list, 1u);
-        if (at < kListed) __hip_atomic_store(&row->list[at], e, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    for_each_wanted(logits + (size_t)seq * c.ld, sh.lo, sh.hi, g, w, [&](uint64_t e) {
+        const uint32_t at = atomicAdd(&s.n_list, 1u);
+        if (at < kListed) s.list[at] = e;
     });
-    __threadfence(); /* this thread's entries are there before its workgroup counts as done */
     __syncthreads();
-    if (threadIdx.x == 0) s.last = __hip_atomic_fetch_add(&row->done, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)parts - 1;
+    /* (one atomic per workgroup: a thousand of them on one address take 100 us) */
+    const uint32_t mine = s.n_list;
+    if (threadIdx.x == 0) s.best = mine ? atomicAdd(&row->n_list, mine) : 0;
     __syncthreads();
-    if (!s.last) return;
-    __threadfence();
-    const uint32_t listed = __hip_atomic_load(&row->n_list, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    for (uint32_t i = threadIdx.x; i < min(mine, (uint32_t)kListed) && s.best + i < kListed; i += kThreads) row->list[s.best + i] = s.list[i];
+}
+
+/* and the pick from it: a launch of its own, since waiting for the other parts' entries inside the one before takes fences between the
+ * dies' L2s, 40 to 60 us where 32 sequences meet them */
+template <class T> __global__ void __launch_bounds__(kThreads) sample_pick_kernel(const T *__restrict__ logits, SampleCall c, int parts) {
+    __shared__ Shared s;
+    const int seq = blockIdx.x, n = c.n_vocab;
+    const Settings set = settings_of(c, seq);
+    if (takes_first(set) || by_candidates(set)) return;
+    Row *row = row_of(c, seq, parts);
+    const Range r = range_of_parts(parts_of(row), parts);
+    if (!is_there(r.max)) return;
+    const Grid g(r, set.t, n);
     int32_t *id = c.ids + seq;
     float *prob = c.probs ? c.probs + seq : nullptr;
-    if (listed > kListed) return sample_by_value(x, n, set, Weights{r.max, g.per_t, 0.0}, id, prob, s);
-    for (int i = threadIdx.x; i < (int)listed; i += kThreads) s.list[i] = __hip_atomic_load(&row->list[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const uint32_t listed = row->n_list;
+    if (listed > kListed) return sample_by_value(logits + (size_t)seq * c.ld, n, set, Weights{r.max, g.per_t, 0.0}, id, prob, s);
+    for (int i = threadIdx.x; i < (int)listed; i += kThreads) s.list[i] = row->list[i];
+    for (int i = threadIdx.x; i < kBins; i += kThreads) s.weight[i] = row->weight[i], s.count[i] = row->count[i];
     __syncthreads();
+    sum_bins(g, set, s);
+    const Wanted w = wanted_bins(g, set, s);
     sort_list((int)listed, s);
     pick_from_list((int)listed, g, set, w, id, prob, s);
 }
 
-/* workgroups per sequence: 1 = the kernel of one, else the three launches */
+/* workgroups per sequence: 1 = the kernel of one, else the four launches */
 int parts_for(int n_seq, int n_vocab) {
     if (n_seq > 64 || n_vocab < 16384) return 1;
-    return n_vocab < 65536 ? n_vocab / 4096 : 16;
+    return n_vocab < 4096 * kMaxParts ? n_vocab / 4096 : kMaxParts;
 }
 
 template <class T> hipError_t sample(const SampleCall &c) {
@@ -898,7 +965,8 @@ template <class T> hipError_t sample(const SampleCall &c) {
     } else {
         sample_parts_kernel<T><<<c.n_seq * parts, kThreads, 0, c.stream>>>(x, c, parts);
         sample_bins_kernel<T><<<c.n_seq * parts, kThreads, 0, c.stream>>>(x, c, parts);
-        sample_pick_kernel<T><<<c.n_seq * parts, kThreads, 0, c.stream>>>(x, c, parts);
+        sample_list_kernel<T><<<c.n_seq * parts, kThreads, 0, c.stream>>>(x, c, parts);
+        sample_pick_kernel<T><<<c.n_seq, kThreads, 0, c.stream>>>(x, c, parts);
     }
     return hipGetLastError();
 }
