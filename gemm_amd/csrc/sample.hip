@@ -402,39 +402,54 @@ template <class F, class G> __device__ Pair first_bins(Shared &s, F one, G other
 }
 template <class F> __device__ int first_bin(Shared &s, F one) { return first_bins(s, one, [](int) { return false; }).one; }
 
-/* the bins to list, as up to four runs in order, and which of them hold which cut */
+/* The bins to list. Each cut has a run of bins in which it may lie, empty (hi < lo) where it does not cut. */
 struct Run { int lo, hi; };
+constexpr int kNowhere = 1 << 30;
 struct Wanted {
-    Run k, p, m, u; /* the bins in which each cut may lie; empty (hi < lo): it does not cut */
-    Run run[4];     /* their union */
-    int n;
+    Run k, p, m, u;
+    Run run[4];     /* the same in order; an empty one begins at kNowhere */
+    int from[4];    /* where the bins that are listed without a gap begin, of each run */
+    double before[4]; /* sums of weights of the bins before that */
+    double total, m_total; /* of all bins; of those up to the end of m's */
+    uint32_t k_before; /* tokens of the bins before k's */
     bool all;       /* the list holds every kept token (run[0] from bin 0) */
 };
-__device__ void add_run(Wanted &w, Run r) {
-    if (r.hi < r.lo) return;
-    int i = 0;
-    while (i < w.n && w.run[i].hi + 1 < r.lo) i++;
-    if (i == w.n || r.hi + 1 < w.run[i].lo) { /* apart from all */
-        for (int j = w.n; j > i; j--) w.run[j] = w.run[j - 1];
-        w.run[i] = r;
-        w.n++;
-        return;
-    }
-    w.run[i].lo = min(w.run[i].lo, r.lo);
-    w.run[i].hi = max(w.run[i].hi, r.hi);
-    while (i + 1 < w.n && w.run[i + 1].lo <= w.run[i].hi + 1) {
-        w.run[i].hi = max(w.run[i].hi, w.run[i + 1].hi);
-        for (int j = i + 1; j + 1 < w.n; j++) w.run[j] = w.run[j + 1];
-        w.n--;
+/* (no index that is not a constant: an array that has one lies in memory, which took 20 us of every row) */
+__device__ __forceinline__ void order_runs(Wanted &w) {
+    w.run[0] = w.k, w.run[1] = w.p, w.run[2] = w.m, w.run[3] = w.u;
+#pragma unroll
+    for (int r = 0; r < 4; r++)
+        if (w.run[r].hi < w.run[r].lo) w.run[r] = {kNowhere, -1};
+    auto by_start = [&](Run &a, Run &b) {
+        if (b.lo < a.lo) {
+            const Run t = a;
+            a = b;
+            b = t;
+        }
+    };
+    by_start(w.run[0], w.run[1]);
+    by_start(w.run[2], w.run[3]);
+    by_start(w.run[0], w.run[2]);
+    by_start(w.run[1], w.run[3]);
+    by_start(w.run[1], w.run[2]);
+    w.from[0] = w.run[0].lo;
+    int reach = w.run[0].hi;
+#pragma unroll
+    for (int r = 1; r < 4; r++) {
+        const bool joins = w.run[r].lo <= reach + 1;
+        w.from[r] = joins ? w.from[r - 1] : w.run[r].lo;
+        reach = joins ? max(reach, w.run[r].hi) : w.run[r].hi;
     }
 }
 __device__ Wanted wanted_bins(const Grid &g, const Settings &set, Shared &s) {
     constexpr double kSlack = 1e-11; /* of the sums' rounding */
     const Run none = {0, -1};
-    Wanted w = {none, none, none, none, {none, none, none, none}, 0, !needs_weights(set)};
+    Wanted w = {};
+    w.k = w.p = w.m = w.u = none;
+    w.all = !needs_weights(set);
     if (w.all) {
-        w.run[0] = {0, min(first_bin(s, [&](int b) { return s.count[b] >= (uint32_t)set.k; }), kLastBin)};
-        w.n = 1;
+        w.k = {0, min(first_bin(s, [&](int b) { return s.count[b] >= (uint32_t)set.k; }), kLastBin)};
+        order_runs(w);
         return w;
     }
     auto before = [&](int b) { return b > 0 ? s.upto[b - 1] : 0.0; };
@@ -464,10 +479,12 @@ __device__ Wanted wanted_bins(const Grid &g, const Settings &set, Shared &s) {
     const double at_most = fmin(u * hi * (1.0 + kSlack), everything * (1.0 - kSlack));
     const Pair f = first_bins(s, [&](int i) { return s.upto[i] > at_least; }, [&](int i) { return s.upto[i] > at_most; });
     w.u = {min(f.one, kLastBin), min(max(f.one, f.other), kLastBin)};
-    add_run(w, w.k);
-    add_run(w, w.p);
-    add_run(w, w.m);
-    add_run(w, w.u);
+    order_runs(w);
+#pragma unroll
+    for (int r = 0; r < 4; r++) w.before[r] = w.from[r] < kNowhere ? before(w.from[r]) : 0.0;
+    w.total = everything;
+    w.m_total = w.m.hi >= w.m.lo ? s.upto[w.m.hi] : 0.0;
+    w.k_before = w.k.hi >= w.k.lo && w.k.lo > 0 ? s.count[w.k.lo - 1] : 0;
     return w;
 }
 
@@ -477,9 +494,7 @@ __device__ __forceinline__ float entry_value(uint64_t e) { return value_of(~(uin
 
 /* fn(entry) for the tokens of the wanted bins: most fail a comparison of floats with bounds a little wider than all of them */
 template <class T, class F> __device__ __forceinline__ void for_each_wanted(const T *x, int lo, int hi, const Grid &g, const Wanted &w, F fn) {
-    int last = w.run[0].hi;
-#pragma unroll
-    for (int r = 1; r < 4; r++) last = max(last, w.run[r].hi);
+    const int last = max(max(w.run[0].hi, w.run[1].hi), max(w.run[2].hi, w.run[3].hi));
     const float low = g.value_below(last + 1), high = w.run[0].lo == 0 ? g.max : g.value_above(w.run[0].lo);
     for_each(x, lo, hi, [&](float v, int i) {
         if (!(v >= low && v <= high && is_there(v))) return;
@@ -537,12 +552,13 @@ template <int E> __device__ void sort_network(int n, int size, Shared &s) {
                 }
             }
         }
-    __syncthreads();
+    if (size > 64) __syncthreads();
     if (t < size) {
 #pragma unroll
         for (int e = 0; e < E; e++) s.list[e * kThreads + t] = v[e];
     }
-    __syncthreads();
+    if (size > 64) __syncthreads(); /* up to 64 entries are wave 0's alone, as is their pick */
+    else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 }
 __device__ void sort_list(int n, Shared &s) {
     int size = 64;
@@ -551,8 +567,8 @@ __device__ void sort_list(int n, Shared &s) {
     else sort_network<1>(n, size, s);
 }
 
-/* The cuts on the sorted list, two entries per thread of `WAVES` waves: one wave for up to 128, which then needs no barrier, else all. */
-constexpr int kOneWave = 128;
+/* The cuts on the sorted list, two entries per thread of `WAVES` waves: one wave for up to 64, which then needs no barrier, else all. */
+constexpr int kOneWave = 64;
 template <int WAVES> __device__ void pick_with(int n, const Grid &g, const Settings &set, const Wanted &w, int32_t *id, float *prob, Shared &s) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i0 = 2 * threadIdx.x;
     auto meet = [&] {
@@ -607,16 +623,16 @@ template <int WAVES> __device__ void pick_with(int n, const Grid &g, const Setti
     if (!w.all) {
 #pragma unroll
         for (int r = 0; r < 4; r++)
-            if (r < w.n) {
-                const int at = first({w.run[r].lo, kBins}, any);
-                base[r] = (w.run[r].lo > 0 ? s.upto[w.run[r].lo - 1] : 0.0) - (at > 0 ? s.run[at - 1] : 0.0);
+            if (w.from[r] < kNowhere) {
+                const int at = first({w.from[r], kBins}, any);
+                base[r] = w.before[r] - (at > 0 ? s.run[at - 1] : 0.0);
             }
     }
     auto sum_to = [&](int i, int b) { /* running sum at entry i, of bin b */
         double off = base[0];
 #pragma unroll
         for (int r = 1; r < 4; r++)
-            if (r < w.n && b >= w.run[r].lo) off = base[r];
+            if (b >= w.run[r].lo) off = base[r];
         return s.run[i] + off;
     };
     double sums[2];
@@ -625,12 +641,12 @@ template <int WAVES> __device__ void pick_with(int n, const Grid &g, const Setti
     auto sum_at = [&](int i) { return sum_to(i, (int)g.place(entry_value(s.list[i]))); };
     const Run everywhere = {0, kBins};
     int kept = n; /* list entries from here on are cut off (those between the runs lie on the right side by construction) */
-    double total = w.all ? s.run[n - 1] : s.upto[kLastBin];
+    double total = w.all ? s.run[n - 1] : w.total;
     if (w.all) {
         kept = min(set.k, n);
         total = s.run[kept - 1];
     } else if (w.k.hi >= w.k.lo) {
-        const uint32_t at = (uint32_t)set.k - (w.k.lo > 0 ? s.count[w.k.lo - 1] : 0u); /* of the bin's tokens, from 1 */
+        const uint32_t at = (uint32_t)set.k - w.k_before; /* of the bin's tokens, from 1 */
         kept = min(first(w.k, any) + (int)at, n);
         total = sum_to(kept - 1, w.k.lo);
     }
@@ -646,7 +662,7 @@ template <int WAVES> __device__ void pick_with(int n, const Grid &g, const Setti
         const int i = first(w.all ? everywhere : w.m, [&](int, double weight, int) { return weight < (double)set.m; });
         const int from = i < n || w.all ? i : first({w.m.hi + 1, kBins}, any);
         if (i < n && i < kept) total = fmin(total, sum_at(i) - g.weight(entry_value(s.list[i])));
-        else if (i >= n && !w.all) total = fmin(total, s.upto[w.m.hi]);
+        else if (i >= n && !w.all) total = fmin(total, w.m_total);
         kept = min(kept, from); /* (what lies behind the bins of this cut is lighter) */
     }
     const double target = (double)set.u * total;
@@ -736,88 +752,52 @@ template <class T> __global__ void __launch_bounds__(kThreads) sample_row_kernel
 
 /* ------------------------------------------------------------------ few sequences: several workgroups for each, four launches */
 
-/* What a sequence keeps in the workspace. A part of the row is a workgroup's; candidates are its tokens that top_k of up to kFewOfParts
- * can keep. */
-struct Part { float max, min; int first; uint32_t n; };
+/* What a sequence keeps in the workspace. A part of the row is a workgroup's, 256 groups of its threads have a largest logit each. */
+struct Part { float max, min; int first; uint32_t unused; };
+constexpr int kGroups = 256, kMaxParts = 16;
 struct Row {
     uint64_t weight[kBins];
     uint64_t list[kListed];
     uint32_t count[kBins];
-    uint32_t n_list, unused[63];
+    Wanted wanted;
+    uint32_t n_list, listed; /* entries; whether the groups' largest logits made the list */
+    Part part[kMaxParts];
+    float group[kMaxParts][kGroups];
 };
-constexpr int kCandidates = 256, kFewOfParts = 128;
-__host__ __device__ constexpr size_t row_bytes(int parts) { return sizeof(Row) + (size_t)parts * (sizeof(Part) + kCandidates * sizeof(uint64_t)); }
-static_assert(sizeof(Row) % 256 == 0 && sizeof(Part) == 16, "alignment of what follows");
-__device__ __forceinline__ Row *row_of(const SampleCall &c, int seq, int parts) { return reinterpret_cast<Row *>(static_cast<uint8_t *>(c.workspace) + (size_t)seq * row_bytes(parts)); }
-__device__ __forceinline__ Part *parts_of(Row *r) { return reinterpret_cast<Part *>(r + 1); }
-__device__ __forceinline__ uint64_t *candidates_of(Row *r, int parts) { return reinterpret_cast<uint64_t *>(parts_of(r) + parts); }
-__device__ __forceinline__ bool by_candidates(const Settings &s) { return s.k > 1 && s.k <= kFewOfParts; }
+constexpr size_t kRowBytes = (sizeof(Row) + 255) / 256 * 256;
+__device__ __forceinline__ Row *row_of(const SampleCall &c, int seq) { return reinterpret_cast<Row *>(static_cast<uint8_t *>(c.workspace) + (size_t)seq * kRowBytes); }
+__device__ __forceinline__ bool by_largest(const Settings &s) { return s.k > 1 && s.k <= kFewOfThreads; }
 struct Share { int lo, hi; };
 __device__ __forceinline__ Share share_of(int n, int parts, int part) {
     const int per = ((n + parts - 1) / parts + 63) & ~63; /* (rows on 16 bytes stay so) */
     return {min(part * per, n), min((part + 1) * per, n)};
 }
 
-/* the range of each part, its candidates, and empty bins */
+/* the range of each part, its groups' largest logits, and empty bins */
 template <class T> __global__ void __launch_bounds__(kThreads) sample_parts_kernel(const T *__restrict__ logits, SampleCall c, int parts) {
     __shared__ Shared s;
     const int seq = blockIdx.x / (unsigned)parts, part = blockIdx.x - seq * parts;
     const T *x = logits + (size_t)seq * c.ld;
-    Row *row = row_of(c, seq, parts);
+    Row *row = row_of(c, seq);
     const Settings set = settings_of(c, seq);
     const Share sh = share_of(c.n_vocab, parts, part);
     for (int i = part * kThreads + threadIdx.x; i < kBins; i += parts * kThreads) row->weight[i] = 0, row->count[i] = 0;
-    if (part == 0 && threadIdx.x == 0) row->n_list = 0;
-    if (threadIdx.x == 0) s.best = (uint32_t)c.n_vocab, s.n_list = 0;
+    if (part == 0 && threadIdx.x == 0) row->n_list = 0, row->listed = 0;
+    if (threadIdx.x == 0) s.best = (uint32_t)c.n_vocab;
     const Range mine = range_of_share(x, sh.lo, sh.hi), r = range_of_workgroup(mine, s);
-    if (takes_first(set)) {
-        if (is_there(r.max) && mine.max == r.max)
-            for_each(x, sh.lo, sh.hi, [&](float v, int i) {
-                if (v == r.max) atomicMin(&s.best, (uint32_t)i);
-            });
-    } else if (by_candidates(set) && is_there(r.max)) {
-        /* the k-th largest of 256 groups' largest logits (equal ones in any order): the part's first k tokens are not below it. Nor
-         * does anything weigh that the bins would not count. */
-        const float group = fmaxf(fmaxf(mine.max, __shfl_xor(mine.max, 1, 64)), fmaxf(__shfl_xor(mine.max, 2, 64), __shfl_xor(mine.max, 3, 64)));
-        float *groups = reinterpret_cast<float *>(s.count);
-        if ((threadIdx.x & 3) == 0) groups[threadIdx.x >> 2] = group;
-        if (threadIdx.x == 0) s.digit = __float_as_uint(kMinusInf);
-        __syncthreads();
-        { /* four threads count for each group */
-            const int i = threadIdx.x >> 2;
-            const float own = groups[i];
-            int rank = 0;
-#pragma unroll
-            for (int b = 0; b < 16; b++) {
-                const int j = 64 * (threadIdx.x & 3) + 4 * b;
-                const float4 v = *reinterpret_cast<const float4 *>(groups + j);
-                rank += (v.x > own || (v.x == own && j < i)) + (v.y > own || (v.y == own && j + 1 < i));
-                rank += (v.z > own || (v.z == own && j + 2 < i)) + (v.w > own || (v.w == own && j + 3 < i));
-            }
-            rank += __shfl_xor(rank, 1, 64);
-            rank += __shfl_xor(rank, 2, 64);
-            if ((threadIdx.x & 3) == 0 && rank == set.k - 1) s.digit = __float_as_uint(own);
-        }
-        __syncthreads();
-        const double reach = (double)r.max - 32.0 * (double)set.t;
-        const float low = fmaxf(__uint_as_float(s.digit), __double2float_rd(reach));
-        uint64_t *to = candidates_of(row, parts) + (size_t)part * kCandidates;
-        if (mine.max >= low)
-            for_each(x, sh.lo, sh.hi, [&](float v, int i) {
-                if (v >= low && is_there(v)) {
-                    const uint32_t at = atomicAdd(&s.n_list, 1u);
-                    if (at < kCandidates) to[at] = entry_of(v, i);
-                }
-            });
-    }
+    const float group = fmaxf(fmaxf(mine.max, __shfl_xor(mine.max, 1, 64)), fmaxf(__shfl_xor(mine.max, 2, 64), __shfl_xor(mine.max, 3, 64)));
+    if ((threadIdx.x & 3) == 0) row->group[part][threadIdx.x >> 2] = group;
+    if (takes_first(set) && is_there(r.max) && mine.max == r.max)
+        for_each(x, sh.lo, sh.hi, [&](float v, int i) {
+            if (v == r.max) atomicMin(&s.best, (uint32_t)i);
+        });
     __syncthreads();
-    if (threadIdx.x == 0) parts_of(row)[part] = {r.max, r.min, (int)s.best, s.n_list};
+    if (threadIdx.x == 0) row->part[part] = {r.max, r.min, (int)s.best, 0};
 }
 
-/* the row's range, in every thread: a lane loads one part's (there are at most kMaxParts) */
-constexpr int kMaxParts = 16;
-__device__ Range range_of_parts(const Part *p, int parts) {
-    const Part mine = p[min((int)threadIdx.x & (kMaxParts - 1), parts - 1)];
+/* the row's range, in every thread: a lane loads one part's */
+__device__ Range range_of_parts(const Row *row, int parts) {
+    const Part mine = row->part[min((int)threadIdx.x & (kMaxParts - 1), parts - 1)];
     Range r = {mine.max, mine.min};
 #pragma unroll
     for (int off = kMaxParts / 2; off; off >>= 1) {
@@ -827,95 +807,9 @@ __device__ Range range_of_parts(const Part *p, int parts) {
     return r;
 }
 
-/* the pick where the parts already hold what it takes; else each part's tokens into the bins */
-template <class T> __global__ void __launch_bounds__(kThreads) sample_bins_kernel(const T *__restrict__ logits, SampleCall c, int parts) {
-    __shared__ Shared s;
-    const int seq = blockIdx.x / (unsigned)parts, part = blockIdx.x - seq * parts, n = c.n_vocab;
-    const T *x = logits + (size_t)seq * c.ld;
-    Row *row = row_of(c, seq, parts);
-    const Part *p = parts_of(row);
-    const Settings set = settings_of(c, seq);
-    const Range r = range_of_parts(p, parts);
-    int32_t *id = c.ids + seq;
-    float *prob = c.probs ? c.probs + seq : nullptr;
-    if (!is_there(r.max) || takes_first(set)) {
-        if (part == 0 && threadIdx.x == 0) {
-            int first = n;
-            for (int i = 0; i < parts; i++)
-                if (p[i].max == r.max) first = min(first, p[i].first);
-            *id = is_there(r.max) ? first : -1;
-            if (prob) *prob = is_there(r.max) ? 1.0f : 0.0f;
-        }
-        return;
-    }
-    const Grid g(r, set.t, n);
-    if (by_candidates(set) && part > 0) return;
-    clear_bins(s);
-    if (threadIdx.x == 0) s.n_list = 0;
-    __syncthreads();
-    if (!by_candidates(set)) {
-        const Share sh = share_of(n, parts, part);
-        fill_bins(x, sh.lo, sh.hi, g, set, s);
-        __syncthreads();
-        for (int i = threadIdx.x; i < kBins; i += kThreads) {
-            if (const uint64_t w = s.weight[i]) atomicAdd((unsigned long long *)&row->weight[i], (unsigned long long)w);
-            if (const uint32_t k = s.count[i]) atomicAdd(&row->count[i], k);
-        }
-        return;
-    }
-    /* every candidate in a register, with the bin that it falls into: one trip to memory */
-    constexpr int kEach = kMaxParts * kCandidates / kThreads;
-    const uint64_t *from = candidates_of(row, parts);
-    uint64_t entry[kEach];
-    int bin[kEach];
-    bool overflow = false;
-#pragma unroll
-    for (int j = 0; j < kEach; j++) {
-        const int i = threadIdx.x + j * kThreads, of = min(i / kCandidates, parts - 1);
-        entry[j] = from[min(i, parts * kCandidates - 1)];
-        const Part q = p[of];
-        const double at = g.place(entry_value(entry[j]));
-        const bool there = i < parts * kCandidates && (uint32_t)(i % kCandidates) < q.n && at < kBins - 1;
-        bin[j] = there ? (int)at : kBins;
-        overflow = overflow || (q.n > kCandidates && g.place(q.max) < kBins - 1);
-    }
-    overflow = __syncthreads_or(overflow);
-#pragma unroll
-    for (int j = 0; j < kEach; j++)
-        if (bin[j] < kBins) atomicAdd(&s.count[bin[j]], 1u);
-    __syncthreads();
-    sum_bins(g, set, s);
-    const Wanted w = wanted_bins(g, set, s);
-#pragma unroll
-    for (int j = 0; j < kEach; j++)
-        if (bin[j] <= w.run[0].hi) {
-            const uint32_t at = atomicAdd(&s.n_list, 1u);
-            if (at < kListed) s.list[at] = entry[j];
-        }
-    __syncthreads();
-    const uint32_t listed = s.n_list;
-    if (overflow || listed > kListed) return sample_by_value(x, n, set, Weights{r.max, g.per_t, 0.0}, id, prob, s);
-    sort_list((int)listed, s);
-    pick_from_list((int)listed, g, set, w, id, prob, s);
-}
-
-/* the list of the wanted bins */
-template <class T> __global__ void __launch_bounds__(kThreads) sample_list_kernel(const T *__restrict__ logits, SampleCall c, int parts) {
-    __shared__ Shared s;
-    const int seq = blockIdx.x / (unsigned)parts, part = blockIdx.x - seq * parts, n = c.n_vocab;
-    const Settings set = settings_of(c, seq);
-    if (takes_first(set) || by_candidates(set)) return;
-    Row *row = row_of(c, seq, parts);
-    const Range r = range_of_parts(parts_of(row), parts);
-    if (!is_there(r.max)) return;
-    const Grid g(r, set.t, n);
-    for (int i = threadIdx.x; i < kBins; i += kThreads) s.weight[i] = row->weight[i], s.count[i] = row->count[i];
-    if (threadIdx.x == 0) s.n_list = 0;
-    __syncthreads();
-    sum_bins(g, set, s);
-    const Wanted w = wanted_bins(g, set, s);
-    const Share sh = share_of(n, parts, part);
-    for_each_wanted(logits + (size_t)seq * c.ld, sh.lo, sh.hi, g, w, [&](uint64_t e) {
+/* this part's tokens of the wanted bins behind those of the others in the row's list; s.n_list is 0 */
+template <class T> __device__ void list_share(const T *x, const Share &sh, const Grid &g, const Wanted &w, Row *row, Shared &s) {
+    for_each_wanted(x, sh.lo, sh.hi, g, w, [&](uint64_t e) {
         const uint32_t at = atomicAdd(&s.n_list, 1u);
         if (at < kListed) s.list[at] = e;
     });
@@ -927,26 +821,99 @@ template <class T> __global__ void __launch_bounds__(kThreads) sample_list_kerne
     for (uint32_t i = threadIdx.x; i < min(mine, (uint32_t)kListed) && s.best + i < kListed; i += kThreads) row->list[s.best + i] = s.list[i];
 }
 
+/* The first token where that is the pick. The list where the groups' largest logits bound the k-th (as the threads' do in the kernel of
+ * one workgroup); else each part's tokens into the bins. */
+template <class T> __global__ void __launch_bounds__(kThreads) sample_bins_kernel(const T *__restrict__ logits, SampleCall c, int parts) {
+    __shared__ Shared s;
+    const int seq = blockIdx.x / (unsigned)parts, part = blockIdx.x - seq * parts, n = c.n_vocab;
+    const T *x = logits + (size_t)seq * c.ld;
+    Row *row = row_of(c, seq);
+    const Settings set = settings_of(c, seq);
+    const Range r = range_of_parts(row, parts);
+    if (!is_there(r.max) || takes_first(set)) {
+        if (part == 0 && threadIdx.x == 0) {
+            int first = n;
+            for (int i = 0; i < parts; i++)
+                if (row->part[i].max == r.max) first = min(first, row->part[i].first);
+            c.ids[seq] = is_there(r.max) ? first : -1;
+            if (c.probs) c.probs[seq] = is_there(r.max) ? 1.0f : 0.0f;
+        }
+        return;
+    }
+    const Grid g(r, set.t, n);
+    const Share sh = share_of(n, parts, part);
+    clear_bins(s);
+    if (threadIdx.x == 0) s.n_list = 0;
+    __syncthreads();
+    if (by_largest(set)) {
+        constexpr int kEach = kMaxParts * kGroups / kThreads;
+        const float *largest = &row->group[0][0];
+        float v[kEach];
+#pragma unroll
+        for (int j = 0; j < kEach; j++) v[j] = largest[min((int)threadIdx.x + j * kThreads, parts * kGroups - 1)];
+#pragma unroll
+        for (int j = 0; j < kEach; j++) {
+            const double at = g.place(v[j]);
+            if ((int)threadIdx.x + j * kThreads < parts * kGroups && is_there(v[j]) && at < kBins - 1) atomicAdd(&s.count[(int)at], 1u);
+        }
+        __syncthreads();
+        sum_bins(g, set, s);
+        if (s.count[kLastBin] >= (uint32_t)set.k) {
+            const Wanted w = wanted_bins(g, set, s);
+            list_share(x, sh, g, w, row, s);
+            if (part == 0 && threadIdx.x == 0) row->wanted = w, row->listed = 1;
+            return;
+        }
+        __syncthreads();
+        clear_bins(s);
+        __syncthreads();
+    }
+    fill_bins(x, sh.lo, sh.hi, g, set, s);
+    __syncthreads();
+    for (int i = threadIdx.x; i < kBins; i += kThreads) {
+        if (const uint64_t w = s.weight[i]) atomicAdd((unsigned long long *)&row->weight[i], (unsigned long long)w);
+        if (const uint32_t k = s.count[i]) atomicAdd(&row->count[i], k);
+    }
+}
+
+/* the list of the wanted bins of a row in bins */
+template <class T> __global__ void __launch_bounds__(kThreads) sample_list_kernel(const T *__restrict__ logits, SampleCall c, int parts) {
+    __shared__ Shared s;
+    const int seq = blockIdx.x / (unsigned)parts, part = blockIdx.x - seq * parts, n = c.n_vocab;
+    const Settings set = settings_of(c, seq);
+    Row *row = row_of(c, seq);
+    if (takes_first(set) || row->listed) return;
+    const Range r = range_of_parts(row, parts);
+    if (!is_there(r.max)) return;
+    const Grid g(r, set.t, n);
+    for (int i = threadIdx.x; i < kBins; i += kThreads) s.weight[i] = row->weight[i], s.count[i] = row->count[i];
+    if (threadIdx.x == 0) s.n_list = 0;
+    __syncthreads();
+    sum_bins(g, set, s);
+    const Wanted w = wanted_bins(g, set, s);
+    if (part == 0 && threadIdx.x == 0) row->wanted = w;
+    list_share(logits + (size_t)seq * c.ld, share_of(n, parts, part), g, w, row, s);
+}
+
 /* and the pick from it: a launch of its own, since waiting for the other parts' entries inside the one before takes fences between the
  * dies' L2s, 40 to 60 us where 32 sequences meet them */
 template <class T> __global__ void __launch_bounds__(kThreads) sample_pick_kernel(const T *__restrict__ logits, SampleCall c, int parts) {
     __shared__ Shared s;
     const int seq = blockIdx.x, n = c.n_vocab;
     const Settings set = settings_of(c, seq);
-    if (takes_first(set) || by_candidates(set)) return;
-    Row *row = row_of(c, seq, parts);
-    const Range r = range_of_parts(parts_of(row), parts);
+    if (takes_first(set)) return;
+    Row *row = row_of(c, seq);
+    const uint32_t listed = row->n_list;
+    const Wanted w = row->wanted;
+    const Range r = range_of_parts(row, parts);
     if (!is_there(r.max)) return;
     const Grid g(r, set.t, n);
     int32_t *id = c.ids + seq;
     float *prob = c.probs ? c.probs + seq : nullptr;
-    const uint32_t listed = row->n_list;
     if (listed > kListed) return sample_by_value(logits + (size_t)seq * c.ld, n, set, Weights{r.max, g.per_t, 0.0}, id, prob, s);
     for (int i = threadIdx.x; i < (int)listed; i += kThreads) s.list[i] = row->list[i];
-    for (int i = threadIdx.x; i < kBins; i += kThreads) s.weight[i] = row->weight[i], s.count[i] = row->count[i];
-    __syncthreads();
-    sum_bins(g, set, s);
-    const Wanted w = wanted_bins(g, set, s);
+    if (listed > 64) __syncthreads();
+    else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); /* (wave 0 loaded, sorts and picks) */
     sort_list((int)listed, s);
     pick_from_list((int)listed, g, set, w, id, prob, s);
 }
@@ -975,7 +942,7 @@ template <class T> hipError_t sample(const SampleCall &c) {
 
 size_t sample_workspace_bytes(int n_seq, int n_vocab) {
     const int parts = parts_for(n_seq, n_vocab);
-    return parts == 1 ? 0 : (size_t)n_seq * row_bytes(parts);
+    return parts == 1 ? 0 : (size_t)n_seq * kRowBytes;
 }
 
 hipError_t launch_sample(uint32_t type, const SampleCall &c) {
