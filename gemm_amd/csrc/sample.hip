@@ -48,6 +48,16 @@ __device__ __forceinline__ uint32_t key_of(float v) {
 __device__ __forceinline__ float value_of(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k); }
 
 
+/* values that are the same in all lanes, into scalar registers: a row's bins and cuts would otherwise hold half of the 128 vector registers
+ * that 1024 threads have each */
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
+__device__ __forceinline__ float uniform(float v) { return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(v))); }
+__device__ __forceinline__ double uniform(double v) {
+    const uint64_t b = (uint64_t)__double_as_longlong(v);
+    return __longlong_as_double((long long)((uint64_t)uniform((uint32_t)(b >> 32)) << 32 | uniform((uint32_t)b)));
+}
+
 /* a sequence's settings */
 struct Settings {
     float t, p, m, u;
@@ -192,7 +202,7 @@ template <class T> __device__ int nth_of_value(const T *x, int n, uint32_t k, ui
 }
 
 /* the whole row by values: for rows whose lists overflow. n tokens, of which the largest is w.max */
-template <class T> __device__ void sample_by_value(const T *x, int n, const Settings &set, Weights w, int32_t *id, float *prob, Shared &s) {
+template <class T> __device__ __noinline__ void sample_by_value(const T *x, int n, const Settings &set, Weights w, int32_t *id, float *prob, Shared &s) {
     int shift = 62; /* n << shift stays below 2^63 */
     while (shift > 0 && ((uint64_t)n >> (62 - shift)) > 1) shift--;
     w.unit = (double)(1ull << shift);
@@ -238,37 +248,59 @@ template <class T> __device__ void sample_by_value(const T *x, int n, const Sett
 
 /* ------------------------------------------------------------------ a row by bins */
 
-/* fn(value, index) for this thread's share of elements lo .. hi - 1 of x: 16-byte loads between the first and the last address on
- * 16 bytes, four in flight per thread */
-template <class T, class F> __device__ __forceinline__ void for_each(const T *x, int lo, int hi, F fn) {
-    constexpr int kPer = 16 / sizeof(T);
-    struct alignas(16) Vec { T v[kPer]; };
+/* This thread's share of elements lo .. hi - 1 of x, in vectors of 16 bytes from the first to the last address on 16, four loads ahead of
+ * their use; an element before or behind those is a vector of its own, whose other places hold NaN. fn(values, index of the first) is
+ * called from one place: a workgroup runs most of this file's code once, and what it has not run yet comes from memory, 64 bytes at a
+ * time. Unrolled over the four vectors, the pass that lists tokens took 15 us instead of 6, most of it for its own instructions. */
+template <class T> constexpr int kPer = 16 / sizeof(T);
+template <class T> struct alignas(16) Vec { T v[kPer<T>]; };
+template <class T, class F> __device__ __forceinline__ void for_vectors(const T *x, int lo, int hi, F fn) {
+    constexpr int N = kPer<T>;
     const int skip = (int)(((16 - (reinterpret_cast<uintptr_t>(x + lo) & 15)) & 15) / sizeof(T));
-    const int first = min(lo + skip, hi), vecs = (hi - first) / kPer, behind = first + vecs * kPer;
-    if ((int)threadIdx.x < first - lo) fn(to_f32(x[lo + threadIdx.x]), lo + (int)threadIdx.x);
-    if ((int)threadIdx.x < hi - behind) fn(to_f32(x[behind + threadIdx.x]), behind + (int)threadIdx.x);
-    const Vec *p = reinterpret_cast<const Vec *>(x + first);
+    const int first = min(lo + skip, hi), vecs = (hi - first) / N, behind = first + vecs * N, before = first - lo;
+    const int all = vecs + before + hi - behind;
+    auto index = [&](int i) { return i < vecs ? first + i * N : i < vecs + before ? lo + i - vecs : behind + i - vecs - before; };
+    auto load = [&](int i) {
+        Vec<T> v;
+        if (i < vecs) return *reinterpret_cast<const Vec<T> *>(x + first + i * N);
+        const uint32_t nan = sizeof(T) == 4 ? 0x7FC00000u : 0x7FFF7FFFu; /* of either 16-bit type */
+        *reinterpret_cast<uint4 *>(&v) = {nan, nan, nan, nan};
+        if (i < all) v.v[0] = x[index(i)];
+        return v;
+    };
     int i = threadIdx.x;
-    for (; i + 3 * kThreads < vecs; i += 4 * kThreads) {
-        const Vec a = p[i], b = p[i + kThreads], c = p[i + 2 * kThreads], d = p[i + 3 * kThreads];
+    Vec<T> a = load(i), b = load(i + kThreads), c = load(i + 2 * kThreads), d = load(i + 3 * kThreads);
+#pragma unroll 1
+    for (; i < all; i += kThreads) {
+        float v[N];
 #pragma unroll
-        for (int j = 0; j < kPer; j++) fn(to_f32(a.v[j]), first + i * kPer + j);
-#pragma unroll
-        for (int j = 0; j < kPer; j++) fn(to_f32(b.v[j]), first + (i + kThreads) * kPer + j);
-#pragma unroll
-        for (int j = 0; j < kPer; j++) fn(to_f32(c.v[j]), first + (i + 2 * kThreads) * kPer + j);
-#pragma unroll
-        for (int j = 0; j < kPer; j++) fn(to_f32(d.v[j]), first + (i + 3 * kThreads) * kPer + j);
+        for (int j = 0; j < N; j++) v[j] = to_f32(a.v[j]);
+        a = b, b = c, c = d, d = load(i + 4 * kThreads);
+        fn(v, index(i));
     }
-    for (; i < vecs; i += kThreads) {
-        const Vec a = p[i];
+}
+template <class T, class F> __device__ __forceinline__ void for_each(const T *x, int lo, int hi, F fn) {
+    for_vectors(x, lo, hi, [&](const float (&v)[kPer<T>], int at) {
 #pragma unroll
-        for (int j = 0; j < kPer; j++) fn(to_f32(a.v[j]), first + i * kPer + j);
-    }
+        for (int j = 0; j < kPer<T>; j++) fn(v[j], at + j);
+    });
+}
+/* fn(value, index) for the few elements that pass a cheap test */
+template <class T, class P, class F> __device__ __forceinline__ void for_each_of(const T *x, int lo, int hi, P test, F fn) {
+    for_vectors(x, lo, hi, [&](const float (&v)[kPer<T>], int at) {
+        uint32_t passed = 0;
+#pragma unroll
+        for (int j = 0; j < kPer<T>; j++) passed |= test(v[j]) ? 1u << j : 0u;
+        while (passed) {
+            const int j = __builtin_ctz(passed);
+            passed &= passed - 1;
+            fn(to_f32(x[at + j]), at + j);
+        }
+    });
 }
 
 struct Range { float max, min; };
-__device__ Range range_of_workgroup(Range r, Shared &s) {
+__device__ __forceinline__ Range range_of_workgroup(Range r, Shared &s) {
     for (int off = 32; off; off >>= 1) {
         r.max = fmaxf(r.max, __shfl_xor(r.max, off, 64));
         r.min = fminf(r.min, __shfl_xor(r.min, off, 64));
@@ -277,7 +309,7 @@ __device__ Range range_of_workgroup(Range r, Shared &s) {
     __syncthreads();
     for (int w = 0; w < kWaves; w++) r.max = fmaxf(r.max, s.wave_max[w]), r.min = fminf(r.min, s.wave_min[w]);
     __syncthreads();
-    return r;
+    return {uniform(r.max), uniform(r.min)};
 }
 template <class T> __device__ __forceinline__ Range range_of_share(const T *x, int lo, int hi) {
     Range r = {kMinusInf, -kMinusInf};
@@ -295,7 +327,7 @@ struct Grid {
     double per_t;  /* 1 / T */
     double scale;  /* bins per unit of logits */
     double step;   /* a bin in units of the exponent: at most 1/64 */
-    double unit;   /* 2^bits: of the sums of exp(offset) */
+    double unit, per_unit; /* 2^bits: of the sums of exp(offset); its inverse */
     __device__ Grid(const Range &r, float t, int n) : max(r.max), per_t(1.0 / (double)t) {
         const double span = (double)r.max - (double)r.min;
         scale = fmax(64.0 * per_t, span > 0.0 ? 2040.0 / span : 0.0);
@@ -304,6 +336,8 @@ struct Grid {
         int bits = 40; /* n << bits stays below 2^62 */
         while (bits > 0 && ((uint64_t)n >> (61 - bits)) > 0) bits--;
         unit = (double)(1ull << bits);
+        max = uniform(max), per_t = uniform(per_t), scale = uniform(scale), step = uniform(step);
+        per_unit = 1.0 / unit;
     }
     /* in bins from the largest; 2047 and more: not counted */
     __device__ __forceinline__ double place(float v) const { return v == max ? 0.0 : ((double)max - (double)v) * scale; }
@@ -324,35 +358,29 @@ struct Grid {
 };
 constexpr int kLastBin = kBins - 2;
 
-/* what a row's bins hold: counts where the list will hold all kept tokens, else weights, and both where top_k is larger than that */
-__device__ __forceinline__ bool needs_counts(const Settings &s) { return s.k > 0; }
-__device__ __forceinline__ bool needs_weights(const Settings &s) { return s.k <= 0 || s.k > kTopList; }
+/* what the bins hold: counts where the list will hold all kept tokens, else weights, and both where top_k is larger than that */
+struct Holds { bool counts, weights; };
+__device__ __forceinline__ Holds holds_for(const Settings &s) { return {s.k > 0, s.k <= 0 || s.k > kTopList}; }
 
-template <class T> __device__ __forceinline__ void fill_bins(const T *x, int lo, int hi, const Grid &g, const Settings &set, Shared &s) {
-    if (!needs_weights(set)) {
-        for_each(x, lo, hi, [&](float v, int) {
-            const double at = g.place(v);
-            if (is_there(v) && at < kBins - 1) atomicAdd(&s.count[(int)at], 1u);
-        });
-    } else {
-        const bool counts = needs_counts(set);
-        for_each(x, lo, hi, [&](float v, int) {
-            const double at = g.place(v);
-            if (is_there(v) && at < kBins - 1) {
-                const int bin = (int)at;
-                atomicAdd((unsigned long long *)&s.weight[bin], (unsigned long long)g.offset_weight(at, bin));
-                if (counts) atomicAdd(&s.count[bin], 1u);
-            }
-        });
-    }
+__device__ __forceinline__ void into_bin(float v, const Grid &g, bool counts, bool weights, Shared &s) {
+    const double at = g.place(v);
+    if (!(at < kBins - 1)) return;
+    const int bin = (int)at;
+    if (weights) atomicAdd((unsigned long long *)&s.weight[bin], (unsigned long long)g.offset_weight(at, bin));
+    if (counts) atomicAdd(&s.count[bin], 1u);
+}
+template <class T> __device__ __forceinline__ void fill_bins(const T *x, int lo, int hi, const Grid &g, const Holds &h, Shared &s) {
+    if (!h.weights) for_each(x, lo, hi, [&](float v, int) { if (is_there(v)) into_bin(v, g, true, false, s); });
+    else if (!h.counts) for_each(x, lo, hi, [&](float v, int) { if (is_there(v)) into_bin(v, g, false, true, s); });
+    else for_each(x, lo, hi, [&](float v, int) { if (is_there(v)) into_bin(v, g, true, true, s); });
 }
 
 /* counts and weights to running sums */
-__device__ void sum_bins(const Grid &g, const Settings &set, Shared &s) {
+__device__ void sum_bins(const Grid &g, const Holds &h, Shared &s) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, b = 2 * threadIdx.x;
-    if (needs_weights(set)) {
-        const double a0 = (double)s.weight[b] / g.unit * exp(-((double)b + 0.5) * g.step);
-        const double a1 = b + 1 > kLastBin ? 0.0 : (double)s.weight[b + 1] / g.unit * exp(-((double)b + 1.5) * g.step);
+    if (h.weights) {
+        const double a0 = (double)s.weight[b] * g.per_unit * exp(-((double)b + 0.5) * g.step);
+        const double a1 = b + 1 > kLastBin ? 0.0 : (double)s.weight[b + 1] * g.per_unit * exp(-((double)b + 1.5) * g.step);
         double run = a0 + a1;
         for (int off = 1; off < 64; off <<= 1) {
             const double o = shfl_up_f64(run, off);
@@ -366,7 +394,7 @@ __device__ void sum_bins(const Grid &g, const Settings &set, Shared &s) {
         s.upto[b + 1] = before + run;
         s.upto[b] = before + run - a1;
     }
-    if (needs_counts(set)) {
+    if (h.counts) {
         const uint32_t a0 = s.count[b], a1 = s.count[b + 1];
         uint32_t run = a0 + a1;
         for (int off = 1; off < 64; off <<= 1) {
@@ -396,7 +424,7 @@ template <class F, class G> __device__ Pair first_bins(Shared &s, F one, G other
         if (b <= kLastBin && other(b) && (b == 0 || !other(b - 1))) s.found[1] = b;
     }
     __syncthreads();
-    const Pair r = {(int)s.found[0], (int)s.found[1]};
+    const Pair r = {uniform((int)s.found[0]), uniform((int)s.found[1])};
     __syncthreads();
     return r;
 }
@@ -441,37 +469,38 @@ __device__ __forceinline__ void order_runs(Wanted &w) {
         reach = joins ? max(reach, w.run[r].hi) : w.run[r].hi;
     }
 }
-__device__ Wanted wanted_bins(const Grid &g, const Settings &set, Shared &s) {
+__device__ Wanted wanted_bins(const Grid &g, const Settings &set, const Holds &h, Shared &s) {
     constexpr double kSlack = 1e-11; /* of the sums' rounding */
     const Run none = {0, -1};
     Wanted w = {};
     w.k = w.p = w.m = w.u = none;
-    w.all = !needs_weights(set);
+    w.all = !h.weights;
     if (w.all) {
         w.k = {0, min(first_bin(s, [&](int b) { return s.count[b] >= (uint32_t)set.k; }), kLastBin)};
         order_runs(w);
         return w;
     }
-    auto before = [&](int b) { return b > 0 ? s.upto[b - 1] : 0.0; };
-    const double everything = s.upto[kLastBin];
+    auto before = [&](int b) { return b > 0 ? uniform(s.upto[b - 1]) : 0.0; };
+    const double everything = uniform(s.upto[kLastBin]);
     double lo = everything, hi = lo; /* between which the sum of the kept lies */
     if (set.k > 0) {
         const int b = first_bin(s, [&](int i) { return s.count[i] >= (uint32_t)set.k; });
-        if (b <= kLastBin) w.k = {b, b}, lo = before(b), hi = s.upto[b];
+        if (b <= kLastBin) w.k = {b, b}, lo = before(b), hi = uniform(s.upto[b]);
     }
     if (set.p < 1.0f) {
         const double p = fmax((double)set.p, 0.0), at_least = p * lo * (1.0 - kSlack), at_most = p * hi * (1.0 + kSlack);
         const Pair f = first_bins(s, [&](int i) { return s.upto[i] >= at_least; }, [&](int i) { return s.upto[i] >= at_most; });
         w.p = {min(f.one, kLastBin), min(f.other, kLastBin)};
         lo = fmin(lo, before(w.p.lo));
-        hi = fmin(hi, s.upto[w.p.hi]);
+        hi = fmin(hi, uniform(s.upto[w.p.hi]));
     }
     if (set.m > 0.0f) {
         const double at = -log((double)set.m) / g.step;
         if (at < kBins) {
-            w.m = {min(max((int)at - 1, 0), kLastBin), min((int)at + 1, kLastBin)};
+            const int bin = uniform((int)at);
+            w.m = {min(max(bin - 1, 0), kLastBin), min(bin + 1, kLastBin)};
             lo = fmin(lo, before(w.m.lo));
-            hi = fmin(hi, s.upto[w.m.hi]);
+            hi = fmin(hi, uniform(s.upto[w.m.hi]));
         }
     }
     /* (beyond the sum of all, for a random number of 1, the last bin that weighs anything) */
@@ -483,8 +512,8 @@ __device__ Wanted wanted_bins(const Grid &g, const Settings &set, Shared &s) {
 #pragma unroll
     for (int r = 0; r < 4; r++) w.before[r] = w.from[r] < kNowhere ? before(w.from[r]) : 0.0;
     w.total = everything;
-    w.m_total = w.m.hi >= w.m.lo ? s.upto[w.m.hi] : 0.0;
-    w.k_before = w.k.hi >= w.k.lo && w.k.lo > 0 ? s.count[w.k.lo - 1] : 0;
+    w.m_total = w.m.hi >= w.m.lo ? uniform(s.upto[w.m.hi]) : 0.0;
+    w.k_before = w.k.hi >= w.k.lo && w.k.lo > 0 ? uniform(s.count[w.k.lo - 1]) : 0;
     return w;
 }
 
@@ -492,19 +521,21 @@ __device__ Wanted wanted_bins(const Grid &g, const Settings &set, Shared &s) {
 __device__ __forceinline__ uint64_t entry_of(float v, int i) { return (uint64_t)(~key_of(v)) << 32 | (uint32_t)i; }
 __device__ __forceinline__ float entry_value(uint64_t e) { return value_of(~(uint32_t)(e >> 32)); }
 
+__device__ __forceinline__ bool is_wanted(int bin, const Wanted &w) {
+    bool in = false;
+#pragma unroll
+    for (int r = 0; r < 4; r++) in = in || (bin >= w.run[r].lo && bin <= w.run[r].hi);
+    return in;
+}
 /* fn(entry) for the tokens of the wanted bins: most fail a comparison of floats with bounds a little wider than all of them */
 template <class T, class F> __device__ __forceinline__ void for_each_wanted(const T *x, int lo, int hi, const Grid &g, const Wanted &w, F fn) {
     const int last = max(max(w.run[0].hi, w.run[1].hi), max(w.run[2].hi, w.run[3].hi));
     const float low = g.value_below(last + 1), high = w.run[0].lo == 0 ? g.max : g.value_above(w.run[0].lo);
-    for_each(x, lo, hi, [&](float v, int i) {
-        if (!(v >= low && v <= high && is_there(v))) return;
+    for_each_of(x, lo, hi, [&](float v) { return v >= low && v <= high; }, [&](float v, int i) {
+        if (!is_there(v)) return;
         const double at = g.place(v);
         if (!(at < kBins - 1)) return;
-        const int b = (int)at;
-        bool in = false;
-#pragma unroll
-        for (int r = 0; r < 4; r++) in = in || (b >= w.run[r].lo && b <= w.run[r].hi);
-        if (in) fn(entry_of(v, i));
+        if (is_wanted((int)at, w)) fn(entry_of(v, i));
     });
 }
 
@@ -567,27 +598,29 @@ __device__ void sort_list(int n, Shared &s) {
     else sort_network<1>(n, size, s);
 }
 
-/* The cuts on the sorted list, two entries per thread of `WAVES` waves: one wave for up to 64, which then needs no barrier, else all. */
+/* The cuts on the sorted list, E entries per thread of `WAVES` waves: one wave for up to 64 entries, which then needs no barrier, else
+ * all. */
 constexpr int kOneWave = 64;
-template <int WAVES> __device__ void pick_with(int n, const Grid &g, const Settings &set, const Wanted &w, int32_t *id, float *prob, Shared &s) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i0 = 2 * threadIdx.x;
+template <int WAVES, int E> __device__ __forceinline__ void pick_with(int n, const Grid &g, const Settings &set, const Wanted &w, int32_t *id, float *prob, Shared &s) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i0 = E * threadIdx.x;
+    double *weight = s.upto; /* the entries' (the bins' sums have gone into w) */
     auto meet = [&] {
         if constexpr (WAVES > 1) __syncthreads();
         else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     };
     /* the least of the waves' least entries for which a test holds, n if there is none; each call has a place of its own */
     if (threadIdx.x < 10) s.least[threadIdx.x] = (uint32_t)n;
-    float value[2];
-    double wt[2];
-    int bin[2];
+    double wt[E], run = 0.0;
+    int bin[E];
 #pragma unroll
-    for (int e = 0; e < 2; e++) {
+    for (int e = 0; e < E; e++) {
         const bool there = i0 + e < n;
-        value[e] = there ? entry_value(s.list[i0 + e]) : 0.0f;
-        wt[e] = there ? g.weight(value[e]) : 0.0;
-        bin[e] = there ? (int)g.place(value[e]) : kBins;
+        const float value = there ? entry_value(s.list[i0 + e]) : 0.0f;
+        wt[e] = there ? g.weight(value) : 0.0;
+        bin[e] = there ? (int)g.place(value) : kBins;
+        weight[i0 + e] = wt[e];
+        run += wt[e];
     }
-    double run = wt[0] + wt[1];
     for (int off = 1; off < 64; off <<= 1) {
         const double o = shfl_up_f64(run, off);
         if (lane >= off) run += o;
@@ -598,21 +631,21 @@ template <int WAVES> __device__ void pick_with(int n, const Grid &g, const Setti
         meet();
         for (int v = 0; v < wave; v++) ahead += s.wave_f64[v];
     }
-    s.run[i0 + 1] = ahead + run;
-    s.run[i0] = ahead + run - wt[1];
+    s.run[i0 + E - 1] = ahead + run;
+    if constexpr (E == 2) s.run[i0] = ahead + run - wt[1];
     meet();
     int calls = 0;
     auto first = [&](Run where, auto test) {
         int best = n;
 #pragma unroll
-        for (int e = 1; e >= 0; e--) {
+        for (int e = E - 1; e >= 0; e--) {
             const uint64_t holds = __ballot(i0 + e < n && bin[e] >= where.lo && bin[e] <= where.hi && test(i0 + e, wt[e], e));
-            if (holds) best = min(best, 2 * (wave * 64 + (int)__builtin_ctzll(holds)) + e);
+            if (holds) best = min(best, E * (wave * 64 + (int)__builtin_ctzll(holds)) + e);
         }
         if constexpr (WAVES > 1) {
             if (lane == 0 && best < n) atomicMin(&s.least[calls], (uint32_t)best);
             meet();
-            best = (int)s.least[calls];
+            best = uniform((int)s.least[calls]);
         }
         calls++;
         return best;
@@ -625,7 +658,7 @@ template <int WAVES> __device__ void pick_with(int n, const Grid &g, const Setti
         for (int r = 0; r < 4; r++)
             if (w.from[r] < kNowhere) {
                 const int at = first({w.from[r], kBins}, any);
-                base[r] = w.before[r] - (at > 0 ? s.run[at - 1] : 0.0);
+                base[r] = uniform(w.before[r] - (at > 0 ? s.run[at - 1] : 0.0));
             }
     }
     auto sum_to = [&](int i, int b) { /* running sum at entry i, of bin b */
@@ -635,9 +668,9 @@ template <int WAVES> __device__ void pick_with(int n, const Grid &g, const Setti
             if (b >= w.run[r].lo) off = base[r];
         return s.run[i] + off;
     };
-    double sums[2];
+    double sums[E];
 #pragma unroll
-    for (int e = 0; e < 2; e++) sums[e] = i0 + e < n ? sum_to(i0 + e, bin[e]) : 0.0;
+    for (int e = 0; e < E; e++) sums[e] = i0 + e < n ? sum_to(i0 + e, bin[e]) : 0.0;
     auto sum_at = [&](int i) { return sum_to(i, (int)g.place(entry_value(s.list[i]))); };
     const Run everywhere = {0, kBins};
     int kept = n; /* list entries from here on are cut off (those between the runs lie on the right side by construction) */
@@ -661,7 +694,7 @@ template <int WAVES> __device__ void pick_with(int n, const Grid &g, const Setti
     if (w.all ? set.m > 0.0f : w.m.hi >= w.m.lo) {
         const int i = first(w.all ? everywhere : w.m, [&](int, double weight, int) { return weight < (double)set.m; });
         const int from = i < n || w.all ? i : first({w.m.hi + 1, kBins}, any);
-        if (i < n && i < kept) total = fmin(total, sum_at(i) - g.weight(entry_value(s.list[i])));
+        if (i < n && i < kept) total = fmin(total, sum_at(i) - weight[i]);
         else if (i >= n && !w.all) total = fmin(total, w.m_total);
         kept = min(kept, from); /* (what lies behind the bins of this cut is lighter) */
     }
@@ -673,12 +706,40 @@ template <int WAVES> __device__ void pick_with(int n, const Grid &g, const Setti
     }
     if (threadIdx.x == 0) {
         *id = (int32_t)(uint32_t)s.list[i];
-        if (prob) *prob = (float)(g.weight(entry_value(s.list[i])) / total);
+        if (prob) *prob = (float)(weight[i] / total);
     }
 }
-__device__ __forceinline__ void pick_from_list(int n, const Grid &g, const Settings &set, const Wanted &w, int32_t *id, float *prob, Shared &s) {
-    if (n > kOneWave) pick_with<kWaves>(n, g, set, w, id, prob, s);
-    else if (threadIdx.x < 64) pick_with<1>(n, g, set, w, id, prob, s);
+/* s.list[0 .. n), in any order, to the pick. A longer list of all kept tokens is itself a row of which bins say where the cuts lie (k = 1000:
+ * sorting all of them took 15 us). */
+__device__ void clear_bins(Shared &s) {
+    for (int i = threadIdx.x; i < kBins; i += kThreads) s.weight[i] = 0, s.count[i] = 0;
+}
+__device__ void pick_from_list(int n, const Grid &g, const Settings &set, Wanted w, int32_t *id, float *prob, Shared &s) {
+    if (w.all && n > kOneWave) {
+        const Holds both = {true, true};
+        __syncthreads();
+        clear_bins(s);
+        if (threadIdx.x == 0) s.n_list = 0;
+        __syncthreads();
+        uint64_t entry[kListed / kThreads];
+#pragma unroll
+        for (int e = 0; e < kListed / kThreads; e++) {
+            const int i = threadIdx.x + e * kThreads;
+            entry[e] = i < n ? s.list[i] : 0; /* (no token's: its value is NaN) */
+            if (i < n) into_bin(entry_value(entry[e]), g, true, true, s);
+        }
+        __syncthreads();
+        sum_bins(g, both, s);
+        w = wanted_bins(g, set, both, s);
+#pragma unroll
+        for (int e = 0; e < kListed / kThreads; e++)
+            if ((int)threadIdx.x + e * kThreads < n && is_wanted((int)g.place(entry_value(entry[e])), w)) s.list[atomicAdd(&s.n_list, 1u)] = entry[e];
+        __syncthreads();
+        n = uniform((int)s.n_list);
+    }
+    sort_list(n, s);
+    if (n > kOneWave) pick_with<kWaves, 2>(n, g, set, w, id, prob, s);
+    else if (threadIdx.x < 64) pick_with<1, 1>(n, g, set, w, id, prob, s);
 }
 
 __device__ __forceinline__ void nothing_there(int32_t *id, float *prob) {
@@ -686,10 +747,6 @@ __device__ __forceinline__ void nothing_there(int32_t *id, float *prob) {
         *id = -1;
         if (prob) *prob = 0.0f;
     }
-}
-
-__device__ __forceinline__ void clear_bins(Shared &s) {
-    for (int i = threadIdx.x; i < kBins; i += kThreads) s.weight[i] = 0, s.count[i] = 0;
 }
 
 /* one workgroup per sequence */
@@ -707,9 +764,7 @@ template <class T> __global__ void __launch_bounds__(kThreads) sample_row_kernel
     __syncthreads();
     if (takes_first(set)) {
         if (mine.max == r.max) /* few threads have it */
-            for_each(x, 0, n, [&](float v, int i) {
-                if (v == r.max) atomicMin(&s.best, (uint32_t)i);
-            });
+            for_each_of(x, 0, n, [&](float v) { return v == r.max; }, [&](float, int i) { atomicMin(&s.best, (uint32_t)i); });
         __syncthreads();
         if (threadIdx.x == 0) {
             *id = (int32_t)s.best;
@@ -718,6 +773,7 @@ template <class T> __global__ void __launch_bounds__(kThreads) sample_row_kernel
         return;
     }
     const Grid g(r, set.t, n);
+    const Holds holds = holds_for(set);
     /* The k-th largest of the threads' own largest logits is not above the k-th of all. For a k that is small beside the threads it is close
      * below (of 128256 logits and k = 512 some 700 are as large), and the pass that counts all tokens into bins is saved. */
     bool counted = false;
@@ -727,26 +783,25 @@ template <class T> __global__ void __launch_bounds__(kThreads) sample_row_kernel
             if (at < kBins - 1) atomicAdd(&s.count[(int)at], 1u);
         }
         __syncthreads();
-        sum_bins(g, set, s);
+        sum_bins(g, holds, s);
         counted = s.count[kLastBin] >= (uint32_t)set.k;
         __syncthreads();
         if (!counted) clear_bins(s);
         __syncthreads();
     }
     if (!counted) {
-        fill_bins(x, 0, n, g, set, s);
+        fill_bins(x, 0, n, g, holds, s);
         __syncthreads();
-        sum_bins(g, set, s);
+        sum_bins(g, holds, s);
     }
-    const Wanted w = wanted_bins(g, set, s);
+    const Wanted w = wanted_bins(g, set, holds, s);
     for_each_wanted(x, 0, n, g, w, [&](uint64_t e) {
         const uint32_t at = atomicAdd(&s.n_list, 1u);
         if (at < kListed) s.list[at] = e;
     });
     __syncthreads();
-    const uint32_t listed = s.n_list;
+    const uint32_t listed = uniform(s.n_list);
     if (listed > kListed) return sample_by_value(x, n, set, Weights{r.max, g.per_t, 0.0}, id, prob, s);
-    sort_list((int)listed, s);
     pick_from_list((int)listed, g, set, w, id, prob, s);
 }
 
@@ -788,9 +843,7 @@ template <class T> __global__ void __launch_bounds__(kThreads) sample_parts_kern
     const float group = fmaxf(fmaxf(mine.max, __shfl_xor(mine.max, 1, 64)), fmaxf(__shfl_xor(mine.max, 2, 64), __shfl_xor(mine.max, 3, 64)));
     if ((threadIdx.x & 3) == 0) row->group[part][threadIdx.x >> 2] = group;
     if (takes_first(set) && is_there(r.max) && mine.max == r.max)
-        for_each(x, sh.lo, sh.hi, [&](float v, int i) {
-            if (v == r.max) atomicMin(&s.best, (uint32_t)i);
-        });
+        for_each_of(x, sh.lo, sh.hi, [&](float v) { return v == r.max; }, [&](float, int i) { atomicMin(&s.best, (uint32_t)i); });
     __syncthreads();
     if (threadIdx.x == 0) row->part[part] = {r.max, r.min, (int)s.best, 0};
 }
@@ -804,7 +857,7 @@ __device__ Range range_of_parts(const Row *row, int parts) {
         r.max = fmaxf(r.max, __shfl_xor(r.max, off, 64));
         r.min = fminf(r.min, __shfl_xor(r.min, off, 64));
     }
-    return r;
+    return {uniform(r.max), uniform(r.min)};
 }
 
 /* this part's tokens of the wanted bins behind those of the others in the row's list; s.n_list is 0 */
@@ -841,6 +894,7 @@ template <class T> __global__ void __launch_bounds__(kThreads) sample_bins_kerne
         return;
     }
     const Grid g(r, set.t, n);
+    const Holds holds = holds_for(set);
     const Share sh = share_of(n, parts, part);
     clear_bins(s);
     if (threadIdx.x == 0) s.n_list = 0;
@@ -857,9 +911,9 @@ template <class T> __global__ void __launch_bounds__(kThreads) sample_bins_kerne
             if ((int)threadIdx.x + j * kThreads < parts * kGroups && is_there(v[j]) && at < kBins - 1) atomicAdd(&s.count[(int)at], 1u);
         }
         __syncthreads();
-        sum_bins(g, set, s);
+        sum_bins(g, holds, s);
         if (s.count[kLastBin] >= (uint32_t)set.k) {
-            const Wanted w = wanted_bins(g, set, s);
+            const Wanted w = wanted_bins(g, set, holds, s);
             list_share(x, sh, g, w, row, s);
             if (part == 0 && threadIdx.x == 0) row->wanted = w, row->listed = 1;
             return;
@@ -868,7 +922,7 @@ template <class T> __global__ void __launch_bounds__(kThreads) sample_bins_kerne
         clear_bins(s);
         __syncthreads();
     }
-    fill_bins(x, sh.lo, sh.hi, g, set, s);
+    fill_bins(x, sh.lo, sh.hi, g, holds, s);
     __syncthreads();
     for (int i = threadIdx.x; i < kBins; i += kThreads) {
         if (const uint64_t w = s.weight[i]) atomicAdd((unsigned long long *)&row->weight[i], (unsigned long long)w);
@@ -886,11 +940,12 @@ template <class T> __global__ void __launch_bounds__(kThreads) sample_list_kerne
     const Range r = range_of_parts(row, parts);
     if (!is_there(r.max)) return;
     const Grid g(r, set.t, n);
+    const Holds holds = holds_for(set);
     for (int i = threadIdx.x; i < kBins; i += kThreads) s.weight[i] = row->weight[i], s.count[i] = row->count[i];
     if (threadIdx.x == 0) s.n_list = 0;
     __syncthreads();
-    sum_bins(g, set, s);
-    const Wanted w = wanted_bins(g, set, s);
+    sum_bins(g, holds, s);
+    const Wanted w = wanted_bins(g, set, holds, s);
     if (part == 0 && threadIdx.x == 0) row->wanted = w;
     list_share(logits + (size_t)seq * c.ld, share_of(n, parts, part), g, w, row, s);
 }
@@ -912,9 +967,8 @@ template <class T> __global__ void __launch_bounds__(kThreads) sample_pick_kerne
     float *prob = c.probs ? c.probs + seq : nullptr;
     if (listed > kListed) return sample_by_value(logits + (size_t)seq * c.ld, n, set, Weights{r.max, g.per_t, 0.0}, id, prob, s);
     for (int i = threadIdx.x; i < (int)listed; i += kThreads) s.list[i] = row->list[i];
-    if (listed > 64) __syncthreads();
+    if (listed > kOneWave) __syncthreads();
     else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); /* (wave 0 loaded, sorts and picks) */
-    sort_list((int)listed, s);
     pick_from_list((int)listed, g, set, w, id, prob, s);
 }
 
