@@ -18,7 +18,7 @@
  *
  * Weights and sums are 64-bit: the borders between tokens lie closer to each other than fp32 sums resolve, and the token is to be the
  * one that the definition gives. A bin's weight is exp(centre) times the sum of exp(offset from the centre), offsets below 1/128, so
- * that a token costs a polynomial of degree 5 (3e-16) instead of an exponential; the sum is of integers of 2^-40, which do not depend on
+ * that a token costs a polynomial of degree 4 instead of an exponential; the sum is of integers of 2^-40, which do not depend on
  * the order of the additions: the same call gives the same token.
  *   A list that overflows (a bin of more than 2048 tokens: rows of equal logits) leaves the row to sample_by_value, which takes
  * several passes for each cut.
@@ -254,29 +254,37 @@ template <class T> __device__ __noinline__ void sample_by_value(const T *x, int 
  * time. Unrolled over the four vectors, the pass that lists tokens took 15 us instead of 6, most of it for its own instructions. */
 template <class T> constexpr int kPer = 16 / sizeof(T);
 template <class T> struct alignas(16) Vec { T v[kPer<T>]; };
-template <class T, class F> __device__ __forceinline__ void for_vectors(const T *x, int lo, int hi, F fn) {
-    constexpr int N = kPer<T>;
-    const int skip = (int)(((16 - (reinterpret_cast<uintptr_t>(x + lo) & 15)) & 15) / sizeof(T));
-    const int first = min(lo + skip, hi), vecs = (hi - first) / N, behind = first + vecs * N, before = first - lo;
-    const int all = vecs + before + hi - behind;
-    auto index = [&](int i) { return i < vecs ? first + i * N : i < vecs + before ? lo + i - vecs : behind + i - vecs - before; };
-    auto load = [&](int i) {
+template <class T> struct Vectors {
+    static constexpr int N = kPer<T>;
+    const T *x;
+    int lo, first, vecs, behind, all;
+    __device__ Vectors(const T *p, int begin, int end) : x(p), lo(begin) {
+        const int skip = (int)(((16 - (reinterpret_cast<uintptr_t>(x + lo) & 15)) & 15) / sizeof(T));
+        first = min(lo + skip, end), vecs = (end - first) / N, behind = first + vecs * N;
+        all = vecs + (first - lo) + (end - behind);
+    }
+    __device__ int index(int i) const { return i < vecs ? first + i * N : i < vecs + first - lo ? lo + i - vecs : behind + i - vecs - (first - lo); }
+    __device__ Vec<T> load(int i) const {
         Vec<T> v;
         if (i < vecs) return *reinterpret_cast<const Vec<T> *>(x + first + i * N);
         const uint32_t nan = sizeof(T) == 4 ? 0x7FC00000u : 0x7FFF7FFFu; /* of either 16-bit type */
         *reinterpret_cast<uint4 *>(&v) = {nan, nan, nan, nan};
         if (i < all) v.v[0] = x[index(i)];
         return v;
-    };
+    }
+};
+template <class T, class F> __device__ __forceinline__ void for_vectors(const T *x, int lo, int hi, F fn) {
+    constexpr int N = kPer<T>;
+    const Vectors<T> vec(x, lo, hi);
     int i = threadIdx.x;
-    Vec<T> a = load(i), b = load(i + kThreads), c = load(i + 2 * kThreads), d = load(i + 3 * kThreads);
+    Vec<T> a = vec.load(i), b = vec.load(i + kThreads), c = vec.load(i + 2 * kThreads), d = vec.load(i + 3 * kThreads);
 #pragma unroll 1
-    for (; i < all; i += kThreads) {
+    for (; i < vec.all; i += kThreads) {
         float v[N];
 #pragma unroll
         for (int j = 0; j < N; j++) v[j] = to_f32(a.v[j]);
-        a = b, b = c, c = d, d = load(i + 4 * kThreads);
-        fn(v, index(i));
+        a = b, b = c, c = d, d = vec.load(i + 4 * kThreads);
+        fn(v, vec.index(i));
     }
 }
 template <class T, class F> __device__ __forceinline__ void for_each(const T *x, int lo, int hi, F fn) {
@@ -314,14 +322,13 @@ __device__ __forceinline__ Range range_of_workgroup(Range r, Shared &s) {
 template <class T> __device__ __forceinline__ Range range_of_share(const T *x, int lo, int hi) {
     Range r = {kMinusInf, -kMinusInf};
     for_each(x, lo, hi, [&](float v, int) {
-        const bool there = is_there(v);
-        r.max = fmaxf(r.max, there ? v : kMinusInf);
-        r.min = fminf(r.min, there ? v : -kMinusInf);
+        r.max = fmaxf(r.max, v); /* (NaN is not taken) */
+        r.min = fminf(r.min, is_there(v) ? v : -kMinusInf);
     });
     return r;
 }
 
-/* the bins of a row */
+/* the bins of a row whose largest logit is finite */
 struct Grid {
     float max;
     double per_t;  /* 1 / T */
@@ -332,29 +339,31 @@ struct Grid {
         const double span = (double)r.max - (double)r.min;
         scale = fmax(64.0 * per_t, span > 0.0 ? 2040.0 / span : 0.0);
         if (!(scale > 0.0)) scale = 1.0;
-        step = per_t / scale;
+        scale = fmin(scale, 1e250); /* (a temperature of 1e-45) */
+        step = fmin(per_t / scale, 1.0 / 64);
         int bits = 40; /* n << bits stays below 2^62 */
         while (bits > 0 && ((uint64_t)n >> (61 - bits)) > 0) bits--;
         unit = (double)(1ull << bits);
         max = uniform(max), per_t = uniform(per_t), scale = uniform(scale), step = uniform(step);
         per_unit = 1.0 / unit;
     }
-    /* in bins from the largest; 2047 and more: not counted */
-    __device__ __forceinline__ double place(float v) const { return v == max ? 0.0 : ((double)max - (double)v) * scale; }
-    __device__ __forceinline__ uint64_t offset_weight(double place, int bin) const {
-        const double g = ((double)bin + 0.5 - place) * step;
-        double e = fma(g, 1.0 / 120, 1.0 / 24);
-        e = fma(e, g, 1.0 / 6);
-        e = fma(e, g, 0.5);
-        e = fma(e, g, 1.0);
-        e = fma(e, g, 1.0);
-        /* the integer nearest to e * unit is what the sum with 2^52 holds below the exponent */
-        return (uint64_t)__double_as_longlong(fma(e, unit, 4503599627370496.0)) & 0x000FFFFFFFFFFFFFull;
+    /* in bins from the largest, which is at 0; never falls from a logit to a smaller one. 2047 and more is not counted, nor what
+     * -infinity (infinity) and NaN (NaN) give */
+    __device__ __forceinline__ double place(float v) const { return ((double)max - (double)v) * scale; }
+    /* exp(centre of the bin - place), by a polynomial of degree 4 (2.4e-13 at the bin's edge, and the errors of its two halves have
+     * opposite signs), as an integer of 1 / unit: the last of the sums rounds at 2^52, whose lower bits are that integer */
+    __device__ __forceinline__ uint64_t offset_weight(double place) const {
+        const double g = fma(-__builtin_amdgcn_fract(place), step, 0.5 * step);
+        double e = fma(g, unit / 24, unit / 6);
+        e = fma(e, g, unit / 2);
+        e = fma(e, g, unit);
+        e = fma(e, g, unit + 4503599627370496.0);
+        return (uint64_t)__double_as_longlong(e) & 0x000FFFFFFFFFFFFFull;
     }
     /* floats below (above) every value of place `at` and less (and more) */
     __device__ float value_below(int at) const { return __double2float_rd((double)max - (double)at / scale * (1.0 + 1e-9)); }
     __device__ float value_above(int at) const { return __double2float_ru((double)max - (double)at / scale * (1.0 - 1e-9)); }
-    __device__ double weight(float v) const { return v == max ? 1.0 : max == -kMinusInf ? 0.0 : exp(((double)v - (double)max) * per_t); }
+    __device__ double weight(float v) const { return exp(((double)v - (double)max) * per_t); }
 };
 constexpr int kLastBin = kBins - 2;
 
@@ -366,13 +375,13 @@ __device__ __forceinline__ void into_bin(float v, const Grid &g, bool counts, bo
     const double at = g.place(v);
     if (!(at < kBins - 1)) return;
     const int bin = (int)at;
-    if (weights) atomicAdd((unsigned long long *)&s.weight[bin], (unsigned long long)g.offset_weight(at, bin));
+    if (weights) atomicAdd((unsigned long long *)&s.weight[bin], (unsigned long long)g.offset_weight(at));
     if (counts) atomicAdd(&s.count[bin], 1u);
 }
 template <class T> __device__ __forceinline__ void fill_bins(const T *x, int lo, int hi, const Grid &g, const Holds &h, Shared &s) {
-    if (!h.weights) for_each(x, lo, hi, [&](float v, int) { if (is_there(v)) into_bin(v, g, true, false, s); });
-    else if (!h.counts) for_each(x, lo, hi, [&](float v, int) { if (is_there(v)) into_bin(v, g, false, true, s); });
-    else for_each(x, lo, hi, [&](float v, int) { if (is_there(v)) into_bin(v, g, true, true, s); });
+    if (!h.weights) for_each(x, lo, hi, [&](float v, int) { into_bin(v, g, true, false, s); });
+    else if (!h.counts) for_each(x, lo, hi, [&](float v, int) { into_bin(v, g, false, true, s); });
+    else for_each(x, lo, hi, [&](float v, int) { into_bin(v, g, true, true, s); });
 }
 
 /* counts and weights to running sums */
@@ -503,6 +512,11 @@ __device__ Wanted wanted_bins(const Grid &g, const Settings &set, const Holds &h
             hi = fmin(hi, uniform(s.upto[w.m.hi]));
         }
     }
+    /* of top-p and min-p the one that cuts off more is enough, where that is clear */
+    if (w.p.hi >= w.p.lo && w.m.hi >= w.m.lo) {
+        if (w.m.hi < w.p.lo) w.p = none;
+        else if (w.p.hi < w.m.lo) w.m = none;
+    }
     /* (beyond the sum of all, for a random number of 1, the last bin that weighs anything) */
     const double u = fmin((double)set.u, 1.0), at_least = fmin(u * lo * (1.0 - kSlack), everything * (1.0 - kSlack));
     const double at_most = fmin(u * hi * (1.0 + kSlack), everything * (1.0 - kSlack));
@@ -527,16 +541,30 @@ __device__ __forceinline__ bool is_wanted(int bin, const Wanted &w) {
     for (int r = 0; r < 4; r++) in = in || (bin >= w.run[r].lo && bin <= w.run[r].hi);
     return in;
 }
-/* fn(entry) for the tokens of the wanted bins: most fail a comparison of floats with bounds a little wider than all of them */
+/* Whether a value can lie in a wanted bin, by floats a little outside of the first bins without a gap, and of all behind them. */
+struct Bounds {
+    float low0, high0, low1, high1;
+    __device__ Bounds(const Grid &g, const Wanted &w) {
+        int end = w.run[0].hi, start = kNowhere, last = -1;
+#pragma unroll
+        for (int r = 1; r < 4; r++) {
+            const bool joins = w.from[r] == w.from[0];
+            if (joins) end = max(end, w.run[r].hi);
+            else start = min(start, w.run[r].lo), last = max(last, w.run[r].hi);
+        }
+        low0 = uniform(g.value_below(end + 1)), high0 = uniform(w.run[0].lo == 0 ? g.max : g.value_above(w.run[0].lo));
+        low1 = uniform(start < kNowhere ? g.value_below(last + 1) : -kMinusInf), high1 = uniform(start < kNowhere ? g.value_above(start) : kMinusInf);
+    }
+    __device__ __forceinline__ bool operator()(float v) const { return (v >= low0 && v <= high0) || (v >= low1 && v <= high1); }
+};
+/* fn(entry) for the tokens of the wanted bins */
+template <class F> __device__ __forceinline__ void if_wanted(float v, int i, const Grid &g, const Wanted &w, F fn) {
+    const double at = g.place(v);
+    if (at < kBins - 1 && is_wanted((int)at, w)) fn(entry_of(v, i));
+}
 template <class T, class F> __device__ __forceinline__ void for_each_wanted(const T *x, int lo, int hi, const Grid &g, const Wanted &w, F fn) {
-    const int last = max(max(w.run[0].hi, w.run[1].hi), max(w.run[2].hi, w.run[3].hi));
-    const float low = g.value_below(last + 1), high = w.run[0].lo == 0 ? g.max : g.value_above(w.run[0].lo);
-    for_each_of(x, lo, hi, [&](float v) { return v >= low && v <= high; }, [&](float v, int i) {
-        if (!is_there(v)) return;
-        const double at = g.place(v);
-        if (!(at < kBins - 1)) return;
-        if (is_wanted((int)at, w)) fn(entry_of(v, i));
-    });
+    const Bounds bounds(g, w);
+    for_each_of(x, lo, hi, bounds, [&](float v, int i) { if_wanted(v, i, g, w, fn); });
 }
 
 __device__ __forceinline__ uint64_t shfl_xor_u64(uint64_t v, int by) {
@@ -683,7 +711,7 @@ template <int WAVES, int E> __device__ __forceinline__ void pick_with(int n, con
         kept = min(first(w.k, any) + (int)at, n);
         total = sum_to(kept - 1, w.k.lo);
     }
-    if (set.p < 1.0f) {
+    if (w.all ? set.p < 1.0f : w.p.hi >= w.p.lo) {
         const double target = fmax((double)set.p, 0.0) * total;
         const int i = first(w.all ? everywhere : w.p, [&](int, double, int e) { return sums[e] >= target; });
         if (i < kept) {
@@ -759,7 +787,7 @@ template <class T> __global__ void __launch_bounds__(kThreads) sample_row_kernel
     const Settings set = settings_of(c, seq);
     const Range mine = range_of_share(x, 0, n), r = range_of_workgroup(mine, s);
     if (!is_there(r.max)) return nothing_there(id, prob);
-    if (threadIdx.x == 0) s.best = (uint32_t)n, s.n_list = 0;
+    if (threadIdx.x == 0) s.best = (uint32_t)n, s.n_list = 0, s.digit = 0;
     clear_bins(s);
     __syncthreads();
     if (takes_first(set)) {
@@ -772,6 +800,7 @@ template <class T> __global__ void __launch_bounds__(kThreads) sample_row_kernel
         }
         return;
     }
+    if (r.max == -kMinusInf) return sample_by_value(x, n, set, Weights{r.max, 1.0 / (double)set.t, 0.0}, id, prob, s);
     const Grid g(r, set.t, n);
     const Holds holds = holds_for(set);
     /* The k-th largest of the threads' own largest logits is not above the k-th of all. For a k that is small beside the threads it is close
@@ -795,10 +824,29 @@ template <class T> __global__ void __launch_bounds__(kThreads) sample_row_kernel
         sum_bins(g, holds, s);
     }
     const Wanted w = wanted_bins(g, set, holds, s);
-    for_each_wanted(x, 0, n, g, w, [&](uint64_t e) {
+    auto list = [&](uint64_t e) {
         const uint32_t at = atomicAdd(&s.n_list, 1u);
         if (at < kListed) s.list[at] = e;
-    });
+    };
+    if (counted) {
+        /* only what the threads read whose largest logit is wanted: their vectors, dealt to all threads (for k = 40 some 720 vectors of
+         * 16032; a pass over all of them takes 12 us) */
+        uint32_t *of = reinterpret_cast<uint32_t *>(s.sorted);
+        const Bounds bounds(g, w);
+        if (mine.max >= bounds.low0) of[atomicAdd(&s.digit, 1u)] = threadIdx.x;
+        __syncthreads();
+        const Vectors<T> vec(x, 0, n);
+        const int rounds = (vec.all + kThreads - 1) / kThreads, tasks = uniform((int)s.digit) * rounds;
+        for (int q = threadIdx.x; q < tasks; q += kThreads) {
+            const int i = (int)of[q / rounds] + q % rounds * kThreads;
+            const Vec<T> v = vec.load(i);
+#pragma unroll
+            for (int j = 0; j < kPer<T>; j++)
+                if (bounds(to_f32(v.v[j]))) if_wanted(to_f32(v.v[j]), vec.index(i) + j, g, w, list);
+        }
+    } else {
+        for_each_wanted(x, 0, n, g, w, list);
+    }
     __syncthreads();
     const uint32_t listed = uniform(s.n_list);
     if (listed > kListed) return sample_by_value(x, n, set, Weights{r.max, g.per_t, 0.0}, id, prob, s);
@@ -893,6 +941,10 @@ template <class T> __global__ void __launch_bounds__(kThreads) sample_bins_kerne
         }
         return;
     }
+    if (r.max == -kMinusInf) {
+        if (part == 0) sample_by_value(x, n, set, Weights{r.max, 1.0 / (double)set.t, 0.0}, c.ids + seq, c.probs ? c.probs + seq : nullptr, s);
+        return;
+    }
     const Grid g(r, set.t, n);
     const Holds holds = holds_for(set);
     const Share sh = share_of(n, parts, part);
@@ -938,7 +990,7 @@ template <class T> __global__ void __launch_bounds__(kThreads) sample_list_kerne
     Row *row = row_of(c, seq);
     if (takes_first(set) || row->listed) return;
     const Range r = range_of_parts(row, parts);
-    if (!is_there(r.max)) return;
+    if (!is_there(r.max) || r.max == -kMinusInf) return;
     const Grid g(r, set.t, n);
     const Holds holds = holds_for(set);
     for (int i = threadIdx.x; i < kBins; i += kThreads) s.weight[i] = row->weight[i], s.count[i] = row->count[i];
@@ -961,7 +1013,7 @@ template <class T> __global__ void __launch_bounds__(kThreads) sample_pick_kerne
     const uint32_t listed = row->n_list;
     const Wanted w = row->wanted;
     const Range r = range_of_parts(row, parts);
-    if (!is_there(r.max)) return;
+    if (!is_there(r.max) || r.max == -kMinusInf) return;
     const Grid g(r, set.t, n);
     int32_t *id = c.ids + seq;
     float *prob = c.probs ? c.probs + seq : nullptr;
