@@ -73,7 +73,9 @@ __device__ __forceinline__ Settings settings_of(const SampleCall &c, int seq) {
     s.u = u > 0.0f ? u : 0.0f;
     return s;
 }
+constexpr int kFewOfThreads = 512; /* top_k up to which the threads' largest logits bound it */
 __device__ __forceinline__ bool takes_first(const Settings &s) { return !(s.t > 0.0f) || s.k == 1; }
+__device__ __forceinline__ bool by_largest(const Settings &s) { return s.k > 1 && s.k <= kFewOfThreads; }
 
 __device__ __forceinline__ uint64_t shfl_u64(uint64_t v, int from) {
     return (uint64_t)__shfl((uint32_t)(v >> 32), from, 64) << 32 | __shfl((uint32_t)v, from, 64);
@@ -98,7 +100,6 @@ struct Sum { uint32_t count; uint64_t weight; };
 __device__ __forceinline__ Sum operator+(Sum a, Sum b) { return {a.count + b.count, a.weight + b.weight}; }
 
 constexpr int kBins = 2048, kListed = 2048, kTopList = 1024; /* bins; tokens of a list; top_k up to which a list holds all kept */
-constexpr int kFewOfThreads = 512; /* top_k up to which the threads' largest logits bound it */
 
 struct Shared {
     union {
@@ -557,6 +558,10 @@ struct Bounds {
     }
     __device__ __forceinline__ bool operator()(float v) const { return (v >= low0 && v <= high0) || (v >= low1 && v <= high1); }
 };
+__device__ __forceinline__ void add_to_list(uint64_t e, Shared &s) {
+    const uint32_t at = atomicAdd(&s.n_list, 1u);
+    if (at < kListed) s.list[at] = e;
+}
 /* fn(entry) for the tokens of the wanted bins */
 template <class F> __device__ __forceinline__ void if_wanted(float v, int i, const Grid &g, const Wanted &w, F fn) {
     const double at = g.place(v);
@@ -777,19 +782,64 @@ __device__ __forceinline__ void nothing_there(int32_t *id, float *prob) {
     }
 }
 
-/* one workgroup per sequence */
-template <class T> __global__ void __launch_bounds__(kThreads) sample_row_kernel(const T *__restrict__ logits, SampleCall c) {
-    __shared__ Shared s;
-    const int seq = blockIdx.x, n = c.n_vocab;
-    const T *x = logits + (size_t)seq * c.ld;
-    int32_t *id = c.ids + seq;
-    float *prob = c.probs ? c.probs + seq : nullptr;
-    const Settings set = settings_of(c, seq);
+/* A row from its bins, or where `filled` is false from its range, to the pick; `mine` is the range of what this thread reads of the row. */
+template <class T> __device__ __forceinline__ void finish_row(const T *x, int n, const Range &r, float mine, bool filled, const Settings &set, int32_t *id, float *prob, Shared &s) {
+    const Grid g(r, set.t, n);
+    const Holds holds = holds_for(set);
+    bool by_value = r.max == -kMinusInf; /* several infinities */
+    if (!by_value) {
+        /* The k-th largest of the threads' own largest logits is not above the k-th of all. For a k that is small beside the threads it is
+         * close below (of 128256 logits and k = 512 some 700 are as large), and the pass that counts all tokens into bins is saved. */
+        bool counted = false;
+        if (!filled) {
+            if (by_largest(set)) {
+                if (is_there(mine)) into_bin(mine, g, true, false, s);
+                __syncthreads();
+                sum_bins(g, holds, s);
+                counted = s.count[kLastBin] >= (uint32_t)set.k;
+                __syncthreads();
+                if (!counted) clear_bins(s);
+                __syncthreads();
+            }
+            if (!counted) fill_bins(x, 0, n, g, holds, s);
+            __syncthreads();
+        }
+        if (!counted) sum_bins(g, holds, s);
+        const Wanted w = wanted_bins(g, set, holds, s);
+        if (counted) {
+            /* and only what those threads read whose largest logit is wanted is looked at again: their vectors, dealt to all threads (for
+             * k = 40 some 720 vectors of 16032; a pass over all of them takes 12 us where all compute units make one) */
+            uint32_t *of = reinterpret_cast<uint32_t *>(s.sorted);
+            const Bounds bounds(g, w);
+            if (mine >= bounds.low0) of[atomicAdd(&s.digit, 1u)] = threadIdx.x;
+            __syncthreads();
+            const Vectors<T> vec(x, 0, n);
+            const int rounds = (vec.all + kThreads - 1) / kThreads, tasks = uniform((int)s.digit) * rounds;
+            for (int q = threadIdx.x; q < tasks; q += kThreads) {
+                const int i = (int)of[q / rounds] + q % rounds * kThreads;
+                const Vec<T> v = vec.load(i);
+#pragma unroll
+                for (int j = 0; j < kPer<T>; j++)
+                    if (bounds(to_f32(v.v[j]))) if_wanted(to_f32(v.v[j]), vec.index(i) + j, g, w, [&](uint64_t e) { add_to_list(e, s); });
+            }
+        } else {
+            for_each_wanted(x, 0, n, g, w, [&](uint64_t e) { add_to_list(e, s); });
+        }
+        __syncthreads();
+        const uint32_t listed = uniform(s.n_list);
+        by_value = listed > kListed;
+        if (!by_value) pick_from_list((int)listed, g, set, w, id, prob, s);
+    }
+    if (by_value) sample_by_value(x, n, set, Weights{r.max, 1.0 / (double)set.t, 0.0}, id, prob, s);
+}
+
+/* a row by one workgroup */
+template <class T> __device__ __forceinline__ void whole_row(const T *x, int n, const Settings &set, int32_t *id, float *prob, Shared &s) {
     const Range mine = range_of_share(x, 0, n), r = range_of_workgroup(mine, s);
-    if (!is_there(r.max)) return nothing_there(id, prob);
     if (threadIdx.x == 0) s.best = (uint32_t)n, s.n_list = 0, s.digit = 0;
     clear_bins(s);
     __syncthreads();
+    if (!is_there(r.max)) return nothing_there(id, prob);
     if (takes_first(set)) {
         if (mine.max == r.max) /* few threads have it */
             for_each_of(x, 0, n, [&](float v) { return v == r.max; }, [&](float, int i) { atomicMin(&s.best, (uint32_t)i); });
@@ -800,100 +850,51 @@ template <class T> __global__ void __launch_bounds__(kThreads) sample_row_kernel
         }
         return;
     }
-    if (r.max == -kMinusInf) return sample_by_value(x, n, set, Weights{r.max, 1.0 / (double)set.t, 0.0}, id, prob, s);
-    const Grid g(r, set.t, n);
-    const Holds holds = holds_for(set);
-    /* The k-th largest of the threads' own largest logits is not above the k-th of all. For a k that is small beside the threads it is close
-     * below (of 128256 logits and k = 512 some 700 are as large), and the pass that counts all tokens into bins is saved. */
-    bool counted = false;
-    if (set.k > 0 && set.k <= kFewOfThreads) {
-        if (is_there(mine.max)) {
-            const double at = g.place(mine.max);
-            if (at < kBins - 1) atomicAdd(&s.count[(int)at], 1u);
-        }
-        __syncthreads();
-        sum_bins(g, holds, s);
-        counted = s.count[kLastBin] >= (uint32_t)set.k;
-        __syncthreads();
-        if (!counted) clear_bins(s);
-        __syncthreads();
-    }
-    if (!counted) {
-        fill_bins(x, 0, n, g, holds, s);
-        __syncthreads();
-        sum_bins(g, holds, s);
-    }
-    const Wanted w = wanted_bins(g, set, holds, s);
-    auto list = [&](uint64_t e) {
-        const uint32_t at = atomicAdd(&s.n_list, 1u);
-        if (at < kListed) s.list[at] = e;
-    };
-    if (counted) {
-        /* only what the threads read whose largest logit is wanted: their vectors, dealt to all threads (for k = 40 some 720 vectors of
-         * 16032; a pass over all of them takes 12 us) */
-        uint32_t *of = reinterpret_cast<uint32_t *>(s.sorted);
-        const Bounds bounds(g, w);
-        if (mine.max >= bounds.low0) of[atomicAdd(&s.digit, 1u)] = threadIdx.x;
-        __syncthreads();
-        const Vectors<T> vec(x, 0, n);
-        const int rounds = (vec.all + kThreads - 1) / kThreads, tasks = uniform((int)s.digit) * rounds;
-        for (int q = threadIdx.x; q < tasks; q += kThreads) {
-            const int i = (int)of[q / rounds] + q % rounds * kThreads;
-            const Vec<T> v = vec.load(i);
-#pragma unroll
-            for (int j = 0; j < kPer<T>; j++)
-                if (bounds(to_f32(v.v[j]))) if_wanted(to_f32(v.v[j]), vec.index(i) + j, g, w, list);
-        }
-    } else {
-        for_each_wanted(x, 0, n, g, w, list);
-    }
-    __syncthreads();
-    const uint32_t listed = uniform(s.n_list);
-    if (listed > kListed) return sample_by_value(x, n, set, Weights{r.max, g.per_t, 0.0}, id, prob, s);
-    pick_from_list((int)listed, g, set, w, id, prob, s);
+    finish_row(x, n, r, mine.max, false, set, id, prob, s);
 }
 
-/* ------------------------------------------------------------------ few sequences: several workgroups for each, four launches */
+template <class T> __global__ void __launch_bounds__(kThreads) sample_row_kernel(const T *__restrict__ logits, SampleCall c) {
+    __shared__ Shared s;
+    const int seq = blockIdx.x;
+    whole_row(logits + (size_t)seq * c.ld, c.n_vocab, settings_of(c, seq), c.ids + seq, c.probs ? c.probs + seq : nullptr, s);
+}
 
-/* What a sequence keeps in the workspace. A part of the row is a workgroup's, 256 groups of its threads have a largest logit each. */
-struct Part { float max, min; int first; uint32_t unused; };
-constexpr int kGroups = 256, kMaxParts = 16;
-struct Row {
+/* ------------------------------------------------------------------ few sequences
+ * Rows that have to be put into bins, by several workgroups each: their ranges, their bins, and the rest by one workgroup, in a launch
+ * each. Other rows are the first launch's first workgroup's alone. (What comes after the bins was spread over the workgroups too, the
+ * list by one launch and the pick by another, or by the last to finish: what a launch gains over 12 us it loses by starting, and fences
+ * between the dies' L2s take 40 to 60 us where 32 sequences meet them.) */
+
+constexpr int kMaxParts = 16;
+struct Part { float max, min; };
+struct Row { /* of the workspace */
     uint64_t weight[kBins];
-    uint64_t list[kListed];
     uint32_t count[kBins];
-    Wanted wanted;
-    uint32_t n_list, listed; /* entries; whether the groups' largest logits made the list */
     Part part[kMaxParts];
-    float group[kMaxParts][kGroups];
+    uint64_t unused[16];
 };
-constexpr size_t kRowBytes = (sizeof(Row) + 255) / 256 * 256;
-__device__ __forceinline__ Row *row_of(const SampleCall &c, int seq) { return reinterpret_cast<Row *>(static_cast<uint8_t *>(c.workspace) + (size_t)seq * kRowBytes); }
-__device__ __forceinline__ bool by_largest(const Settings &s) { return s.k > 1 && s.k <= kFewOfThreads; }
+static_assert(sizeof(Row) % 256 == 0, "rows start on 256 bytes");
+__device__ __forceinline__ bool by_parts(const Settings &s) { return !takes_first(s) && !by_largest(s); }
 struct Share { int lo, hi; };
 __device__ __forceinline__ Share share_of(int n, int parts, int part) {
     const int per = ((n + parts - 1) / parts + 63) & ~63; /* (rows on 16 bytes stay so) */
     return {min(part * per, n), min((part + 1) * per, n)};
 }
 
-/* the range of each part, its groups' largest logits, and empty bins */
 template <class T> __global__ void __launch_bounds__(kThreads) sample_parts_kernel(const T *__restrict__ logits, SampleCall c, int parts) {
     __shared__ Shared s;
     const int seq = blockIdx.x / (unsigned)parts, part = blockIdx.x - seq * parts;
     const T *x = logits + (size_t)seq * c.ld;
-    Row *row = row_of(c, seq);
     const Settings set = settings_of(c, seq);
-    const Share sh = share_of(c.n_vocab, parts, part);
+    if (!by_parts(set)) {
+        if (part == 0) whole_row(x, c.n_vocab, set, c.ids + seq, c.probs ? c.probs + seq : nullptr, s);
+        return;
+    }
+    Row *row = static_cast<Row *>(c.workspace) + seq;
     for (int i = part * kThreads + threadIdx.x; i < kBins; i += parts * kThreads) row->weight[i] = 0, row->count[i] = 0;
-    if (part == 0 && threadIdx.x == 0) row->n_list = 0, row->listed = 0;
-    if (threadIdx.x == 0) s.best = (uint32_t)c.n_vocab;
-    const Range mine = range_of_share(x, sh.lo, sh.hi), r = range_of_workgroup(mine, s);
-    const float group = fmaxf(fmaxf(mine.max, __shfl_xor(mine.max, 1, 64)), fmaxf(__shfl_xor(mine.max, 2, 64), __shfl_xor(mine.max, 3, 64)));
-    if ((threadIdx.x & 3) == 0) row->group[part][threadIdx.x >> 2] = group;
-    if (takes_first(set) && is_there(r.max) && mine.max == r.max)
-        for_each_of(x, sh.lo, sh.hi, [&](float v) { return v == r.max; }, [&](float, int i) { atomicMin(&s.best, (uint32_t)i); });
-    __syncthreads();
-    if (threadIdx.x == 0) row->part[part] = {r.max, r.min, (int)s.best, 0};
+    const Share sh = share_of(c.n_vocab, parts, part);
+    const Range r = range_of_workgroup(range_of_share(x, sh.lo, sh.hi), s);
+    if (threadIdx.x == 0) row->part[part] = {r.max, r.min};
 }
 
 /* the row's range, in every thread: a lane loads one part's */
@@ -908,73 +909,19 @@ __device__ Range range_of_parts(const Row *row, int parts) {
     return {uniform(r.max), uniform(r.min)};
 }
 
-/* this part's tokens of the wanted bins behind those of the others in the row's list; s.n_list is 0 */
-template <class T> __device__ void list_share(const T *x, const Share &sh, const Grid &g, const Wanted &w, Row *row, Shared &s) {
-    for_each_wanted(x, sh.lo, sh.hi, g, w, [&](uint64_t e) {
-        const uint32_t at = atomicAdd(&s.n_list, 1u);
-        if (at < kListed) s.list[at] = e;
-    });
-    __syncthreads();
-    /* (one atomic per workgroup: a thousand of them on one address take 100 us) */
-    const uint32_t mine = s.n_list;
-    if (threadIdx.x == 0) s.best = mine ? atomicAdd(&row->n_list, mine) : 0;
-    __syncthreads();
-    for (uint32_t i = threadIdx.x; i < min(mine, (uint32_t)kListed) && s.best + i < kListed; i += kThreads) row->list[s.best + i] = s.list[i];
-}
-
-/* The first token where that is the pick. The list where the groups' largest logits bound the k-th (as the threads' do in the kernel of
- * one workgroup); else each part's tokens into the bins. */
 template <class T> __global__ void __launch_bounds__(kThreads) sample_bins_kernel(const T *__restrict__ logits, SampleCall c, int parts) {
     __shared__ Shared s;
-    const int seq = blockIdx.x / (unsigned)parts, part = blockIdx.x - seq * parts, n = c.n_vocab;
-    const T *x = logits + (size_t)seq * c.ld;
-    Row *row = row_of(c, seq);
+    const int seq = blockIdx.x / (unsigned)parts, part = blockIdx.x - seq * parts;
     const Settings set = settings_of(c, seq);
+    if (!by_parts(set)) return;
+    Row *row = static_cast<Row *>(c.workspace) + seq;
     const Range r = range_of_parts(row, parts);
-    if (!is_there(r.max) || takes_first(set)) {
-        if (part == 0 && threadIdx.x == 0) {
-            int first = n;
-            for (int i = 0; i < parts; i++)
-                if (row->part[i].max == r.max) first = min(first, row->part[i].first);
-            c.ids[seq] = is_there(r.max) ? first : -1;
-            if (c.probs) c.probs[seq] = is_there(r.max) ? 1.0f : 0.0f;
-        }
-        return;
-    }
-    if (r.max == -kMinusInf) {
-        if (part == 0) sample_by_value(x, n, set, Weights{r.max, 1.0 / (double)set.t, 0.0}, c.ids + seq, c.probs ? c.probs + seq : nullptr, s);
-        return;
-    }
-    const Grid g(r, set.t, n);
-    const Holds holds = holds_for(set);
-    const Share sh = share_of(n, parts, part);
+    if (!is_there(r.max) || r.max == -kMinusInf) return;
+    const Grid g(r, set.t, c.n_vocab);
     clear_bins(s);
-    if (threadIdx.x == 0) s.n_list = 0;
     __syncthreads();
-    if (by_largest(set)) {
-        constexpr int kEach = kMaxParts * kGroups / kThreads;
-        const float *largest = &row->group[0][0];
-        float v[kEach];
-#pragma unroll
-        for (int j = 0; j < kEach; j++) v[j] = largest[min((int)threadIdx.x + j * kThreads, parts * kGroups - 1)];
-#pragma unroll
-        for (int j = 0; j < kEach; j++) {
-            const double at = g.place(v[j]);
-            if ((int)threadIdx.x + j * kThreads < parts * kGroups && is_there(v[j]) && at < kBins - 1) atomicAdd(&s.count[(int)at], 1u);
-        }
-        __syncthreads();
-        sum_bins(g, holds, s);
-        if (s.count[kLastBin] >= (uint32_t)set.k) {
-            const Wanted w = wanted_bins(g, set, holds, s);
-            list_share(x, sh, g, w, row, s);
-            if (part == 0 && threadIdx.x == 0) row->wanted = w, row->listed = 1;
-            return;
-        }
-        __syncthreads();
-        clear_bins(s);
-        __syncthreads();
-    }
-    fill_bins(x, sh.lo, sh.hi, g, holds, s);
+    const Share sh = share_of(c.n_vocab, parts, part);
+    fill_bins(logits + (size_t)seq * c.ld, sh.lo, sh.hi, g, holds_for(set), s);
     __syncthreads();
     for (int i = threadIdx.x; i < kBins; i += kThreads) {
         if (const uint64_t w = s.weight[i]) atomicAdd((unsigned long long *)&row->weight[i], (unsigned long long)w);
@@ -982,52 +929,30 @@ template <class T> __global__ void __launch_bounds__(kThreads) sample_bins_kerne
     }
 }
 
-/* the list of the wanted bins of a row in bins */
-template <class T> __global__ void __launch_bounds__(kThreads) sample_list_kernel(const T *__restrict__ logits, SampleCall c, int parts) {
+template <class T> __global__ void __launch_bounds__(kThreads) sample_finish_kernel(const T *__restrict__ logits, SampleCall c, int parts) {
     __shared__ Shared s;
-    const int seq = blockIdx.x / (unsigned)parts, part = blockIdx.x - seq * parts, n = c.n_vocab;
+    const int seq = blockIdx.x;
     const Settings set = settings_of(c, seq);
-    Row *row = row_of(c, seq);
-    if (takes_first(set) || row->listed) return;
+    if (!by_parts(set)) return;
+    const Row *row = static_cast<const Row *>(c.workspace) + seq;
+    const T *x = logits + (size_t)seq * c.ld;
+    int32_t *id = c.ids + seq;
+    float *prob = c.probs ? c.probs + seq : nullptr;
     const Range r = range_of_parts(row, parts);
-    if (!is_there(r.max) || r.max == -kMinusInf) return;
-    const Grid g(r, set.t, n);
-    const Holds holds = holds_for(set);
+    if (!is_there(r.max)) return nothing_there(id, prob);
     for (int i = threadIdx.x; i < kBins; i += kThreads) s.weight[i] = row->weight[i], s.count[i] = row->count[i];
     if (threadIdx.x == 0) s.n_list = 0;
     __syncthreads();
-    sum_bins(g, holds, s);
-    const Wanted w = wanted_bins(g, set, holds, s);
-    if (part == 0 && threadIdx.x == 0) row->wanted = w;
-    list_share(logits + (size_t)seq * c.ld, share_of(n, parts, part), g, w, row, s);
+    finish_row(x, c.n_vocab, r, 0.0f, true, set, id, prob, s);
 }
 
-/* and the pick from it: a launch of its own, since waiting for the other parts' entries inside the one before takes fences between the
- * dies' L2s, 40 to 60 us where 32 sequences meet them */
-template <class T> __global__ void __launch_bounds__(kThreads) sample_pick_kernel(const T *__restrict__ logits, SampleCall c, int parts) {
-    __shared__ Shared s;
-    const int seq = blockIdx.x, n = c.n_vocab;
-    const Settings set = settings_of(c, seq);
-    if (takes_first(set)) return;
-    Row *row = row_of(c, seq);
-    const uint32_t listed = row->n_list;
-    const Wanted w = row->wanted;
-    const Range r = range_of_parts(row, parts);
-    if (!is_there(r.max) || r.max == -kMinusInf) return;
-    const Grid g(r, set.t, n);
-    int32_t *id = c.ids + seq;
-    float *prob = c.probs ? c.probs + seq : nullptr;
-    if (listed > kListed) return sample_by_value(logits + (size_t)seq * c.ld, n, set, Weights{r.max, g.per_t, 0.0}, id, prob, s);
-    for (int i = threadIdx.x; i < (int)listed; i += kThreads) s.list[i] = row->list[i];
-    if (listed > kOneWave) __syncthreads();
-    else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); /* (wave 0 loaded, sorts and picks) */
-    pick_from_list((int)listed, g, set, w, id, prob, s);
-}
-
-/* workgroups per sequence: 1 = the kernel of one, else the four launches */
+/* Workgroups per sequence: 1 = the kernel of one, else the three launches. Of 128256 bf16 logits, rows that need bins (no top_k) take 51, 53
+ * and 57 us by one workgroup each for 1, 4 and 16 sequences, 36, 39 and 47 by parts; rows that do not (top_k 40) 20 and 24 to 27, for the
+ * two launches more; 16 sequences with settings of all kinds 57 and 70. Of 32003 logits a row takes 24 us at most by one. The rule follows
+ * sizes alone, as the settings are on the GPU. */
 int parts_for(int n_seq, int n_vocab) {
-    if (n_seq > 64 || n_vocab < 16384) return 1;
-    return n_vocab < 4096 * kMaxParts ? n_vocab / 4096 : kMaxParts;
+    if (n_seq > 8 || n_vocab < 65536) return 1;
+    return kMaxParts;
 }
 
 template <class T> hipError_t sample(const SampleCall &c) {
@@ -1038,8 +963,7 @@ template <class T> hipError_t sample(const SampleCall &c) {
     } else {
         sample_parts_kernel<T><<<c.n_seq * parts, kThreads, 0, c.stream>>>(x, c, parts);
         sample_bins_kernel<T><<<c.n_seq * parts, kThreads, 0, c.stream>>>(x, c, parts);
-        sample_list_kernel<T><<<c.n_seq * parts, kThreads, 0, c.stream>>>(x, c, parts);
-        sample_pick_kernel<T><<<c.n_seq, kThreads, 0, c.stream>>>(x, c, parts);
+        sample_finish_kernel<T><<<c.n_seq, kThreads, 0, c.stream>>>(x, c, parts);
     }
     return hipGetLastError();
 }
@@ -1048,7 +972,7 @@ template <class T> hipError_t sample(const SampleCall &c) {
 
 size_t sample_workspace_bytes(int n_seq, int n_vocab) {
     const int parts = parts_for(n_seq, n_vocab);
-    return parts == 1 ? 0 : (size_t)n_seq * kRowBytes;
+    return parts == 1 ? 0 : (size_t)n_seq * sizeof(Row);
 }
 
 hipError_t launch_sample(uint32_t type, const SampleCall &c) {

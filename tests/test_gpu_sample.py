@@ -85,7 +85,7 @@ def random_settings(rng, n_seq):
 @pytest.mark.parametrize("type_id", [F32, F16, BF16])
 @pytest.mark.parametrize("n_seq,n,pad", [(1, 1, 0), (3, 2, 1), (5, 7, 0), (9, 63, 0), (4, 64, 3), (7, 65, 0), (40, 1000, 0), (12, 1025, 7), (33, 4097, 0), (300, 500, 0), (2, 32003, 0),
                                          (3, 32768, 64), (1, 151936, 0), (5, 128256, 8),
-                                         (64, 16384, 0), (65, 16385, 3), (20, 16383, 0), (66, 70000, 0)])
+                                         (8, 65536, 0), (9, 65536, 3), (20, 16383, 0), (66, 70000, 0), (8, 65541, 1)])
 def test_picks(type_id, n_seq, n, pad):
     rng = np.random.default_rng(n_seq * 1000 + n)
     x = np.pad(random_logits(rng, n_seq, n), ((0, 0), (0, pad)), constant_values=99.0)  # what lies behind a row is larger than all of it
@@ -96,28 +96,28 @@ def test_picks(type_id, n_seq, n, pad):
 
 @pytest.mark.parametrize("name,value", [("k", 5), ("k", 40), ("k", 128), ("k", 129), ("k", 512), ("k", 600), ("k", 1024), ("k", 1025), ("k", 5000), ("p", 0.9), ("p", 0.5), ("p", 0.0), ("p", -1.0), ("m", 0.05), ("m", 1.0), ("m", 2.0), ("t", 0.0), ("t", -1.0),
                                         ("t", 100.0), ("t", 1e-3), ("t", np.inf), ("t", np.nan), ("p", np.nan), ("m", np.nan), ("k", -3)])
-@pytest.mark.parametrize("n_seq,n", [(16, 5000), (16, 20000), (70, 20000)])  # one workgroup per sequence, several, and one again
+@pytest.mark.parametrize("n_seq,n", [(16, 5000), (8, 66000), (70, 20000)])  # by one workgroup per sequence, by several, and by one
 def test_one_setting(n_seq, n, name, value):
     rng = np.random.default_rng(11)
     compare(F32, random_logits(rng, n_seq, n), rng.random(n_seq), **{name: [value] * n_seq})
 
 
-@pytest.mark.parametrize("n", [50, 3000, 40000])
-def test_equal_logits(n):
+@pytest.mark.parametrize("rows,n", [(24, 50), (24, 3000), (24, 40000), (8, 66000)])
+def test_equal_logits(rows, n):
     """equal tokens: the lower index first, wherever a cut falls between them"""
     rng = np.random.default_rng(n)
-    few = rng.integers(0, 4, (24, n)).astype(np.float64)  # four values
-    flat = np.full((24, n), -3.25)
-    zeros = np.where(rng.random((24, n)) < 0.5, 0.0, -0.0)
+    few = rng.integers(0, 4, (rows, n)).astype(np.float64)  # four values
+    flat = np.full((rows, n), -3.25)
+    zeros = np.where(rng.random((rows, n)) < 0.5, 0.0, -0.0)
     for x in (few, flat, zeros):
         for type_id in (F32, BF16):
-            u = rng.random(24)
+            u = rng.random(rows)
             compare(type_id, x, u)
-            compare(type_id, x, u, **random_settings(rng, 24))
-            compare(type_id, x, u, k=rng.integers(2, n + 5, 24))
+            compare(type_id, x, u, **random_settings(rng, rows))
+            compare(type_id, x, u, k=rng.integers(2, n + 5, rows))
 
 
-@pytest.mark.parametrize("n", [3001, 20011])
+@pytest.mark.parametrize("n", [3001, 66001])
 def test_masks(n):
     """tokens that are ruled out by -infinity or NaN, or pushed down to the type's lowest value; rows of which nothing is left"""
     rng = np.random.default_rng(5)
@@ -138,10 +138,11 @@ def test_masks(n):
     x[12] = np.where(rng.random(n) < 0.5, np.finfo(np.float32).max, np.finfo(np.float32).min)
     x[13, :] = 1e-40  # subnormal logits
     x[13, 7] = 2e-40
-    u = rng.random(14)
-    compare(F32, x, u)
-    for _ in range(4):
-        compare(F32, x, rng.random(14), **random_settings(rng, 14))
+    for rows in (slice(0, 14), slice(0, 7), slice(7, 14)):  # the halves by several workgroups per row where rows are long
+        m = len(x[rows])
+        compare(F32, x[rows], rng.random(m))
+        for _ in range(4):
+            compare(F32, x[rows], rng.random(m), **random_settings(rng, m))
     lowest = random_logits(rng, 4, n)
     lowest[:, 20:] = -65504.0
     compare(F16, lowest, rng.random(4), p=[0.9] * 4)
