@@ -330,12 +330,14 @@ template <class T> __device__ __forceinline__ Range range_of_share(const T *x, i
 }
 
 /* the bins of a row whose largest logit is finite */
+constexpr double kTicks = 4503599627370496.0; /* 2^52 */
 struct Grid {
     float max;
     double per_t;  /* 1 / T */
     double scale;  /* bins per unit of logits */
     double step;   /* a bin in units of the exponent: at most 1/64 */
     double unit, per_unit; /* 2^bits: of the sums of exp(offset); its inverse */
+    double c1, c2, c3, c4; /* unit exp(-step f) in powers of f */
     __device__ Grid(const Range &r, float t, int n) : max(r.max), per_t(1.0 / (double)t) {
         const double span = (double)r.max - (double)r.min;
         scale = fmax(64.0 * per_t, span > 0.0 ? 2040.0 / span : 0.0);
@@ -347,23 +349,32 @@ struct Grid {
         unit = (double)(1ull << bits);
         max = uniform(max), per_t = uniform(per_t), scale = uniform(scale), step = uniform(step);
         per_unit = 1.0 / unit;
+        c1 = -step * unit, c2 = 0.5 * step * step * unit, c3 = -step * step * step * unit / 6, c4 = step * step * step * step * unit / 24;
     }
-    /* in bins from the largest, which is at 0; never falls from a logit to a smaller one. 2047 and more is not counted, nor what
-     * -infinity (infinity) and NaN (NaN) give */
-    __device__ __forceinline__ double place(float v) const { return ((double)max - (double)v) * scale; }
-    /* exp(centre of the bin - place), by a polynomial of degree 4 (2.4e-13 at the bin's edge, and the errors of its two halves have
-     * opposite signs), as an integer of 1 / unit: the last of the sums rounds at 2^52, whose lower bits are that integer */
-    __device__ __forceinline__ uint64_t offset_weight(double place) const {
-        const double g = fma(-__builtin_amdgcn_fract(place), step, 0.5 * step);
-        double e = fma(g, unit / 24, unit / 6);
-        e = fma(e, g, unit / 2);
-        e = fma(e, g, unit);
-        e = fma(e, g, unit + 4503599627370496.0);
+    /* The bin of a value is its distance from the largest in bins, rounded: the sum with 2^52 rounds at 1 and holds it in its lower half.
+     * One rounding, so that it never falls from a logit to a smaller one. NaN where the value is; infinite for -infinity. */
+    __device__ __forceinline__ double distance(float v) const { return (double)max - (double)v; }
+    __device__ __forceinline__ double ticks(double distance) const { return fma(distance, scale, kTicks); }
+    static __device__ __forceinline__ bool counts(double ticks) { return ticks < kTicks + (kBins - 1); }
+    static __device__ __forceinline__ int bin(double ticks) { return (int)__double_as_longlong(ticks); }
+    __device__ __forceinline__ int bin_of(float v) const { /* kBins: not counted */
+        const double t = ticks(distance(v));
+        return counts(t) ? bin(t) : kBins;
+    }
+    /* exp(centre of the bin - distance), by a polynomial of degree 4 (2.4e-13 at the bin's edge), as an integer of 1 / unit: the last of
+     * the sums rounds as above. (Eight 64-bit operations; with the conversions to an integer and back, which take four times an
+     * addition, a pass took a quarter longer.) */
+    __device__ __forceinline__ uint64_t offset_weight(double distance, double ticks) const {
+        const double f = fma(distance, scale, kTicks - ticks); /* from the centre, in bins */
+        double e = fma(f, c4, c3);
+        e = fma(e, f, c2);
+        e = fma(e, f, c1);
+        e = fma(e, f, unit + kTicks);
         return (uint64_t)__double_as_longlong(e) & 0x000FFFFFFFFFFFFFull;
     }
-    /* floats below (above) every value of place `at` and less (and more) */
-    __device__ float value_below(int at) const { return __double2float_rd((double)max - (double)at / scale * (1.0 + 1e-9)); }
-    __device__ float value_above(int at) const { return __double2float_ru((double)max - (double)at / scale * (1.0 - 1e-9)); }
+    /* floats below (above) every value of the bins up to (from) `bin` */
+    __device__ float value_below(int bin) const { return __double2float_rd((double)max - ((double)bin + 1.0) / scale); }
+    __device__ float value_above(int bin) const { return __double2float_ru((double)max - ((double)bin - 1.0) / scale); }
     __device__ double weight(float v) const { return exp(((double)v - (double)max) * per_t); }
 };
 constexpr int kLastBin = kBins - 2;
@@ -373,11 +384,10 @@ struct Holds { bool counts, weights; };
 __device__ __forceinline__ Holds holds_for(const Settings &s) { return {s.k > 0, s.k <= 0 || s.k > kTopList}; }
 
 __device__ __forceinline__ void into_bin(float v, const Grid &g, bool counts, bool weights, Shared &s) {
-    const double at = g.place(v);
-    if (!(at < kBins - 1)) return;
-    const int bin = (int)at;
-    if (weights) atomicAdd((unsigned long long *)&s.weight[bin], (unsigned long long)g.offset_weight(at));
-    if (counts) atomicAdd(&s.count[bin], 1u);
+    const double d = g.distance(v), t = g.ticks(d);
+    if (!g.counts(t)) return;
+    if (weights) atomicAdd((unsigned long long *)&s.weight[g.bin(t)], (unsigned long long)g.offset_weight(d, t));
+    if (counts) atomicAdd(&s.count[g.bin(t)], 1u);
 }
 template <class T> __device__ __forceinline__ void fill_bins(const T *x, int lo, int hi, const Grid &g, const Holds &h, Shared &s) {
     if (!h.weights) for_each(x, lo, hi, [&](float v, int) { into_bin(v, g, true, false, s); });
@@ -389,8 +399,8 @@ template <class T> __device__ __forceinline__ void fill_bins(const T *x, int lo,
 __device__ void sum_bins(const Grid &g, const Holds &h, Shared &s) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, b = 2 * threadIdx.x;
     if (h.weights) {
-        const double a0 = (double)s.weight[b] * g.per_unit * exp(-((double)b + 0.5) * g.step);
-        const double a1 = b + 1 > kLastBin ? 0.0 : (double)s.weight[b + 1] * g.per_unit * exp(-((double)b + 1.5) * g.step);
+        const double a0 = (double)s.weight[b] * g.per_unit * exp(-(double)b * g.step);
+        const double a1 = b + 1 > kLastBin ? 0.0 : (double)s.weight[b + 1] * g.per_unit * exp(-((double)b + 1.0) * g.step);
         double run = a0 + a1;
         for (int off = 1; off < 64; off <<= 1) {
             const double o = shfl_up_f64(run, off);
@@ -553,8 +563,8 @@ struct Bounds {
             if (joins) end = max(end, w.run[r].hi);
             else start = min(start, w.run[r].lo), last = max(last, w.run[r].hi);
         }
-        low0 = uniform(g.value_below(end + 1)), high0 = uniform(w.run[0].lo == 0 ? g.max : g.value_above(w.run[0].lo));
-        low1 = uniform(start < kNowhere ? g.value_below(last + 1) : -kMinusInf), high1 = uniform(start < kNowhere ? g.value_above(start) : kMinusInf);
+        low0 = uniform(g.value_below(end)), high0 = uniform(w.run[0].lo == 0 ? g.max : g.value_above(w.run[0].lo));
+        low1 = uniform(start < kNowhere ? g.value_below(last) : -kMinusInf), high1 = uniform(start < kNowhere ? g.value_above(start) : kMinusInf);
     }
     __device__ __forceinline__ bool operator()(float v) const { return (v >= low0 && v <= high0) || (v >= low1 && v <= high1); }
 };
@@ -564,8 +574,8 @@ __device__ __forceinline__ void add_to_list(uint64_t e, Shared &s) {
 }
 /* fn(entry) for the tokens of the wanted bins */
 template <class F> __device__ __forceinline__ void if_wanted(float v, int i, const Grid &g, const Wanted &w, F fn) {
-    const double at = g.place(v);
-    if (at < kBins - 1 && is_wanted((int)at, w)) fn(entry_of(v, i));
+    const int bin = g.bin_of(v);
+    if (bin < kBins && is_wanted(bin, w)) fn(entry_of(v, i));
 }
 template <class T, class F> __device__ __forceinline__ void for_each_wanted(const T *x, int lo, int hi, const Grid &g, const Wanted &w, F fn) {
     const Bounds bounds(g, w);
@@ -650,7 +660,7 @@ template <int WAVES, int E> __device__ __forceinline__ void pick_with(int n, con
         const bool there = i0 + e < n;
         const float value = there ? entry_value(s.list[i0 + e]) : 0.0f;
         wt[e] = there ? g.weight(value) : 0.0;
-        bin[e] = there ? (int)g.place(value) : kBins;
+        bin[e] = there ? g.bin_of(value) : kBins;
         weight[i0 + e] = wt[e];
         run += wt[e];
     }
@@ -704,7 +714,7 @@ template <int WAVES, int E> __device__ __forceinline__ void pick_with(int n, con
     double sums[E];
 #pragma unroll
     for (int e = 0; e < E; e++) sums[e] = i0 + e < n ? sum_to(i0 + e, bin[e]) : 0.0;
-    auto sum_at = [&](int i) { return sum_to(i, (int)g.place(entry_value(s.list[i]))); };
+    auto sum_at = [&](int i) { return sum_to(i, g.bin_of(entry_value(s.list[i]))); };
     const Run everywhere = {0, kBins};
     int kept = n; /* list entries from here on are cut off (those between the runs lie on the right side by construction) */
     double total = w.all ? s.run[n - 1] : w.total;
@@ -766,7 +776,7 @@ __device__ void pick_from_list(int n, const Grid &g, const Settings &set, Wanted
         w = wanted_bins(g, set, both, s);
 #pragma unroll
         for (int e = 0; e < kListed / kThreads; e++)
-            if ((int)threadIdx.x + e * kThreads < n && is_wanted((int)g.place(entry_value(entry[e])), w)) s.list[atomicAdd(&s.n_list, 1u)] = entry[e];
+            if ((int)threadIdx.x + e * kThreads < n && is_wanted(g.bin_of(entry_value(entry[e])), w)) s.list[atomicAdd(&s.n_list, 1u)] = entry[e];
         __syncthreads();
         n = uniform((int)s.n_list);
     }
