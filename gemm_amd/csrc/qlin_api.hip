@@ -1537,7 +1537,7 @@ int qlin_sample_dev(uint32_t type, const void *logits, int n_seq, int n_vocab, i
     if (!float_bytes(type)) return fail(QLIN_ERR_TYPE, "logits are F32, F16 or BF16 (got type %u)", type);
     if (int rc = check_float_rows("logits", type, logits, n_seq, n_vocab, ld)) return rc;
     if (n_seq == 0) return QLIN_OK;
-    if (n_vocab == 0) return fail(QLIN_ERR_ARG, "sampling from no tokens");
+    if (n_vocab == 0 || n_vocab > 1 << 30) return fail(QLIN_ERR_ARG, "sampling from %d tokens", n_vocab);
     if (!u || !ids) return fail(QLIN_ERR_ARG, "null pointer");
     for (const void *p : {(const void *)temperature, (const void *)top_k, (const void *)top_p, (const void *)min_p, (const void *)u, (const void *)ids, (const void *)probs})
         if (!aligned(p, 4)) return fail(QLIN_ERR_ARG, "misaligned pointer");

@@ -389,11 +389,12 @@ int qlin_mxfp4_gemm_silu_mul_dev(const void *Wgate, const void *Wup, uint32_t x_
  * probs (may be NULL): the pick's weight divided by the sum of the kept; 1 for the first of the order, 0 for id -1.
  * temperature, top_k, top_p, min_p and u are device arrays of n_seq elements, u of numbers in [0, 1) (a smaller one or NaN counts as
  * 0); each of the first four may be NULL, which is 1, 0, 1 and 0 for every sequence (so is a NaN among top_p and min_p; NaN as a
- * temperature is 0). Several +infinities share the weight among them. Weights are 64-bit exponentials and their sums integers of at
- * most 2^-44 (up to 262144 tokens) of the largest weight: the same call gives the same token, and a token below half a unit is never
- * picked.
+ * temperature is 0). Several +infinities share the weight among them. Weights and sums are 64-bit and do not depend on the order in
+ * which the GPU adds them: the same call gives the same token. A token that weighs less than 2e-14 of the first one (31.9 temperatures
+ * below it) may count as one without weight, which is never picked; a u within about 1e-12 of a border between two tokens may pick either.
+ * n_vocab up to 2^30. Rows of more than a few thousand equal logits, or that hold +infinity, take several times as long as others.
  * workspace: device memory, 256-byte aligned, qlin_sample_workspace_bytes(n_seq, n_vocab) bytes (0: it may be NULL), which holds
- * nothing between calls; calls that share one must be ordered on one stream. */
+ * nothing between calls; calls that share one must be ordered on one stream, and graphs that share one must not run at the same time. */
 size_t qlin_sample_workspace_bytes(int n_seq, int n_vocab);
 int qlin_sample_dev(uint32_t logits_type, const void *logits, int n_seq, int n_vocab, int ld, const float *temperature, const int32_t *top_k,
                     const float *top_p, const float *min_p, const float *u, int32_t *ids, float *probs, void *workspace,

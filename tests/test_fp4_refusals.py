@@ -72,9 +72,9 @@ def test_gate_and_up_refuse_a_missing_operand(lib):
 
 
 @pytest.mark.parametrize("code,change", [
-    (TYPE, dict(type=Q4K)), (ARG, dict(n_seq=-1)), (ARG, dict(n_vocab=-1)), (ARG, dict(n_vocab=0)), (ARG, dict(ld=99)), (ARG, dict(logits=None)), (ARG, dict(logits=P + 2)),
+    (TYPE, dict(type=Q4K)), (ARG, dict(n_seq=-1)), (ARG, dict(n_vocab=-1)), (ARG, dict(n_vocab=0)), (ARG, dict(n_vocab=(1 << 30) + 1, ld=(1 << 31) - 1)), (ARG, dict(ld=99)), (ARG, dict(logits=None)), (ARG, dict(logits=P + 2)),
     (ARG, dict(u=None)), (ARG, dict(ids=None)), (ARG, dict(u=P + 2)), (ARG, dict(ids=P + 1)), (ARG, dict(probs=P + 2)), (ARG, dict(t=P + 2)), (ARG, dict(k=P + 2)), (ARG, dict(p=P + 2)),
-    (ARG, dict(m=P + 2)),
+    (ARG, dict(m=P + 2)), (ARG, dict(n_vocab=100000, ld=100000, ws=None)), (ARG, dict(n_vocab=100000, ld=100000, ws=P + 128)), (ARG, dict(n_vocab=100000, ld=100000, ws_bytes=1000)),
 ])
 def test_sample_refuses(lib, code, change):
     a = dict(dict(type=F32, logits=P, n_seq=4, n_vocab=100, ld=100, t=P, k=P, p=P, m=P, u=P, ids=P, probs=P, ws=P, ws_bytes=1 << 30), **change)
