@@ -12,7 +12,7 @@
  * Four lanes share a block, 8 consecutive elements each, so that a wave reads 512 consecutive elements of a row, 16 bytes per lane
  * and load in 16-bit types. The 4 KB of codes that a workgroup makes pass LDS once: out of the lanes they would go to memory in
  * pieces of 4 bytes. Bound by memory for many rows (4096 x 14336 fp32 to blocks 48 to 59 us, 4.5 to 5.5 TB/s) and by the launch for
- * few (2048 x 4096 bf16 to an operand 6.5 us, 24 x 14336 4).
+ * few (2048 x 4096 bf16 to an operand 6.5 us, 24 x 14336 4). Blocks of 151936 x 4096 to an operand 117 us, 5.7 TB/s (429 by single bytes).
  */
 #include "mxfp4_quant.h"
 
@@ -54,28 +54,28 @@ __global__ void __launch_bounds__(256) operand_kernel(const T *__restrict__ X, u
             *reinterpret_cast<const uint4 *>(scales + threadIdx.x * 16);
 }
 
-/* the same from GGML blocks: codes and exponents are moved, not changed */
+/* the same from GGML blocks: codes and exponents are moved, not changed. A lane loads a block, 16 bytes at any address: sixteen lanes read a
+ * row's 272 bytes */
 __global__ void __launch_bounds__(256) operand_of_blocks_kernel(const uint8_t *__restrict__ W, uint8_t *__restrict__ op, int n_rows, int n_blocks, Shape s) {
-    constexpr int kRow = 16 * kBlockBytes;
-    __shared__ uint8_t raw[16 * kRow];
+    constexpr int kRun = 16 * 4 + 4; /* as in operand_kernel */
+    __shared__ __attribute__((aligned(16))) uint32_t codes[16 * kRun];
     __shared__ __attribute__((aligned(16))) uint8_t scales[kScaleBytes];
     const int group = blockIdx.x / (unsigned)s.quads, quad = blockIdx.x - group * s.quads;
-    const int here = min(16, n_blocks - quad * 16) * kBlockBytes; /* bytes of a row */
-    for (int i = threadIdx.x; i < 16 * kRow; i += 256) {
-        const int r = i / kRow, at = i - r * kRow, row = group * 16 + r;
-        uint8_t v = 0;
-        if (row < n_rows && at < here) v = W[((size_t)row * n_blocks + quad * 16) * kBlockBytes + at];
-        raw[i] = v;
+    const int r = threadIdx.x >> 4, block = threadIdx.x & 15, row = group * 16 + r, n = quad * 16 + block;
+    u32x4 v = {};
+    uint8_t e = 0;
+    if (row < n_rows && n < n_blocks) {
+        const uint8_t *b = W + ((size_t)row * n_blocks + n) * kBlockBytes;
+        e = b[0];
+        __builtin_memcpy(&v, b + 1, 16);
     }
+    *reinterpret_cast<u32x4 *>(codes + block * kRun + r * 4) = v;
+    scales[((block & 3) * 16 + r) * 4 + (block >> 2)] = e;
     __syncthreads();
-    const int r = threadIdx.x & 15, block = threadIdx.x >> 4, tile = quad * 4 + (block >> 2);
-    const uint8_t *b = raw + r * kRow + block * kBlockBytes;
-    u32x4 v;
-    __builtin_memcpy(&v, b + 1, 16);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, tile = quad * 4 + wave;
     if (tile < s.tiles)
-        *reinterpret_cast<u32x4 *>(op + ((size_t)group * s.tiles + tile) * kTileBytes + ((block & 3) * 16 + r) * 16) = v;
-    scales[((block & 3) * 16 + r) * 4 + (block >> 2)] = b[0];
-    __syncthreads();
+        *reinterpret_cast<uint4 *>(op + ((size_t)group * s.tiles + tile) * kTileBytes + lane * 16) =
+            *reinterpret_cast<const uint4 *>(codes + (4 * wave + (lane >> 4)) * kRun + (lane & 15) * 4);
     if (threadIdx.x < 16)
         *reinterpret_cast<uint4 *>(op + s.code_bytes() + ((size_t)group * s.quads + quad) * kScaleBytes + threadIdx.x * 16) =
             *reinterpret_cast<const uint4 *>(scales + threadIdx.x * 16);
