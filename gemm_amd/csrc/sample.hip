@@ -23,10 +23,11 @@
  *   A list that overflows (a bin of more than 2048 tokens: rows of equal logits) leaves the row to sample_by_value, which takes
  * several passes for each cut.
  *
- * What bounds it, 256 rows of 128256 bf16 logits, by the clock in the kernel: without filters 12 us for the first pass (5.5 TB/s), 21 for
+ * What bounds it, 256 rows of 128256 bf16 logits, by the clock in the kernel: without filters 12 us for the first pass (5.5 TB/s), 19 for
  * the bins (14 64-bit vector instructions and an LDS addition per token), 13 to 15 for the list (the row comes from the last-level cache
- * again), 8 for sums, sort and cuts, which are chains of a few hundred instructions; with top_k 40 the first 12, 3.5 for the list, 8 for the
- * rest. A row alone is bound by what one compute unit loads (128256 logits with top_k 20 us, without 36 by several workgroups).
+ * again), 8 for sums, sort and cuts, which are chains of a few hundred instructions; with top_k 40 the first 9, 3.5 for the list, 8 for the
+ * rest. A row alone is bound by what one compute unit loads and executes (16 sequences with top_k 15.9 us, one 19.8 with the two launches
+ * that such a row leaves empty, without top_k 37 by several workgroups).
  */
 #include "qlin_device.h"
 #include "qlin_internal.h"
@@ -254,10 +255,11 @@ template <class T> __device__ __noinline__ void sample_by_value(const T *x, int 
 
 /* ------------------------------------------------------------------ a row by bins */
 
-/* This thread's share of elements lo .. hi - 1 of x, in vectors of 16 bytes from the first to the last address on 16, four loads ahead of
- * their use; an element before or behind those is a vector of its own, whose other places hold NaN. fn(values, index of the first) is
+/* This thread's share of elements lo .. hi - 1 of x, in vectors of 16 bytes from the first to the last address on 16; an element before or
+ * behind those is a vector of its own, whose other places hold NaN. One load ahead of its use: four waves per SIMD cover the rest, and
+ * vectors handed on from register to register are instructions (256 rows without filters 65.5 us, four loads ahead 68). fn(values, index of the first) is
  * called from one place: a workgroup runs most of this file's code once, and what it has not run yet comes from memory, 64 bytes at a
- * time. Unrolled over the four vectors, the pass that lists tokens took 15 us instead of 6, most of it for its own instructions. */
+ * time. Unrolled over four vectors, the pass that lists tokens took 15 us instead of 6, most of it for its own instructions. */
 template <class T> constexpr int kPer = 16 / sizeof(T);
 template <class T> struct alignas(16) Vec { T v[kPer<T>]; };
 template <class T> struct Vectors {
@@ -283,13 +285,13 @@ template <class T, class F> __device__ __forceinline__ void for_vectors(const T 
     constexpr int N = kPer<T>;
     const Vectors<T> vec(x, lo, hi);
     int i = threadIdx.x;
-    Vec<T> a = vec.load(i), b = vec.load(i + kThreads), c = vec.load(i + 2 * kThreads), d = vec.load(i + 3 * kThreads);
+    Vec<T> a = vec.load(i);
 #pragma unroll 1
     for (; i < vec.all; i += kThreads) {
         float v[N];
 #pragma unroll
         for (int j = 0; j < N; j++) v[j] = to_f32(a.v[j]);
-        a = b, b = c, c = d, d = vec.load(i + 4 * kThreads);
+        a = vec.load(i + kThreads);
         fn(v, vec.index(i));
     }
 }
@@ -325,12 +327,35 @@ __device__ __forceinline__ Range range_of_workgroup(Range r, Shared &s) {
     __syncthreads();
     return {uniform(r.max), uniform(r.min)};
 }
-template <class T> __device__ __forceinline__ Range range_of_share(const T *x, int lo, int hi) {
+/* The range of what for_vectors would give this thread; without MIN its largest alone. Four loads ahead, each into the registers that
+ * were just used: one row is bound by its vector instructions here, of which handing vectors on took a third (151936 fp32 logits, top_k
+ * 40: 25.6 -> 22.1 us; eight ahead spill). */
+template <bool MIN, class T> __device__ __forceinline__ Range range_of_share(const T *x, int lo, int hi) {
+    constexpr int kAhead = 4;
+    const Vectors<T> vec(x, lo, hi);
     Range r = {kMinusInf, -kMinusInf};
-    for_each(x, lo, hi, [&](float v, int) {
+    auto take = [&](float v) {
         r.max = fmaxf(r.max, v); /* (NaN is not taken) */
-        r.min = fminf(r.min, is_there(v) ? v : -kMinusInf);
-    });
+        if constexpr (MIN) r.min = fminf(r.min, is_there(v) ? v : -kMinusInf);
+    };
+    const int behind = vec.vecs + ((int)(threadIdx.x - (unsigned)vec.vecs) & (kThreads - 1)); /* of this thread's, the first that is no whole vector */
+    if (behind < vec.all) take(to_f32(x[vec.index(behind)]));
+    int i = threadIdx.x;
+    if (i >= vec.vecs) return r;
+    const Vec<T> *from = reinterpret_cast<const Vec<T> *>(x + vec.first);
+    Vec<T> a[kAhead];
+#pragma unroll
+    for (int d = 0; d < kAhead; d++) a[d] = from[i + d * kThreads < vec.vecs ? i + d * kThreads : i];
+#pragma unroll 1
+    for (; i < vec.vecs; i += kAhead * kThreads) {
+#pragma unroll
+        for (int d = 0; d < kAhead; d++) {
+#pragma unroll
+            for (int j = 0; j < kPer<T>; j++) take(to_f32(a[d].v[j]));
+            const int next = i + (kAhead + d) * kThreads;
+            if (next < vec.vecs) a[d] = from[next]; /* (else the same again, which changes nothing) */
+        }
+    }
     return r;
 }
 
@@ -797,32 +822,21 @@ __device__ __forceinline__ void nothing_there(int32_t *id, float *prob) {
     }
 }
 
-/* A row from its bins, or where `filled` is false from its range, to the pick; `mine` is the range of what this thread reads of the row. */
-template <class T> __device__ __forceinline__ void finish_row(const T *x, int n, const Range &r, float mine, bool filled, const Settings &set, int32_t *id, float *prob, Shared &s) {
-    const Grid g(r, set.t, n);
+/* A row to the pick: from its bins, where they are `filled` or are here; or where the threads' largest logits have been `counted` (`mine` is
+ * this thread's) from those. */
+enum class Bins { empty, filled, counted };
+template <class T> __device__ __forceinline__ void finish_row(const T *x, int n, const Grid &g, float mine, Bins bins, const Settings &set, int32_t *id, float *prob, Shared &s) {
     const Holds holds = holds_for(set);
-    bool by_value = r.max == -kMinusInf; /* several infinities */
+    bool by_value = g.max == -kMinusInf; /* several infinities */
     if (!by_value) {
-        /* The k-th largest of the threads' own largest logits is not above the k-th of all. For a k that is small beside the threads it is
-         * close below (of 128256 logits and k = 512 some 700 are as large), and the pass that counts all tokens into bins is saved. */
-        bool counted = false;
-        if (!filled) {
-            if (by_largest(set)) {
-                if (is_there(mine)) into_bin(mine, g, true, false, s);
-                __syncthreads();
-                sum_bins(g, holds, s);
-                counted = s.count[kLastBin] >= (uint32_t)set.k;
-                __syncthreads();
-                if (!counted) clear_bins(s);
-                __syncthreads();
-            }
-            if (!counted) fill_bins(x, 0, n, g, holds, s);
+        if (bins == Bins::empty) {
+            fill_bins(x, 0, n, g, holds, s);
             __syncthreads();
         }
-        if (!counted) sum_bins(g, holds, s);
+        if (bins != Bins::counted) sum_bins(g, holds, s);
         const Wanted w = wanted_bins(g, set, holds, s);
-        if (counted) {
-            /* and only what those threads read whose largest logit is wanted is looked at again: their vectors, dealt to all threads (for
+        if (bins == Bins::counted) {
+            /* only what those threads read whose largest logit is wanted is looked at again: their vectors, dealt to all threads (for
              * k = 40 some 720 vectors of 16032; a pass over all of them takes 12 us where all compute units make one) */
             uint32_t *of = reinterpret_cast<uint32_t *>(s.sorted);
             const Bounds bounds(g, w);
@@ -845,27 +859,55 @@ template <class T> __device__ __forceinline__ void finish_row(const T *x, int n,
         by_value = listed > kListed;
         if (!by_value) pick_from_list((int)listed, g, set, w, id, prob, s);
     }
-    if (by_value) sample_by_value(x, n, set, Weights{r.max, 1.0 / (double)set.t, 0.0}, id, prob, s);
+    if (by_value) sample_by_value(x, n, set, Weights{g.max, 1.0 / (double)set.t, 0.0}, id, prob, s);
 }
 
 /* a row by one workgroup */
 template <class T> __device__ __forceinline__ void whole_row(const T *x, int n, const Settings &set, int32_t *id, float *prob, Shared &s) {
-    const Range mine = range_of_share(x, 0, n), r = range_of_workgroup(mine, s);
     if (threadIdx.x == 0) s.best = (uint32_t)n, s.n_list = 0, s.digit = 0;
     clear_bins(s);
-    __syncthreads();
-    if (!is_there(r.max)) return nothing_there(id, prob);
-    if (takes_first(set)) {
-        if (mine.max == r.max) /* few threads have it */
-            for_each_of(x, 0, n, [&](float v) { return v == r.max; }, [&](float, int i) { atomicMin(&s.best, (uint32_t)i); });
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            *id = (int32_t)s.best;
-            if (prob) *prob = 1.0f;
+    const bool first = takes_first(set);
+    bool largest = first || by_largest(set), counted = false;
+    float mine = kMinusInf;
+    /* The k-th largest of the threads' own largest logits is not above the k-th of all. For a k that is small beside the threads it is
+     * close below (of 128256 logits and k = 512 some 700 are as large), so that bins of those alone, over the range of those alone, say
+     * what to list. Where fewer than k threads have one within the bins, all tokens are counted. */
+#pragma unroll 1
+    for (;; largest = false) {
+        Range r;
+        if (largest) {
+            mine = range_of_share<false>(x, 0, n).max;
+            r = {mine, is_there(mine) ? mine : -kMinusInf};
+        } else {
+            r = range_of_share<true>(x, 0, n);
         }
-        return;
+        r = range_of_workgroup(r, s);
+        if (!is_there(r.max)) return nothing_there(id, prob);
+        if (first) {
+            if (mine == r.max) /* few threads have it */
+                for_each_of(x, 0, n, [&](float v) { return v == r.max; }, [&](float, int i) { atomicMin(&s.best, (uint32_t)i); });
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                *id = (int32_t)s.best;
+                if (prob) *prob = 1.0f;
+            }
+            return;
+        }
+        const Grid g(r, set.t, n);
+        if (largest && r.max < -kMinusInf) {
+            if (is_there(mine)) into_bin(mine, g, true, false, s);
+            __syncthreads();
+            sum_bins(g, holds_for(set), s);
+            counted = uniform(s.count[kLastBin]) >= (uint32_t)set.k;
+            __syncthreads();
+            if (!counted) {
+                clear_bins(s);
+                __syncthreads();
+                continue;
+            }
+        }
+        return finish_row(x, n, g, mine, counted ? Bins::counted : Bins::empty, set, id, prob, s);
     }
-    finish_row(x, n, r, mine.max, false, set, id, prob, s);
 }
 
 template <class T> __global__ void __launch_bounds__(kThreads) sample_row_kernel(const T *__restrict__ logits, SampleCall c) {
@@ -908,7 +950,7 @@ template <class T> __global__ void __launch_bounds__(kThreads) sample_parts_kern
     Row *row = static_cast<Row *>(c.workspace) + seq;
     for (int i = part * kThreads + threadIdx.x; i < kBins; i += parts * kThreads) row->weight[i] = 0, row->count[i] = 0;
     const Share sh = share_of(c.n_vocab, parts, part);
-    const Range r = range_of_workgroup(range_of_share(x, sh.lo, sh.hi), s);
+    const Range r = range_of_workgroup(range_of_share<true>(x, sh.lo, sh.hi), s);
     if (threadIdx.x == 0) row->part[part] = {r.max, r.min};
 }
 
@@ -958,11 +1000,11 @@ template <class T> __global__ void __launch_bounds__(kThreads) sample_finish_ker
     for (int i = threadIdx.x; i < kBins; i += kThreads) s.weight[i] = row->weight[i], s.count[i] = row->count[i];
     if (threadIdx.x == 0) s.n_list = 0;
     __syncthreads();
-    finish_row(x, c.n_vocab, r, 0.0f, true, set, id, prob, s);
+    finish_row(x, c.n_vocab, Grid(r, set.t, c.n_vocab), 0.0f, Bins::filled, set, id, prob, s);
 }
 
 /* Workgroups per sequence: 1 = the kernel of one, else the three launches. Of 128256 bf16 logits, rows that need bins (no top_k) take 51, 53
- * and 57 us by one workgroup each for 1, 4 and 16 sequences, 36, 39 and 47 by parts; rows that do not (top_k 40) 20 and 24 to 27, for the
+ * and 57 us by one workgroup each for 1, 4 and 16 sequences, 36, 39 and 47 by parts; rows that do not (top_k 40) 16 and 20, for the
  * two launches more; 16 sequences with settings of all kinds 57 and 70. Of 32003 logits a row takes 24 us at most by one. The rule follows
  * sizes alone, as the settings are on the GPU. */
 int parts_for(int n_seq, int n_vocab) {

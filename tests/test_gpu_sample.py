@@ -202,3 +202,28 @@ def test_same_token_every_time(n_seq):
     for _ in range(3):
         again = draw(F32, x, u, **s)
         assert np.array_equal(again[0], first[0]) and np.array_equal(again[1], first[1])
+
+
+@pytest.mark.parametrize("type_id,n", [(F32, 40960), (BF16, 81920), (F16, 20483)])
+def test_top_k_where_few_threads_hold_tokens(type_id, n):
+    """one workgroup's thread reads 16 bytes in every 16 KB: rows whose tokens, or whose large ones, are a few threads'; rows that fall off so
+    fast that the 64th token weighs nothing; the largest tokens at the very ends"""
+    rng = np.random.default_rng(n)
+    per = 4 if type_id == F32 else 8
+    thread = np.arange(n) // per % 1024
+    x = random_logits(rng, 18, n)
+    for s, mine in enumerate(([0], [5], [1023], [0, 512], list(range(40)), list(range(63)))):
+        x[s, ~np.isin(thread, mine)] = -np.inf
+        x[6 + s, np.isin(thread, mine)] += 15.0
+    x[12] = -np.arange(n) * 0.5
+    x[13] = np.arange(n) * 0.5
+    x[14, :3] = x[14, -3:] = 40.0
+    x[15, :] = -np.inf
+    x[15, -1] = 3.0
+    x[16] = np.where(thread == 7, x[16], -50.0)
+    x[17] = 8.0 - 4.0 * (thread == 1)
+    for k in (2, 40, 64, 512):
+        for t in (1.0, 0.05, 30.0):
+            u = rng.random(18)
+            compare(type_id, x, u, t=[t] * 18, k=[k] * 18)
+            compare(type_id, x, u, t=[t] * 18, k=[k] * 18, p=[0.9] * 18, m=[0.02] * 18)
