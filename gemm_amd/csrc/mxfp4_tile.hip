@@ -347,7 +347,8 @@ namespace {
  * itself, `rest` per tile) or side by side (`work`: what they take of the unit from each other); the weights from memory; and the
  * results to it, per MB. Fitted to 229 measured products of 17 to 4096 tokens, 256 to 28672 rows and 256 to 14336 columns, which
  * the smallest estimate's kernel takes 1.6 % longer than the fastest in the mean and 28 % at most (23551 rows x 6912, 169 tokens: 39 us against
- * 30 of a 128 x 256 tile, which was built with two more shapes and left out: together they gain 0.1 %). */
+ * 30 of a 128 x 256 tile, which was built with two more shapes and left out: together they gain 0.1 %). 420 others, F32 and BF16 in
+ * equal parts and rows of any alignment, 2.5 % and 30 % (with costs of results by type and alignment, fitted to them, 2.1 %). */
 struct TileCost { int mb, nb, resident; float start, wait, work, rest, result, weights; };
 constexpr TileCost kTileCosts[] = {{1, 1, 4, 2.888f, 0.123f, 0.097f, 0.552f, 0.108f, 0.163f},
                                    {2, 1, 3, 3.019f, 0.105f, 0.149f, 1.114f, 0.114f, 0.167f},
