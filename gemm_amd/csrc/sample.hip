@@ -13,7 +13,7 @@
  * long as an earlier cut inside a bin leaves a sum open, in which few of them. Only the tokens of those bins are listed and sorted (from
  * one to a few hundred of 150000), and the cuts are made exactly on the list. With top_k of up to 1024 all kept tokens fit the list, and the
  * bins hold counts instead of weights; with top_k of up to 512 what the threads read largest says enough, and the bins hold only that.
- *   One pass over the row finds the largest and smallest logit, one fills the bins, one lists; the second and third read from the
+ *   One pass over the row finds the largest and smallest logit, one fills the bins, one lists; the second and third read from LDS and the
  * caches what the first brought, and a row with top_k up to 512 makes the first alone.
  *
  * Weights and sums are 64-bit: the borders between tokens lie closer to each other than fp32 sums resolve, and the token is to be the
@@ -24,8 +24,8 @@
  * several passes for each cut.
  *
  * What bounds it, 256 rows of 128256 bf16 logits, by the clock in the kernel: without filters 12 us for the first pass (5.5 TB/s), 19 for
- * the bins (14 64-bit vector instructions and an LDS addition per token), 13 to 15 for the list (the row comes from the last-level cache
- * again), 8 for sums, sort and cuts, which are chains of a few hundred instructions; with top_k 40 the first 9, 3.5 for the list, 8 for the
+ * the bins (14 64-bit vector instructions and an LDS addition per token), 9 to 12 for the list (what LDS does not hold of the row comes from the last-level
+ * cache again), 8 for sums, sort and cuts, which are chains of a few hundred instructions; with top_k 40 the first 9, 3.5 for the list, 8 for the
  * rest. A row alone is bound by what one compute unit loads and executes (16 sequences with top_k 15.9 us, one 19.8 with the two launches
  * that such a row leaves empty, without top_k 37 by several workgroups).
  */
@@ -262,18 +262,29 @@ template <class T> __device__ __noinline__ void sample_by_value(const T *x, int 
  * time. Unrolled over four vectors, the pass that lists tokens took 15 us instead of 6, most of it for its own instructions. */
 template <class T> constexpr int kPer = 16 / sizeof(T);
 template <class T> struct alignas(16) Vec { T v[kPer<T>]; };
+/* The first vectors of a row, which its first pass leaves in LDS for the next ones, each thread its own: 96 KB of the 160 that a workgroup of
+ * 1024 threads has to itself (its registers leave no room for another). 256 rows of 128256 bf16 logits without filters 66 -> 62.5 us. */
+constexpr int kKept = 6 * kThreads;
+struct Kept { uint4 *at; int n; };
 template <class T> struct Vectors {
     static constexpr int N = kPer<T>;
     const T *x;
-    int lo, first, vecs, behind, all;
-    __device__ Vectors(const T *p, int begin, int end) : x(p), lo(begin) {
+    int lo, first, vecs, behind, all, kept;
+    const uint4 *in_lds;
+    __device__ Vectors(const T *p, int begin, int end, Kept k = {nullptr, 0}) : x(p), lo(begin), in_lds(k.at) {
         const int skip = (int)(((16 - (reinterpret_cast<uintptr_t>(x + lo) & 15)) & 15) / sizeof(T));
         first = min(lo + skip, end), vecs = (end - first) / N, behind = first + vecs * N;
         all = vecs + (first - lo) + (end - behind);
+        kept = min(k.n, vecs);
     }
     __device__ int index(int i) const { return i < vecs ? first + i * N : i < vecs + first - lo ? lo + i - vecs : behind + i - vecs - (first - lo); }
     __device__ Vec<T> load(int i) const {
         Vec<T> v;
+        if (i < kept) {
+            const uint4 bits = in_lds[i];
+            __builtin_memcpy(&v, &bits, 16);
+            return v;
+        }
         if (i < vecs) return *reinterpret_cast<const Vec<T> *>(x + first + i * N);
         const uint32_t nan = sizeof(T) == 4 ? 0x7FC00000u : 0x7FFF7FFFu; /* of either 16-bit type */
         *reinterpret_cast<uint4 *>(&v) = {nan, nan, nan, nan};
@@ -281,9 +292,9 @@ template <class T> struct Vectors {
         return v;
     }
 };
-template <class T, class F> __device__ __forceinline__ void for_vectors(const T *x, int lo, int hi, F fn) {
+template <class T, class F> __device__ __forceinline__ void for_vectors(const T *x, int lo, int hi, Kept kept, F fn) {
     constexpr int N = kPer<T>;
-    const Vectors<T> vec(x, lo, hi);
+    const Vectors<T> vec(x, lo, hi, kept);
     int i = threadIdx.x;
     Vec<T> a = vec.load(i);
 #pragma unroll 1
@@ -295,15 +306,15 @@ template <class T, class F> __device__ __forceinline__ void for_vectors(const T 
         fn(v, vec.index(i));
     }
 }
-template <class T, class F> __device__ __forceinline__ void for_each(const T *x, int lo, int hi, F fn) {
-    for_vectors(x, lo, hi, [&](const float (&v)[kPer<T>], int at) {
+template <class T, class F> __device__ __forceinline__ void for_each(const T *x, int lo, int hi, Kept kept, F fn) {
+    for_vectors(x, lo, hi, kept, [&](const float (&v)[kPer<T>], int at) {
 #pragma unroll
         for (int j = 0; j < kPer<T>; j++) fn(v[j], at + j);
     });
 }
 /* fn(value, index) for the few elements that pass a cheap test */
-template <class T, class P, class F> __device__ __forceinline__ void for_each_of(const T *x, int lo, int hi, P test, F fn) {
-    for_vectors(x, lo, hi, [&](const float (&v)[kPer<T>], int at) {
+template <class T, class P, class F> __device__ __forceinline__ void for_each_of(const T *x, int lo, int hi, Kept kept, P test, F fn) {
+    for_vectors(x, lo, hi, kept, [&](const float (&v)[kPer<T>], int at) {
         uint32_t passed = 0;
 #pragma unroll
         for (int j = 0; j < kPer<T>; j++) passed |= test(v[j]) ? 1u << j : 0u;
@@ -330,9 +341,9 @@ __device__ __forceinline__ Range range_of_workgroup(Range r, Shared &s) {
 /* The range of what for_vectors would give this thread; without MIN its largest alone. Four loads ahead, each into the registers that
  * were just used: one row is bound by its vector instructions here, of which handing vectors on took a third (151936 fp32 logits, top_k
  * 40: 25.6 -> 22.1 us; eight ahead spill). */
-template <bool MIN, class T> __device__ __forceinline__ Range range_of_share(const T *x, int lo, int hi) {
+template <bool MIN, class T> __device__ __forceinline__ Range range_of_share(const T *x, int lo, int hi, Kept keep = {nullptr, 0}) {
     constexpr int kAhead = 4;
-    const Vectors<T> vec(x, lo, hi);
+    const Vectors<T> vec(x, lo, hi, keep);
     Range r = {kMinusInf, -kMinusInf};
     auto take = [&](float v) {
         r.max = fmaxf(r.max, v); /* (NaN is not taken) */
@@ -352,6 +363,7 @@ template <bool MIN, class T> __device__ __forceinline__ Range range_of_share(con
         for (int d = 0; d < kAhead; d++) {
 #pragma unroll
             for (int j = 0; j < kPer<T>; j++) take(to_f32(a[d].v[j]));
+            if (i + d * kThreads < vec.kept) __builtin_memcpy(&keep.at[i + d * kThreads], &a[d], 16);
             const int next = i + (kAhead + d) * kThreads;
             if (next < vec.vecs) a[d] = from[next]; /* (else the same again, which changes nothing) */
         }
@@ -419,10 +431,10 @@ __device__ __forceinline__ void into_bin(float v, const Grid &g, bool counts, bo
     if (weights) atomicAdd((unsigned long long *)&s.weight[g.bin(t)], (unsigned long long)g.offset_weight(d, t));
     if (counts) atomicAdd(&s.count[g.bin(t)], 1u);
 }
-template <class T> __device__ __forceinline__ void fill_bins(const T *x, int lo, int hi, const Grid &g, const Holds &h, Shared &s) {
-    if (!h.weights) for_each(x, lo, hi, [&](float v, int) { into_bin(v, g, true, false, s); });
-    else if (!h.counts) for_each(x, lo, hi, [&](float v, int) { into_bin(v, g, false, true, s); });
-    else for_each(x, lo, hi, [&](float v, int) { into_bin(v, g, true, true, s); });
+template <class T> __device__ __forceinline__ void fill_bins(const T *x, int lo, int hi, Kept kept, const Grid &g, const Holds &h, Shared &s) {
+    if (!h.weights) for_each(x, lo, hi, kept, [&](float v, int) { into_bin(v, g, true, false, s); });
+    else if (!h.counts) for_each(x, lo, hi, kept, [&](float v, int) { into_bin(v, g, false, true, s); });
+    else for_each(x, lo, hi, kept, [&](float v, int) { into_bin(v, g, true, true, s); });
 }
 
 /* counts and weights to running sums */
@@ -607,9 +619,9 @@ template <class F> __device__ __forceinline__ void if_wanted(float v, int i, con
     const int bin = g.bin_of(v);
     if (bin < kBins && is_wanted(bin, w)) fn(entry_of(v, i));
 }
-template <class T, class F> __device__ __forceinline__ void for_each_wanted(const T *x, int lo, int hi, const Grid &g, const Wanted &w, F fn) {
+template <class T, class F> __device__ __forceinline__ void for_each_wanted(const T *x, int lo, int hi, Kept kept, const Grid &g, const Wanted &w, F fn) {
     const Bounds bounds(g, w);
-    for_each_of(x, lo, hi, bounds, [&](float v, int i) { if_wanted(v, i, g, w, fn); });
+    for_each_of(x, lo, hi, kept, bounds, [&](float v, int i) { if_wanted(v, i, g, w, fn); });
 }
 
 __device__ __forceinline__ uint64_t shfl_xor_u64(uint64_t v, int by) {
@@ -825,12 +837,12 @@ __device__ __forceinline__ void nothing_there(int32_t *id, float *prob) {
 /* A row to the pick: from its bins, where they are `filled` or are here; or where the threads' largest logits have been `counted` (`mine` is
  * this thread's) from those. */
 enum class Bins { empty, filled, counted };
-template <class T> __device__ __forceinline__ void finish_row(const T *x, int n, const Grid &g, float mine, Bins bins, const Settings &set, int32_t *id, float *prob, Shared &s) {
+template <class T> __device__ __forceinline__ void finish_row(const T *x, int n, Kept kept, const Grid &g, float mine, Bins bins, const Settings &set, int32_t *id, float *prob, Shared &s) {
     const Holds holds = holds_for(set);
     bool by_value = g.max == -kMinusInf; /* several infinities */
     if (!by_value) {
         if (bins == Bins::empty) {
-            fill_bins(x, 0, n, g, holds, s);
+            fill_bins(x, 0, n, kept, g, holds, s);
             __syncthreads();
         }
         if (bins != Bins::counted) sum_bins(g, holds, s);
@@ -852,7 +864,7 @@ template <class T> __device__ __forceinline__ void finish_row(const T *x, int n,
                     if (bounds(to_f32(v.v[j]))) if_wanted(to_f32(v.v[j]), vec.index(i) + j, g, w, [&](uint64_t e) { add_to_list(e, s); });
             }
         } else {
-            for_each_wanted(x, 0, n, g, w, [&](uint64_t e) { add_to_list(e, s); });
+            for_each_wanted(x, 0, n, kept, g, w, [&](uint64_t e) { add_to_list(e, s); });
         }
         __syncthreads();
         const uint32_t listed = uniform(s.n_list);
@@ -864,6 +876,7 @@ template <class T> __device__ __forceinline__ void finish_row(const T *x, int n,
 
 /* a row by one workgroup */
 template <class T> __device__ __forceinline__ void whole_row(const T *x, int n, const Settings &set, int32_t *id, float *prob, Shared &s) {
+    __shared__ uint4 keep[kKept];
     if (threadIdx.x == 0) s.best = (uint32_t)n, s.n_list = 0, s.digit = 0;
     clear_bins(s);
     const bool first = takes_first(set);
@@ -879,13 +892,13 @@ template <class T> __device__ __forceinline__ void whole_row(const T *x, int n, 
             mine = range_of_share<false>(x, 0, n).max;
             r = {mine, is_there(mine) ? mine : -kMinusInf};
         } else {
-            r = range_of_share<true>(x, 0, n);
+            r = range_of_share<true>(x, 0, n, Kept{keep, kKept});
         }
         r = range_of_workgroup(r, s);
         if (!is_there(r.max)) return nothing_there(id, prob);
         if (first) {
             if (mine == r.max) /* few threads have it */
-                for_each_of(x, 0, n, [&](float v) { return v == r.max; }, [&](float, int i) { atomicMin(&s.best, (uint32_t)i); });
+                for_each_of(x, 0, n, Kept{nullptr, 0}, [&](float v) { return v == r.max; }, [&](float, int i) { atomicMin(&s.best, (uint32_t)i); });
             __syncthreads();
             if (threadIdx.x == 0) {
                 *id = (int32_t)s.best;
@@ -906,7 +919,7 @@ template <class T> __device__ __forceinline__ void whole_row(const T *x, int n, 
                 continue;
             }
         }
-        return finish_row(x, n, g, mine, counted ? Bins::counted : Bins::empty, set, id, prob, s);
+        return finish_row(x, n, Kept{keep, counted ? 0 : kKept}, g, mine, counted ? Bins::counted : Bins::empty, set, id, prob, s);
     }
 }
 
@@ -978,7 +991,7 @@ template <class T> __global__ void __launch_bounds__(kThreads) sample_bins_kerne
     clear_bins(s);
     __syncthreads();
     const Share sh = share_of(c.n_vocab, parts, part);
-    fill_bins(logits + (size_t)seq * c.ld, sh.lo, sh.hi, g, holds_for(set), s);
+    fill_bins(logits + (size_t)seq * c.ld, sh.lo, sh.hi, Kept{nullptr, 0}, g, holds_for(set), s);
     __syncthreads();
     for (int i = threadIdx.x; i < kBins; i += kThreads) {
         if (const uint64_t w = s.weight[i]) atomicAdd((unsigned long long *)&row->weight[i], (unsigned long long)w);
@@ -1000,7 +1013,7 @@ template <class T> __global__ void __launch_bounds__(kThreads) sample_finish_ker
     for (int i = threadIdx.x; i < kBins; i += kThreads) s.weight[i] = row->weight[i], s.count[i] = row->count[i];
     if (threadIdx.x == 0) s.n_list = 0;
     __syncthreads();
-    finish_row(x, c.n_vocab, Grid(r, set.t, c.n_vocab), 0.0f, Bins::filled, set, id, prob, s);
+    finish_row(x, c.n_vocab, Kept{nullptr, 0}, Grid(r, set.t, c.n_vocab), 0.0f, Bins::filled, set, id, prob, s);
 }
 
 /* Workgroups per sequence: 1 = the kernel of one, else the three launches. Of 128256 bf16 logits, rows that need bins (no top_k) take 51, 53
