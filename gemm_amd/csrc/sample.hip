@@ -23,11 +23,12 @@
  *   A list that overflows (a bin of more than 2048 tokens: rows of equal logits) leaves the row to sample_by_value, which takes
  * several passes for each cut.
  *
- * What bounds it, 256 rows of 128256 bf16 logits, by the clock in the kernel: without filters 12 us for the first pass (5.5 TB/s), 19 for
- * the bins (14 64-bit vector instructions and an LDS addition per token), 9 to 12 for the list (what LDS does not hold of the row comes from the last-level
- * cache again), 8 for sums, sort and cuts, which are chains of a few hundred instructions; with top_k 40 the first 9, 3.5 for the list, 8 for the
- * rest. A row alone is bound by what one compute unit loads and executes (16 sequences with top_k 15.9 us, one 19.8 with the two launches
- * that such a row leaves empty, without top_k 37 by several workgroups).
+ * What bounds it, 256 rows of 128256 bf16 logits, by the clock in the kernel when it took 70 us without filters (62.5 now, with fewer
+ * register moves in the passes and a part of the row in LDS): 12 us for the first pass (5.5 TB/s), 21 for the bins (14 64-bit vector
+ * instructions and an LDS addition per token), 13 to 15 for the list (the row came from the last-level cache again), 8 for sums, sort
+ * and cuts, which are chains of a few hundred instructions; with top_k 40, when it took 27 (23.8 now), 12 for the first pass, 3.5 for
+ * the list, 8 for the rest. A row alone is bound by what one compute unit loads and executes (16 sequences with top_k 15.8 us, one 19.7 with
+ * the two launches that such a row leaves empty, without top_k 36 by several workgroups).
  */
 #include "qlin_device.h"
 #include "qlin_internal.h"
