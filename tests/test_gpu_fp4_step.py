@@ -194,3 +194,23 @@ def test_two_threads_on_streams_of_their_own(model):
             assert np.array_equal(a, b)
     for stream in streams:
         assert hip.hipStreamDestroy(stream) == 0
+
+
+@pytest.mark.parametrize("tokens", [1, 3, 40])
+def test_a_sequence_that_is_lost(model, tokens):
+    """a sequence whose activations hold a NaN has no token left: id -1, probability 0 and an embedding of zeros, and the others' step is
+    what it was"""
+    step = Step(model, tokens, 7)
+    step.enqueue(None)
+    qlinear.sync()
+    before = step.results()
+    bad = step.x_host.copy()
+    bad[tokens - 1, 300] = 0x7FC0
+    assert qlinear.load().qlin_dev_upload(step.x.ptr, bad.ctypes.data, bad.nbytes) == 0
+    step.enqueue(None)
+    qlinear.sync()
+    for a, b in zip(step.results(), before):
+        assert np.array_equal(a[:tokens - 1], b[:tokens - 1])
+    assert step.ids.to_numpy(np.int32, (tokens,))[-1] == -1 and step.probs.to_numpy(np.float32, (tokens,))[-1] == 0
+    assert not step.next.to_numpy(np.float32, (tokens, HIDDEN))[-1].any()
+    assert (before[3] >= 0).all()
