@@ -44,18 +44,18 @@ __device__ __forceinline__ void store4(__bf16 *y, f32x4 a, int left) {
     }
 }
 
-constexpr int kFewFloats = 4; /* tokens that a workgroup quantises itself, at most */
+constexpr int kFewFloats = 8; /* tokens that a workgroup quantises itself, at most */
 
-/* MATS 2: gate and up; NT: token groups of 16 per workgroup; XT: uint8_t for an operand, or the floats' type (at most kFewFloats tokens,
- * rows that can be read in 16-byte loads) */
-template <int MATS, int NT, int WAVES, class XT, class OUT>
+/* MATS 2: gate and up; NT: token groups of 16 per workgroup; XT: uint8_t for an operand, or the floats' type (FLOATS tokens at most, rows
+ * that can be read in 16-byte loads) */
+template <int MATS, int NT, int WAVES, int FLOATS, class XT, class OUT>
 __global__ void __launch_bounds__(64 * WAVES)
 few_kernel(const uint8_t *__restrict__ W, const uint8_t *__restrict__ up, const XT *__restrict__ X, OUT *__restrict__ Y, int n_rows, int n_tok, Shape w, Shape x,
            int n_cols, size_t ldx, size_t ldy) {
     constexpr bool kFloats = !std::is_same<XT, uint8_t>::value;
-    static_assert(!kFloats || NT == 1, "floats come in one token group");
+    static_assert(!kFloats || (NT == 1 && FLOATS <= kFewFloats), "floats come in one token group");
     __shared__ f32x4 sums[WAVES][MATS * NT][64];
-    __shared__ __attribute__((aligned(16))) uint32_t packed[kFloats ? WAVES : 1][kFewFloats][64 + 4]; /* of a piece: codes, exponents */
+    __shared__ __attribute__((aligned(16))) uint32_t packed[kFloats ? WAVES : 1][FLOATS][64 + 4]; /* of a piece: codes, exponents */
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int token_blocks = (x.groups + NT - 1) / NT;
     const int group = blockIdx.x / (unsigned)token_blocks, t0 = (blockIdx.x - group * token_blocks) * NT;
@@ -63,10 +63,10 @@ few_kernel(const uint8_t *__restrict__ W, const uint8_t *__restrict__ up, const 
     for (int q = wave; q < w.quads; q += WAVES) {
         u32x4 a[MATS][4], b[NT][4];
         int sa[MATS], sb[NT];
-        float v[kFloats ? kFewFloats : 1][8];
+        float v[FLOATS][8];
         if constexpr (kFloats) { /* ahead of the weights, so that waiting for them does not wait for those */
 #pragma unroll
-            for (int t = 0; t < kFewFloats; t++)
+            for (int t = 0; t < FLOATS; t++)
                 if (t < n_tok) load8<XT, true>(X + t * ldx + q * 512 + lane * 8, n_cols - q * 512 - lane * 8, v[t]);
         }
 #pragma unroll
@@ -85,7 +85,7 @@ few_kernel(const uint8_t *__restrict__ W, const uint8_t *__restrict__ up, const 
             sa[m] = *reinterpret_cast<const int *>((m ? up : W) + w.code_bytes() + ((size_t)group * w.quads + q) * kScaleBytes + lane * 4);
         if constexpr (kFloats) {
 #pragma unroll
-            for (int t = 0; t < kFewFloats; t++)
+            for (int t = 0; t < FLOATS; t++)
                 if (t < n_tok) {
                     const Packed p = pack8(v[t], lane & 3);
                     const int block = lane >> 2;
@@ -140,23 +140,26 @@ few_kernel(const uint8_t *__restrict__ W, const uint8_t *__restrict__ up, const 
     }
 }
 
-template <int MATS, int NT, class XT, class OUT> hipError_t few(const Mxfp4Product &p) {
+template <int MATS, int NT, int FLOATS, class XT, class OUT> hipError_t few(const Mxfp4Product &p) {
     constexpr int kWaves = 8;
     const Shape w = shape_of(p.n_rows, p.n_cols), x = shape_of(p.n_tok, p.n_cols);
     const dim3 grid((unsigned)w.groups * (unsigned)((x.groups + NT - 1) / NT));
-    few_kernel<MATS, NT, kWaves, XT, OUT><<<grid, 64 * kWaves, 0, p.stream>>>(p.W, p.up, static_cast<const XT *>(p.X), static_cast<OUT *>(p.Y), p.n_rows, p.n_tok, w, x,
+    few_kernel<MATS, NT, kWaves, FLOATS, XT, OUT><<<grid, 64 * kWaves, 0, p.stream>>>(p.W, p.up, static_cast<const XT *>(p.X), static_cast<OUT *>(p.Y), p.n_rows, p.n_tok, w, x,
                                                                              p.n_cols, (size_t)p.ldx, (size_t)p.ldy);
     return hipGetLastError();
 }
+template <int MATS, class XT, class OUT> hipError_t few_floats(const Mxfp4Product &p) {
+    return p.n_tok <= 4 ? few<MATS, 1, 4, XT, OUT>(p) : few<MATS, 1, kFewFloats, XT, OUT>(p);
+}
 template <int MATS, class OUT> hipError_t few_tokens(const Mxfp4Product &p) {
-    if (p.x_type == T_F32) return few<MATS, 1, float, OUT>(p);
-    if (p.x_type == T_F16) return few<MATS, 1, _Float16, OUT>(p);
-    if (p.x_type == T_BF16) return few<MATS, 1, Bf16, OUT>(p);
+    if (p.x_type == T_F32) return few_floats<MATS, float, OUT>(p);
+    if (p.x_type == T_F16) return few_floats<MATS, _Float16, OUT>(p);
+    if (p.x_type == T_BF16) return few_floats<MATS, Bf16, OUT>(p);
     const int groups = (p.n_tok + 15) / 16;
-    if (groups == 1) return few<MATS, 1, uint8_t, OUT>(p);
-    if (groups == 2) return few<MATS, 2, uint8_t, OUT>(p);
-    if (groups == 3) return few<MATS, 3, uint8_t, OUT>(p);
-    return few<MATS, 4, uint8_t, OUT>(p);
+    if (groups == 1) return few<MATS, 1, 1, uint8_t, OUT>(p);
+    if (groups == 2) return few<MATS, 2, 1, uint8_t, OUT>(p);
+    if (groups == 3) return few<MATS, 3, 1, uint8_t, OUT>(p);
+    return few<MATS, 4, 1, uint8_t, OUT>(p);
 }
 
 }  // namespace
@@ -168,9 +171,12 @@ hipError_t launch_mxfp4_few(const Mxfp4Product &p) {
 
 /* A launch of its own to quantise costs about 2.7 us. Here a piece (512 columns of a token) costs each of the row groups about 0.07 us per
  * thousand: 14336 x 4096, 4 tokens (29 k pieces) 9.0 us against 10; 4096 x 14336, 4 tokens (29 k) 8.4 to 10.5 against 10.6; 151936 x 4096
- * (76 k per token) 1 token 58.4 against 57, 4 tokens 74 against 60. */
+ * (76 k per token) 1 token 58.4 against 57, 4 tokens 74 against 60. From five tokens on their registers cost workgroups in flight too. In a
+ * graph, bf16: 4096 x 4096, 8 tokens (16 k) 6.1 against 7.0, gate and up of 6144 x 4096, 5 tokens (15 k) 8.2 against 8.45 and 6 tokens
+ * (18 k) 8.9 against 8.5; one tensor of that size, 8 tokens (25 k) 7.5 against 7.7. With nine tokens and more (a third variant, left out) 512 x 2048
+ * 5.7 against 5.4, 14336 x 4096 22 against 12. */
 bool mxfp4_quantises_in_product(const Mxfp4Product &p) {
-    constexpr size_t kPieces = 32768;
+    const size_t kPieces = p.n_tok <= 4 ? 32768 : 16384;
     const Shape w = shape_of(p.n_rows, p.n_cols);
     if (p.x_type == T_MXFP4 || p.n_tok > kFewFloats || (size_t)w.groups * w.quads * p.n_tok > kPieces) return false;
     return p.x_type == T_F32 ? reads_wide<float>(p.X, p.n_cols, p.ldx) : reads_wide<Bf16>(p.X, p.n_cols, p.ldx);

@@ -316,3 +316,20 @@ def test_sizes_of_nothing():
     qlinear.mxfp4_gemm_dev(buf, F32, buf, F32, buf, 4, 64, 0, 64, 4, ws)
     qlinear.sync()
     assert (buf.to_numpy(np.uint8, (4096,)) == FILL).all()
+
+
+@pytest.mark.parametrize("tok", [4, 5, 6, 7, 8, 9])
+@pytest.mark.parametrize("rows,cols", [(1, 8), (200, 520), (48, 4104), (257, 1536), (4000, 4096)])
+def test_tokens_quantised_in_the_product(rows, cols, tok):
+    """some tokens are quantised by the product where rows can be read 16 bytes at a time and the sizes are small, and in a launch of their own
+    else: the same bits either way, whatever lies behind a row"""
+    (G, g_type, _), (U, _, _) = weights(rows, cols, rows), weights(rows, cols, rows + 1)
+    ops = [operand(g_type, W, rows, cols)[0] for W in (G, U)]
+    for x_type in (F32, F16, BF16):
+        a, _ = as_type(activations(tok, cols, tok + cols), x_type)
+        x_op, _ = operand(x_type, a, tok, cols)
+        for some in (ops[:1], ops):
+            for y_type in (F32, BF16):
+                want = multiply(some, MXFP4, x_op, y_type, rows, cols, tok)
+                for pad in (0, 8, 1):
+                    assert np.array_equal(multiply(some, x_type, upload_rows(a, cols + pad), y_type, rows, cols, tok, pad, cols + pad), want)
