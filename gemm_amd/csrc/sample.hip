@@ -243,8 +243,8 @@ template <class T> __device__ __noinline__ void sample_by_value(const T *x, int 
         }
         total = sum_of_workgroup(kept, s, nullptr).weight;
     }
-    uint64_t target = (uint64_t)fmin((double)set.u * (double)total, 9.0e18);
-    target = min(target, total - 1) + 1;
+    const double t = (double)set.u * (double)total;
+    const uint64_t target = min(t < (double)total ? (uint64_t)t : total, total - 1) + 1; /* (u of 1 and more: the last) */
     const Cut c = find_cut<true>(x, n, w, target, s);
     const uint64_t each = w(value_of(c.key));
     const int at = nth_of_value(x, n, c.key, (uint32_t)((target - c.above.weight + each - 1) / each), s);
