@@ -532,6 +532,13 @@ __device__ __forceinline__ void order_runs(Wanted &w) {
         reach = joins ? max(reach, w.run[r].hi) : w.run[r].hi;
     }
 }
+/* The bins in which min-p may cut; empty: it cuts nothing that has a weight. The weights and the logarithm are rounded, by less than 1e-15 of
+ * the exponent and 1e-15: a part of a bin, but many bins where logits lie closer together than 64-bit weights tell apart. */
+__device__ __forceinline__ Run min_p_bins(const Grid &g, float m) {
+    const double at = -log((double)m), off = 1e-15 * (at + 1.0), lo = (at - off) / g.step - 1.0, hi = (at + off) / g.step + 1.0;
+    if (!(lo < kBins)) return {0, -1};
+    return {uniform((int)fmax(lo, 0.0)), uniform((int)fmin(hi, (double)kLastBin))};
+}
 __device__ Wanted wanted_bins(const Grid &g, const Settings &set, const Holds &h, Shared &s) {
     constexpr double kSlack = 1e-11; /* of the sums' rounding */
     const Run none = {0, -1};
@@ -558,10 +565,8 @@ __device__ Wanted wanted_bins(const Grid &g, const Settings &set, const Holds &h
         hi = fmin(hi, uniform(s.upto[w.p.hi]));
     }
     if (set.m > 0.0f) {
-        const double at = -log((double)set.m) / g.step;
-        if (at < kBins) {
-            const int bin = uniform((int)at);
-            w.m = {min(max(bin - 1, 0), kLastBin), min(bin + 1, kLastBin)};
+        w.m = min_p_bins(g, set.m);
+        if (w.m.hi >= w.m.lo) {
             lo = fmin(lo, before(w.m.lo));
             hi = fmin(hi, uniform(s.upto[w.m.hi]));
         }
