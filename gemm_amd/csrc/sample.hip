@@ -20,8 +20,9 @@
  * one that the definition gives. A bin's weight is exp(centre) times the sum of exp(offset from the centre), offsets up to 1/128, so
  * that a token costs a polynomial of degree 4 instead of an exponential; the sum is of integers of 2^-40, which do not depend on
  * the order of the additions: the same call gives the same token.
- *   A list that overflows (a bin of more than 2048 tokens: rows of equal logits) leaves the row to sample_by_value, which takes
- * several passes for each cut.
+ *   A list that overflows leaves the row to sample_by_value, which takes three passes over it for each cut: rows of equal logits, of 16-bit
+ * logits so large that few values lie near the top, of which a finite mask leaves the others a few bins. 256 rows of 128256 bf16
+ * logits of one value 0.5 to 0.8 ms, around -30 instead of 0 0.3 ms, 0.46 with top-p (by 64-bit integer weights of the whole row 1.0 to 2.4, 0.48 and 0.86).
  *
  * What bounds it, 256 rows of 128256 bf16 logits, by the clock in the kernel when it took 70 us without filters (62.5 now, with fewer
  * register moves in the passes and a part of the row in LDS): 12 us for the first pass (5.5 TB/s), 21 for the bins (14 64-bit vector
@@ -88,20 +89,6 @@ __device__ __forceinline__ uint64_t shfl_u64(uint64_t v, int from) {
 }
 __device__ __forceinline__ double shfl_up_f64(double v, int by) { return __shfl_up(v, by, 64); }
 
-/* ------------------------------------------------------------------ a row by the bits of its values */
-
-struct Weights {
-    float max;
-    double per_t; /* 1 / T */
-    double unit;  /* 2^shift */
-    __device__ double real(float v) const {
-        if (v == max) return 1.0;
-        if (max == -kMinusInf) return 0.0;
-        return exp(((double)v - (double)max) * per_t);
-    }
-    __device__ uint64_t operator()(float v) const { return (uint64_t)__double2ull_rn(real(v) * unit); }
-};
-
 struct Sum { uint32_t count; uint64_t weight; };
 __device__ __forceinline__ Sum operator+(Sum a, Sum b) { return {a.count + b.count, a.weight + b.weight}; }
 
@@ -147,44 +134,6 @@ __device__ Sum sum_of_workgroup(Sum v, Shared &s, Sum *before) {
     return total;
 }
 
-/* The value at which the running sum down the order reaches `target` (of counts or of weights; the row's sum does): its key, and the
- * sum over larger ones */
-struct Cut { uint32_t key; Sum above; };
-template <bool BY_WEIGHT, class T> __device__ Cut find_cut(const T *x, int n, const Weights &w, uint64_t target, Shared &s) {
-    Cut c = {0, {0, 0}};
-    for (int pass = 0; pass < 3; pass++) {
-        const int low = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
-        for (int i = threadIdx.x; i < 2048; i += kThreads) s.count[i] = 0, s.weight[i] = 0;
-        __syncthreads();
-        for (int i = threadIdx.x; i < n; i += kThreads) {
-            const float v = to_f32(x[i]);
-            if (!is_there(v)) continue;
-            const uint32_t k = key_of(v);
-            if (pass && (pass == 1 ? k >> 21 : k >> 10) != c.key) continue;
-            const uint32_t d = (k >> low) & (bins - 1);
-            atomicAdd(&s.count[d], 1u);
-            if (const uint64_t m = w(v)) atomicAdd((unsigned long long *)&s.weight[d], (unsigned long long)m);
-        }
-        __syncthreads();
-        const int hi = 2047 - 2 * threadIdx.x; /* two bins per thread, the largest first */
-        const Sum a = {s.count[hi], s.weight[hi]}, b = {s.count[hi - 1], s.weight[hi - 1]};
-        Sum before;
-        (void)sum_of_workgroup(a + b, s, &before);
-        before = before + c.above;
-        const Sum mid = before + a, after = mid + b;
-        auto reached = [&](const Sum &v) { return (BY_WEIGHT ? v.weight : (uint64_t)v.count) >= target; };
-        if (!reached(before) && reached(after)) {
-            s.digit = reached(mid) ? hi : hi - 1;
-            s.above = reached(mid) ? before : mid;
-        }
-        __syncthreads();
-        c.key = c.key << (pass == 2 ? 10 : 11) | s.digit;
-        c.above = s.above;
-        __syncthreads();
-    }
-    return c;
-}
-
 /* index of the nth (from 1) element of value key k */
 template <class T> __device__ int nth_of_value(const T *x, int n, uint32_t k, uint32_t nth, Shared &s) {
     const int per = (n + kWaves - 1) / kWaves, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -207,51 +156,6 @@ template <class T> __device__ int nth_of_value(const T *x, int n, uint32_t k, ui
     }
     __syncthreads();
     return s.picked;
-}
-
-/* the whole row by values: for rows whose lists overflow. n tokens, of which the largest is w.max */
-template <class T> __device__ __noinline__ void sample_by_value(const T *x, int n, const Settings &set, Weights w, int32_t *id, float *prob, Shared &s) {
-    int shift = 62; /* n << shift stays below 2^63 */
-    while (shift > 0 && ((uint64_t)n >> (62 - shift)) > 1) shift--;
-    w.unit = (double)(1ull << shift);
-    Sum all = {0, 0};
-    for (int i = threadIdx.x; i < n; i += kThreads) {
-        const float v = to_f32(x[i]);
-        if (is_there(v)) all = all + Sum{1, w(v)};
-    }
-    all = sum_of_workgroup(all, s, nullptr);
-
-    uint32_t last = 0; /* key of the last kept token's value (0: everything is kept) */
-    uint64_t total = all.weight;
-    if (set.k > 0 && (uint32_t)set.k < all.count) {
-        const Cut c = find_cut<false>(x, n, w, (uint64_t)set.k, s);
-        last = c.key;
-        total = c.above.weight + (set.k - c.above.count) * w(value_of(c.key));
-    }
-    if (set.p < 1.0f) {
-        const uint64_t target = min(max((uint64_t)ceil(fmax((double)set.p, 0.0) * (double)total), (uint64_t)1), total);
-        const Cut c = find_cut<true>(x, n, w, target, s);
-        const uint64_t each = w(value_of(c.key)); /* not 0: the sum grows here */
-        last = c.key;
-        total = c.above.weight + (target - c.above.weight + each - 1) / each * each;
-    }
-    if (set.m > 0.0f && (last == 0 || w.real(value_of(last)) < (double)set.m)) {
-        Sum kept = {0, 0};
-        for (int i = threadIdx.x; i < n; i += kThreads) {
-            const float v = to_f32(x[i]);
-            if (is_there(v) && (v == w.max || (key_of(v) > last && w.real(v) >= (double)set.m))) kept = kept + Sum{1, w(v)};
-        }
-        total = sum_of_workgroup(kept, s, nullptr).weight;
-    }
-    const double t = (double)set.u * (double)total;
-    const uint64_t target = min(t < (double)total ? (uint64_t)t : total, total - 1) + 1; /* (u of 1 and more: the last) */
-    const Cut c = find_cut<true>(x, n, w, target, s);
-    const uint64_t each = w(value_of(c.key));
-    const int at = nth_of_value(x, n, c.key, (uint32_t)((target - c.above.weight + each - 1) / each), s);
-    if (threadIdx.x == 0) {
-        *id = at;
-        if (prob) *prob = (float)((double)each / (double)total);
-    }
 }
 
 /* ------------------------------------------------------------------ a row by bins */
@@ -393,6 +297,12 @@ struct Grid {
         max = uniform(max), per_t = uniform(per_t), scale = uniform(scale), step = uniform(step);
         per_unit = 1.0 / unit;
         c1 = -step * unit, c2 = 0.5 * step * step * unit, c3 = -step * step * step * unit / 6, c4 = step * step * step * step * unit / 24;
+    }
+    __device__ Grid scalar() const { /* (the arguments of a function that is not inlined come in vector registers) */
+        Grid g = *this;
+        g.max = uniform(max), g.per_t = uniform(per_t), g.scale = uniform(scale), g.step = uniform(step), g.unit = uniform(unit), g.per_unit = uniform(per_unit);
+        g.c1 = uniform(c1), g.c2 = uniform(c2), g.c3 = uniform(c3), g.c4 = uniform(c4);
+        return g;
     }
     /* The bin of a value is its distance from the largest in bins, rounded: the sum with 2^52 rounds at 1 and holds it in its lower half.
      * One rounding, so that it never falls from a logit to a smaller one. NaN where the value is; infinite for -infinity. */
@@ -833,6 +743,204 @@ __device__ void pick_from_list(int n, const Grid &g, const Settings &set, Wanted
     else if (threadIdx.x < 64) pick_with<1, 1>(n, g, set, w, id, prob, s);
 }
 
+/* ------------------------------------------------------------------ a row by values
+ * Where the bins of the cuts hold more tokens than a list, a cut is searched for in its bin by the bits of the values: three passes over the
+ * row, each with sums by 11 (10) of the bits. Weights are the bins', multiples of 2^-40 of the bin's own, so that a tail far below
+ * the largest logit is as sharp as its head (integers of the whole row's weights put 6 to 87 % of the picks from a flat tail 21
+ * temperatures down on a neighbour). */
+
+/* the first bin with tokens of which `test` holds (kBins: none) */
+template <class F> __device__ int first_filled(Shared &s, F test) {
+    if (threadIdx.x == 0) s.found[0] = kBins;
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+        const int b = 2 * threadIdx.x + e;
+        if (b <= kLastBin && s.count[b] > (b ? s.count[b - 1] : 0) && test(b)) atomicMin(&s.found[0], (uint32_t)b);
+    }
+    __syncthreads();
+    const int r = uniform((int)s.found[0]);
+    __syncthreads();
+    return r;
+}
+
+/* what the bins before `bin` weigh, and what 1 of its own sums does */
+__device__ __forceinline__ double before_bin(int bin, Shared &s) { return bin > 0 ? uniform(s.upto[bin - 1]) : 0.0; }
+__device__ __forceinline__ double unit_of_bin(int bin, const Grid &g) { return g.per_unit * exp(-(double)bin * g.step); }
+
+/* A thread's additions to sums by bin or digit, those that follow each other to the same place as one: of a row of one value all threads' go to
+ * one place, and wait for each other there (128256 equal logits 1050 -> 310 us). */
+struct Additions {
+    uint32_t *count;
+    uint64_t *weight;
+    int at = -1;
+    Sum held = {0, 0};
+    __device__ __forceinline__ void flush() {
+        if (at < 0) return;
+        atomicAdd(&count[at], held.count);
+        atomicAdd((unsigned long long *)&weight[at], (unsigned long long)held.weight);
+    }
+    __device__ __forceinline__ void add(int to, uint64_t w) {
+        if (to != at) {
+            flush();
+            at = to, held = {0, 0};
+        }
+        held = held + Sum{1, w};
+    }
+};
+
+/* where the kept end: with the bin, or inside it at `upto` of its sum; the sum of all kept */
+struct End {
+    int bin;
+    uint64_t upto;
+    double total;
+};
+/* the end that min-p makes: its lightest token is in one of `bins`, or those before them stay and no more */
+template <class T> __device__ __forceinline__ End end_by_min_p(const T *x, int n, const Grid &g, float m, Run bins, Shared &s) {
+    const Kept nothing = {nullptr, 0};
+    if (threadIdx.x == 0) s.best = ~0u;
+    __syncthreads();
+    uint32_t least = ~0u;
+    for_each(x, 0, n, nothing, [&](float v, int) {
+        const int b = g.bin_of(v);
+        if (b >= bins.lo && b <= bins.hi && g.weight(v) >= (double)m) least = min(least, key_of(v));
+    });
+    if (least != ~0u) atomicMin(&s.best, least);
+    __syncthreads();
+    least = uniform(s.best);
+    if (least == ~0u) { /* (never from bin 0 on: the largest token stays) */
+        const uint32_t heavier = uniform(s.count[bins.lo - 1]);
+        const int b = first_filled(s, [&](int i) { return s.count[i] >= heavier; });
+        return {b, ~0ull, uniform(s.upto[b])};
+    }
+    const int bin = g.bin_of(value_of(least));
+    Sum kept = {0, 0};
+    for_each(x, 0, n, nothing, [&](float v, int) {
+        const double d = g.distance(v), t = g.ticks(d);
+        if (g.counts(t) && g.bin(t) == bin && key_of(v) >= least) kept = kept + Sum{1, g.offset_weight(d, t)};
+    });
+    kept = sum_of_workgroup(kept, s, nullptr);
+    return {bin, kept.weight, before_bin(bin, s) + unit_of_bin(bin, g) * (double)kept.weight};
+}
+
+/* The value in a bin, which has tokens, at which the bin's running sum reaches `target` (a number of tokens, or a sum in the bin's unit; at
+ * least 1), its last one if none does: its key, which of its tokens it is (from 1), what each weighs, and the bin's sum with that token */
+struct Cut {
+    uint32_t key, nth;
+    uint64_t each, upto;
+};
+template <class T> __device__ __forceinline__ Cut find_cut(const T *x, int n, const Grid &g, int bin, bool by_weight, uint64_t target, Shared &s) {
+    uint64_t *weight = s.list;
+    uint32_t *count = reinterpret_cast<uint32_t *>(s.sorted);
+    uint32_t key = 0;
+    Sum above = {0, 0};
+#pragma unroll 1
+    for (int pass = 0; pass < 3; pass++) {
+        const int low = pass == 0 ? 21 : pass == 1 ? 10 : 0, known = pass == 0 ? 32 : low + (pass == 1 ? 11 : 10), digits = pass == 2 ? 1024 : 2048;
+        for (int i = threadIdx.x; i < 2048; i += kThreads) count[i] = 0, weight[i] = 0;
+        __syncthreads();
+        Additions sums = {count, weight};
+        for_each(x, 0, n, Kept{nullptr, 0}, [&](float v, int) {
+            const double d = g.distance(v), t = g.ticks(d);
+            if (!g.counts(t) || g.bin(t) != bin) return;
+            const uint32_t k = key_of(v);
+            if (pass && k >> known != key) return;
+            sums.add((k >> low) & (digits - 1), g.offset_weight(d, t));
+        });
+        sums.flush();
+        __syncthreads();
+        const int hi = 2047 - 2 * threadIdx.x; /* two digits per thread, the largest first */
+        const Sum a = {count[hi], weight[hi]}, b = {count[hi - 1], weight[hi - 1]};
+        Sum before;
+        const Sum all = sum_of_workgroup(a + b, s, &before);
+        if (pass == 0) target = min(target, by_weight ? all.weight : (uint64_t)all.count);
+        before = before + above;
+        const Sum mid = before + a, after = mid + b;
+        auto reached = [&](const Sum &v) { return (by_weight ? v.weight : (uint64_t)v.count) >= target; };
+        if (!reached(before) && reached(after)) {
+            s.digit = reached(mid) ? hi : hi - 1;
+            s.above = reached(mid) ? before : mid;
+        }
+        __syncthreads();
+        key = key << (known - low) | uniform(s.digit);
+        above = s.above;
+        __syncthreads();
+    }
+    const double d = g.distance(value_of(key));
+    const uint64_t each = g.offset_weight(d, g.ticks(d));
+    const uint32_t nth = by_weight ? (uint32_t)((target - above.weight + each - 1) / each) : (uint32_t)target - above.count;
+    return {key, nth, each, above.weight + nth * each};
+}
+
+/* the whole row, whose largest logit is finite, from bins of its own */
+template <class T> __device__ __noinline__ void sample_by_value(const T *x, int n, Settings set, Grid grid, int32_t *id, float *prob, Shared &s) {
+    const Grid g = grid.scalar();
+    clear_bins(s);
+    __syncthreads();
+    Additions sums = {s.count, s.weight};
+    for_each(x, 0, n, Kept{nullptr, 0}, [&](float v, int) {
+        const double d = g.distance(v), t = g.ticks(d);
+        if (g.counts(t)) sums.add(g.bin(t), g.offset_weight(d, t));
+    });
+    sums.flush();
+    __syncthreads();
+    sum_bins(g, Holds{true, true}, s);
+    const uint32_t tokens = uniform(s.count[kLastBin]);
+    End end = {first_filled(s, [&](int b) { return s.count[b] >= tokens; }), ~0ull, 0.0};
+    end.total = uniform(s.upto[end.bin]);
+    enum Step { top_k, top_p, min_p, pick };
+#pragma unroll 1
+    for (int step = top_k; step <= pick; step++) {
+        int bin = end.bin;
+        uint64_t goal = end.upto;
+        if (step == top_k) {
+            if (set.k <= 0 || (uint32_t)set.k >= tokens) continue;
+            bin = first_filled(s, [&](int b) { return s.count[b] >= (uint32_t)set.k; });
+            goal = (uint32_t)set.k - (bin > 0 ? uniform(s.count[bin - 1]) : 0);
+        } else if (step == min_p) {
+            const Run bins = set.m > 0.0f ? min_p_bins(g, set.m) : Run{0, -1};
+            if (bins.hi < bins.lo) continue;
+            const End m = end_by_min_p(x, n, g, set.m, bins, s);
+            if (m.bin < end.bin || (m.bin == end.bin && m.upto < end.upto)) end = m;
+            continue;
+        } else { /* the first kept token at which the running sum reaches p times the sum, or is past u times the sum */
+            if (step == top_p && !(set.p < 1.0f)) continue;
+            const double target = (step == top_p ? fmax((double)set.p, 0.0) : (double)set.u) * end.total;
+            if (target < end.total) {
+                bin = min(first_filled(s, [&](int b) { return step == top_p ? s.upto[b] >= target : s.upto[b] > target; }), end.bin);
+                const double in_bin = fmax(target - before_bin(bin, s), 0.0) / unit_of_bin(bin, g);
+                goal = max((uint64_t)fmin(step == top_p ? ceil(in_bin) : floor(in_bin) + 1.0, 9.0e18), (uint64_t)1); /* (a bin's sum is below 2^62.1) */
+                if (bin == end.bin) goal = min(goal, end.upto);
+            }
+        }
+        const Cut c = find_cut(x, n, g, bin, step != top_k, goal, s);
+        const double unit = unit_of_bin(bin, g);
+        if (step == pick) {
+            const int at = nth_of_value(x, n, c.key, c.nth, s);
+            if (threadIdx.x == 0) {
+                *id = at;
+                if (prob) *prob = (float)(unit * (double)c.each / end.total);
+            }
+        }
+        end = {bin, c.upto, before_bin(bin, s) + unit * (double)c.upto};
+    }
+}
+
+/* a row whose largest logits are infinite: each of them weighs 1, the others nothing */
+template <class T> __device__ __noinline__ void sample_infinities(const T *x, int n, Settings set, int32_t *id, float *prob, Shared &s) {
+    Sum mine = {0, 0};
+    for_each(x, 0, n, Kept{nullptr, 0}, [&](float v, int) { mine.count += v == -kMinusInf; });
+    uint32_t kept = sum_of_workgroup(mine, s, nullptr).count;
+    if (set.k > 0) kept = min(kept, (uint32_t)set.k);
+    if (set.p < 1.0f) kept = max((uint32_t)ceil(fmax((double)set.p, 0.0) * kept), 1u);
+    const double target = (double)set.u * kept;
+    const int at = nth_of_value(x, n, key_of(-kMinusInf), target < kept ? (uint32_t)target + 1 : kept, s);
+    if (threadIdx.x == 0) {
+        *id = at;
+        if (prob) *prob = (float)(1.0 / kept);
+    }
+}
+
 __device__ __forceinline__ void nothing_there(int32_t *id, float *prob) {
     if (threadIdx.x == 0) {
         *id = -1;
@@ -845,39 +953,36 @@ __device__ __forceinline__ void nothing_there(int32_t *id, float *prob) {
 enum class Bins { empty, filled, counted };
 template <class T> __device__ __forceinline__ void finish_row(const T *x, int n, Kept kept, const Grid &g, float mine, Bins bins, const Settings &set, int32_t *id, float *prob, Shared &s) {
     const Holds holds = holds_for(set);
-    bool by_value = g.max == -kMinusInf; /* several infinities */
-    if (!by_value) {
-        if (bins == Bins::empty) {
-            fill_bins(x, 0, n, kept, g, holds, s);
-            __syncthreads();
-        }
-        if (bins != Bins::counted) sum_bins(g, holds, s);
-        const Wanted w = wanted_bins(g, set, holds, s);
-        if (bins == Bins::counted) {
-            /* only what those threads read whose largest logit is wanted is looked at again: their vectors, dealt to all threads (for
-             * k = 40 some 720 vectors of 16032; a pass over all of them takes 12 us where all compute units make one) */
-            uint32_t *of = reinterpret_cast<uint32_t *>(s.sorted);
-            const Bounds bounds(g, w);
-            if (mine >= bounds.low0) of[atomicAdd(&s.digit, 1u)] = threadIdx.x;
-            __syncthreads();
-            const Vectors<T> vec(x, 0, n);
-            const int rounds = (vec.all + kThreads - 1) / kThreads, tasks = uniform((int)s.digit) * rounds;
-            for (int q = threadIdx.x; q < tasks; q += kThreads) {
-                const int i = (int)of[q / rounds] + q % rounds * kThreads;
-                const Vec<T> v = vec.load(i);
-#pragma unroll
-                for (int j = 0; j < kPer<T>; j++)
-                    if (bounds(to_f32(v.v[j]))) if_wanted(to_f32(v.v[j]), vec.index(i) + j, g, w, [&](uint64_t e) { add_to_list(e, s); });
-            }
-        } else {
-            for_each_wanted(x, 0, n, kept, g, w, [&](uint64_t e) { add_to_list(e, s); });
-        }
+    if (g.max == -kMinusInf) return sample_infinities(x, n, set, id, prob, s);
+    if (bins == Bins::empty) {
+        fill_bins(x, 0, n, kept, g, holds, s);
         __syncthreads();
-        const uint32_t listed = uniform(s.n_list);
-        by_value = listed > kListed;
-        if (!by_value) pick_from_list((int)listed, g, set, w, id, prob, s);
     }
-    if (by_value) sample_by_value(x, n, set, Weights{g.max, 1.0 / (double)set.t, 0.0}, id, prob, s);
+    if (bins != Bins::counted) sum_bins(g, holds, s);
+    const Wanted w = wanted_bins(g, set, holds, s);
+    if (bins == Bins::counted) {
+        /* only what those threads read whose largest logit is wanted is looked at again: their vectors, dealt to all threads (for
+         * k = 40 some 720 vectors of 16032; a pass over all of them takes 12 us where all compute units make one) */
+        uint32_t *of = reinterpret_cast<uint32_t *>(s.sorted);
+        const Bounds bounds(g, w);
+        if (mine >= bounds.low0) of[atomicAdd(&s.digit, 1u)] = threadIdx.x;
+        __syncthreads();
+        const Vectors<T> vec(x, 0, n);
+        const int rounds = (vec.all + kThreads - 1) / kThreads, tasks = uniform((int)s.digit) * rounds;
+        for (int q = threadIdx.x; q < tasks; q += kThreads) {
+            const int i = (int)of[q / rounds] + q % rounds * kThreads;
+            const Vec<T> v = vec.load(i);
+#pragma unroll
+            for (int j = 0; j < kPer<T>; j++)
+                if (bounds(to_f32(v.v[j]))) if_wanted(to_f32(v.v[j]), vec.index(i) + j, g, w, [&](uint64_t e) { add_to_list(e, s); });
+        }
+    } else {
+        for_each_wanted(x, 0, n, kept, g, w, [&](uint64_t e) { add_to_list(e, s); });
+    }
+    __syncthreads();
+    const uint32_t listed = uniform(s.n_list);
+    if (listed > kListed) return sample_by_value(x, n, set, g, id, prob, s);
+    pick_from_list((int)listed, g, set, w, id, prob, s);
 }
 
 /* a row by one workgroup */
