@@ -486,9 +486,7 @@ __device__ Wanted wanted_bins(const Grid &g, const Settings &set, const Holds &h
         if (w.m.hi < w.p.lo) w.p = none;
         else if (w.p.hi < w.m.lo) w.m = none;
     }
-    /* (beyond the sum of all, for a random number of 1, the last bin that weighs anything) */
-    const double u = fmin((double)set.u, 1.0), at_least = fmin(u * lo * (1.0 - kSlack), everything * (1.0 - kSlack));
-    const double at_most = fmin(u * hi * (1.0 + kSlack), everything * (1.0 - kSlack));
+    const double u = (double)set.u, at_least = u * lo * (1.0 - kSlack), at_most = u * hi * (1.0 + kSlack); /* (u < 1: some bin is past both) */
     const Pair f = first_bins(s, [&](int i) { return s.upto[i] > at_least; }, [&](int i) { return s.upto[i] > at_most; });
     w.u = {min(f.one, kLastBin), min(max(f.one, f.other), kLastBin)};
     order_runs(w);
@@ -701,7 +699,7 @@ template <int WAVES, int E> __device__ __forceinline__ void pick_with(int n, con
     }
     const double target = (double)set.u * total;
     int i = first(w.all ? everywhere : w.u, [&](int at, double weight, int e) { return at < kept && weight > 0.0 && sums[e] > target; });
-    if (i >= n) { /* u of 1, or the last border rounded away: the last kept token that weighs anything, which is before the first that does not */
+    if (i >= n) { /* the last border rounded away: the last kept token that weighs anything, which is before the first that does not */
         const int none = first(everywhere, [&](int at, double weight, int) { return at >= kept || !(weight > 0.0); });
         i = max(none - 1, 0);
     }
@@ -980,7 +978,8 @@ template <class T> __device__ __forceinline__ void finish_row(const T *x, int n,
         for_each_wanted(x, 0, n, kept, g, w, [&](uint64_t e) { add_to_list(e, s); });
     }
     __syncthreads();
-    const uint32_t listed = uniform(s.n_list);
+    /* (a u of 1 or more takes the last token with a weight: sums do not find its bin, to which it adds next to nothing) */
+    const uint32_t listed = set.u >= 1.0f ? kListed + 1 : uniform(s.n_list);
     if (listed > kListed) return sample_by_value(x, n, set, g, id, prob, s);
     pick_from_list((int)listed, g, set, w, id, prob, s);
 }

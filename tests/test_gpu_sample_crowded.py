@@ -47,6 +47,8 @@ class ByValue:
     def reaching(self, target, past):
         """-> (tokens until the running sum reaches, or is past, `target`; distance of the target from the nearest border of the value)"""
         upto = np.cumsum(self.w * self.counts)
+        if past and target >= upto[-1]:
+            return int(np.sum(self.counts)), 1.0
         i = min(int(np.searchsorted(upto, target, side="right" if past else "left")), len(upto) - 1)
         before = upto[i - 1] if i else np.longdouble(0)
         if self.w[i] == 0:
@@ -152,6 +154,7 @@ def test_crowded_bins(type_id, centre, sigma, t, mask, rows):
     check(type_id, x, rng.random(rows), t=[t] * rows, p=rng.choice([0.0, 0.3, 0.9, 0.95, 0.999], rows))
     for _ in range(2):
         check(type_id, x, rng.random(rows), t=[t] * rows, k=rng.choice([0, 2, 20, 400, 1000, 1500, 30000], rows), p=rng.choice([1.0, 0.3, 0.95, 0.999], rows), m=rng.choice([0.0, 1e-3, 0.05, 0.9], rows))
+    check(type_id, x, [0.0, LAST, 1.0, 2.0, 1e-30, 0.5][:rows] * (rows // 6) + [0.25] * (rows % 6), t=[t] * rows)
 
 
 @pytest.mark.parametrize("n", [9001, 66001])
@@ -192,3 +195,16 @@ def test_min_p_of_one_among_logits_that_weigh_the_same(n, rows):
         compare(F32, x, rng.random(rows), t=[t] * rows, m=[1.0] * rows)
         compare(F32, x, rng.random(rows), t=[t] * rows, m=[1.0] * rows, k=[n // 2] * rows, p=[0.7] * rows)
     compare(F32, x, rng.random(rows), t=[1.0] * rows, m=[1.0 - 2.0 ** -24] * rows)
+
+
+@pytest.mark.parametrize("n", [3, 900, 5000, 66000])
+@pytest.mark.parametrize("rows", [4, 12])
+def test_random_numbers_of_one_and_more(n, rows):
+    """nothing is past the whole sum: the last of the kept tokens, however little it weighs"""
+    rng = np.random.default_rng(n)
+    x = 2.0 * rng.standard_normal((rows, n)) - np.linspace(0.0, 10.0, n)
+    u = np.resize([1.0, 2.0, np.inf, LAST], rows)
+    check(F32, x, u)
+    check(F32, x, u, t=[0.8] * rows, k=[0, 40, 700, 1500][:rows] * (rows // 4))
+    check(F32, x, u, p=[0.95] * rows)
+    check(F32, x, u, m=[1e-4] * rows, k=[0, 40, 700, 1500][:rows] * (rows // 4))
