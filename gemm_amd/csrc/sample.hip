@@ -363,7 +363,7 @@ __device__ void sum_bins(const Grid &g, const Holds &h, Shared &s) {
         __syncthreads();
         double before = 0.0;
         for (int w = 0; w < wave; w++) before += s.wave_f64[w];
-        /* (a running sum must not fall from one bin to the next: both are the same sum and a1) */
+        /* (both are the same sum and a1: within a pair no sum falls; from pair to pair one may, by a rounding) */
         s.upto[b + 1] = before + run;
         s.upto[b] = before + run - a1;
     }
@@ -384,8 +384,9 @@ __device__ void sum_bins(const Grid &g, const Holds &h, Shared &s) {
     __syncthreads();
 }
 
-/* The first bin of which `one` holds, and the first of which `other` holds (running sums: once true, true to the end); kLastBin + 1 if there
- * is none. All threads of the workgroup call it. */
+/* The first bin of which `one` holds, and the first of which `other` holds; kLastBin + 1 if there is none. The tests are of running sums, which fall by
+ * a rounding here and there: what holds of a bin need not of the next, and of several firsts the least counts. All threads
+ * of the workgroup call it. */
 struct Pair { int one, other; };
 template <class F, class G> __device__ Pair first_bins(Shared &s, F one, G other) {
     if (threadIdx.x < 2) s.found[threadIdx.x] = kLastBin + 1;
@@ -393,8 +394,8 @@ template <class F, class G> __device__ Pair first_bins(Shared &s, F one, G other
 #pragma unroll
     for (int e = 0; e < 2; e++) {
         const int b = 2 * threadIdx.x + e;
-        if (b <= kLastBin && one(b) && (b == 0 || !one(b - 1))) s.found[0] = b;
-        if (b <= kLastBin && other(b) && (b == 0 || !other(b - 1))) s.found[1] = b;
+        if (b <= kLastBin && one(b) && (b == 0 || !one(b - 1))) atomicMin(&s.found[0], (uint32_t)b);
+        if (b <= kLastBin && other(b) && (b == 0 || !other(b - 1))) atomicMin(&s.found[1], (uint32_t)b);
     }
     __syncthreads();
     const Pair r = {uniform((int)s.found[0]), uniform((int)s.found[1])};
