@@ -451,7 +451,7 @@ __device__ __forceinline__ Run min_p_bins(const Grid &g, float m) {
     return {uniform((int)fmax(lo, 0.0)), uniform((int)fmin(hi, (double)kLastBin))};
 }
 __device__ Wanted wanted_bins(const Grid &g, const Settings &set, const Holds &h, Shared &s) {
-    constexpr double kSlack = 1e-11; /* of the sums' rounding */
+    const double slack = 1e-11 + 2.0 * g.per_unit; /* of the sums' rounding: half a unit for each of a bin's tokens, which may all go one way */
     const Run none = {0, -1};
     Wanted w = {};
     w.k = w.p = w.m = w.u = none;
@@ -469,7 +469,7 @@ __device__ Wanted wanted_bins(const Grid &g, const Settings &set, const Holds &h
         if (b <= kLastBin) w.k = {b, b}, lo = before(b), hi = uniform(s.upto[b]);
     }
     if (set.p < 1.0f) {
-        const double p = fmax((double)set.p, 0.0), at_least = p * lo * (1.0 - kSlack), at_most = p * hi * (1.0 + kSlack);
+        const double p = fmax((double)set.p, 0.0), at_least = p * lo * (1.0 - slack), at_most = p * hi * (1.0 + slack);
         const Pair f = first_bins(s, [&](int i) { return s.upto[i] >= at_least; }, [&](int i) { return s.upto[i] >= at_most; });
         w.p = {min(f.one, kLastBin), min(f.other, kLastBin)};
         lo = fmin(lo, before(w.p.lo));
@@ -487,7 +487,7 @@ __device__ Wanted wanted_bins(const Grid &g, const Settings &set, const Holds &h
         if (w.m.hi < w.p.lo) w.p = none;
         else if (w.p.hi < w.m.lo) w.m = none;
     }
-    const double u = (double)set.u, at_least = u * lo * (1.0 - kSlack), at_most = u * hi * (1.0 + kSlack); /* (u < 1: some bin is past both) */
+    const double u = (double)set.u, at_least = u * lo * (1.0 - slack), at_most = u * hi * (1.0 + slack); /* (u < 1: some bin is past both) */
     const Pair f = first_bins(s, [&](int i) { return s.upto[i] > at_least; }, [&](int i) { return s.upto[i] > at_most; });
     w.u = {min(f.one, kLastBin), min(max(f.one, f.other), kLastBin)};
     order_runs(w);

@@ -208,3 +208,35 @@ def test_random_numbers_of_one_and_more(n, rows):
     check(F32, x, u, t=[0.8] * rows, k=[0, 40, 700, 1500][:rows] * (rows // 4))
     check(F32, x, u, p=[0.95] * rows)
     check(F32, x, u, m=[1e-4] * rows, k=[0, 40, 700, 1500][:rows] * (rows // 4))
+
+
+def test_a_border_between_bins_in_a_row_of_2_to_the_27():
+    """The bins of a row so long hold weights in 2^-33, so that their sums are off by up to 2^-34. A crowd whose weights all round up, and a
+    random number that falls between its sum and the bin's: the pick is the crowd's last token or the first behind it, not a token of another
+    cut's bins far down the row."""
+    n, unit = 1 << 27, 2.0 ** 33
+    light = -20.7  # three tokens that weigh about 1e-9, which min-p keeps
+    scale = 2040.0 / -float(np.float32(light))
+
+    def in_bin(logit):
+        """what a bin holds for a token"""
+        at = np.round(-np.float64(logit) * scale)
+        return np.round(np.exp((at / scale) + np.float64(logit)) * unit) / unit * np.exp(-at / scale)
+
+    crowd = np.linspace(-0.31, -0.29, 20001).astype(np.float32)
+    crowd = crowd[np.argmax(in_bin(crowd) / np.exp(crowd.astype(np.float64)))]
+    assert in_bin(crowd) / math.exp(crowd) - 1 > 5e-11
+    behind = np.float32(-0.32)
+    assert np.round(-behind * scale) > np.round(-crowd * scale)
+    head = 1.0 + 2000 * in_bin(crowd)
+    fill, rest = [], head * (1 - 6e-11) - 1990 * in_bin(behind) - 3 * in_bin(light)  # the tail weighs 6e-11 less than the head by the bins
+    while rest > 1e-9:
+        fill.append(np.float32(min(math.log(rest), -0.5)))
+        rest -= in_bin(fill[-1])
+    head_exact, tail_exact = 1.0 + 2000 * math.exp(crowd), 1990 * math.exp(behind) + sum(math.exp(v) for v in fill) + 3 * math.exp(light)
+    assert abs(head_exact / tail_exact - 1) < 1e-10
+    x = np.full((1, n), -np.inf, np.float32)
+    places = np.sort(np.random.default_rng(1).choice(n, 1 + 2000 + 1990 + len(fill) + 3, replace=False))
+    x[0, places] = np.concatenate([[0.0], np.full(2000, crowd), np.full(1990, behind), fill, np.full(3, light)]).astype(np.float32)
+    ids, _ = draw(F32, x, np.float32([0.5]), m=[1.0215e-9])  # a fifth of a bin below the three
+    assert ids[0] in (places[2000], places[2001])
