@@ -32,6 +32,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kGroupRows = 16, kTileCols = 128, kTileBytes = 1024, kScaleBytes = 256;
 constexpr int kBlock = 32, kBlockBytes = 17; /* of the GGML format: [exponent][16 bytes of codes] */
+constexpr int kPackThreads = 256, kFewThreads = 512, kTileThreads = 256; /* of a workgroup that makes operands or blocks, of those that multiply */
 
 /* where an operand's parts lie */
 struct Shape {
@@ -85,6 +86,9 @@ hipError_t launch_mxfp4_few(const Mxfp4Product &p);
 hipError_t launch_mxfp4_tiles(int mb, int nb, const Mxfp4Product &p);
 /* the kernel for a product: 0 = launch_mxfp4_few, 10 mb + nb = tiles */
 int mxfp4_choice(const Mxfp4Product &p, int n_cu);
+/* what its launch consists of */
+struct Mxfp4Launch { size_t workgroups, threads; };
+Mxfp4Launch mxfp4_launch(int kernel, const Mxfp4Product &p);
 hipError_t launch_mxfp4_product(const Mxfp4Product &p, int n_cu);
 
 }  // namespace qlin

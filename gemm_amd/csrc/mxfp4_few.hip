@@ -141,10 +141,10 @@ few_kernel(const uint8_t *__restrict__ W, const uint8_t *__restrict__ up, const 
 }
 
 template <int MATS, int NT, int FLOATS, class XT, class OUT> hipError_t few(const Mxfp4Product &p) {
-    constexpr int kWaves = 8;
+    constexpr int kWaves = kFewThreads / 64;
     const Shape w = shape_of(p.n_rows, p.n_cols), x = shape_of(p.n_tok, p.n_cols);
-    const dim3 grid((unsigned)w.groups * (unsigned)((x.groups + NT - 1) / NT));
-    few_kernel<MATS, NT, kWaves, FLOATS, XT, OUT><<<grid, 64 * kWaves, 0, p.stream>>>(p.W, p.up, static_cast<const XT *>(p.X), static_cast<OUT *>(p.Y), p.n_rows, p.n_tok, w, x,
+    const dim3 grid((unsigned)mxfp4_launch(0, p).workgroups);
+    few_kernel<MATS, NT, kWaves, FLOATS, XT, OUT><<<grid, kFewThreads, 0, p.stream>>>(p.W, p.up, static_cast<const XT *>(p.X), static_cast<OUT *>(p.Y), p.n_rows, p.n_tok, w, x,
                                                                              p.n_cols, (size_t)p.ldx, (size_t)p.ldy);
     return hipGetLastError();
 }

@@ -23,7 +23,7 @@ namespace {
 
 /* one workgroup: a row group's 512 columns */
 template <class T, bool VEC>
-__global__ void __launch_bounds__(256) operand_kernel(const T *__restrict__ X, uint8_t *__restrict__ op, int n_rows, int n_cols, size_t ldx, Shape s) {
+__global__ void __launch_bounds__(kPackThreads) operand_kernel(const T *__restrict__ X, uint8_t *__restrict__ op, int n_rows, int n_cols, size_t ldx, Shape s) {
     constexpr int kRun = 16 * 4 + 4; /* dwords from one block of a tile to the next: 16 rows, and 4 against bank conflicts */
     __shared__ __attribute__((aligned(16))) uint32_t codes[16 * kRun];
     __shared__ __attribute__((aligned(16))) uint8_t scales[kScaleBytes];
@@ -56,7 +56,7 @@ __global__ void __launch_bounds__(256) operand_kernel(const T *__restrict__ X, u
 
 /* the same from GGML blocks: codes and exponents are moved, not changed. A lane loads a block, 16 bytes at any address: sixteen lanes read a
  * row's 272 bytes */
-__global__ void __launch_bounds__(256) operand_of_blocks_kernel(const uint8_t *__restrict__ W, uint8_t *__restrict__ op, int n_rows, int n_blocks, Shape s) {
+__global__ void __launch_bounds__(kPackThreads) operand_of_blocks_kernel(const uint8_t *__restrict__ W, uint8_t *__restrict__ op, int n_rows, int n_blocks, Shape s) {
     constexpr int kRun = 16 * 4 + 4; /* as in operand_kernel */
     __shared__ __attribute__((aligned(16))) uint32_t codes[16 * kRun];
     __shared__ __attribute__((aligned(16))) uint8_t scales[kScaleBytes];
@@ -83,7 +83,7 @@ __global__ void __launch_bounds__(256) operand_of_blocks_kernel(const uint8_t *_
 
 /* one workgroup: 256 consecutive blocks of the rows end to end, 4352 bytes of the result */
 template <class T, bool VEC>
-__global__ void __launch_bounds__(256) blocks_kernel(const T *__restrict__ X, uint8_t *__restrict__ W, size_t n_blocks, int per_row, size_t ldx, bool wide) {
+__global__ void __launch_bounds__(kPackThreads) blocks_kernel(const T *__restrict__ X, uint8_t *__restrict__ W, size_t n_blocks, int per_row, size_t ldx, bool wide) {
     constexpr int kBytes = 256 * kBlockBytes;
     __shared__ __attribute__((aligned(16))) uint8_t out[kBytes];
     const size_t first = (size_t)blockIdx.x * 256;
@@ -122,8 +122,8 @@ template <class T> hipError_t operand_of(const void *X, void *op, int n_rows, in
     const dim3 grid((unsigned)s.groups * (unsigned)s.quads);
     const T *x = static_cast<const T *>(X);
     uint8_t *o = static_cast<uint8_t *>(op);
-    if (reads_wide<T>(X, n_cols, ldx)) operand_kernel<T, true><<<grid, 256, 0, stream>>>(x, o, n_rows, n_cols, (size_t)ldx, s);
-    else operand_kernel<T, false><<<grid, 256, 0, stream>>>(x, o, n_rows, n_cols, (size_t)ldx, s);
+    if (reads_wide<T>(X, n_cols, ldx)) operand_kernel<T, true><<<grid, kPackThreads, 0, stream>>>(x, o, n_rows, n_cols, (size_t)ldx, s);
+    else operand_kernel<T, false><<<grid, kPackThreads, 0, stream>>>(x, o, n_rows, n_cols, (size_t)ldx, s);
     return hipGetLastError();
 }
 
@@ -134,8 +134,8 @@ template <class T> hipError_t blocks_of(const void *X, void *W, int n_rows, int 
     const bool wide = (reinterpret_cast<uintptr_t>(W) & 15) == 0;
     const T *x = static_cast<const T *>(X);
     uint8_t *w = static_cast<uint8_t *>(W);
-    if (reads_wide<T>(X, n_cols, ldx)) blocks_kernel<T, true><<<grid, 256, 0, stream>>>(x, w, n_blocks, per_row, (size_t)ldx, wide);
-    else blocks_kernel<T, false><<<grid, 256, 0, stream>>>(x, w, n_blocks, per_row, (size_t)ldx, wide);
+    if (reads_wide<T>(X, n_cols, ldx)) blocks_kernel<T, true><<<grid, kPackThreads, 0, stream>>>(x, w, n_blocks, per_row, (size_t)ldx, wide);
+    else blocks_kernel<T, false><<<grid, kPackThreads, 0, stream>>>(x, w, n_blocks, per_row, (size_t)ldx, wide);
     return hipGetLastError();
 }
 
@@ -146,7 +146,7 @@ hipError_t launch_mxfp4_operand(uint32_t type, const void *X, void *op, int n_ro
     if (type == T_F16) return operand_of<_Float16>(X, op, n_rows, n_cols, ldx, stream);
     if (type == T_BF16) return operand_of<Bf16>(X, op, n_rows, n_cols, ldx, stream);
     const Shape s = shape_of(n_rows, n_cols);
-    operand_of_blocks_kernel<<<dim3((unsigned)s.groups * (unsigned)s.quads), 256, 0, stream>>>(
+    operand_of_blocks_kernel<<<dim3((unsigned)s.groups * (unsigned)s.quads), kPackThreads, 0, stream>>>(
         static_cast<const uint8_t *>(X), static_cast<uint8_t *>(op), n_rows, n_cols / kBlock, s);
     return hipGetLastError();
 }

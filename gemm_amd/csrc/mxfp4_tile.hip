@@ -193,7 +193,7 @@ QLIN_INL uint32_t bytes_from(int groups, int from, uint32_t pitch) {
 }
 
 template <int MB, int NB, bool PAIR, class OUT>
-__global__ void __launch_bounds__(256, MB + NB > 4 ? 1 : 2)
+__global__ void __launch_bounds__(kTileThreads, MB + NB > 4 ? 1 : 2)
 tile_kernel(const uint8_t *__restrict__ W, const uint8_t *__restrict__ up, const uint8_t *__restrict__ X, OUT *__restrict__ Y, int n_rows, int n_tok, Shape w,
             Shape x, size_t ldy, int row_tiles, int tok_tiles, bool stream) {
     /* Consecutive workgroups go to different dies, each with an L2 of its own: a die takes a run of the tiles, numbered through groups of
@@ -315,9 +315,9 @@ template <int MB, int NB, bool PAIR, class OUT> hipError_t tiles(const Mxfp4Prod
     const Shape w = shape_of(p.n_rows, p.n_cols), x = shape_of(p.n_tok, p.n_cols);
     constexpr int kRows = (PAIR ? 32 : 64) * MB, kTok = 64 * NB;
     const int row_tiles = (p.n_rows + kRows - 1) / kRows, tok_tiles = (p.n_tok + kTok - 1) / kTok;
-    const dim3 grid(((unsigned)row_tiles * (unsigned)tok_tiles + 7) / 8 * 8);
+    const dim3 grid((unsigned)mxfp4_launch(10 * MB + NB, p).workgroups);
     const bool stream = (reinterpret_cast<uintptr_t>(p.Y) & 63) == 0 && (size_t)p.ldy * sizeof(OUT) % 64 == 0;
-    tile_kernel<MB, NB, PAIR, OUT><<<grid, 256, 0, p.stream>>>(p.W, p.up, static_cast<const uint8_t *>(p.X), static_cast<OUT *>(p.Y), p.n_rows, p.n_tok, w, x, (size_t)p.ldy, row_tiles, tok_tiles, stream);
+    tile_kernel<MB, NB, PAIR, OUT><<<grid, kTileThreads, 0, p.stream>>>(p.W, p.up, static_cast<const uint8_t *>(p.X), static_cast<OUT *>(p.Y), p.n_rows, p.n_tok, w, x, (size_t)p.ldy, row_tiles, tok_tiles, stream);
     return hipGetLastError();
 }
 template <int MB, int NB> hipError_t tiles_for(const Mxfp4Product &p) {
@@ -385,6 +385,14 @@ int mxfp4_choice(const Mxfp4Product &p, int n_cu) {
         if (t < least) least = t, best = 10 * c.mb + c.nb;
     }
     return best;
+}
+
+Mxfp4Launch mxfp4_launch(int kernel, const Mxfp4Product &p) {
+    const Shape w = shape_of(p.n_rows, p.n_cols), x = shape_of(p.n_tok, p.n_cols);
+    if (kernel == 0) return {(size_t)w.groups * ((x.groups + 3) / 4), kFewThreads}; /* (up to four token groups each) */
+    const size_t rows = (p.up ? 32 : 64) * (kernel / 10), tok = 64 * (kernel % 10);
+    const size_t tiles = (p.n_rows + rows - 1) / rows * ((p.n_tok + tok - 1) / tok);
+    return {(tiles + 7) / 8 * 8, kTileThreads}; /* (as many for each die) */
 }
 
 hipError_t launch_mxfp4_product(const Mxfp4Product &p, int n_cu) {

@@ -1448,11 +1448,20 @@ int check_float_rows(const char *what, uint32_t type, const void *X, int n_rows,
     if (!aligned(X, float_bytes(type))) return fail(QLIN_ERR_ARG, "%s: misaligned pointer", what);
     return QLIN_OK;
 }
+/* HIP launches less than 2^32 threads */
+bool launch_takes(size_t workgroups, size_t threads) { return workgroups < (1ull << 32) / threads; }
 /* sizes that the kernels of an operand can number */
 constexpr int kMaxOperandCols = (1 << 24) - 1;
 bool operand_fits(int n_rows, int n_cols) {
     const mxfp4::Shape s = mxfp4::shape_of(n_rows, n_cols);
-    return n_cols <= kMaxOperandCols && (size_t)s.groups * s.quads <= INT_MAX;
+    return n_cols <= kMaxOperandCols && launch_takes((size_t)s.groups * s.quads, mxfp4::kPackThreads);
+}
+bool product_fits(const Mxfp4Product &p, int kernel = -1) { /* by the kernel that is chosen, if none is named */
+    if (!operand_fits(p.n_rows, p.n_cols) || !operand_fits(p.n_tok, p.n_cols)) return false;
+    const size_t most = (size_t)mxfp4::shape_of(p.n_rows, p.n_cols).groups * mxfp4::shape_of(p.n_tok, p.n_cols).groups;
+    if (launch_takes(most, mxfp4::kFewThreads)) return true; /* (16 rows x 16 tokens: no kernel has more workgroups, nor larger ones) */
+    const Mxfp4Launch l = mxfp4_launch(kernel < 0 ? mxfp4_choice(p, g.n_cu) : kernel, p);
+    return launch_takes(l.workgroups, l.threads);
 }
 }  // namespace
 
@@ -1462,7 +1471,7 @@ int qlin_quantize_mxfp4_dev(uint32_t x_type, const void *X, void *W, int n_rows,
     if (int rc = check_float_rows("X", x_type, X, n_rows, n_cols, ldx)) return rc;
     if (n_rows == 0 || n_cols == 0) return QLIN_OK;
     if (!W) return fail(QLIN_ERR_ARG, "null pointer");
-    if ((size_t)n_rows * (n_cols / mxfp4::kBlock) > (size_t)INT_MAX * 256) return fail(QLIN_ERR_ARG, "%d x %d elements in one call", n_rows, n_cols);
+    if (!launch_takes(((size_t)n_rows * (n_cols / mxfp4::kBlock) + 255) / 256, mxfp4::kPackThreads)) return fail(QLIN_ERR_ARG, "%d x %d elements in one call", n_rows, n_cols);
     if (int rc = init_once()) return rc;
     HIP_TRY(launch_mxfp4_blocks(x_type, X, W, n_rows, n_cols, ldx, (hipStream_t)stream));
     return QLIN_OK;
@@ -1503,12 +1512,11 @@ static int mxfp4_gemm(const void *W, const void *up, bool pair, uint32_t x_type,
     if (!W || (pair && !up) || !X || !Y) return fail(QLIN_ERR_ARG, "null pointer");
     if (!aligned(W, 16) || !aligned(up, 16) || (x_type == T_MXFP4 && !aligned(X, 16)) || !aligned(Y, float_bytes(y_type)))
         return fail(QLIN_ERR_ARG, "operands need 16-byte alignment, Y an element's");
-    if (!operand_fits(n_rows, n_cols) || !operand_fits(n_tok, n_cols) || (size_t)((n_rows + 15ll) / 16) * ((n_tok + 15ll) / 16) > INT_MAX)
-        return fail(QLIN_ERR_ARG, "a product of %d x %d x %d is too large", n_rows, n_cols, n_tok);
+    Mxfp4Product p = {static_cast<const uint8_t *>(W), static_cast<const uint8_t *>(up), x_type, X, Y, n_rows, n_cols, n_tok, ldx, ldy, y_type == T_BF16, (hipStream_t)stream};
+    if (!product_fits(p)) return fail(QLIN_ERR_ARG, "a product of %d x %d x %d is too large", n_rows, n_cols, n_tok);
     if (x_type != T_MXFP4 && (!workspace || !aligned(workspace, 16) || workspace_bytes < qlin_mxfp4_gemm_workspace_bytes(n_cols, n_tok)))
         return fail(QLIN_ERR_ARG, "the workspace needs %zu bytes, 16-byte aligned", qlin_mxfp4_gemm_workspace_bytes(n_cols, n_tok));
     if (int rc = init_once()) return rc;
-    Mxfp4Product p = {static_cast<const uint8_t *>(W), static_cast<const uint8_t *>(up), x_type, X, Y, n_rows, n_cols, n_tok, ldx, ldy, y_type == T_BF16, (hipStream_t)stream};
     if (x_type != T_MXFP4 && !mxfp4_quantises_in_product(p)) {
         HIP_TRY(launch_mxfp4_operand(x_type, X, workspace, n_tok, n_cols, ldx, (hipStream_t)stream));
         p.x_type = T_MXFP4;
@@ -1538,6 +1546,7 @@ int qlin_sample_dev(uint32_t type, const void *logits, int n_seq, int n_vocab, i
     if (int rc = check_float_rows("logits", type, logits, n_seq, n_vocab, ld)) return rc;
     if (n_seq == 0) return QLIN_OK;
     if (n_vocab == 0 || n_vocab > 1 << 30) return fail(QLIN_ERR_ARG, "sampling from %d tokens", n_vocab);
+    if (!launch_takes((size_t)n_seq, kSampleThreads)) return fail(QLIN_ERR_ARG, "sampling for %d sequences in one call", n_seq);
     if (!u || !ids) return fail(QLIN_ERR_ARG, "null pointer");
     for (const void *p : {(const void *)temperature, (const void *)top_k, (const void *)top_p, (const void *)min_p, (const void *)u, (const void *)ids, (const void *)probs})
         if (!aligned(p, 4)) return fail(QLIN_ERR_ARG, "misaligned pointer");
@@ -1631,10 +1640,12 @@ int qlin_probe_gemm_tile(int tile, uint32_t type, const void *W, const uint16_t 
 int qlin_probe_mxfp4_gemm(int kernel, const void *W, const void *up, const void *X, uint32_t y_type, void *Y, int n_rows, int n_cols, int n_tok, int ldy,
                           void *stream) {
     if (y_type != T_F32 && y_type != T_BF16) return fail(QLIN_ERR_TYPE, "results are F32 or BF16 (got type %u)", y_type);
-    if (kernel < 0 || n_rows <= 0 || n_cols <= 0 || n_tok <= 0 || ldy < n_rows || !operand_fits(n_rows, n_cols) || !operand_fits(n_tok, n_cols)) return fail(QLIN_ERR_ARG, "bad kernel or size");
+    if (kernel < 0 || n_rows <= 0 || n_cols <= 0 || n_tok <= 0 || ldy < n_rows) return fail(QLIN_ERR_ARG, "bad kernel or size");
     if (!W || !X || !Y || !aligned(W, 16) || !aligned(up, 16) || !aligned(X, 16) || !aligned(Y, float_bytes(y_type))) return fail(QLIN_ERR_ARG, "null or misaligned pointer");
-    if (int rc = init_once()) return rc;
     const Mxfp4Product p = {static_cast<const uint8_t *>(W), static_cast<const uint8_t *>(up), T_MXFP4, X, Y, n_rows, n_cols, n_tok, n_cols, ldy, y_type == T_BF16, (hipStream_t)stream};
+    if (kernel != 0 && kernel != 11 && kernel != 21 && kernel != 22 && kernel != 44) return fail(QLIN_ERR_ARG, "no kernel %d", kernel);
+    if (!product_fits(p, kernel)) return fail(QLIN_ERR_ARG, "a product of %d x %d x %d is too large", n_rows, n_cols, n_tok);
+    if (int rc = init_once()) return rc;
     if (kernel == 0) HIP_TRY(launch_mxfp4_few(p));
     else HIP_TRY(launch_mxfp4_tiles(kernel / 10, kernel % 10, p));
     return QLIN_OK;

@@ -281,6 +281,7 @@ struct SampleCall {
     void *workspace;
     hipStream_t stream;
 };
+constexpr int kSampleThreads = 1024; /* of a workgroup; one for each sequence at least */
 size_t sample_workspace_bytes(int n_seq, int n_vocab);
 hipError_t launch_sample(uint32_t type, const SampleCall &c);
 /* measurement probes (probe.hip): a register-only MFMA loop (flops issued come back in *flops) with the

@@ -38,7 +38,7 @@ namespace qlin {
 
 namespace {
 
-constexpr int kThreads = 1024, kWaves = kThreads / 64;
+constexpr int kThreads = kSampleThreads, kWaves = kThreads / 64;
 
 struct Bf16 { uint16_t bits; };
 __device__ __forceinline__ float to_f32(float v) { return v; }

@@ -80,3 +80,30 @@ def test_sample_refuses(lib, code, change):
     a = dict(dict(type=F32, logits=P, n_seq=4, n_vocab=100, ld=100, t=P, k=P, p=P, m=P, u=P, ids=P, probs=P, ws=P, ws_bytes=1 << 30), **change)
     assert lib.qlin_sample_dev(*[a[n] for n in ("type", "logits", "n_seq", "n_vocab", "ld", "t", "k", "p", "m", "u", "ids", "probs", "ws", "ws_bytes")], None) == code
     assert lib.qlin_last_error()
+
+
+@pytest.mark.parametrize("args", [(F32, P, P, 1 << 28, 128, 128), (F32, P, P, 2 ** 31 - 1, 1, 1), (MXFP4, P, P, 1 << 28, 32, 32), (BF16, P, P, 1 << 20, 1 << 19, 1 << 19)])
+def test_operands_of_more_workgroups_than_a_launch_takes(lib, args):
+    """a launch has less than 2^32 threads, 256 for each 16 rows of 512 columns"""
+    assert lib.qlin_mxfp4_operand_dev(*args, None) == ARG
+
+
+@pytest.mark.parametrize("pair", [False, True])
+@pytest.mark.parametrize("change", [dict(n_rows=2 ** 31 - 1, n_cols=1, n_tok=1, ldy=2 ** 31 - 1), dict(n_rows=1 << 27, n_tok=1, ldy=1 << 27), dict(n_rows=1 << 27, n_tok=16, ldy=1 << 27),
+                                    dict(n_rows=17, n_tok=2 ** 31 - 1, x_type=MXFP4), dict(n_rows=1 << 26, n_tok=1 << 26, ldy=1 << 26, x_type=MXFP4)])
+def test_products_of_more_workgroups_than_a_launch_takes(lib, pair, change):
+    a = dict(GOOD, ws_bytes=1 << 60, **change)
+    call = lib.qlin_mxfp4_gemm_silu_mul_dev if pair else lib.qlin_mxfp4_gemm_dev
+    rc = call(*([a["W"], a["up"]] if pair else [a["W"]]), a["x_type"], a["X"], a["y_type"], a["Y"], a["n_rows"], a["n_cols"], a["n_tok"], a["ldx"], a["ldy"], a["ws"], a["ws_bytes"], None)
+    assert rc == ARG
+
+
+@pytest.mark.parametrize("n_seq", [1 << 22, 2 ** 31 - 1])
+def test_more_sequences_than_a_launch_takes(lib, n_seq):
+    """1024 threads for each"""
+    assert lib.qlin_sample_dev(F32, P, n_seq, 100, 100, None, None, None, None, P, P, None, None, 0, None) == ARG
+
+
+def test_blocks_of_more_workgroups_than_a_launch_takes(lib):
+    """256 blocks for each"""
+    assert lib.qlin_quantize_mxfp4_dev(BF16, P, P, 1 << 17, 1 << 20, 1 << 20, None) == ARG
