@@ -46,6 +46,14 @@ __device__ __forceinline__ void store4(__bf16 *y, f32x4 a, int left) {
 
 constexpr int kFewFloats = 8; /* tokens that a workgroup quantises itself, at most */
 
+/* A wave's lanes read from LDS what others of its lanes wrote, and write it anew: one wave's requests to LDS stay in order, and this keeps the compiler from
+ * changing it. No instruction. */
+__device__ __forceinline__ void wave_meets() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 /* MATS 2: gate and up; NT: token groups of 16 per workgroup; XT: uint8_t for an operand, or the floats' type (FLOATS tokens at most, rows
  * that can be read in 16-byte loads) */
 template <int MATS, int NT, int WAVES, int FLOATS, class XT, class OUT>
@@ -84,6 +92,7 @@ few_kernel(const uint8_t *__restrict__ W, const uint8_t *__restrict__ up, const 
         for (int m = 0; m < MATS; m++)
             sa[m] = *reinterpret_cast<const int *>((m ? up : W) + w.code_bytes() + ((size_t)group * w.quads + q) * kScaleBytes + lane * 4);
         if constexpr (kFloats) {
+            wave_meets();
 #pragma unroll
             for (int t = 0; t < FLOATS; t++)
                 if (t < n_tok) {
@@ -93,6 +102,7 @@ few_kernel(const uint8_t *__restrict__ W, const uint8_t *__restrict__ up, const 
                     to[block * 4 + dword_of(lane & 3)] = p.codes;
                     if ((lane & 3) == 0) reinterpret_cast<uint8_t *>(to + 64)[(block & 3) * 4 + (block >> 2)] = (uint8_t)p.exponent;
                 }
+            wave_meets();
             /* lane 16 g + t of the instruction: block g of token t (those past the last repeat it) */
             const uint32_t *from = packed[wave][min(lane & 15, n_tok - 1)];
 #pragma unroll
