@@ -333,3 +333,10 @@ def test_tokens_quantised_in_the_product(rows, cols, tok):
                 want = multiply(some, MXFP4, x_op, y_type, rows, cols, tok)
                 for pad in (0, 8, 1):
                     assert np.array_equal(multiply(some, x_type, upload_rows(a, cols + pad), y_type, rows, cols, tok, pad, cols + pad), want)
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("rows,cols,tok", [(130, 200, 130), (640, 256, 300), (257, 768, 70), (513, 736, 255), (70, 896, 257), (300, 850, 129), (65, 1408, 513)])
+def test_every_kernel_two_and_three_tiles_past_a_quad(kernel, rows, cols, tok):
+    """2, 6, 7 and 11 column tiles: what follows the last four together, which takes other waits and exponents than they do"""
+    test_every_kernel(kernel, rows, cols, tok)
