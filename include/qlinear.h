@@ -365,7 +365,7 @@ int qlin_mxfp4_operand_dev(uint32_t ggml_type, const void *X, void *operand, int
  * (x_type 39; ldx and workspace are not looked at, qlin_mxfp4_operand_dev makes one for several products) or F32, F16 or BF16
  * rows of pitch ldx, which are quantised into the workspace first: device memory, 16-byte aligned,
  * qlin_mxfp4_gemm_workspace_bytes(n_cols, n_tok) bytes; calls that share one must be ordered on one stream, and graphs that share
- * one must not run at the same time. Y F32 or BF16 (y_type), any pitch >= n_rows and any element alignment. The products of codes are
+ * one must not run at the same time. Y must not overlap with what is read, nor with the workspace. Y F32 or BF16 (y_type), any pitch >= n_rows and any element alignment. The products of codes are
  * exact and their sums fp32 (relative L2 ~1e-7 for F32 results against a double-precision product of the same operands); BF16
  * results are rounded once. The same call gives the same bits. n_cols below 2^24. What would take 2^32 threads or more is refused (16 rows x 512
  * columns of an operand or 8192 elements of blocks take 256 to make, 16 rows x 64 tokens of a product 512 at most). */
@@ -373,7 +373,8 @@ size_t qlin_mxfp4_gemm_workspace_bytes(int n_cols, int n_tok);
 int qlin_mxfp4_gemm_dev(const void *W, uint32_t x_type, const void *X, uint32_t y_type, void *Y, int n_rows, int n_cols, int n_tok, int ldx,
                         int ldy, void *workspace, size_t workspace_bytes, void *stream);
 /* Y[t*ldy + r] = silu(X . Wgate) * (X . Wup), silu(g) = g / (1 + exp(-g)): qlin_gemv_silu_mul_dev for these operands and any number of
- * tokens, the activation applied to the fp32 sums. Wgate and Wup are operands of n_rows x n_cols each. */
+ * tokens, the activation applied to the fp32 sums. Wgate and Wup are operands of n_rows x n_cols each. Where the gate is below -87.3, and
+ * silu of it smaller than 1.1e-36, the result may be 0. */
 int qlin_mxfp4_gemm_silu_mul_dev(const void *Wgate, const void *Wup, uint32_t x_type, const void *X, uint32_t y_type, void *Y, int n_rows,
                                  int n_cols, int n_tok, int ldx, int ldy, void *workspace, size_t workspace_bytes, void *stream);
 

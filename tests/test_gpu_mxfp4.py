@@ -340,3 +340,34 @@ def test_tokens_quantised_in_the_product(rows, cols, tok):
 def test_every_kernel_two_and_three_tiles_past_a_quad(kernel, rows, cols, tok):
     """2, 6, 7 and 11 column tiles: what follows the last four together, which takes other waits and exponents than they do"""
     test_every_kernel(kernel, rows, cols, tok)
+
+
+@pytest.mark.parametrize("tok", [1, 20, 130, 300])
+@pytest.mark.parametrize("sign", [-1.0, 1.0])
+def test_gates_far_from_zero(tok, sign):
+    """gates of 80 to 95 on either side, exact in fp32: silu within 8 half steps and a product's, down to where its reciprocal is subnormal
+    (below -87.3, where it is smaller than 1.1e-36: there it may be lost, not more)"""
+    rows, cols = 144, 64
+    G = np.zeros((rows, 2, 32))
+    G[:, 0, :2] = 64.0, 16.0
+    for r in range(rows):
+        left = 0.5 * (30 * r // rows)  # 0 to 14.5 of numbers that are codes
+        for j, c in enumerate((6.0, 6.0, 2.0, 1.0, 0.5)):
+            if left >= c:
+                G[r, 1, j] = c
+                left -= c
+    G[:, 1, 30:] = 4.0, -4.0  # (keep the block's power of two at 1)
+    G = sign * G.reshape(rows, cols)
+    U = np.zeros((rows, cols))
+    U[:, 2] = np.where(np.arange(rows) % 2 == 0, 1.0, -6.0)
+    x = np.ones((tok, cols))
+    for m in (G, U):
+        assert np.array_equal(f.values_of(f.quantized(m)), m)
+    ops = [operand(F32, m.astype(np.float32), rows, cols)[0] for m in (G, U)]
+    got = multiply(ops, F32, upload_rows(x.astype(np.float32), cols), F32, rows, cols, tok)
+    gate, up = G.sum(axis=1), U.sum(axis=1)
+    assert gate.min() * sign >= -95.0 and np.abs(gate).min() == 80.0 and np.abs(gate).max() >= 94.0
+    want = f.silu_mul(gate, up)
+    lost = gate < -87.3
+    assert (np.abs(got - want)[:, ~lost] <= 9 * 2.0 ** -24 * np.abs(want)[~lost]).all()
+    assert (np.abs(got)[:, lost] <= (1 + 9 * 2.0 ** -24) * np.abs(want)[lost] + 2.0 ** -149).all()
