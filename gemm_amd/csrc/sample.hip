@@ -19,17 +19,20 @@
  * Weights and sums are 64-bit: the borders between tokens lie closer to each other than fp32 sums resolve, and the token is to be the
  * one that the definition gives. A bin's weight is exp(centre) times the sum of exp(offset from the centre), offsets up to 1/128, so
  * that a token costs a polynomial of degree 4 instead of an exponential; the sum is of integers of 2^-40, which do not depend on
- * the order of the additions: the same call gives the same token.
+ * the order of the additions: the same call gives the same token. A bin's sum is off by 2^-41 of itself for the rounding and 2.4e-13 for
+ * the polynomial (of n tokens above 2^21, whose sums must stay within 64 bits, by 2^-62 to 2^-61 n), and all sums lack what is too far down
+ * for a bin, at most 1.3e-14 n.
  *   A list that overflows leaves the row to sample_by_value, which takes three passes over it for each cut: rows of equal logits, of 16-bit
  * logits so large that few values lie near the top, of which a finite mask leaves the others a few bins. 256 rows of 128256 bf16
- * logits of one value 0.5 to 0.8 ms, around -30 instead of 0 0.3 ms, 0.46 with top-p (by 64-bit integer weights of the whole row 1.0 to 2.4, 0.48 and 0.86).
+ * logits of one value 0.5 to 0.8 ms, around -30 instead of 0 0.3 ms, 0.46 with top-p (by 64-bit integer weights of the whole row 1.0 to
+ * 2.4, 0.48 and 0.86).
  *
- * What bounds it, 256 rows of 128256 bf16 logits, by the clock in the kernel when it took 70 us without filters (62.5 now, with fewer
- * register moves in the passes and a part of the row in LDS): 12 us for the first pass (5.5 TB/s), 21 for the bins (14 64-bit vector
- * instructions and an LDS addition per token), 13 to 15 for the list (the row came from the last-level cache again), 8 for sums, sort
- * and cuts, which are chains of a few hundred instructions; with top_k 40, when it took 27 (23.8 now), 12 for the first pass, 3.5 for
- * the list, 8 for the rest. A row alone is bound by what one compute unit loads and executes (16 sequences with top_k 15.8 us, one 19.7 with
- * the two launches that such a row leaves empty, without top_k 36 by several workgroups).
+ * What bounds it, 256 rows of 128256 bf16 logits without filters, 67 us, by the clock in the kernel: 11 us for the first pass (6 TB/s), 21 for
+ * the bins (14 64-bit vector instructions and an LDS addition per token), 14 for the list (what LDS does not hold of the row comes from the
+ * last-level cache again), 9 for sums, sort and cuts, which are chains of a few hundred instructions; the rest is how far the workgroups'
+ * starts and ends lie apart. With top_k 40, 24 us: 9 for the first pass, 2 for the bins of the threads' largest, 3 for the list, 5 for the
+ * rest. A row alone is bound by what one compute unit loads and executes (9 rows of 151936 fp32 logits with top_k 40 19 us, one 22 with the
+ * two launches that such a row leaves empty, 16 bf16 rows without top_k 55, one 36 by several workgroups).
  */
 #include "qlin_device.h"
 #include "qlin_internal.h"
@@ -162,9 +165,9 @@ template <class T> __device__ int nth_of_value(const T *x, int n, uint32_t k, ui
 
 /* This thread's share of elements lo .. hi - 1 of x, in vectors of 16 bytes from the first to the last address on 16; an element before or
  * behind those is a vector of its own, whose other places hold NaN. One load ahead of its use: four waves per SIMD cover the rest, and
- * vectors handed on from register to register are instructions (256 rows without filters 65.5 us, four loads ahead 68). fn(values, index of the first) is
- * called from one place: a workgroup runs most of this file's code once, and what it has not run yet comes from memory, 64 bytes at a
- * time. Unrolled over four vectors, the pass that lists tokens took 15 us instead of 6, most of it for its own instructions. */
+ * vectors handed on from register to register are instructions (256 rows without filters 65.5 us, four loads ahead 68). fn(values, index of
+ * the first) is called from one place: a workgroup runs most of this file's code once, and what it has not run yet comes from memory, 64
+ * bytes at a time. Unrolled over four vectors, the pass that lists tokens took 15 us instead of 6, most of it for its own instructions. */
 template <class T> constexpr int kPer = 16 / sizeof(T);
 template <class T> struct alignas(16) Vec { T v[kPer<T>]; };
 /* The first vectors of a row, which its first pass leaves in LDS for the next ones, each thread its own: 96 KB of the 160 that a workgroup of
@@ -384,9 +387,9 @@ __device__ void sum_bins(const Grid &g, const Holds &h, Shared &s) {
     __syncthreads();
 }
 
-/* The first bin of which `one` holds, and the first of which `other` holds; kLastBin + 1 if there is none. The tests are of running sums, which fall by
- * a rounding here and there: what holds of a bin need not of the next, and of several firsts the least counts. All threads
- * of the workgroup call it. */
+/* The first bin of which `one` holds, and the first of which `other` holds; kLastBin + 1 if there is none. The tests are of running sums,
+ * which fall by a rounding here and there: what holds of a bin need not of the next, and of several firsts the least counts. All threads of
+ * the workgroup call it. */
 struct Pair { int one, other; };
 template <class F, class G> __device__ Pair first_bins(Shared &s, F one, G other) {
     if (threadIdx.x < 2) s.found[threadIdx.x] = kLastBin + 1;
@@ -1044,7 +1047,7 @@ template <class T> __global__ void __launch_bounds__(kThreads) sample_row_kernel
  * Rows that have to be put into bins, by several workgroups each: their ranges, their bins, and the rest by one workgroup, in a launch
  * each. Other rows are the first launch's first workgroup's alone. (What comes after the bins was spread over the workgroups too, the
  * list by one launch and the pick by another, or by the last to finish: what a launch gains over 12 us it loses by starting, and fences
- * between the dies' L2s take 40 to 60 us where 32 sequences meet them.) */
+ * between the dies' L2s took 40 to 60 us where 32 sequences met them; with the eight at most that this route has now it was not measured.) */
 
 constexpr int kMaxParts = 16;
 struct Part { float max, min; };

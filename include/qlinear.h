@@ -365,10 +365,11 @@ int qlin_mxfp4_operand_dev(uint32_t ggml_type, const void *X, void *operand, int
  * (x_type 39; ldx and workspace are not looked at, qlin_mxfp4_operand_dev makes one for several products) or F32, F16 or BF16
  * rows of pitch ldx, which are quantised into the workspace first: device memory, 16-byte aligned,
  * qlin_mxfp4_gemm_workspace_bytes(n_cols, n_tok) bytes; calls that share one must be ordered on one stream, and graphs that share
- * one must not run at the same time. Y must not overlap with what is read, nor with the workspace. Y F32 or BF16 (y_type), any pitch >= n_rows and any element alignment. The products of codes are
- * exact and their sums fp32 (relative L2 ~1e-7 for F32 results against a double-precision product of the same operands); BF16
- * results are rounded once. The same call gives the same bits. n_cols below 2^24. What would take 2^32 threads or more is refused (16 rows x 512
- * columns of an operand or 8192 elements of blocks take 256 to make, 16 rows x 64 tokens of a product 512 at most). */
+ * one must not run at the same time. Y must not overlap with what is read, nor with the workspace. Y F32 or BF16 (y_type), any pitch >=
+ * n_rows and any element alignment. The products of codes are exact and their sums fp32 (relative L2 ~1e-7 for F32 results against a
+ * double-precision product of the same operands); BF16 results are rounded once. The same call gives the same bits. n_cols below 2^24. What
+ * would take 2^32 threads or more is refused (16 rows x 512 columns of an operand or 8192 elements of blocks take 256 to make, 16 rows x 64
+ * tokens of a product 512 at most). */
 size_t qlin_mxfp4_gemm_workspace_bytes(int n_cols, int n_tok);
 int qlin_mxfp4_gemm_dev(const void *W, uint32_t x_type, const void *X, uint32_t y_type, void *Y, int n_rows, int n_cols, int n_tok, int ldx,
                         int ldy, void *workspace, size_t workspace_bytes, void *stream);
@@ -393,8 +394,13 @@ int qlin_mxfp4_gemm_silu_mul_dev(const void *Wgate, const void *Wup, uint32_t x_
  * 0); each of the first four may be NULL, which is 1, 0, 1 and 0 for every sequence (so is a NaN among top_p and min_p; NaN as a
  * temperature is 0). Several +infinities share the weight among them. Weights and sums are 64-bit and do not depend on the order in
  * which the GPU adds them: the same call gives the same token. A token that weighs less than 2e-14 of the first one (31.9 temperatures
- * below it) may count as one without weight, which is never picked; a u within about 1e-12 of a border between two tokens may pick either.
- * n_vocab up to 2^30, n_seq below 2^22. Rows of more than a few thousand equal logits, or that hold +infinity, take several times as long as others.
+ * below it) may count as one without weight: it is never picked, and the sums lack it. A u within 1e-12 of a border between two tokens
+ * (of more than 2^21 tokens, within 5e-19 n_vocab) and what the sums lack (at most 2e-14 n_vocab of the first token's weight) may pick
+ * either. n_vocab up to 2^30, n_seq below 2^22.
+ * Rows of which more than 2048 tokens lie next to a cut take several times as long as others (256 rows of 128256 tokens 0.3 to 0.8 ms
+ * instead of 0.07): equal logits; 16-bit logits around -30 or 30 and further from 0, where they are 1/8 apart and more; a finite mask
+ * (-65504, -1e30) beside logits that spread little over the temperature, while -infinity slows no row down; a u of 1 or more. Rows with
+ * +infinity take about twice as long.
  * workspace: device memory, 256-byte aligned, qlin_sample_workspace_bytes(n_seq, n_vocab) bytes (0: it may be NULL), which holds
  * nothing between calls; calls that share one must be ordered on one stream, and graphs that share one must not run at the same time. */
 size_t qlin_sample_workspace_bytes(int n_seq, int n_vocab);
