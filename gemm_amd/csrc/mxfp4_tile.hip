@@ -15,7 +15,7 @@
  *   What bounds it: 256 x 256 tiles take 0.80 us per column tile on random operands, 5.4 PFLOP/s over the chip, and 0.50 on zeros: the
  * power limit. Beside that the results of a round of tiles leave at its end, with nothing left to multiply: 4096 x 4096 of them 13 us
  * in fp32 and 9 in bf16, launch and first loads included. 4096 x 4096 columns x 4096 tokens 39 us in fp32 (3.5 PFLOP/s) and 35 in bf16, 4096 x 16384 x
- * 4096 113 to 115 (4.8), 14336 x 4096 x 2048 in bf16 63 to 66, gate and up of 512 tokens 35.5.
+ * 4096 113 to 115 (4.8), 14336 x 4096 x 2048 in bf16 63 to 69, gate and up of 512 tokens 35.5 to 37.
  */
 #include "mxfp4.h"
 
