@@ -343,7 +343,7 @@ int qlin_moe_ffn_static_dev(uint32_t type_gate, uint32_t type_up, uint32_t type_
  * Products whose both factors are MXFP4, on the scaled 4-bit matrix instructions: 32 elements share a power of two and hold an
  * e2m1 number each (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign). No counterpart in the reference, which decodes MXFP4 weights
  * (common/ggml_dequant.h:2818-2830) and multiplies in fp32; what these calls round and the others do not are the activations.
- * Pointers and stream belong to the current device, as in the group above.
+ * Pointers and stream belong to the current device, as in the group above. What a call writes must not overlap with what it reads.
  *
  * Quantisation: a block's power of two is that of its largest magnitude, divided by four (exponent byte floor(log2 max|x|) + 125, at
  * least 0); its codes are the nearest e2m1 numbers, on a tie the one with the even code, 6 beyond 6. A block with an infinity or a
@@ -365,8 +365,8 @@ int qlin_mxfp4_operand_dev(uint32_t ggml_type, const void *X, void *operand, int
  * (x_type 39; ldx and workspace are not looked at, qlin_mxfp4_operand_dev makes one for several products) or F32, F16 or BF16
  * rows of pitch ldx, which are quantised into the workspace first: device memory, 16-byte aligned,
  * qlin_mxfp4_gemm_workspace_bytes(n_cols, n_tok) bytes; calls that share one must be ordered on one stream, and graphs that share
- * one must not run at the same time. Y must not overlap with what is read, nor with the workspace. Y F32 or BF16 (y_type), any pitch >=
- * n_rows and any element alignment. The products of codes are exact and their sums fp32 (relative L2 ~1e-7 for F32 results against a
+ * one must not run at the same time. Nor may Y overlap with the workspace. Y F32 or BF16 (y_type), any pitch >= n_rows and any element
+ * alignment. The products of codes are exact and their sums fp32 (relative L2 ~1e-7 for F32 results against a
  * double-precision product of the same operands); BF16 results are rounded once. The same call gives the same bits. n_cols below 2^24. What
  * would take 2^32 threads or more is refused (16 rows x 512 columns of an operand or 8192 elements of blocks take 256 to make, 16 rows x 64
  * tokens of a product 512 at most). */
