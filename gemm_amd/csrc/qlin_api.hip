@@ -1536,6 +1536,80 @@ int qlin_mxfp4_gemm_silu_mul_dev(const void *Wgate, const void *Wup, uint32_t x_
     return mxfp4_gemm(Wgate, Wup, true, x_type, X, y_type, Y, n_rows, n_cols, n_tok, ldx, ldy, workspace, workspace_bytes, stream);
 }
 
+/* ------------------------------------------------------------------ routing by scores, low-rank adapters */
+
+int qlin_moe_route_scores_dev(int score, uint32_t type, const void *logits, int n_tok, int n_expert, int ld, const float *bias, int n_group, int n_group_used,
+                              int group_top, int top_k, int renorm, float scale, int32_t *expert_idx, float *expert_w, void *stream) {
+    if (!float_bytes(type)) return fail(QLIN_ERR_TYPE, "logits are F32, F16 or BF16 (got type %u)", type);
+    if (score != QLIN_ROUTE_SOFTMAX && score != QLIN_ROUTE_SIGMOID) return fail(QLIN_ERR_ARG, "score %d: QLIN_ROUTE_SOFTMAX or QLIN_ROUTE_SIGMOID", score);
+    if (n_expert < 1 || n_expert > kRouteMaxExperts) return fail(QLIN_ERR_ARG, "routing to %d experts (1 to %d)", n_expert, kRouteMaxExperts);
+    if (n_group < 1 || n_group > kRouteMaxGroups || n_expert % n_group || n_group_used < 1 || n_group_used > n_group || group_top < 1 || group_top > 2)
+        return fail(QLIN_ERR_ARG, "%d of %d groups of %d experts by their %d largest", n_group_used, n_group, n_expert, group_top);
+    if (top_k < 1 || top_k > n_expert / n_group * n_group_used) return fail(QLIN_ERR_ARG, "%d experts out of %d groups of %d", top_k, n_group_used, n_expert / n_group);
+    if (int rc = check_float_rows("logits", type, logits, n_tok, n_expert, ld)) return rc;
+    if (n_tok == 0) return QLIN_OK;
+    if (!launch_takes((size_t)n_tok, 64)) return fail(QLIN_ERR_ARG, "routing %d tokens in one call", n_tok);
+    if (!expert_idx || !expert_w) return fail(QLIN_ERR_ARG, "null pointer");
+    if (!aligned(bias, 4) || !aligned(expert_idx, 4) || !aligned(expert_w, 4)) return fail(QLIN_ERR_ARG, "misaligned pointer");
+    if (int rc = init_once()) return rc;
+    const RouteCall c = {score, logits, n_tok, n_expert, ld, bias, n_group, n_group_used, group_top, top_k, renorm != 0, scale, expert_idx, expert_w, (hipStream_t)stream};
+    HIP_TRY(launch_moe_route_scores(type, c));
+    return QLIN_OK;
+}
+
+static_assert(sizeof(qlin_lora) == sizeof(LoraEntry) && sizeof(qlin_lora) == 24 && sizeof(qlin_lora_tensor) == sizeof(LoraTensor) && kLoraMaxRank == QLIN_LORA_MAX_RANK,
+              "the kernels' structures are the public header's");
+
+size_t qlin_lora_workspace_bytes(int n_mat, int max_rank, int n_cols, int n_tok) {
+    if (n_mat <= 0 || max_rank <= 0 || n_cols <= 0 || n_tok <= 0) return 0;
+    return lora_workspace_bytes(n_mat, max_rank, n_cols, n_tok);
+}
+
+static int lora_call(LoraCall &c, uint32_t lora_type, void *workspace, size_t workspace_bytes) {
+    if (!float_bytes(lora_type) || !float_bytes(c.x_type) || !float_bytes(c.y_type) || !float_bytes(c.out_type))
+        return fail(QLIN_ERR_TYPE, "adapters, activations and results are F32, F16 or BF16 (got types %u, %u, %u, %u)", lora_type, c.x_type, c.y_type, c.out_type);
+    if (c.n_adapter < 0 || c.max_rank < 1 || c.max_rank > kLoraMaxRank) return fail(QLIN_ERR_ARG, "%d adapters of rank %d (1 to %d)", c.n_adapter, c.max_rank, kLoraMaxRank);
+    if (c.n_cols < 1 || c.n_cols >= 1 << 24) return fail(QLIN_ERR_ARG, "rows of %d columns", c.n_cols);
+    if (int rc = check_float_rows("X", c.x_type, c.X, c.n_tok, c.n_cols, c.ldx)) return rc;
+    bool rows = false;
+    for (int i = 0; i < c.n_mat; i++) {
+        const LoraTensor &m = c.m[i];
+        if (m.n_rows < 0 || m.ldy < m.n_rows || m.ldo < m.n_rows) return fail(QLIN_ERR_ARG, "negative size or a row pitch below the row");
+        if (m.n_rows == 0 || c.n_tok == 0) continue;
+        rows = true;
+        if (!m.Y || (!m.out && (i == 0 || !c.pair)) || (!m.adapters && c.n_adapter)) return fail(QLIN_ERR_ARG, "null pointer");
+        if (!aligned(m.adapters, 8) || !aligned(m.Y, float_bytes(c.y_type)) || !aligned(m.out, float_bytes(c.out_type))) return fail(QLIN_ERR_ARG, "misaligned pointer");
+    }
+    if (!rows) return QLIN_OK;
+    if (!c.ids || !aligned(c.ids, 4)) return fail(QLIN_ERR_ARG, "null or misaligned pointer");
+    const LoraPlan p = lora_plan(c);
+    if (!launch_takes(p.shrink_workgroups(), kLoraThreads) || !launch_takes(p.expand_workgroups(), kLoraThreads)) return fail(QLIN_ERR_ARG, "%d tokens in one call", c.n_tok);
+    const size_t need = lora_workspace_bytes(c.n_mat, c.max_rank, c.n_cols, c.n_tok);
+    if (!workspace || !aligned(workspace, 16) || workspace_bytes < need) return fail(QLIN_ERR_ARG, "the workspace needs %zu bytes, 16-byte aligned", need);
+    if (int rc = init_once()) return rc;
+    c.workspace = static_cast<float *>(workspace);
+    HIP_TRY(launch_lora(lora_type, c, p));
+    return QLIN_OK;
+}
+
+int qlin_lora_add_dev(int n_mat, const qlin_lora_tensor *tensors, uint32_t lora_type, int n_adapter, int max_rank, const int32_t *ids, uint32_t x_type, const void *X,
+                      uint32_t y_type, uint32_t out_type, int n_cols, int n_tok, int ldx, void *workspace, size_t workspace_bytes, void *stream) {
+    if (n_mat < 1 || n_mat > 3 || !tensors) return fail(QLIN_ERR_ARG, "one to three tensors per call");
+    LoraCall c = {n_mat, false, {}, n_adapter, max_rank, ids, x_type, y_type, out_type, X, n_cols, n_tok, ldx, nullptr, (hipStream_t)stream};
+    for (int i = 0; i < n_mat; i++)
+        c.m[i] = {reinterpret_cast<const LoraEntry *>(tensors[i].adapters), tensors[i].Y, tensors[i].out, tensors[i].n_rows, tensors[i].ldy, tensors[i].ldo, 0};
+    return lora_call(c, lora_type, workspace, workspace_bytes);
+}
+
+int qlin_lora_silu_mul_dev(const qlin_lora *gate_adapters, const qlin_lora *up_adapters, uint32_t lora_type, int n_adapter, int max_rank, const int32_t *ids, uint32_t x_type,
+                           const void *X, uint32_t y_type, const void *gate, const void *up, uint32_t out_type, void *out, int n_rows, int n_cols, int n_tok, int ldx, int ldy,
+                           int ldo, void *workspace, size_t workspace_bytes, void *stream) {
+    LoraCall c = {2, true, {}, n_adapter, max_rank, ids, x_type, y_type, out_type, X, n_cols, n_tok, ldx, nullptr, (hipStream_t)stream};
+    c.m[0] = {reinterpret_cast<const LoraEntry *>(gate_adapters), gate, out, n_rows, ldy, ldo, 0};
+    c.m[1] = {reinterpret_cast<const LoraEntry *>(up_adapters), up, nullptr, n_rows, ldy, ldo, 0};
+    return lora_call(c, lora_type, workspace, workspace_bytes);
+}
+
 /* ------------------------------------------------------------------ sampling */
 
 size_t qlin_sample_workspace_bytes(int n_seq, int n_vocab) { return n_seq > 0 && n_vocab > 0 ? sample_workspace_bytes(n_seq, n_vocab) : 0; }

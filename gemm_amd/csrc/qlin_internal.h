@@ -284,6 +284,54 @@ struct SampleCall {
 constexpr int kSampleThreads = 1024; /* of a workgroup; one for each sequence at least */
 size_t sample_workspace_bytes(int n_seq, int n_vocab);
 hipError_t launch_sample(uint32_t type, const SampleCall &c);
+/* low-rank adapters beside a shared projection (lora.hip): the layouts of the public header's qlin_lora and qlin_lora_tensor */
+struct LoraEntry {
+    const void *A, *B;
+    int32_t rank;
+    float scale;
+};
+struct LoraTensor {
+    const LoraEntry *adapters;
+    const void *Y;
+    void *out;
+    int32_t n_rows, ldy, ldo, unused;
+};
+constexpr int kLoraMaxRank = 256; /* = QLIN_LORA_MAX_RANK of the public header */
+constexpr int kLoraThreads = 256;
+struct LoraCall {
+    int n_mat; /* 1..3; pair (gate and up): 2, the result where m[0] says */
+    bool pair;
+    LoraTensor m[3];
+    int n_adapter, max_rank;
+    const int32_t *ids;
+    uint32_t x_type, y_type, out_type;
+    const void *X;
+    int n_cols, n_tok, ldx;
+    float *workspace;
+    hipStream_t stream;
+};
+struct LoraPlan {
+    int tiles, slots, parts, rank_pad, rank_tiles, rank_blocks, row_tiles, row_blocks[3], row_blocks_all, n_mat;
+    unsigned long long shrink_workgroups() const { return (unsigned long long)tiles * n_mat * rank_blocks * parts * slots; }
+    unsigned long long expand_workgroups() const { return (unsigned long long)tiles * row_blocks_all * slots; }
+};
+size_t lora_workspace_bytes(int n_mat, int max_rank, int n_cols, int n_tok);
+LoraPlan lora_plan(const LoraCall &c);
+hipError_t launch_lora(uint32_t w_type, const LoraCall &c, const LoraPlan &p);
+/* the experts of each token and their weights (moe_route_scores.hip); bias may be null */
+struct RouteCall {
+    int score; /* 0: softmax, 1: sigmoid */
+    const void *logits;
+    int n_tok, n_expert, ld;
+    const float *bias;
+    int n_group, n_group_used, group_top, top_k, renorm;
+    float scale;
+    int32_t *idx;
+    float *w;
+    hipStream_t stream;
+};
+constexpr int kRouteMaxExperts = 4096, kRouteMaxGroups = 256;
+hipError_t launch_moe_route_scores(uint32_t type, const RouteCall &c);
 /* measurement probes (probe.hip): a register-only MFMA loop (flops issued come back in *flops) with the
  * cycle and 100 MHz counters around it, and a streaming read of a device buffer */
 hipError_t launch_probe_mfma(int iters, int n_cu, hipStream_t stream, double *flops);

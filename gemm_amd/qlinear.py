@@ -82,6 +82,8 @@ SIGNATURES = {
     "qlin_gemm_f32_dev": (C.c_int, [C.c_uint32, _vp, _vp, _vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, _vp]),
     "qlin_moe_workspace_bytes": (C.c_size_t, [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int]),
     "qlin_moe_route_dev": (C.c_int, [_vp, C.c_int, C.c_int, C.c_int, _vp, _vp, _vp]),
+    "qlin_moe_route_scores_dev": (C.c_int, [C.c_int, C.c_uint32, _vp, C.c_int, C.c_int, C.c_int, _vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int,
+                                            C.c_float, _vp, _vp, _vp]),
     "qlin_moe_ffn_dev": (C.c_int, [C.c_uint32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, C.c_int, C.c_int, C.c_int,
                                    C.c_int, C.c_int, _vp, _vp]),
     "qlin_moe_ffn_types_dev": (C.c_int, [C.c_uint32, C.c_uint32, C.c_uint32, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
@@ -95,6 +97,11 @@ SIGNATURES = {
     "qlin_mxfp4_gemm_dev": (C.c_int, [_vp, C.c_uint32, _vp, C.c_uint32, _vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, _vp, C.c_size_t, _vp]),
     "qlin_mxfp4_gemm_silu_mul_dev": (C.c_int, [_vp, _vp, C.c_uint32, _vp, C.c_uint32, _vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, _vp,
                                                C.c_size_t, _vp]),
+    "qlin_lora_workspace_bytes": (C.c_size_t, [C.c_int, C.c_int, C.c_int, C.c_int]),
+    "qlin_lora_add_dev": (C.c_int, [C.c_int, _vp, C.c_uint32, C.c_int, C.c_int, _vp, C.c_uint32, _vp, C.c_uint32, C.c_uint32, C.c_int, C.c_int, C.c_int,
+                                    _vp, C.c_size_t, _vp]),
+    "qlin_lora_silu_mul_dev": (C.c_int, [_vp, _vp, C.c_uint32, C.c_int, C.c_int, _vp, C.c_uint32, _vp, C.c_uint32, _vp, _vp, C.c_uint32, _vp, C.c_int, C.c_int,
+                                         C.c_int, C.c_int, C.c_int, C.c_int, _vp, C.c_size_t, _vp]),
     "qlin_sample_workspace_bytes": (C.c_size_t, [C.c_int, C.c_int]),
     "qlin_sample_dev": (C.c_int, [C.c_uint32, _vp, C.c_int, C.c_int, C.c_int, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, C.c_size_t, _vp]),
     "qlin_gguf_open": (C.c_int, [C.c_char_p, _vp]),
@@ -368,6 +375,16 @@ def moe_route_dev(dlogits, n_tok, n_expert, top_k, didx, dw, stream=None):
     check(load().qlin_moe_route_dev(dlogits.ptr, n_tok, n_expert, top_k, didx.ptr, dw.ptr, stream))
 
 
+ROUTE_SOFTMAX, ROUTE_SIGMOID = 0, 1  # QLIN_ROUTE_* of include/qlinear.h
+
+
+def moe_route_scores_dev(score, logits_type, dlogits, n_tok, n_expert, ld, dbias, n_group, n_group_used, group_top, top_k, renorm, scale, didx, dw,
+                         stream=None):
+    """dbias may be None"""
+    check(load().qlin_moe_route_scores_dev(score, logits_type, dlogits.ptr, n_tok, n_expert, ld, dbias.ptr if dbias is not None else None, n_group,
+                                           n_group_used, group_top, top_k, int(renorm), scale, didx.ptr, dw.ptr, stream))
+
+
 def moe_ffn_dev(type_id, dgate, dup, ddown, dX, didx, dw, dout, n_tok, top_k, n_embd, n_ff, n_expert, dws,
                 stream=None):
     check(load().qlin_moe_ffn_dev(type_id, dgate.ptr, dup.ptr, ddown.ptr, dX.ptr, didx.ptr, dw.ptr, dout.ptr,
@@ -408,6 +425,36 @@ def mxfp4_gemm_dev(dW, x_type, dX, y_type, dY, n_rows, n_cols, n_tok, ldx, ldy, 
 def mxfp4_gemm_silu_mul_dev(dWgate, dWup, x_type, dX, y_type, dY, n_rows, n_cols, n_tok, ldx, ldy, dws, stream=None):
     check(load().qlin_mxfp4_gemm_silu_mul_dev(dWgate.ptr, dWup.ptr, x_type, dX.ptr, y_type, dY.ptr, n_rows, n_cols, n_tok, ldx, ldy,
                                               dws.ptr if dws is not None else None, dws.nbytes if dws is not None else 0, stream))
+
+
+LORA_MAX_RANK = 256  # QLIN_LORA_MAX_RANK of include/qlinear.h
+# an entry of a tensor's table of adapters, struct qlin_lora
+LORA_DTYPE = np.dtype([("A", np.uint64), ("B", np.uint64), ("rank", np.int32), ("scale", np.float32)])
+
+
+class LoraTensor(C.Structure):
+    """struct qlin_lora_tensor"""
+    _fields_ = [("adapters", _vp), ("Y", _vp), ("out", _vp), ("n_rows", C.c_int32), ("ldy", C.c_int32), ("ldo", C.c_int32), ("unused", C.c_int32)]
+
+
+def lora_tensors(projections):
+    """projections: (dadapters, dY, dout, n_rows, ldy, ldo) each, one to three; to be kept and passed to lora_add_dev as often as they are used"""
+    return (LoraTensor * len(projections))(*[LoraTensor(a.ptr, y.ptr, o.ptr, n_rows, ldy, ldo, 0) for a, y, o, n_rows, ldy, ldo in projections])
+
+
+def lora_workspace_bytes(n_mat, max_rank, n_cols, n_tok):
+    return load().qlin_lora_workspace_bytes(n_mat, max_rank, n_cols, n_tok)
+
+
+def lora_add_dev(tensors, lora_type, n_adapter, max_rank, dids, x_type, dX, y_type, out_type, n_cols, n_tok, ldx, dws, stream=None):
+    check(load().qlin_lora_add_dev(len(tensors), C.addressof(tensors), lora_type, n_adapter, max_rank, dids.ptr, x_type, dX.ptr, y_type, out_type, n_cols, n_tok,
+                                   ldx, dws.ptr, dws.nbytes, stream))
+
+
+def lora_silu_mul_dev(dgate_adapters, dup_adapters, lora_type, n_adapter, max_rank, dids, x_type, dX, y_type, dgate, dup, out_type, dout, n_rows, n_cols, n_tok,
+                      ldx, ldy, ldo, dws, stream=None):
+    check(load().qlin_lora_silu_mul_dev(dgate_adapters.ptr, dup_adapters.ptr, lora_type, n_adapter, max_rank, dids.ptr, x_type, dX.ptr, y_type, dgate.ptr,
+                                        dup.ptr, out_type, dout.ptr, n_rows, n_cols, n_tok, ldx, ldy, ldo, dws.ptr, dws.nbytes, stream))
 
 
 def sample_workspace_bytes(n_seq, n_vocab):

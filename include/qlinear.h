@@ -313,6 +313,22 @@ int qlin_gemm_f32_any_dev(uint32_t ggml_type, const void *W, const float *X, flo
 size_t qlin_moe_workspace_bytes(int n_tok, int top_k, int n_embd, int n_ff, int n_expert);
 int qlin_moe_route_dev(const float *router_logits, int n_tok, int n_expert, int top_k,
                        int32_t *expert_idx, float *expert_w, void *stream);
+/* The experts of each token and their weights for the routers that qlin_moe_route_dev does not cover, in the layout that
+ * qlin_moe_ffn_dev takes. logits: F32, F16 or BF16 rows of n_expert, row pitch ld elements. Expert e scores s_e = exp(x_e - max) / sum of
+ * exp(x - max) (QLIN_ROUTE_SOFTMAX) or 1 / (1 + exp(-x_e)) (QLIN_ROUTE_SIGMOID), and is chosen by s_e + bias[e] (bias: n_expert floats, the
+ * balance that a model learned; NULL: by s_e, whose order is the logits'). Of n_group groups of consecutive experts the n_group_used with the
+ * largest sum of their group_top (1 or 2) largest values stay; of the experts in those the top_k largest are chosen. The choice is that of
+ * 64-bit values, equal ones by index, and expert_idx has them in that order, largest first.
+ * expert_w = scale * s_e, with renorm not 0 divided by the sum of the chosen scores (the bias is in the choice only).
+ * A logit of NaN or -infinity takes its expert out of the softmax and of the choice, a bias of NaN or -infinity out of the choice; a token
+ * of which fewer than top_k experts are left has the index -1 and the weight 0 in the last places, which qlin_moe_ffn_dev passes over.
+ * Several logits of +infinity share the softmax among them. n_expert up to 4096, n_group up to 256 and a divisor of n_expert, top_k up to
+ * the number of experts in n_group_used groups. No workspace. What the call writes must not overlap with what it reads. */
+#define QLIN_ROUTE_SOFTMAX 0
+#define QLIN_ROUTE_SIGMOID 1
+int qlin_moe_route_scores_dev(int score, uint32_t logits_type, const void *logits, int n_tok, int n_expert, int ld, const float *bias,
+                              int n_group, int n_group_used, int group_top, int top_k, int renorm, float scale, int32_t *expert_idx,
+                              float *expert_w, void *stream);
 int qlin_moe_ffn_dev(uint32_t ggml_type, const void *gate_exps, const void *up_exps,
                      const void *down_exps, const uint16_t *X, const int32_t *expert_idx,
                      const float *expert_w, float *out, int n_tok, int top_k, int n_embd,
@@ -378,6 +394,51 @@ int qlin_mxfp4_gemm_dev(const void *W, uint32_t x_type, const void *X, uint32_t 
  * silu of it smaller than 1.1e-36, the result may be 0. */
 int qlin_mxfp4_gemm_silu_mul_dev(const void *Wgate, const void *Wup, uint32_t x_type, const void *X, uint32_t y_type, void *Y, int n_rows,
                                  int n_cols, int n_tok, int ldx, int ldy, void *workspace, size_t workspace_bytes, void *stream);
+
+/* ------------------------------------------------------------------ low-rank adapters
+ * What the adapters of many requests add to projections that all requests share:
+ *   out[t*ldo + r] = Y[t*ldy + r] + scale * sum_k B[r, k] sum_c A[k, c] X[t*ldx + c]      with the A, B and scale of adapter ids[t]
+ * after the call that made Y (qlin_gemv_multi_dev, qlin_gemm_bf16_multi_dev, qlin_mxfp4_gemm_dev, ...). No counterpart in the reference.
+ * Pointers and stream belong to the current device, as in the groups above.
+ *
+ * A tensor's adapters are a table in device memory, one entry each; A and B are packed rows, as the lora_a and lora_b tensors of an
+ * adapter file are, all of one type (F32, F16 or BF16). The kernels read the table when they run: an engine changes an entry on the stream
+ * between two calls, or between two replays of a graph. An entry with a null pointer, or whose rank is not in 1..max_rank, is no adapter,
+ * nor is an id outside of 0..n_adapter-1 (-1 for a request without one): such a token's out is its Y. A and B need an element's
+ * alignment; 16 bytes, and n_cols of a multiple of 8, X on 16 bytes and ldx of 16 bytes, are read faster, as are ranks of a multiple of 4. */
+#define QLIN_LORA_MAX_RANK 256
+typedef struct qlin_lora {
+    const void *A;  /* [rank, n_cols] */
+    const void *B;  /* [n_rows, rank] */
+    int32_t rank;
+    float scale;    /* alpha / rank, as the adapter's file says */
+} qlin_lora;
+typedef struct qlin_lora_tensor { /* one projection; in host memory, read before the call returns */
+    const qlin_lora *adapters;    /* n_adapter entries in device memory */
+    const void *Y;                /* [n_tok, n_rows], y_type, row pitch ldy elements */
+    void *out;                    /* out_type, row pitch ldo; Y itself where type and pitch are the same */
+    int32_t n_rows, ldy, ldo, unused;
+} qlin_lora_tensor;
+/* One to three tensors that share the activations X (F32, F16 or BF16, row pitch ldx). ids: n_tok adapter numbers in device memory, in any
+ * order (neighbours that share an adapter share its loads). y_type and out_type: F32, F16 or BF16. The sums are fp32, the products of an
+ * adapter and X exact, and a 16-bit result is rounded once; the same call gives the same bits. An infinity or a NaN in X or in an adapter
+ * stays with its tokens. workspace: device memory, 16-byte aligned, qlin_lora_workspace_bytes(n_mat, max_rank, n_cols, n_tok) bytes (0 for
+ * sizes that are not positive), which holds nothing between calls; calls that share one must be ordered on one stream, and graphs that
+ * share one must not run at the same time. What a call writes must not overlap with what it reads, but for an out that is its Y. n_cols
+ * below 2^24, max_rank up to QLIN_LORA_MAX_RANK; what would take 2^32 threads or more is refused (64 tokens x 64 rows take 256). */
+size_t qlin_lora_workspace_bytes(int n_mat, int max_rank, int n_cols, int n_tok);
+int qlin_lora_add_dev(int n_mat, const qlin_lora_tensor *tensors, uint32_t lora_type, int n_adapter, int max_rank, const int32_t *ids,
+                      uint32_t x_type, const void *X, uint32_t y_type, uint32_t out_type, int n_cols, int n_tok, int ldx, void *workspace,
+                      size_t workspace_bytes, void *stream);
+/* Gate and up with their adapters and the activation: out[t*ldo + r] = silu(gate[t*ldy + r] + its adapter's) * (up[t*ldy + r] + its
+ * adapter's), silu(g) = g / (1 + exp(-g)), from the fp32 sums. gate and up are n_rows x n_tok results of y_type, made before by
+ * qlin_gemv_multi_dev or qlin_gemm_bf16_multi_dev (the fused calls with silu have no place for an adapter); out may be either of them where
+ * type and pitch are the same. workspace as above with n_mat 2. Where the gate is below -87.3, and silu of it smaller than 1.1e-36,
+ * the result may be 0. */
+int qlin_lora_silu_mul_dev(const qlin_lora *gate_adapters, const qlin_lora *up_adapters, uint32_t lora_type, int n_adapter, int max_rank,
+                           const int32_t *ids, uint32_t x_type, const void *X, uint32_t y_type, const void *gate, const void *up,
+                           uint32_t out_type, void *out, int n_rows, int n_cols, int n_tok, int ldx, int ldy, int ldo, void *workspace,
+                           size_t workspace_bytes, void *stream);
 
 /* ------------------------------------------------------------------ sampling
  * ids[s] = the next token of sequence s from its logits (F32, F16 or BF16, row pitch ld elements), where the greedy pick of

@@ -1,0 +1,154 @@
+"""qlin_moe_route_scores_dev against its definition in 64 bits: every score, group and type, rows of which nothing or too little is there,
+equal and nearly equal values, one expert to 4096, one token to thousands."""
+import numpy as np
+import pytest
+
+from gemm_amd import qlinear
+from tests import adapter_formulas as f
+
+pytestmark = pytest.mark.gpu
+F32, F16, BF16 = f.F32, f.F16, f.BF16
+NAN, INF = np.nan, np.inf
+
+
+def call(x, t, sigmoid, bias, n_group, used, group_top, k, renorm, scale, pad=0, stream=None):
+    """x: float rows -> (indices, weights, the logits' values)"""
+    n_tok, n = x.shape
+    wide = np.full((n_tok, n + pad), 1e4, np.float32)
+    wide[:, :n] = x
+    raw, v = f.as_type(wide, t)
+    dx, db = qlinear.DevBuf.from_numpy(raw), qlinear.DevBuf.from_numpy(np.asarray(bias, np.float32)) if bias is not None else None
+    guard = 64
+    didx = qlinear.DevBuf.from_numpy(np.full(n_tok * k + guard, 77, np.int32))
+    dw = qlinear.DevBuf.from_numpy(np.full(n_tok * k + guard, 77, np.float32))
+    qlinear.moe_route_scores_dev(int(sigmoid), t, dx, n_tok, n, n + pad, db, n_group, used, group_top, k, renorm, scale, didx, dw, stream)
+    qlinear.sync(stream)
+    idx, w = didx.to_numpy(np.int32, (n_tok * k + guard,)), dw.to_numpy(np.float32, (n_tok * k + guard,))
+    assert (idx[n_tok * k:] == 77).all() and (w[n_tok * k:] == 77).all()
+    return idx[:n_tok * k].reshape(n_tok, k), w[:n_tok * k].reshape(n_tok, k), v[:, :n]
+
+
+def check(x, t, sigmoid, bias, n_group, used, group_top, k, renorm, scale, pad=0):
+    idx, w, v = call(x, t, sigmoid, bias, n_group, used, group_top, k, renorm, scale, pad)
+    b = None if bias is None else np.asarray(bias, np.float32).astype(np.float64)
+    for row in range(len(x)):
+        want_idx, want_w = f.route(v[row], sigmoid, b, n_group, used, group_top, k, renorm, float(np.float32(scale)))
+        assert idx[row].tolist() == want_idx.tolist(), row
+        assert (np.abs(w[row] - want_w) <= f.route_bound(v[row], sigmoid, want_idx, want_w)).all(), (row, w[row], want_w)
+    return idx, w
+
+
+def rows(seed, n_tok, n, spread=1.5):
+    return spread * np.random.default_rng(seed).standard_normal((n_tok, n))
+
+
+def small_bias(seed, n):
+    return 0.05 * np.random.default_rng(seed).standard_normal(n)
+
+
+@pytest.mark.parametrize("sigmoid", [False, True])
+@pytest.mark.parametrize("biased", [False, True])
+@pytest.mark.parametrize("t", [F32, F16, BF16])
+@pytest.mark.parametrize("n_tok,n,n_group,used,group_top,k,pad", [
+    (1, 128, 1, 1, 1, 8, 0), (3, 256, 8, 4, 2, 8, 0), (5, 60, 1, 1, 1, 4, 4), (4, 160, 8, 3, 1, 6, 3), (70, 64, 4, 2, 2, 6, 0), (2, 1, 1, 1, 1, 1, 0), (7, 2, 2, 1, 1, 1, 1),
+    (2, 17, 1, 1, 1, 17, 0), (3, 512, 16, 5, 2, 10, 0), (2, 513, 27, 11, 2, 9, 2), (9, 96, 32, 7, 2, 5, 0), (2, 384, 1, 1, 1, 22, 5), (3, 72, 72, 9, 2, 9, 0)])
+def test_routes(sigmoid, biased, t, n_tok, n, n_group, used, group_top, k, pad):
+    x = rows(n_tok * n + k, n_tok, n)
+    check(x, t, sigmoid, small_bias(n, n) if biased else None, n_group, used, group_top, k, biased != sigmoid, 2.5 if sigmoid else 1.0, pad)
+
+
+@pytest.mark.parametrize("n,n_group,k", [(1024, 1, 64), (1000, 8, 65), (4096, 256, 100), (4096, 1, 4096), (300, 1, 300)])
+def test_many_experts_and_places(n, n_group, k):
+    check(rows(n, 2, n), F32, True, small_bias(1, n), n_group, max(1, n_group // 2), 2, min(k, n // n_group * max(1, n_group // 2)), True, 1.0)
+    check(rows(n, 2, n), BF16, False, None, n_group, n_group, 1, k, False, 1.0)
+
+
+@pytest.mark.parametrize("n_tok", [64, 65, 1000, 4097])
+def test_many_tokens(n_tok):
+    check(rows(n_tok, n_tok, 64), F32, True, small_bias(2, 64), 8, 4, 2, 6, True, 2.5)
+
+
+@pytest.mark.parametrize("sigmoid", [False, True])
+@pytest.mark.parametrize("biased", [False, True])
+@pytest.mark.parametrize("n,n_group", [(64, 1), (64, 8), (200, 4)])
+def test_what_is_not_there(sigmoid, biased, n, n_group):
+    """nothing, one expert, fewer than top_k, one group, the type's lowest value, infinities and NaN"""
+    x = rows(3, 12, n)
+    x[0] = -INF
+    x[1] = NAN
+    x[2] = -INF
+    x[2, n // 2 + 1] = -3.0
+    x[3, 3:] = -INF
+    x[4, n // n_group:] = NAN
+    x[5] = np.finfo(np.float32).min
+    x[6, :] = np.finfo(np.float32).min
+    x[6, 5:9] = [1.0, 2.0, 0.5, 0.25]
+    x[7, [4, 9, 30]] = INF
+    x[8, ::2] = NAN
+    x[9] = 0.0
+    x[10, :n - 1] = -INF
+    x[11, 7] = INF
+    bias = small_bias(4, n) if biased else None
+    if biased:
+        bias[[8, 40]] = [-INF, NAN]
+    for k in (1, 5, 8):
+        for renorm in (False, True):
+            check(x, F32, sigmoid, bias, n_group, max(1, n_group // 2), 2, k, renorm, 1.0)
+    check(np.where(x < -1e38, -INF, x), BF16, sigmoid, bias, n_group, max(1, n_group // 2), 1, 6, True, 1.0)
+
+
+@pytest.mark.parametrize("t", [F32, BF16])
+@pytest.mark.parametrize("biased", [False, True])
+def test_equal_values_go_by_index(t, biased):
+    rng = np.random.default_rng(5)
+    x = rng.integers(-2, 3, (40, 128)).astype(np.float32)
+    bias = rng.integers(0, 2, 128) * 0.25 if biased else None
+    for sigmoid in (False, True):
+        for group_top in (1, 2):
+            check(x, t, sigmoid, bias, 8, 3, group_top, 12, True, 1.0)
+            check(x, t, sigmoid, bias, 1, 1, group_top, 12, True, 1.0)
+
+
+@pytest.mark.parametrize("sigmoid", [False, True])
+@pytest.mark.parametrize("n,n_group,k", [(256, 8, 8), (128, 1, 8), (60, 1, 4)])
+def test_neighbours(sigmoid, n, n_group, k):
+    """values an fp32 step or less apart: the choice is the one of 64 bits"""
+    rng = np.random.default_rng(n)
+    x = np.float32(0.7) + rng.integers(-3, 4, (64, n)) * np.float32(2.0 ** -24)
+    bias = (np.float32(0.3) + rng.integers(-3, 4, n) * np.float32(2.0 ** -25)).astype(np.float32)
+    check(x, F32, sigmoid, None, n_group, max(1, n_group // 2), 2, k, True, 1.0)
+    check(x, F32, sigmoid, bias, n_group, max(1, n_group // 2), 2, k, True, 1.0)
+    check(x, F32, sigmoid, bias, n_group, max(1, n_group // 2), 1, k, False, 1.0)
+
+
+def test_saturated_sigmoid():
+    """scores of 1 in 64 bits stay in the order of their logits without a bias, and go by index with one"""
+    x = np.tile(np.linspace(38, 60, 64, dtype=np.float32), (2, 1))
+    idx, w = check(x, F32, True, None, 1, 1, 1, 5, False, 1.0)
+    assert idx[0].tolist() == [63, 62, 61, 60, 59]
+    idx, w = check(x, F32, True, np.zeros(64), 1, 1, 1, 5, False, 1.0)
+    assert idx[0].tolist() == [0, 1, 2, 3, 4]
+    x = np.tile(np.linspace(-120, -60, 64, dtype=np.float32), (2, 1))
+    check(x, F32, True, np.zeros(64), 1, 1, 1, 5, True, 1.0)
+    check(x, F32, False, np.zeros(64), 1, 1, 1, 5, True, 1.0)
+
+
+def test_agrees_with_the_plain_router():
+    """softmax over all, top_k, renormalised is what qlin_moe_route_dev does, but for its order among equal ones"""
+    x = rows(8, 33, 128).astype(np.float32)
+    idx, w, _ = call(x, F32, False, None, 1, 1, 1, 8, True, 1.0)
+    d = [qlinear.DevBuf.from_numpy(x), qlinear.DevBuf(33 * 8 * 4), qlinear.DevBuf(33 * 8 * 4)]
+    qlinear.moe_route_dev(d[0], 33, 128, 8, d[1], d[2])
+    qlinear.sync()
+    assert np.array_equal(d[1].to_numpy(np.int32, (33, 8)), idx)
+    assert np.abs(d[2].to_numpy(np.float32, (33, 8)) - w).max() <= 2.0 ** -19  # both in fp32, logits of at most 8: 2^-23 (8 + 8 + 24) and less than half
+
+
+def test_same_bits_again():
+    x = rows(9, 500, 256)
+    a = call(x, F32, True, small_bias(1, 256), 8, 4, 2, 8, True, 2.5)
+    b = call(x, F32, True, small_bias(1, 256), 8, 4, 2, 8, True, 2.5)
+    assert np.array_equal(a[0], b[0]) and np.array_equal(a[1], b[1])
+    for n in (1, 3, 64):  # and a token's result does not depend on the others
+        c = call(x[:n], F32, True, small_bias(1, 256), 8, 4, 2, 8, True, 2.5)
+        assert np.array_equal(a[0][:n], c[0]) and np.array_equal(a[1][:n], c[1])
