@@ -18,11 +18,16 @@
 #include "qlin_device.h"
 #include "qlin_internal.h"
 
+#include <type_traits>
+
+#include "mxfp4.h"
+
 namespace qlin {
 
 namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
@@ -36,18 +41,40 @@ template <class T, int N> struct alignas(sizeof(T) * N < 16 ? sizeof(T) * N : 16
 template <class A, class B> struct Same { static constexpr bool value = false; };
 template <class A> struct Same<A, A> { static constexpr bool value = true; };
 
-constexpr int kTile = 64; /* tokens of a tile: a lane each */
-constexpr int kWaves = 4;
+constexpr int kTile = kLoraTile; /* tokens of a tile */
+constexpr int kShrinkWaves = kLoraShrinkThreads / 64, kExpandWaves = kLoraExpandThreads / 64;
+
+/* A wave's lanes read from LDS what others of its lanes wrote, and write it anew: one wave's requests to LDS stay in order, and this keeps the
+ * compiler from changing it. No instruction. */
+__device__ __forceinline__ void wave_meets() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+/* addresses that come out of a table are global ones: without this the loads would ask LDS as well */
+template <class T> using Global = const T __attribute__((address_space(1))) *;
 
 /* N elements p[at..], zeros from `end` on; VEC: p + at on the vector's alignment, at and end multiples of N */
 template <class T, int N, bool VEC> __device__ __forceinline__ Vec<T, N> load(const T *p, int at, int end) {
     Vec<T, N> e = {};
     if constexpr (VEC) {
-        if (at < end) e = *reinterpret_cast<const Vec<T, N> *>(p + at);
+        typedef uint32_t Words __attribute__((ext_vector_type(sizeof(T) * N / 4 < 4 ? sizeof(T) * N / 4 : 4)));
+        constexpr int kPieces = sizeof(T) * N / sizeof(Words);
+        struct { Words w[kPieces]; } raw = {};
+        if (at < end) {
+#pragma unroll
+            for (int i = 0; i < kPieces; i++) raw.w[i] = ((Global<Words>)(p + at))[i];
+        }
+        e = __builtin_bit_cast(Vec<T, N>, raw);
     } else {
+        const Global<T> g = (Global<T>)p;
 #pragma unroll
         for (int i = 0; i < N; i++)
-            if (at + i < end) e.v[i] = p[at + i];
+            if (at + i < end) {
+                if constexpr (Same<T, Bf16>::value) e.v[i].bits = ((Global<uint16_t>)p)[at + i];
+                else e.v[i] = g[at + i];
+            }
     }
     return e;
 }
@@ -61,349 +88,572 @@ struct Entry {
     float scale;
 };
 __device__ __forceinline__ Entry entry_of(const LoraEntry *table, int id, int max_rank) {
-    Entry e = {nullptr, nullptr, 0, 0.0f};
-    if (id >= 0 && table) { /* (no table where a tensor has no rows) */
-        const LoraEntry v = table[id];
-        if (v.A && v.B && v.rank > 0 && v.rank <= max_rank) e = {v.A, v.B, v.rank, v.scale};
-    }
-    return e;
+    if (id < 0 || !table) return {nullptr, nullptr, 0, 0.0f}; /* (no table where a tensor has no rows) */
+    const LoraEntry *v = table + id;
+    const void *A = v->A, *B = v->B;
+    const int rank = v->rank;
+    return {A, B, A && B && rank > 0 && rank <= max_rank ? rank : 0, v->scale};
+}
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ const void *uniform(const void *p) {
+    const uint64_t v = (uint64_t)p;
+    return (const void *)((uint64_t)(uint32_t)uniform((int)(v >> 32)) << 32 | (uint32_t)uniform((int)v));
 }
 
-/* The classes of a tile of tokens, one after the other: which tokens share an id (a lane's bit is its token's), and which. An id
- * outside of the table counts as -1. */
-struct Classes {
-    int mine;
-    uint64_t left;
-    __device__ Classes(const int32_t *ids, int n_tok, int n_adapter, int tile) {
-        const long long t = (long long)tile * kTile + (threadIdx.x & 63);
-        mine = -2;
-        if (t < n_tok) {
-            const int v = ids[t];
-            mine = v >= 0 && v < n_adapter ? v : -1;
+/* A group: up to 16 tokens of a tile that share an id, with what the second launch needs of their adapters. The first launch writes them. */
+struct alignas(16) Group {
+    int32_t id, n; /* n 0: none */
+    uint8_t token[16];
+    int32_t unused[2];
+    struct {
+        const void *B;
+        int32_t rank;
+        float scale;
+    } of[3];
+};
+static_assert(sizeof(Group) == kLoraGroupBytes, "as the workspace is sized");
+
+/* The tokens of a tile by adapter, found by the workgroup's first 256 threads, a token each. Tokens that share an id (-1 for one outside of the table)
+ * are a class, in order, and a class is cut into groups of G; a token is the first of a group where a multiple of G tokens before it share its
+ * id, which all threads count together. */
+template <int G> struct Tile {
+    struct Shared {
+        alignas(16) int id[kTile];
+        int equal[kShrinkWaves * 64 / kTile][kTile]; /* earlier tokens with the same id, by quarters of the tile */
+        int before[kTile], first[kTile], list[G], in_wave[4];
+        Entry entry[kTile];
+    };
+    int id, before;
+    __device__ int find(Shared &s, const LoraCall &c, const LoraEntry *table, int tile) {
+        const int t = threadIdx.x % kTile, quarter = threadIdx.x / kTile;
+        const long long left = (long long)c.n_tok - (long long)tile * kTile;
+        const int here = left < kTile ? (int)left : kTile;
+        id = -2;
+        Entry e = {nullptr, nullptr, 0, 0.0f};
+        if (threadIdx.x < kTile) {
+            if (t < here) {
+                const int v = c.ids[(size_t)tile * kTile + t];
+                id = v >= 0 && v < c.n_adapter ? v : -1;
+                e = entry_of(table, id, c.max_rank);
+            }
+            s.id[t] = id;
         }
-        left = __ballot(mine != -2);
+        __syncthreads();
+        const int mine = s.id[t], low = 64 * quarter, word = __builtin_amdgcn_readfirstlane(t / 64);
+        int equal = 0;
+        if (quarter <= word)
+            for (int j = 0; j < 64 && low + j < here; j += 4) {
+                const int4 v = *reinterpret_cast<const int4 *>(&s.id[low + j]);
+                equal += (v.x == mine && low + j < t) + (v.y == mine && low + j + 1 < t) + (v.z == mine && low + j + 2 < t) + (v.w == mine && low + j + 3 < t);
+            }
+        s.equal[quarter][t] = equal;
+        __syncthreads();
+        before = 0;
+        uint64_t firsts = 0;
+        if (threadIdx.x < kTile) {
+#pragma unroll
+            for (int q = 0; q < kShrinkWaves * 64 / kTile; q++) before += s.equal[q][t];
+            s.before[t] = before;
+            s.entry[t] = e;
+            firsts = __ballot(id != -2 && before % G == 0);
+            s.in_wave[t / 64] = __popcll(firsts);
+        }
+        __syncthreads();
+        int start = 0, all = 0;
+#pragma unroll
+        for (int w = 0; w < kTile / 64; w++) {
+            if (w < t / 64) start += s.in_wave[w];
+            all += s.in_wave[w];
+        }
+        if (threadIdx.x < kTile && (firsts >> (t & 63)) & 1) s.first[start + __builtin_amdgcn_mbcnt_hi((uint32_t)(firsts >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)firsts, 0))] = t;
+        __syncthreads();
+        return all;
     }
-    __device__ uint64_t next(int &id) {
-        id = __builtin_amdgcn_readlane(mine, __builtin_ctzll(left));
-        const uint64_t same = __ballot(mine == id);
-        left &= ~same;
-        return same;
+    /* the tokens of the group that token t0 is the first of, into the list; their number */
+    __device__ int gather(Shared &s, int t0) {
+        if (threadIdx.x < kTile) {
+            const int place = before - s.before[t0];
+            const bool in = id == s.id[t0] && place >= 0 && place < G;
+            if (in) s.list[place] = threadIdx.x;
+            s.in_wave[threadIdx.x / 64] = __popcll(__ballot(in));
+        }
+        __syncthreads();
+        return s.in_wave[0] + s.in_wave[1] + s.in_wave[2] + s.in_wave[3];
     }
 };
 
-/* lane q: the token (of the tile's 64) that is the q-th of a class; past the class some other */
-__device__ __forceinline__ int packed_order(uint64_t same) {
-    const int lane = threadIdx.x & 63;
-    const int before = __builtin_amdgcn_mbcnt_hi((uint32_t)(same >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)same, 0));
-    const int place = (same >> lane) & 1 ? before : __popcll(same) + lane - before;
-    return __builtin_amdgcn_ds_permute(place * 4, lane);
-}
-
 /* ------------------------------------------------------------------ h = A x */
 
-/* sums over steps [k0, k1) of 32 columns for RT groups of 16 ranks and NJ groups of 16 tokens; rows of A from its rank on are not looked at */
-template <class W, class X, int RT, bool VEC>
-__device__ __forceinline__ void shrink_sums(const W *A, int rank0, int rank, const X *const (&x)[4], int n_groups, int n_cols, int k0, int k1, f32x4 (&acc)[4][RT]) {
-    const int lane = threadIdx.x & 63, g = lane >> 4;
+/* acc += w . x over 32 columns, eight to a lane */
+template <class W, class X> __device__ __forceinline__ f32x4 multiply(const Vec<W, 8> &w, const Vec<X, 8> &x, f32x4 acc) {
+    if constexpr (Same<W, Bf16>::value && Same<X, Bf16>::value) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w), __builtin_bit_cast(bf16x8, x), acc, 0, 0, 0);
+    } else if constexpr (Same<W, _Float16>::value && Same<X, _Float16>::value) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, w), __builtin_bit_cast(f16x8, x), acc, 0, 0, 0);
+    } else { /* the e-th of a lane's eight columns with the e-th of the other lanes': any order of columns does, the same on both sides */
+#pragma unroll
+        for (int e = 0; e < 8; e++) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(to_f32(w.v[e]), to_f32(x.v[e]), acc, 0, 0, 0);
+        return acc;
+    }
+}
+
+/* a stage: U x 32 columns, as a fragment each per group of 16 ranks or tokens; WHOLE: all of its columns are there */
+template <class W, class X, int RT, int NJ, int U> struct Stage {
+    Vec<W, 8> w[U][RT];
+    Vec<X, 8> x[U][NJ];
+    template <bool WHOLE> __device__ __forceinline__ void fetch(const W *const (&a)[RT], const X *const (&t)[NJ], int stage, int n_cols) {
+        const int at = 32 * U * stage + 8 * ((threadIdx.x & 63) >> 4), end = WHOLE ? 0x7FFFFFFF : n_cols;
+#pragma unroll
+        for (int j = 0; j < NJ; j++)
+#pragma unroll
+            for (int u = 0; u < U; u++) x[u][j] = load<X, 8, true>(t[j], at + 32 * u, end);
+#pragma unroll
+        for (int i = 0; i < RT; i++)
+#pragma unroll
+            for (int u = 0; u < U; u++) w[u][i] = load<W, 8, true>(a[i], at + 32 * u, end);
+    }
+    __device__ __forceinline__ void add_to(f32x4 (&acc)[NJ][RT]) const {
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int j = 0; j < NJ; j++)
+#pragma unroll
+                for (int i = 0; i < RT; i++) acc[j][i] = multiply(w[u][i], x[u][j], acc[j][i]);
+    }
+};
+/* 64 columns, a whole line of 128 bytes of a row in 16 bits, where two such stages leave the registers of four waves per SIMD */
+template <class W, class X, int RT, int NJ> constexpr int stage_steps() { return (RT * sizeof(W) + NJ * sizeof(X)) <= 8 ? 2 : 1; }
+
+/* sums over steps [k0, k1) of 32 columns for RT groups of 16 ranks and NJ groups of 16 tokens; k0 even; rows of A from its rank on give sums that are
+ * not looked at */
+template <class W, class X, int RT, int NJ>
+__device__ __forceinline__ void shrink_sums(bool vec, const W *A, int rank0, int rank, const X *const (&x)[NJ], int n_cols, int k0, int k1, f32x4 (&acc)[NJ][RT]) {
+    const int lane = threadIdx.x & 63;
     const W *a[RT];
 #pragma unroll
     for (int i = 0; i < RT; i++) {
         const int row = rank0 + 16 * i + (lane & 15);
         a[i] = A + (size_t)(row < rank ? row : rank - 1) * n_cols;
     }
-    for (int s = k0; s < k1; s++) {
-        const int at = 32 * s + 8 * g;
-        Vec<W, 8> w[RT];
-#pragma unroll
-        for (int i = 0; i < RT; i++)
-            if (rank0 + 16 * i < rank) w[i] = load<W, 8, VEC>(a[i], at, n_cols);
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            if (j >= n_groups) break;
-            const Vec<X, 8> v = load<X, 8, VEC>(x[j], at, n_cols);
+    if (vec) { /* the next stage is on its way while one is multiplied; behind the last one it is that once more */
+        constexpr int U = stage_steps<W, X, RT, NJ>();
+        const int whole = n_cols / (32 * U), all = (k1 + U - 1) / U, end = all < whole ? all : whole;
+        Stage<W, X, RT, NJ, U> s[2];
+        int k = k0 / U;
+        if (k < end) {
+            s[0].template fetch<true>(a, x, k, n_cols);
+            for (;;) {
+                s[1].template fetch<true>(a, x, k + 1 < end ? k + 1 : k, n_cols);
+                s[0].add_to(acc);
+                if (++k == end) break;
+                s[0].template fetch<true>(a, x, k + 1 < end ? k + 1 : k, n_cols);
+                s[1].add_to(acc);
+                if (++k == end) break;
+            }
+        }
+        if (end < all) {
+            s[0].template fetch<false>(a, x, end, n_cols);
+            s[0].add_to(acc);
+        }
+    } else { /* rows that do not lie on 16 bytes: element by element, eight at a time */
+        const int end = 32 * k1 < n_cols ? 32 * k1 : n_cols;
+#pragma unroll 1
+        for (int first = 32 * k0; first < end; first += 32) {
+            const int at = first + 8 * (lane >> 4);
 #pragma unroll
             for (int i = 0; i < RT; i++) {
-                if (rank0 + 16 * i >= rank) break;
-                if constexpr (Same<W, Bf16>::value && Same<X, Bf16>::value) {
-                    acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w[i]), __builtin_bit_cast(bf16x8, v), acc[j][i], 0, 0, 0);
-                } else if constexpr (Same<W, _Float16>::value && Same<X, _Float16>::value) {
-                    acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, w[i]), __builtin_bit_cast(f16x8, v), acc[j][i], 0, 0, 0);
-                } else { /* the e-th of a lane's eight columns with the e-th of the other lanes': any order of columns does, the same on both sides */
+                const Vec<W, 8> w = load<W, 8, false>(a[i], at, n_cols);
 #pragma unroll
-                    for (int e = 0; e < 8; e++) acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(to_f32(w[i].v[e]), to_f32(v.v[e]), acc[j][i], 0, 0, 0);
-                }
+                for (int j = 0; j < NJ; j++) acc[j][i] = multiply(w, load<X, 8, false>(x[j], at, n_cols), acc[j][i]);
             }
         }
     }
 }
 
-template <class W, class X, int RT>
-__global__ void __launch_bounds__(64 * kWaves)
+template <class W, class X, int RT, int NJ>
+__global__ void __launch_bounds__(64 * kShrinkWaves)
 lora_shrink_kernel(LoraCall c, LoraPlan p) {
-    __shared__ f32x4 red[kWaves][RT][64];
+    __shared__ f32x4 red[kShrinkWaves][NJ * RT][64];
+    __shared__ typename Tile<16 * NJ>::Shared shared;
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    uint32_t b = blockIdx.x;
-    const int slot = b % p.slots; b /= p.slots;
+    /* workgroups b and b + 8 share a die: the tensors of the same tokens, one after the other */
+    uint32_t b = blockIdx.x % 8 + blockIdx.x / 8 / c.n_mat * 8;
+    const int mat = blockIdx.x / 8 % c.n_mat;
+    if (b >= p.shrink_units()) return;
     const int part = b % p.parts; b /= p.parts;
-    const int block = b % p.rank_blocks; b /= p.rank_blocks;
-    const int mat = b % c.n_mat, tile = b / c.n_mat;
-    const LoraTensor *m = mat == 0 ? &c.m[0] : mat == 1 ? &c.m[1] : &c.m[2];
+    const int slot = b % p.shrink_slots; b /= p.shrink_slots;
+    const int block = b % p.rank_blocks, tile = b / p.rank_blocks;
     const X *x0 = static_cast<const X *>(c.X);
     const int rank0 = block * 16 * RT;
-    const int steps = (c.n_cols + 31) / 32, share = part * kWaves + wv, shares = p.parts * kWaves;
-    const int k0 = (int)((long long)steps * share / shares), k1 = (int)((long long)steps * (share + 1) / shares);
+    const int pairs = (c.n_cols + 63) / 64, share = part * kShrinkWaves + wv, shares = p.parts * kShrinkWaves;
+    const int k0 = 2 * (int)((long long)pairs * share / shares), k1 = 2 * (int)((long long)pairs * (share + 1) / shares);
     const bool x_vec = c.n_cols % 8 == 0 && on(c.X, 16) && (size_t)c.ldx * sizeof(X) % 16 == 0;
-    float *h = c.workspace + ((size_t)part * c.n_mat + mat) * c.n_tok * p.rank_pad;
-    Classes classes(c.ids, c.n_tok, c.n_adapter, tile);
-    for (int k = 0; classes.left; k++) {
-        int id;
-        const uint64_t same = classes.next(id);
-        if (k % p.slots != slot) continue;
-        const Entry e = entry_of(m->adapters, id, c.max_rank);
-        if (e.rank <= rank0) continue; /* no adapter, or none of its ranks here: nothing is read of h either */
-        const int count = __popcll(same), groups = (count + 15) / 16;
-        const int order = packed_order(same);
-        const X *x[4];
-        size_t token[4];
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const int q = 16 * j + (lane & 15);
-            token[j] = (size_t)tile * kTile + __shfl(order, q < count ? q : 0, 64);
-            x[j] = x0 + token[j] * c.ldx;
+    Group *records = static_cast<Group *>(c.workspace) + (size_t)tile * p.groups;
+    Tile<16 * NJ> tokens;
+    const int all = tokens.find(shared, c, mat == 0 ? c.m[0].adapters : mat == 1 ? c.m[1].adapters : c.m[2].adapters, tile);
+    for (int s = slot; s * NJ < p.groups; s += p.shrink_slots) {
+        if (s >= all) { /* the second launch looks at every record */
+            if (part == 0 && block == 0 && mat == 0 && threadIdx.x < NJ) records[s * NJ + threadIdx.x].n = 0;
+            continue;
         }
-        f32x4 acc[4][RT] = {};
-        const W *A = static_cast<const W *>(e.A);
-        if (x_vec && on(A, 16))
-            shrink_sums<W, X, RT, true>(A, rank0, e.rank, x, groups, c.n_cols, k0, k1, acc);
-        else
-            shrink_sums<W, X, RT, false>(A, rank0, e.rank, x, groups, c.n_cols, k0, k1, acc);
-        /* the waves' sums, added in the waves' order */
+        const int t0 = uniform(shared.first[s]), n = uniform(tokens.gather(shared, t0));
+        const Entry e = {uniform(shared.entry[t0].A), uniform(shared.entry[t0].B), uniform(shared.entry[t0].rank), shared.entry[t0].scale};
+        size_t token[NJ];
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            if (j >= groups) break;
+        for (int j = 0; j < NJ; j++) {
+            const int q = 16 * j + (lane & 15);
+            token[j] = (size_t)tile * kTile + (q < n ? shared.list[q] : t0);
+            if (part == 0 && block == 0 && wv == 0 && lane < 16) {
+                Group &r = records[s * NJ + j];
+                if (mat == 0) r.token[lane] = (uint8_t)(token[j] % kTile);
+                if (lane == 0) {
+                    if (mat == 0) r.n = n - 16 * j > 16 ? 16 : n - 16 * j > 0 ? n - 16 * j : 0;
+                    r.of[mat].B = e.B;
+                    r.of[mat].rank = e.rank;
+                    r.of[mat].scale = e.scale;
+                }
+            }
+        }
+        if (e.rank > rank0) { /* else no adapter, or none of its ranks here: nothing is read of h either */
+            const X *x[NJ];
 #pragma unroll
-            for (int i = 0; i < RT; i++) red[wv][i][lane] = acc[j][i];
+            for (int j = 0; j < NJ; j++) x[j] = x0 + token[j] * c.ldx;
+            f32x4 acc[NJ][RT] = {};
+            if (k0 < k1) shrink_sums<W, X, RT, NJ>(x_vec && on(e.A, 16), static_cast<const W *>(e.A), rank0, e.rank, x, c.n_cols, k0, k1, acc);
+            /* the waves' sums, added in the waves' order */
+#pragma unroll
+            for (int j = 0; j < NJ; j++)
+#pragma unroll
+                for (int i = 0; i < RT; i++) red[wv][j * RT + i][lane] = acc[j][i];
             __syncthreads();
-            for (int i = wv; i < RT; i += kWaves) {
-                f32x4 v = red[0][i][lane];
+            for (int f = wv; f < NJ * RT; f += kShrinkWaves) {
+                const int j = f / RT, i = f % RT;
+                f32x4 v = red[0][f][lane];
 #pragma unroll
-                for (int w = 1; w < kWaves; w++) v += red[w][i][lane];
+                for (int w = 1; w < kShrinkWaves; w++) v += red[w][f][lane];
                 const int r = rank0 + 16 * i + 4 * (lane >> 4);
 #pragma unroll
                 for (int q = 0; q < 4; q++)
                     if (r + q >= e.rank) v[q] = 0.0f;
-                if (16 * j + (lane & 15) < count && r < p.rank_pad) *reinterpret_cast<f32x4 *>(h + token[j] * p.rank_pad + r) = v;
+                const size_t t = (j > 0 ? token[NJ - 1] : token[0]) + (size_t)mat * c.n_tok;
+                if (16 * j + (lane & 15) >= n || r >= p.rank_pad) continue;
+                char *h = static_cast<char *>(c.workspace) + p.h_at;
+                if (p.split) {
+                    v *= e.scale;
+                    bf16x4 three[3];
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        three[0][q] = (__bf16)v[q];
+                        const float rest = v[q] - (float)three[0][q];
+                        three[1][q] = (__bf16)rest;
+                        three[2][q] = (__bf16)(rest - (float)three[1][q]);
+                    }
+                    uint16_t *to = reinterpret_cast<uint16_t *>(h) + (t * p.rank_pad + r / 16 * 16) * 3 + r % 16;
+#pragma unroll
+                    for (int q = 0; q < 3; q++) *reinterpret_cast<bf16x4 *>(to + 16 * q) = three[q];
+                } else {
+                    *reinterpret_cast<f32x4 *>(reinterpret_cast<float *>(h) + ((size_t)part * c.n_mat * c.n_tok + t) * p.rank_pad + r) = v;
+                }
             }
-            __syncthreads();
         }
+        __syncthreads();
     }
 }
 
 /* ------------------------------------------------------------------ Y + B h */
 
-/* four consecutive elements of a row, of which `left` are there; VEC-aligned rows in one load */
-__device__ __forceinline__ f32x4 load4(const void *base, size_t at, int left, uint32_t type, bool vec) {
-    f32x4 y = {};
-    if (type == T_F32) {
-        const float *p = static_cast<const float *>(base) + at;
-        if (vec && left > 3) return *reinterpret_cast<const f32x4 *>(p);
-        for (int i = 0; i < 4; i++)
-            if (i < left) y[i] = p[i];
+/* four consecutive elements of a row, T float or the bits of a 16-bit type; WHOLE: all four are there, on the vector's alignment */
+template <class T, bool WHOLE> __device__ __forceinline__ f32x4 load4(const void *base, size_t at, int left, bool bf16) {
+    const T *p = static_cast<const T *>(base) + at;
+    Vec<T, 4> v = {};
+    if constexpr (WHOLE) {
+        v = *reinterpret_cast<const Vec<T, 4> *>(p);
     } else {
-        Vec<uint16_t, 4> v = {};
-        const uint16_t *p = static_cast<const uint16_t *>(base) + at;
-        if (vec && left > 3)
-            v = *reinterpret_cast<const Vec<uint16_t, 4> *>(p);
-        else
-            for (int i = 0; i < 4; i++)
-                if (i < left) v.v[i] = p[i];
 #pragma unroll
-        for (int i = 0; i < 4; i++) y[i] = type == T_BF16 ? to_f32(Bf16{v.v[i]}) : to_f32(__builtin_bit_cast(_Float16, v.v[i]));
+        for (int i = 0; i < 4; i++)
+            if (i < left) v.v[i] = p[i];
+    }
+    f32x4 y;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if constexpr (sizeof(T) == 4) y[i] = v.v[i];
+        else y[i] = bf16 ? to_f32(Bf16{v.v[i]}) : to_f32(__builtin_bit_cast(_Float16, v.v[i]));
     }
     return y;
 }
 /* the one rounding of a result in 16 bits: to the nearest, ties to even */
-__device__ __forceinline__ void store4(void *base, size_t at, int left, uint32_t type, bool vec, f32x4 y) {
-    if (type == T_F32) {
-        float *p = static_cast<float *>(base) + at;
-        if (vec && left > 3) {
-            *reinterpret_cast<f32x4 *>(p) = y;
-            return;
-        }
-        for (int i = 0; i < 4; i++)
-            if (i < left) p[i] = y[i];
-    } else {
-        Vec<uint16_t, 4> v;
+template <class T, bool WHOLE> __device__ __forceinline__ void store4(void *base, size_t at, int left, bool bf16, f32x4 y) {
+    T *p = static_cast<T *>(base) + at;
+    Vec<T, 4> v;
 #pragma unroll
-        for (int i = 0; i < 4; i++) v.v[i] = type == T_BF16 ? __builtin_bit_cast(uint16_t, (__bf16)y[i]) : __builtin_bit_cast(uint16_t, (_Float16)y[i]);
-        uint16_t *p = static_cast<uint16_t *>(base) + at;
-        if (vec && left > 3) {
-            *reinterpret_cast<Vec<uint16_t, 4> *>(p) = v;
-            return;
-        }
+    for (int i = 0; i < 4; i++) {
+        if constexpr (sizeof(T) == 4) v.v[i] = y[i];
+        else v.v[i] = bf16 ? __builtin_bit_cast(uint16_t, (__bf16)y[i]) : __builtin_bit_cast(uint16_t, (_Float16)y[i]);
+    }
+    if constexpr (WHOLE) {
+        *reinterpret_cast<Vec<T, 4> *>(p) = v;
+    } else {
+#pragma unroll
         for (int i = 0; i < 4; i++)
             if (i < left) p[i] = v.v[i];
     }
 }
 
-/* sums over an adapter's ranks for one group of 16 rows x 16 tokens; h: the tokens' in LDS */
-template <class W, bool VEC>
-__device__ __forceinline__ f32x4 expand_sums(const W *row, int rank, const float *h, f32x4 acc) {
-    const int g = (threadIdx.x & 63) >> 4;
-    for (int r = 0; r < rank; r += 16) {
-        const Vec<W, 4> w = load<W, 4, VEC>(row, r + 4 * g, rank);
-        const f32x4 v = *reinterpret_cast<const f32x4 *>(h + r + 4 * g);
+/* acc += B h over an adapter's ranks, for MT groups of 16 rows x 16 tokens; h: the lane's token in the workspace, of which the parts are
+ * added in their order */
+template <class W, int MT, bool VEC>
+__device__ __forceinline__ void expand_sums(const Entry &e, int row0, int n_rows, const float *h, size_t part, int parts, f32x4 (&acc)[MT]) {
+    const int lane = threadIdx.x & 63, g = lane >> 4;
+    const W *b[MT];
 #pragma unroll
-        for (int i = 0; i < 4; i++) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(to_f32(w.v[i]), v[i], acc, 0, 0, 0);
+    for (int i = 0; i < MT; i++) {
+        const int row = row0 + 16 * i + (lane & 15);
+        b[i] = static_cast<const W *>(e.B) + (size_t)(row < n_rows ? row : n_rows - 1) * e.rank;
     }
-    return acc;
+    for (int r = 4 * g; r < e.rank + 4 * g; r += 16) {
+        Vec<W, 4> w[MT];
+#pragma unroll
+        for (int i = 0; i < MT; i++) w[i] = load<W, 4, VEC>(b[i], r, e.rank);
+        f32x4 v = *reinterpret_cast<const f32x4 *>(h + r);
+        for (int s = 1; s < parts; s += 4) { /* (four on their way at a time) */
+            f32x4 more[4];
+#pragma unroll
+            for (int q = 0; q < 4; q++) more[q] = *reinterpret_cast<const f32x4 *>(h + (s + q < parts ? s + q : 0) * part + r);
+#pragma unroll
+            for (int q = 0; q < 4; q++)
+                if (s + q < parts) v += more[q];
+        }
+        v *= e.scale;
+#pragma unroll
+        for (int q = 0; q < 4; q++)
+#pragma unroll
+            for (int i = 0; i < MT; i++) acc[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(to_f32(w[i].v[q]), v[q], acc[i], 0, 0, 0);
+    }
 }
 
-/* a workgroup: 16 MT rows on each of its waves, of one tensor or, PAIR, of gate and up */
-template <class W, int MT, bool PAIR>
-__global__ void __launch_bounds__(64 * kWaves)
-lora_expand_kernel(LoraCall c, LoraPlan p) {
-    extern __shared__ __attribute__((aligned(16))) float hs[]; /* [PAIR ? 2 : 1][16 tokens][rank_pad + 4] */
-    constexpr int MATS = PAIR ? 2 : 1;
-    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
-    uint32_t b = blockIdx.x;
-    const int slot = b % p.slots; b /= p.slots;
-    int mat = 0, block = b % p.row_blocks_all;
-    const int tile = b / p.row_blocks_all;
-    if (!PAIR) {
-        if (block >= p.row_blocks[0]) { block -= p.row_blocks[0]; mat = 1; }
-        if (mat == 1 && block >= p.row_blocks[1]) { block -= p.row_blocks[1]; mat = 2; }
+/* the same where the workspace holds scale h as three numbers in bf16, whose sum it is: 16 first parts of 16 ranks, their second and their third
+ * ones. The first instruction takes first parts in its first 16 columns and second parts in the others, the second one third parts, with
+ * the same 16 columns of B on both halves: the products are exact. */
+template <int MT, bool VEC>
+__device__ __forceinline__ void expand_split(const Entry &e, int row0, int n_rows, const uint16_t *h, f32x4 (&acc)[MT]) {
+    const int lane = threadIdx.x & 63, g = lane >> 4;
+    const Bf16 *b[MT];
+#pragma unroll
+    for (int i = 0; i < MT; i++) {
+        const int row = row0 + 16 * i + (lane & 15);
+        b[i] = static_cast<const Bf16 *>(e.B) + (size_t)(row < n_rows ? row : n_rows - 1) * e.rank;
     }
-    const LoraTensor *m = mat == 0 ? &c.m[0] : mat == 1 ? &c.m[1] : &c.m[2];
-    const int n_rows = m->n_rows, ldy = m->ldy, ldo = m->ldo;
-    const int row0 = (block * kWaves + wv) * 16 * MT;
-    const int stride = p.rank_pad + 4;
-    const bool y_vec = on(m->Y, c.y_type == T_F32 ? 16 : 8) && (!PAIR || on(c.m[1].Y, c.y_type == T_F32 ? 16 : 8)) && ldy % 4 == 0;
-    const bool o_vec = on(m->out, c.out_type == T_F32 ? 16 : 8) && ldo % 4 == 0;
-    Classes classes(c.ids, c.n_tok, c.n_adapter, tile);
-    for (int k = 0; classes.left; k++) {
-        int id;
-        const uint64_t same = classes.next(id);
-        if (k % p.slots != slot) continue;
-        Entry e[MATS];
+    for (int r = 0; r < e.rank; r += 16) {
+        Vec<Bf16, 8> w[MT];
 #pragma unroll
-        for (int a = 0; a < MATS; a++) e[a] = entry_of(PAIR ? c.m[a].adapters : m->adapters, id, c.max_rank);
-        const int count = __popcll(same);
-        const int order = packed_order(same);
-        for (int j = 0; 16 * j < count; j++) {
-            const int q = 16 * j + (lane & 15);
-            const size_t token = (size_t)tile * kTile + __shfl(order, q < count ? q : 0, 64);
-            /* h of the group's tokens: the parts' sums in their order */
-            __syncthreads();
+        for (int i = 0; i < MT; i++) w[i] = load<Bf16, 8, VEC>(b[i], r + 8 * (g & 1), e.rank);
+        const bf16x8 v = *reinterpret_cast<const bf16x8 *>(h + 3 * r + 8 * g);
+        bf16x8 rest = *reinterpret_cast<const bf16x8 *>(h + 3 * r + 32 + 8 * (g & 1));
+        if (g > 1) rest = bf16x8{};
 #pragma unroll
-            for (int a = 0; a < MATS; a++) {
-                for (int v = wv; 16 * v < e[a].rank; v += kWaves) { /* lane: token lane & 15, four ranks */
-                    const size_t part = (size_t)c.n_mat * c.n_tok * p.rank_pad;
-                    const float *from = c.workspace + ((size_t)(mat + a) * c.n_tok + token) * p.rank_pad + 16 * v + 4 * g;
-                    f32x4 sum = *reinterpret_cast<const f32x4 *>(from);
-                    for (int s = 1; s < p.parts; s++) sum += *reinterpret_cast<const f32x4 *>(from + s * part);
-                    *reinterpret_cast<f32x4 *>(hs + (a * 16 + (lane & 15)) * stride + 16 * v + 4 * g) = sum * e[a].scale;
-                }
-            }
-            __syncthreads();
+        for (int i = 0; i < MT; i++) acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w[i]), rest, acc[i], 0, 0, 0);
 #pragma unroll
-            for (int i = 0; i < MT; i++) {
-                if (row0 + 16 * i >= n_rows) break;
-                f32x4 acc[MATS] = {};
-#pragma unroll
-                for (int a = 0; a < MATS; a++) {
-                    const int row = row0 + 16 * i + (lane & 15);
-                    const W *w = static_cast<const W *>(e[a].B) + (size_t)(row < n_rows ? row : n_rows - 1) * e[a].rank;
-                    const float *h = hs + (a * 16 + (lane & 15)) * stride;
-                    if (e[a].rank % 4 == 0 && on(e[a].B, 4 * sizeof(W)))
-                        acc[a] = expand_sums<W, true>(w, e[a].rank, h, acc[a]);
-                    else
-                        acc[a] = expand_sums<W, false>(w, e[a].rank, h, acc[a]);
-                }
-                const int row = row0 + 16 * i + 4 * g, left = n_rows - row;
-                if (q < count && left > 0) {
-                    f32x4 y = load4(m->Y, token * ldy + row, left, c.y_type, y_vec) + acc[0];
-                    if constexpr (PAIR) {
-                        const f32x4 u = load4(c.m[1].Y, token * ldy + row, left, c.y_type, y_vec) + acc[1];
-#pragma unroll
-                        for (int r = 0; r < 4; r++) y[r] = y[r] / (1.0f + expf(-y[r])) * u[r];
-                    }
-                    store4(m->out, token * ldo + row, left, c.out_type, o_vec, y);
-                }
+        for (int i = 0; i < MT; i++) acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w[i]), v, acc[i], 0, 0, 0);
+    }
+}
+
+/* a wave: 16 MT rows of one tensor or, PAIR, of gate and up; T, O: Y's and the result's type, float or the bits of a 16-bit one. The sums come
+ * out of the matrix instruction with a lane's four rows 16 tokens apart; they go through LDS, so that Y is read and results are written in
+ * runs of a token's 16 MT rows. */
+template <class W, class T, class O, int MT, bool PAIR, bool SPLIT>
+__global__ void __launch_bounds__(64 * kExpandWaves)
+lora_expand_kernel(LoraCall c, LoraPlan p) {
+    constexpr int MATS = PAIR ? 2 : 1, kRows = 16 * MT, kStride = kRows + 4; /* (a token's run behind the one before: other banks) */
+    constexpr int kLanes = kRows / 4, kRuns = 64 / kLanes, kSteps = 16 / kRuns; /* lanes of a run, runs at a time */
+    __shared__ float turn[kExpandWaves][16 * kStride];
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int mat = 0, block = blockIdx.x % p.row_blocks_all;
+    const int unit = blockIdx.x / p.row_blocks_all, slot = unit % p.expand_slots, tile = unit / p.expand_slots;
+    LoraTensor m = c.m[0];
+    if (!PAIR) {
+        if (block >= p.row_blocks[0]) {
+            block -= p.row_blocks[0];
+            mat = 1;
+            m = c.m[1];
+            if (block >= p.row_blocks[1]) {
+                block -= p.row_blocks[1];
+                mat = 2;
+                m = c.m[2];
             }
         }
     }
+    const int row0 = (block * kExpandWaves + wv) * kRows;
+    if (row0 >= m.n_rows) return;
+    const bool y_bf16 = c.y_type == T_BF16, o_bf16 = c.out_type == T_BF16;
+    const bool whole = row0 + kRows <= m.n_rows && on(m.Y, 4 * sizeof(T)) && (!PAIR || on(c.m[1].Y, 4 * sizeof(T))) && m.ldy % 4 == 0 && on(m.out, 4 * sizeof(O)) && m.ldo % 4 == 0;
+    const size_t part = (size_t)c.n_mat * c.n_tok * p.rank_pad;
+    const int row = 4 * (lane % kLanes), left = m.n_rows - row0 - row; /* of the run */
+    const char *hs = static_cast<const char *>(c.workspace) + p.h_at;
+    for (int u = slot; u < p.groups; u += p.expand_slots) {
+        const Group *group = static_cast<const Group *>(c.workspace) + (size_t)tile * p.groups + u;
+        const int n = uniform(group->n);
+        if (n == 0) continue;
+        const size_t token = (size_t)tile * kTile + group->token[lane & 15]; /* (behind the group's tokens: the first) */
+        size_t run[kSteps]; /* the tokens of the lane's runs */
+#pragma unroll
+        for (int s = 0; s < kSteps; s++) run[s] = (size_t)tile * kTile + group->token[s * kRuns + lane / kLanes];
+        Entry of[MATS];
+#pragma unroll
+        for (int a = 0; a < MATS; a++) of[a] = {nullptr, uniform(group->of[mat + a].B), uniform(group->of[mat + a].rank), group->of[mat + a].scale};
+        f32x4 y[MATS][kSteps];
+        auto load_all = [&](auto w) {
+#pragma unroll
+            for (int s = 0; s < kSteps; s++) {
+                y[0][s] = load4<T, decltype(w)::value>(m.Y, run[s] * m.ldy + row0 + row, left, y_bf16);
+                if constexpr (PAIR) y[1][s] = load4<T, decltype(w)::value>(c.m[1].Y, run[s] * m.ldy + row0 + row, left, y_bf16);
+            }
+        };
+        if (whole) load_all(std::true_type{});
+        else load_all(std::false_type{});
+#pragma unroll
+        for (int a = 0; a < MATS; a++) {
+            const Entry e = of[a];
+            if (e.rank == 0) continue;
+            f32x4 acc[MT] = {};
+            const size_t h_at = ((size_t)(mat + a) * c.n_tok + token) * p.rank_pad;
+            if constexpr (SPLIT) {
+                const uint16_t *h = reinterpret_cast<const uint16_t *>(hs) + 3 * h_at;
+                if (e.rank % 8 == 0 && on(e.B, 16))
+                    expand_split<MT, true>(e, row0, m.n_rows, h, acc);
+                else
+                    expand_split<MT, false>(e, row0, m.n_rows, h, acc);
+            } else {
+                const float *h = reinterpret_cast<const float *>(hs) + h_at;
+                if (e.rank % 4 == 0 && on(e.B, 4 * sizeof(W)))
+                    expand_sums<W, MT, true>(e, row0, m.n_rows, h, part, p.parts, acc);
+                else
+                    expand_sums<W, MT, false>(e, row0, m.n_rows, h, part, p.parts, acc);
+            }
+            wave_meets();
+#pragma unroll
+            for (int i = 0; i < MT; i++) *reinterpret_cast<f32x4 *>(&turn[wv][(lane & 15) * kStride + 16 * i + 4 * (lane >> 4)]) = acc[i];
+            wave_meets();
+#pragma unroll
+            for (int s = 0; s < kSteps; s++) y[a][s] += *reinterpret_cast<const f32x4 *>(&turn[wv][(s * kRuns + lane / kLanes) * kStride + row]);
+        }
+        if constexpr (PAIR) {
+#pragma unroll
+            for (int s = 0; s < kSteps; s++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) y[0][s][r] = mxfp4::silu_mul(y[0][s][r], y[MATS - 1][s][r]);
+        }
+        auto store_all = [&](auto w) {
+#pragma unroll
+            for (int s = 0; s < kSteps; s++)
+                if (s * kRuns + lane / kLanes < n) store4<O, decltype(w)::value>(m.out, run[s] * m.ldo + row0 + row, left, o_bf16, y[0][s]);
+        };
+        if (whole) store_all(std::true_type{});
+        else store_all(std::false_type{});
+    }
 }
 
-template <class W, class X> hipError_t launch_shrink(const LoraCall &c, const LoraPlan &p) {
-    const dim3 grid((uint32_t)p.shrink_workgroups()), block(64 * kWaves);
-    if (p.rank_tiles == 1)
-        hipLaunchKernelGGL((lora_shrink_kernel<W, X, 1>), grid, block, 0, c.stream, c, p);
-    else if (p.rank_tiles == 2)
-        hipLaunchKernelGGL((lora_shrink_kernel<W, X, 2>), grid, block, 0, c.stream, c, p);
+template <class W, class X, int RT> void launch_shrink(const LoraCall &c, const LoraPlan &p) {
+    const dim3 grid((uint32_t)p.shrink_workgroups()), block(kLoraShrinkThreads);
+    if (p.token_groups == 1)
+        hipLaunchKernelGGL((lora_shrink_kernel<W, X, RT, 1>), grid, block, 0, c.stream, c, p);
     else
-        hipLaunchKernelGGL((lora_shrink_kernel<W, X, 4>), grid, block, 0, c.stream, c, p);
-    return hipGetLastError();
+        hipLaunchKernelGGL((lora_shrink_kernel<W, X, RT, 2>), grid, block, 0, c.stream, c, p);
+}
+template <class W, class X> void launch_shrink(const LoraCall &c, const LoraPlan &p) {
+    if (p.rank_tiles == 1) launch_shrink<W, X, 1>(c, p);
+    else if (p.rank_tiles == 2) launch_shrink<W, X, 2>(c, p);
+    else launch_shrink<W, X, 4>(c, p);
+}
+
+template <class W, class T, class O, bool PAIR> void launch_expand(const LoraCall &c, const LoraPlan &p) {
+    const dim3 grid((uint32_t)p.expand_workgroups()), block(kLoraExpandThreads);
+    if constexpr (Same<W, Bf16>::value) {
+        if (p.split) {
+            hipLaunchKernelGGL((lora_expand_kernel<W, T, O, 4, PAIR, true>), grid, block, 0, c.stream, c, p);
+            return;
+        }
+    }
+    if (p.row_tiles == 1)
+        hipLaunchKernelGGL((lora_expand_kernel<W, T, O, 1, PAIR, false>), grid, block, 0, c.stream, c, p);
+    else
+        hipLaunchKernelGGL((lora_expand_kernel<W, T, O, 4, PAIR, false>), grid, block, 0, c.stream, c, p);
+}
+template <class W, bool PAIR> void launch_expand(const LoraCall &c, const LoraPlan &p) {
+    const bool y32 = c.y_type == T_F32, o32 = c.out_type == T_F32;
+    if (y32 && o32) launch_expand<W, float, float, PAIR>(c, p);
+    else if (y32) launch_expand<W, float, uint16_t, PAIR>(c, p);
+    else if (o32) launch_expand<W, uint16_t, float, PAIR>(c, p);
+    else launch_expand<W, uint16_t, uint16_t, PAIR>(c, p);
 }
 
 template <class W> hipError_t launch_both(const LoraCall &c, const LoraPlan &p) {
-    hipError_t err = c.x_type == T_F32 ? launch_shrink<W, float>(c, p) : c.x_type == T_F16 ? launch_shrink<W, _Float16>(c, p) : launch_shrink<W, Bf16>(c, p);
+    if (c.x_type == T_F32) launch_shrink<W, float>(c, p);
+    else if (c.x_type == T_F16) launch_shrink<W, _Float16>(c, p);
+    else launch_shrink<W, Bf16>(c, p);
+    const hipError_t err = hipGetLastError();
     if (err != hipSuccess) return err;
-    const dim3 grid((uint32_t)p.expand_workgroups()), block(64 * kWaves);
-    const size_t lds = (size_t)(c.pair ? 2 : 1) * 16 * (p.rank_pad + 4) * sizeof(float);
-    if (c.pair) {
-        if (p.row_tiles == 1)
-            hipLaunchKernelGGL((lora_expand_kernel<W, 1, true>), grid, block, lds, c.stream, c, p);
-        else
-            hipLaunchKernelGGL((lora_expand_kernel<W, 4, true>), grid, block, lds, c.stream, c, p);
-    } else {
-        if (p.row_tiles == 1)
-            hipLaunchKernelGGL((lora_expand_kernel<W, 1, false>), grid, block, lds, c.stream, c, p);
-        else
-            hipLaunchKernelGGL((lora_expand_kernel<W, 4, false>), grid, block, lds, c.stream, c, p);
-    }
+    if (c.pair) launch_expand<W, true>(c, p);
+    else launch_expand<W, false>(c, p);
     return hipGetLastError();
 }
 
 }  // namespace
 
-/* how many parts the columns are cut into: enough workgroups for the chip without the classes, whose number is not known here, and at least
- * two steps of 32 columns for a wave */
+/* 16 ranks, 32 or 64 to a workgroup */
+static int lora_rank_tiles(int max_rank) { return max_rank <= 16 ? 1 : max_rank <= 32 ? 2 : 4; }
+static int lora_token_groups(int n_tok) { return n_tok >= 1024 ? 2 : 1; }
+
+/* how many parts the columns are cut into: enough workgroups for the chip, as far as their number is known without the ids, and at
+ * least 64 columns for a wave; the second launch reads every part of h again for each of its rows' workgroups */
 static int lora_parts(int n_mat, int max_rank, int n_cols, int n_tok) {
-    const long long tiles = ((long long)n_tok + kTile - 1) / kTile, ranks = ((long long)max_rank + 63) / 64;
-    const long long want = 1024 / (tiles * n_mat * ranks), most = (n_cols + 255) / 256;
+    const int rt = lora_rank_tiles(max_rank);
+    const long long tokens = 16ll * lora_token_groups(n_tok), groups = (n_tok + tokens - 1) / tokens * n_mat * ((max_rank + 16 * rt - 1) / (16 * rt));
+    const long long want = groups >= 96 ? 1 : 256 / groups, most = n_cols / (64 * kShrinkWaves);
     const long long parts = want < most ? want : most;
-    return (int)(parts > 16 ? 16 : parts < 1 ? 1 : parts);
+    return (int)(parts > 8 ? 8 : parts < 1 ? 1 : parts);
 }
 
+/* the groups of every tile, of which there are at most as many as tokens, or half of them twice as many; then h in fp32 for each part, or, of
+ * one part, as three numbers in bf16 */
+static size_t lora_records(int n_tok, int groups) { return ((size_t)n_tok + kTile - 1) / kTile * groups * sizeof(Group); }
 size_t lora_workspace_bytes(int n_mat, int max_rank, int n_cols, int n_tok) {
-    return (size_t)lora_parts(n_mat, max_rank, n_cols, n_tok) * n_mat * n_tok * ((max_rank + 15) / 16 * 16) * sizeof(float);
+    const int parts = lora_parts(n_mat, max_rank, n_cols, n_tok);
+    return lora_records(n_tok, (n_tok < kTile ? n_tok : kTile) * lora_token_groups(n_tok)) + (size_t)n_mat * n_tok * ((max_rank + 15) / 16 * 16) * (parts == 1 ? 6 : 4 * (size_t)parts);
 }
 
 LoraPlan lora_plan(const LoraCall &c) {
     LoraPlan p;
     p.tiles = (int)(((long long)c.n_tok + kTile - 1) / kTile);
     p.rank_pad = (c.max_rank + 15) / 16 * 16;
-    p.rank_tiles = p.rank_pad <= 16 ? 1 : p.rank_pad <= 32 ? 2 : 4;
-    p.rank_blocks = (p.rank_pad + 16 * p.rank_tiles - 1) / (16 * p.rank_tiles);
+    p.rank_tiles = lora_rank_tiles(c.max_rank);
+    p.rank_blocks = (c.max_rank + 16 * p.rank_tiles - 1) / (16 * p.rank_tiles);
+    p.token_groups = lora_token_groups(c.n_tok);
     p.parts = lora_parts(c.n_mat, c.max_rank, c.n_cols, c.n_tok);
-    p.row_tiles = c.n_tok <= kTile ? 1 : 4;
+    p.split = p.parts == 1 && c.lora_type == T_BF16;
+    p.row_tiles = c.n_tok <= 8 && !p.split ? 1 : 4;
     p.n_mat = c.n_mat;
     p.row_blocks_all = 0;
     for (int i = 0; i < 3; i++) {
-        p.row_blocks[i] = i < c.n_mat && (i == 0 || !c.pair) ? (int)(((long long)c.m[i].n_rows + 16 * kWaves * p.row_tiles - 1) / (16 * kWaves * p.row_tiles)) : 0;
+        const int rows = 16 * kExpandWaves * p.row_tiles;
+        p.row_blocks[i] = i < c.n_mat && (i == 0 || !c.pair) ? (int)(((long long)c.m[i].n_rows + rows - 1) / rows) : 0;
         p.row_blocks_all += p.row_blocks[i];
     }
-    long long classes = c.n_tok < kTile ? c.n_tok : kTile;
-    if (c.n_adapter + 1ll < classes) classes = c.n_adapter + 1ll;
-    const long long others = (long long)p.tiles * p.n_mat * p.rank_blocks * p.parts;
-    const long long want = 4096 / (others > 0 ? others : 1);
-    p.slots = (int)(want < 1 ? 1 : want < classes ? want : classes);
+    /* a workgroup for each group of tokens that a tile can have, unless that makes too many, but then one for each that a prompt of one adapter has */
+    const int tokens = c.n_tok < kTile ? c.n_tok : kTile, size = 16 * p.token_groups;
+    const long long classes = c.n_adapter + 1ll < tokens ? c.n_adapter + 1ll : tokens, bound = (tokens - classes) / size + classes, full = (tokens + size - 1) / size;
+    auto slots = [&](long long bound, long long full, long long others, long long most) {
+        const long long want = others > 0 && most / others > full ? most / others : full;
+        return (int)(want < bound ? want : bound);
+    };
+    p.groups = (int)bound * p.token_groups;
+    p.h_at = lora_records(c.n_tok, p.groups);
+    p.shrink_slots = slots(bound, full, (long long)p.tiles * p.n_mat * p.rank_blocks * p.parts, 1024);
+    p.expand_slots = slots(p.groups, full * p.token_groups, (long long)p.tiles * p.row_blocks_all, 16384);
     return p;
 }
 
-hipError_t launch_lora(uint32_t w_type, const LoraCall &c, const LoraPlan &p) {
-    return w_type == T_F32 ? launch_both<float>(c, p) : w_type == T_F16 ? launch_both<_Float16>(c, p) : launch_both<Bf16>(c, p);
+hipError_t launch_lora(const LoraCall &c, const LoraPlan &p) {
+    return c.lora_type == T_F32 ? launch_both<float>(c, p) : c.lora_type == T_F16 ? launch_both<_Float16>(c, p) : launch_both<Bf16>(c, p);
 }
 
 }  // namespace qlin

@@ -1565,9 +1565,9 @@ size_t qlin_lora_workspace_bytes(int n_mat, int max_rank, int n_cols, int n_tok)
     return lora_workspace_bytes(n_mat, max_rank, n_cols, n_tok);
 }
 
-static int lora_call(LoraCall &c, uint32_t lora_type, void *workspace, size_t workspace_bytes) {
-    if (!float_bytes(lora_type) || !float_bytes(c.x_type) || !float_bytes(c.y_type) || !float_bytes(c.out_type))
-        return fail(QLIN_ERR_TYPE, "adapters, activations and results are F32, F16 or BF16 (got types %u, %u, %u, %u)", lora_type, c.x_type, c.y_type, c.out_type);
+static int lora_call(LoraCall &c, void *workspace, size_t workspace_bytes) {
+    if (!float_bytes(c.lora_type) || !float_bytes(c.x_type) || !float_bytes(c.y_type) || !float_bytes(c.out_type))
+        return fail(QLIN_ERR_TYPE, "adapters, activations and results are F32, F16 or BF16 (got types %u, %u, %u, %u)", c.lora_type, c.x_type, c.y_type, c.out_type);
     if (c.n_adapter < 0 || c.max_rank < 1 || c.max_rank > kLoraMaxRank) return fail(QLIN_ERR_ARG, "%d adapters of rank %d (1 to %d)", c.n_adapter, c.max_rank, kLoraMaxRank);
     if (c.n_cols < 1 || c.n_cols >= 1 << 24) return fail(QLIN_ERR_ARG, "rows of %d columns", c.n_cols);
     if (int rc = check_float_rows("X", c.x_type, c.X, c.n_tok, c.n_cols, c.ldx)) return rc;
@@ -1583,31 +1583,31 @@ static int lora_call(LoraCall &c, uint32_t lora_type, void *workspace, size_t wo
     if (!rows) return QLIN_OK;
     if (!c.ids || !aligned(c.ids, 4)) return fail(QLIN_ERR_ARG, "null or misaligned pointer");
     const LoraPlan p = lora_plan(c);
-    if (!launch_takes(p.shrink_workgroups(), kLoraThreads) || !launch_takes(p.expand_workgroups(), kLoraThreads)) return fail(QLIN_ERR_ARG, "%d tokens in one call", c.n_tok);
+    if (!launch_takes(p.shrink_workgroups(), kLoraShrinkThreads) || !launch_takes(p.expand_workgroups(), kLoraExpandThreads)) return fail(QLIN_ERR_ARG, "%d tokens in one call", c.n_tok);
     const size_t need = lora_workspace_bytes(c.n_mat, c.max_rank, c.n_cols, c.n_tok);
     if (!workspace || !aligned(workspace, 16) || workspace_bytes < need) return fail(QLIN_ERR_ARG, "the workspace needs %zu bytes, 16-byte aligned", need);
     if (int rc = init_once()) return rc;
-    c.workspace = static_cast<float *>(workspace);
-    HIP_TRY(launch_lora(lora_type, c, p));
+    c.workspace = workspace;
+    HIP_TRY(launch_lora(c, p));
     return QLIN_OK;
 }
 
 int qlin_lora_add_dev(int n_mat, const qlin_lora_tensor *tensors, uint32_t lora_type, int n_adapter, int max_rank, const int32_t *ids, uint32_t x_type, const void *X,
                       uint32_t y_type, uint32_t out_type, int n_cols, int n_tok, int ldx, void *workspace, size_t workspace_bytes, void *stream) {
     if (n_mat < 1 || n_mat > 3 || !tensors) return fail(QLIN_ERR_ARG, "one to three tensors per call");
-    LoraCall c = {n_mat, false, {}, n_adapter, max_rank, ids, x_type, y_type, out_type, X, n_cols, n_tok, ldx, nullptr, (hipStream_t)stream};
+    LoraCall c = {n_mat, false, {}, n_adapter, max_rank, ids, lora_type, x_type, y_type, out_type, X, n_cols, n_tok, ldx, nullptr, (hipStream_t)stream};
     for (int i = 0; i < n_mat; i++)
         c.m[i] = {reinterpret_cast<const LoraEntry *>(tensors[i].adapters), tensors[i].Y, tensors[i].out, tensors[i].n_rows, tensors[i].ldy, tensors[i].ldo, 0};
-    return lora_call(c, lora_type, workspace, workspace_bytes);
+    return lora_call(c, workspace, workspace_bytes);
 }
 
 int qlin_lora_silu_mul_dev(const qlin_lora *gate_adapters, const qlin_lora *up_adapters, uint32_t lora_type, int n_adapter, int max_rank, const int32_t *ids, uint32_t x_type,
                            const void *X, uint32_t y_type, const void *gate, const void *up, uint32_t out_type, void *out, int n_rows, int n_cols, int n_tok, int ldx, int ldy,
                            int ldo, void *workspace, size_t workspace_bytes, void *stream) {
-    LoraCall c = {2, true, {}, n_adapter, max_rank, ids, x_type, y_type, out_type, X, n_cols, n_tok, ldx, nullptr, (hipStream_t)stream};
+    LoraCall c = {2, true, {}, n_adapter, max_rank, ids, lora_type, x_type, y_type, out_type, X, n_cols, n_tok, ldx, nullptr, (hipStream_t)stream};
     c.m[0] = {reinterpret_cast<const LoraEntry *>(gate_adapters), gate, out, n_rows, ldy, ldo, 0};
     c.m[1] = {reinterpret_cast<const LoraEntry *>(up_adapters), up, nullptr, n_rows, ldy, ldo, 0};
-    return lora_call(c, lora_type, workspace, workspace_bytes);
+    return lora_call(c, workspace, workspace_bytes);
 }
 
 /* ------------------------------------------------------------------ sampling */

@@ -297,27 +297,30 @@ struct LoraTensor {
     int32_t n_rows, ldy, ldo, unused;
 };
 constexpr int kLoraMaxRank = 256; /* = QLIN_LORA_MAX_RANK of the public header */
-constexpr int kLoraThreads = 256;
+constexpr int kLoraTile = 256, kLoraGroupBytes = 80; /* tokens of a tile, bytes of a group's record */
+constexpr int kLoraShrinkThreads = 1024, kLoraExpandThreads = 256;
 struct LoraCall {
     int n_mat; /* 1..3; pair (gate and up): 2, the result where m[0] says */
     bool pair;
     LoraTensor m[3];
     int n_adapter, max_rank;
     const int32_t *ids;
-    uint32_t x_type, y_type, out_type;
+    uint32_t lora_type, x_type, y_type, out_type;
     const void *X;
     int n_cols, n_tok, ldx;
-    float *workspace;
+    void *workspace;
     hipStream_t stream;
 };
 struct LoraPlan {
-    int tiles, slots, parts, rank_pad, rank_tiles, rank_blocks, row_tiles, row_blocks[3], row_blocks_all, n_mat;
-    unsigned long long shrink_workgroups() const { return (unsigned long long)tiles * n_mat * rank_blocks * parts * slots; }
-    unsigned long long expand_workgroups() const { return (unsigned long long)tiles * row_blocks_all * slots; }
+    int tiles, n_mat, parts, rank_pad, rank_tiles, rank_blocks, token_groups, split, groups, shrink_slots, row_tiles, row_blocks[3], row_blocks_all, expand_slots;
+    size_t h_at;
+    __host__ __device__ unsigned long long shrink_units() const { return (unsigned long long)tiles * rank_blocks * parts * shrink_slots; }
+    unsigned long long shrink_workgroups() const { return (shrink_units() + 7) / 8 * 8 * n_mat; }
+    unsigned long long expand_workgroups() const { return (unsigned long long)tiles * row_blocks_all * expand_slots; }
 };
 size_t lora_workspace_bytes(int n_mat, int max_rank, int n_cols, int n_tok);
 LoraPlan lora_plan(const LoraCall &c);
-hipError_t launch_lora(uint32_t w_type, const LoraCall &c, const LoraPlan &p);
+hipError_t launch_lora(const LoraCall &c, const LoraPlan &p);
 /* the experts of each token and their weights (moe_route_scores.hip); bias may be null */
 struct RouteCall {
     int score; /* 0: softmax, 1: sigmoid */
