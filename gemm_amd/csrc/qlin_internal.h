@@ -298,7 +298,7 @@ struct LoraTensor {
 };
 constexpr int kLoraMaxRank = 256; /* = QLIN_LORA_MAX_RANK of the public header */
 constexpr int kLoraTile = 256, kLoraGroupBytes = 80; /* tokens of a tile, bytes of a group's record */
-constexpr int kLoraShrinkThreads = 1024, kLoraExpandThreads = 256;
+constexpr int kLoraShrinkThreads = 1024, kLoraExpandThreads = 256, kLoraFewThreads = 1024;
 struct LoraCall {
     int n_mat; /* 1..3; pair (gate and up): 2, the result where m[0] says */
     bool pair;
@@ -312,9 +312,9 @@ struct LoraCall {
     hipStream_t stream;
 };
 struct LoraPlan {
-    int tiles, n_mat, parts, rank_pad, rank_tiles, rank_blocks, token_groups, split, groups, shrink_slots, row_tiles, row_blocks[3], row_blocks_all, expand_slots;
+    int tiles, n_mat, parts, rank_pad, rank_tiles, rank_blocks, token_groups, split, few, groups, shrink_slots, row_tiles, row_blocks[3], row_blocks_all, expand_slots;
     size_t h_at;
-    __host__ __device__ unsigned long long shrink_units() const { return (unsigned long long)tiles * rank_blocks * parts * shrink_slots; }
+    __host__ __device__ unsigned long long shrink_units() const { return (unsigned long long)parts * shrink_slots * rank_blocks * tiles; }
     unsigned long long shrink_workgroups() const { return (shrink_units() + 7) / 8 * 8 * n_mat; }
     unsigned long long expand_workgroups() const { return (unsigned long long)tiles * row_blocks_all * expand_slots; }
 };
