@@ -46,10 +46,10 @@ __device__ __forceinline__ double score_of(int kind, double x, double max, doubl
     return (x >= 0 ? 1.0 : e) / (1.0 + e);
 }
 
-/* One wave per token, the experts' 64-bit values in LDS. */
+/* A token by one wave, its experts' 64-bit values in LDS: any number of experts, places and groups. */
 template <class X>
 __global__ void __launch_bounds__(64)
-moe_route_scores_kernel(RouteCall c) {
+moe_route_any_kernel(RouteCall c) {
     extern __shared__ double key[]; /* [n_expert], then [n_group] */
     double *of_group = key + c.n_expert;
     const int lane = threadIdx.x;
@@ -143,18 +143,340 @@ moe_route_scores_kernel(RouteCall c) {
         }
 }
 
+
+/* ------------------------------------------------------------------ up to 512 experts and 16 places */
+
+template <int CTRL> __device__ __forceinline__ int mov(int v) { return __builtin_amdgcn_mov_dpp(v, CTRL, 0xf, 0xf, true); }
+template <int CTRL> __device__ __forceinline__ float mov(float v) { return __int_as_float(mov<CTRL>(__float_as_int(v))); }
+template <int CTRL> __device__ __forceinline__ double mov(double v) { return __hiloint2double(mov<CTRL>(__double2hiint(v)), mov<CTRL>(__double2loint(v))); }
+constexpr int kSwap1 = 0xB1, kSwap2 = 0x4E, kMirror8 = 0x141, kMirror16 = 0x140; /* the four moves after which each of 16 lanes has seen all others */
+template <class T, class F> __device__ __forceinline__ T row_all(T v, F f) {
+    v = f(v, mov<kSwap1>(v));
+    v = f(v, mov<kSwap2>(v));
+    v = f(v, mov<kMirror8>(v));
+    return f(v, mov<kMirror16>(v));
+}
+__device__ __forceinline__ float row_max(float v) { return row_all(v, [](float a, float b) { return fmaxf(a, b); }); }
+__device__ __forceinline__ float row_sum(float v) { return row_all(v, [](float a, float b) { return a + b; }); }
+__device__ __forceinline__ double row_sum(double v) { return row_all(v, [](double a, double b) { return a + b; }); }
+
+/* exp in 64 bits for arguments up to 0, to about 2^-52: 2^n exp(r), r to degree 12 of its series; 0 below the least number */
+__device__ __forceinline__ double exp_to_one(double x) {
+    if (!(x > -745.2)) return 0.0;
+    const double n = rint(x * 1.4426950408889634);
+    double r = fma(n, -0.6931471805599453, x);
+    r = fma(n, -2.3190468138462996e-17, r);
+    double p = 1.0 / 479001600;
+    p = fma(p, r, 1.0 / 39916800);
+    p = fma(p, r, 1.0 / 3628800);
+    p = fma(p, r, 1.0 / 362880);
+    p = fma(p, r, 1.0 / 40320);
+    p = fma(p, r, 1.0 / 5040);
+    p = fma(p, r, 1.0 / 720);
+    p = fma(p, r, 1.0 / 120);
+    p = fma(p, r, 1.0 / 24);
+    p = fma(p, r, 1.0 / 6);
+    p = fma(p, r, 0.5);
+    p = fma(p, r, 1.0);
+    p = fma(p, r, 1.0);
+    return ldexp(p, (int)n);
+}
+__device__ __forceinline__ double quotient(double a, double b) { /* b from 1 up */
+    double r = __builtin_amdgcn_rcp(b);
+    r = fma(fma(-b, r, 1.0), r, r);
+    r = fma(fma(-b, r, 1.0), r, r);
+    const double q = a * r;
+    return fma(fma(-b, q, a), r, q);
+}
+
+/* keeps what is computed of x in the branch that asks for it: the compiler would do it for every token, ahead of a loop */
+__device__ __forceinline__ float here(float x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
+/* 16 lanes to a token, N experts to a lane in registers (its next `per`), a place of the result in each of the 16 lanes.
+ *   Without a bias the experts' order is that of their logits, which fp32 holds. With one, values are computed in fp32, and where one lies so close to
+ * the largest that their errors could change the order (`away`), those that do are computed once more in 64 bits: the choice is always the one of
+ * 64-bit values, and hardly a wave has to. Groups go the same way, by the sum of their largest values.
+ *   A pick: the lanes' largest, the largest of 16 lanes by four moves between lanes, the first lane and in it the first expert that has it. */
+template <class X, int N, bool BIAS>
+__global__ void __launch_bounds__(256, N <= 16 ? 4 : 2)
+moe_route_row_kernel(RouteCall c, int per, int group_lanes) {
+    const int lane = threadIdx.x & 15;
+    const long long row = (long long)blockIdx.x * 16 + threadIdx.x / 16;
+    if (row - (threadIdx.x & 48) / 16 >= c.n_tok) return; /* none of the wave's */
+    const bool there = row < c.n_tok;
+    const X *x = static_cast<const X *>(c.logits) + (size_t)(there ? row : c.n_tok - 1) * c.ld;
+    const int e0 = lane * per, n = c.n_expert - e0 < per ? c.n_expert - e0 : per; /* the lane's experts: e0 .. e0 + n - 1 */
+    const float none = -INFINITY;
+    float v[N], key[N];
+    constexpr int kVec = 16 / sizeof(X);
+    const bool whole = c.n_expert % per == 0;
+    if (per % kVec == 0 && whole && ((uintptr_t)c.logits & 15) == 0 && (size_t)c.ld * sizeof(X) % 16 == 0) {
+        struct alignas(16) Vec { X v[kVec]; };
+#pragma unroll
+        for (int j = 0; j < N; j += kVec) {
+            Vec w = {};
+            if (j < n) w = *reinterpret_cast<const Vec *>(x + e0 + j);
+#pragma unroll
+            for (int i = 0; i < kVec && j + i < N; i++) v[j + i] = j + i < n ? to_f32(w.v[i]) : none;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; j++) v[j] = j < n ? to_f32(x[e0 + j]) : none;
+    }
+    if constexpr (BIAS) {
+        if (per % 4 == 0 && whole && ((uintptr_t)c.bias & 15) == 0) {
+#pragma unroll
+            for (int j = 0; j < N; j += 4) {
+                float4 w = {};
+                if (j < n) w = *reinterpret_cast<const float4 *>(c.bias + e0 + j);
+                key[j] = w.x;
+                key[j + 1] = w.y;
+                key[j + 2] = w.z;
+                key[j + 3] = w.w;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; j++) key[j] = j < n ? c.bias[e0 + j] : none;
+        }
+    }
+    float most = none;
+#pragma unroll
+    for (int j = 0; j < N; j++) {
+        v[j] = v[j] > none ? v[j] : none; /* (a NaN compares false) */
+        most = fmaxf(most, v[j]);
+    }
+    most = row_max(most);
+    constexpr float kLog2e = 1.44269504088896341f;
+    auto power = [&](float x) { return x == most ? 1.0f : __builtin_amdgcn_exp2f((x - most) * kLog2e); }; /* (infinities share) */
+    float sum = 1.0f; /* of the softmax */
+    if (c.score == 0) {
+        sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < N; j++) sum += v[j] > none ? power(v[j]) : 0.0f;
+        sum = row_sum(sum);
+    }
+    /* in 64 bits; every lane of the row takes part in the sum */
+    auto below = [&](float x) { return x == most ? 0.0 : (double)x - (double)most; };
+    auto sum64 = [&]() {
+        double s = 1.0;
+        if (c.score == 0) {
+            s = 0.0;
+#pragma unroll
+            for (int j = 0; j < N; j++) {
+                const float x = here(v[j]);
+                s += x > none ? exp_to_one(below(x)) : 0.0;
+            }
+            s = row_sum(s);
+        }
+        return s;
+    };
+    auto score64 = [&](float x, double sum64) { /* of an expert that is there */
+        const double e = exp_to_one(c.score == 0 ? below(x) : -fabs((double)x));
+        return quotient(c.score == 0 || x < 0.0f ? e : 1.0, c.score == 0 ? sum64 : 1.0 + e);
+    };
+    /* how far an fp32 value may be from another to be taken for it: twice their error. A sigmoid's is below 4e-7 (argument, exponential and reciprocal), a
+     * softmax's 2e-6 of itself (the sum's most of all), and no score is above 1 / sum; adding the bias rounds by 2^-24 */
+    float away = 0.0f;
+    auto threshold = [&](float m) { return !BIAS || m == INFINITY ? m : m - (away + 2.4e-7f * fabsf(m)); };
+    if constexpr (BIAS) {
+        const float inverse = __builtin_amdgcn_rcpf(sum);
+        away = c.score == 0 ? 4e-6f * inverse : 8e-7f;
+        auto values = [&](auto score) {
+#pragma unroll
+            for (int j = 0; j < N; j++) {
+                const float value = score(v[j]) + key[j];
+                key[j] = v[j] > none && value > none ? value : none;
+            }
+        };
+        if (c.score == 0) values([&](float x) { return power(x) * inverse; });
+        else values([&](float x) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * -kLog2e)); });
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; j++) key[j] = v[j];
+    }
+    float top = none, next = none; /* the lane's two largest */
+    auto rank_again = [&]() {
+        top = next = none;
+#pragma unroll
+        for (int j = 0; j < N; j++) {
+            next = __builtin_amdgcn_fmed3f(top, next, key[j]);
+            top = fmaxf(top, key[j]);
+        }
+    };
+    rank_again();
+    if (group_lanes) {
+        bool kept;
+        float first = top, second = next; /* of the group */
+        auto join = [&](auto &a, auto &b, auto c, auto d) {
+            b = fmax(fmin(a, c), fmax(b, d));
+            a = fmax(a, c);
+        };
+        auto join_lanes = [&](auto &a, auto &b) {
+            if (group_lanes > 1) join(a, b, mov<kSwap1>(a), mov<kSwap1>(b));
+            if (group_lanes > 2) join(a, b, mov<kSwap2>(a), mov<kSwap2>(b));
+            if (group_lanes > 4) join(a, b, mov<kMirror8>(a), mov<kMirror8>(b));
+        };
+        join_lanes(first, second);
+        auto look = [&](auto see) { /* at the other groups of the row, and the lane of each */
+#define QLIN_LOOK(N_) \
+    if ((N_) % group_lanes == 0) see([](auto w) { return mov<0x120 + (N_)>(w); });
+            QLIN_LOOK(1) QLIN_LOOK(2) QLIN_LOOK(3) QLIN_LOOK(4) QLIN_LOOK(5) QLIN_LOOK(6) QLIN_LOOK(7) QLIN_LOOK(8)
+            QLIN_LOOK(9) QLIN_LOOK(10) QLIN_LOOK(11) QLIN_LOOK(12) QLIN_LOOK(13) QLIN_LOOK(14) QLIN_LOOK(15)
+#undef QLIN_LOOK
+        };
+        bool close = false;
+        if (BIAS) {
+            const bool two = c.group_top > 1 && second > none;
+            const float worth = two ? first + second : first;
+            const float size = row_max(first > none ? fabsf(first) + (two ? fabsf(second) : 0.0f) : 0.0f), apart = 2.0f * away + 5e-7f * size;
+            int surely = 0, maybe = 0;
+            look([&](auto other) {
+                const float w = other(worth);
+                surely += w - worth > apart ? 1 : 0;
+                maybe += w - worth >= -apart ? 1 : 0;
+            });
+            kept = surely < c.n_group_used;
+            close = first > none && (!(apart < INFINITY) || (kept && maybe >= c.n_group_used));
+        }
+        if (!BIAS || __ballot(close)) { /* by 64-bit values, equal ones by index */
+            double a = top, b = next;
+            double s64 = 1.0;
+            if (BIAS || c.group_top > 1) s64 = sum64();
+            if constexpr (BIAS) {
+                a = b = none;
+                const float least = next > none ? threshold(next) : top > none ? threshold(top) : INFINITY;
+#pragma unroll
+                for (int j = 0; j < N; j++)
+                    if (__ballot(key[j] >= least)) {
+                        const double d = key[j] >= least ? score64(here(v[j]), s64) + (double)c.bias[e0 + j] : (double)none;
+                        b = fmax(b, fmin(a, d));
+                        a = fmax(a, d);
+                    }
+            }
+            join_lanes(a, b);
+            double worth = a;
+            if (c.group_top > 1 && a > (double)none) {
+                if constexpr (!BIAS) {
+                    worth = score64((float)a, s64);
+                    if (b > (double)none) worth += score64((float)b, s64);
+                } else if (b > (double)none) {
+                    worth += b;
+                }
+            }
+            int before = 0;
+            look([&](auto other) {
+                const double w = other(worth);
+                const int from = other(lane); /* (with all lanes) */
+                before += w > worth || (w == worth && from < lane) ? 1 : 0;
+            });
+            kept = before < c.n_group_used;
+        }
+        if (!kept) {
+#pragma unroll
+            for (int j = 0; j < N; j++) key[j] = none;
+            top = next = none;
+        }
+    }
+    int pick = -1; /* of place `lane` */
+    const int shift = threadIdx.x & 48; /* the row's 16 bits of a ballot */
+    auto of_row = [&](bool b) { return (uint32_t)(__ballot(b) >> shift) & 0xFFFFu; };
+    for (int k = 0; k < c.top_k; k++) {
+        const float m = row_max(top), least = threshold(m);
+        uint32_t lanes = of_row(top >= least && m > none);
+        const uint32_t doubles = of_row(next >= least && m > none);
+        int at = N;
+        if (!__ballot(doubles || (lanes & (lanes - 1)))) { /* one alone in every row */
+            const float mine = (lanes >> lane) & 1 ? m : NAN;
+            top = next = none;
+#pragma unroll
+            for (int j = 0; j < N; j++) {
+                const bool hit = key[j] == mine;
+                at = hit ? j : at;
+                key[j] = hit ? none : key[j];
+                next = __builtin_amdgcn_fmed3f(top, next, key[j]);
+                top = fmaxf(top, key[j]);
+            }
+        } else {
+            if constexpr (BIAS) {
+                double best = none;
+                const double s64 = sum64();
+#pragma unroll
+                for (int j = 0; j < N; j++)
+                    if (__ballot(key[j] >= least)) {
+                        const double d = key[j] >= least && m > none ? score64(here(v[j]), s64) + (double)c.bias[e0 + j] : (double)none;
+                        at = d > best ? j : at;
+                        best = fmax(best, d);
+                    }
+                const double row_best = row_all(best, [](double a, double b) { return fmax(a, b); });
+                lanes = of_row(at < N && best == row_best);
+            } else {
+#pragma unroll
+                for (int j = N - 1; j >= 0; j--) at = key[j] == m ? j : at;
+                lanes = of_row(at < N && m > none);
+            }
+            const int taken = __builtin_ctz(lanes | 0x10000u) == lane ? at : N;
+#pragma unroll
+            for (int j = 0; j < N; j++) key[j] = taken == j ? none : key[j];
+            rank_again();
+        }
+        const int winner = __builtin_ctz(lanes | 0x10000u); /* 16: nothing is left */
+        const int chosen = __shfl(e0 + at, winner & 15, 16);
+        if (lane == k) pick = winner < 16 ? chosen : -1;
+    }
+    float w = 0.0f;
+    if (pick >= 0) {
+        const float p = to_f32(x[pick]);
+        if (c.score == 0) {
+            w = (p == most ? 1.0f : expf(p - most)) / sum;
+        } else {
+            const float e = expf(-fabsf(p));
+            w = (p >= 0.0f ? 1.0f : e) / (1.0f + e);
+        }
+    }
+    if (c.renorm) {
+        const float total = row_sum(w);
+        if (total > 0.0f) w /= total;
+    }
+    if (there && lane < c.top_k) {
+        c.idx[row * c.top_k + lane] = pick;
+        c.w[row * c.top_k + lane] = w * c.scale;
+    }
+}
+
+template <class X, int N> void launch_rows(const RouteCall &c, int per, int group_lanes) {
+    const dim3 grid((uint32_t)(((long long)c.n_tok + 15) / 16)), block(256);
+    if (c.bias)
+        hipLaunchKernelGGL((moe_route_row_kernel<X, N, true>), grid, block, 0, c.stream, c, per, group_lanes);
+    else
+        hipLaunchKernelGGL((moe_route_row_kernel<X, N, false>), grid, block, 0, c.stream, c, per, group_lanes);
+}
+
+template <class X> hipError_t launch_route(const RouteCall &c) {
+    const int per = (c.n_expert + 15) / 16, of_group = c.n_expert / c.n_group;
+    /* lanes to a group: 0 where all groups stay, else a power of two */
+    const int group_lanes = c.n_group_used == c.n_group ? 0 : of_group % per ? -1 : of_group / per;
+    if (c.top_k > 16 || per > 32 || (group_lanes && group_lanes != 1 && group_lanes != 2 && group_lanes != 4 && group_lanes != 8)) {
+        const size_t lds = ((size_t)c.n_expert + c.n_group) * sizeof(double);
+        hipLaunchKernelGGL(moe_route_any_kernel<X>, dim3(c.n_tok), dim3(64), lds, c.stream, c);
+    } else if (per <= 4) {
+        launch_rows<X, 4>(c, per, group_lanes);
+    } else if (per <= 8) {
+        launch_rows<X, 8>(c, per, group_lanes);
+    } else if (per <= 16) {
+        launch_rows<X, 16>(c, per, group_lanes);
+    } else {
+        launch_rows<X, 32>(c, per, group_lanes);
+    }
+    return hipGetLastError();
+}
+
 }  // namespace
 
 hipError_t launch_moe_route_scores(uint32_t type, const RouteCall &c) {
-    const size_t lds = ((size_t)c.n_expert + c.n_group) * sizeof(double);
-    const dim3 grid(c.n_tok), block(64);
-    if (type == T_F32)
-        hipLaunchKernelGGL(moe_route_scores_kernel<float>, grid, block, lds, c.stream, c);
-    else if (type == T_F16)
-        hipLaunchKernelGGL(moe_route_scores_kernel<_Float16>, grid, block, lds, c.stream, c);
-    else
-        hipLaunchKernelGGL(moe_route_scores_kernel<Bf16>, grid, block, lds, c.stream, c);
-    return hipGetLastError();
+    return type == T_F32 ? launch_route<float>(c) : type == T_F16 ? launch_route<_Float16>(c) : launch_route<Bf16>(c);
 }
 
 }  // namespace qlin
