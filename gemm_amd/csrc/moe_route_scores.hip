@@ -12,6 +12,8 @@
 #include "qlin_device.h"
 #include "qlin_internal.h"
 
+#include <type_traits>
+
 namespace qlin {
 
 namespace {
@@ -297,16 +299,27 @@ moe_route_row_kernel(RouteCall c, int per, int group_lanes) {
 #pragma unroll
         for (int j = 0; j < N; j++) key[j] = v[j];
     }
-    float top = none, next = none; /* the lane's two largest */
-    auto rank_again = [&]() {
-        top = next = none;
+    /* the lane's four largest in order, equal ones by index, and which they are; `gone` has a bit for each that is picked */
+    float top = none, next = none, third = none, fourth = none;
+    int at = 0, next_at = 0, third_at = 0, fourth_at = 0;
+    uint32_t gone = 0;
+    auto rank = [&](auto some_gone) {
+        top = next = third = fourth = none;
 #pragma unroll
         for (int j = 0; j < N; j++) {
-            next = __builtin_amdgcn_fmed3f(top, next, key[j]);
-            top = fmaxf(top, key[j]);
+            const float k = decltype(some_gone)::value && (gone >> j) & 1 ? none : key[j];
+            const bool a = k > top, b = k > next, d = k > third, e = k > fourth;
+            fourth_at = d ? third_at : e ? j : fourth_at;
+            third_at = b ? next_at : d ? j : third_at;
+            next_at = a ? at : b ? j : next_at;
+            at = a ? j : at;
+            fourth = __builtin_amdgcn_fmed3f(third, fourth, k);
+            third = __builtin_amdgcn_fmed3f(next, third, k);
+            next = __builtin_amdgcn_fmed3f(top, next, k);
+            top = fmaxf(top, k);
         }
     };
-    rank_again();
+    rank(std::false_type{});
     if (group_lanes) {
         bool kept;
         float first = top, second = next; /* of the group */
@@ -375,56 +388,62 @@ moe_route_row_kernel(RouteCall c, int per, int group_lanes) {
             kept = before < c.n_group_used;
         }
         if (!kept) {
-#pragma unroll
-            for (int j = 0; j < N; j++) key[j] = none;
-            top = next = none;
+            gone = ~0u;
+            top = next = third = fourth = none;
         }
     }
     int pick = -1; /* of place `lane` */
     const int shift = threadIdx.x & 48; /* the row's 16 bits of a ballot */
     auto of_row = [&](bool b) { return (uint32_t)(__ballot(b) >> shift) & 0xFFFFu; };
+    int left_in_list = 4;
+    constexpr int kRankAt = BIAS ? 1 : 0; /* (where values may be close, the one behind the first has to be known) */
     for (int k = 0; k < c.top_k; k++) {
-        const float m = row_max(top), least = threshold(m);
-        uint32_t lanes = of_row(top >= least && m > none);
-        const uint32_t doubles = of_row(next >= least && m > none);
-        int at = N;
-        if (!__ballot(doubles || (lanes & (lanes - 1)))) { /* one alone in every row */
-            const float mine = (lanes >> lane) & 1 ? m : NAN;
-            top = next = none;
-#pragma unroll
-            for (int j = 0; j < N; j++) {
-                const bool hit = key[j] == mine;
-                at = hit ? j : at;
-                key[j] = hit ? none : key[j];
-                next = __builtin_amdgcn_fmed3f(top, next, key[j]);
-                top = fmaxf(top, key[j]);
-            }
-        } else {
-            if constexpr (BIAS) {
+        const float m = row_max(top);
+        uint32_t lanes;
+        bool looked = false; /* at all experts once more */
+        int which = at;
+        if constexpr (BIAS) {
+            const float least = threshold(m);
+            lanes = of_row(top >= least && m > none);
+            looked = __ballot((next >= least && m > none) || (lanes & (lanes - 1))); /* several that could be the largest */
+            if (looked) {
                 double best = none;
                 const double s64 = sum64();
 #pragma unroll
-                for (int j = 0; j < N; j++)
-                    if (__ballot(key[j] >= least)) {
-                        const double d = key[j] >= least && m > none ? score64(here(v[j]), s64) + (double)c.bias[e0 + j] : (double)none;
-                        at = d > best ? j : at;
+                for (int j = 0; j < N; j++) {
+                    const bool may = key[j] >= least && m > none && !((gone >> j) & 1);
+                    if (__ballot(may)) {
+                        const double d = may ? score64(here(v[j]), s64) + (double)c.bias[e0 + j] : (double)none;
+                        which = d > best ? j : which;
                         best = fmax(best, d);
                     }
+                }
                 const double row_best = row_all(best, [](double a, double b) { return fmax(a, b); });
-                lanes = of_row(at < N && best == row_best);
-            } else {
-#pragma unroll
-                for (int j = N - 1; j >= 0; j--) at = key[j] == m ? j : at;
-                lanes = of_row(at < N && m > none);
+                lanes = of_row(best > (double)none && best == row_best);
             }
-            const int taken = __builtin_ctz(lanes | 0x10000u) == lane ? at : N;
-#pragma unroll
-            for (int j = 0; j < N; j++) key[j] = taken == j ? none : key[j];
-            rank_again();
+        } else {
+            lanes = of_row(top == m && m > none);
         }
         const int winner = __builtin_ctz(lanes | 0x10000u); /* 16: nothing is left */
-        const int chosen = __shfl(e0 + at, winner & 15, 16);
+        const int chosen = __shfl(e0 + which, winner & 15, 16);
         if (lane == k) pick = winner < 16 ? chosen : -1;
+        const bool mine = winner == lane;
+        if (mine) {
+            gone |= 1u << which;
+            left_in_list--;
+        }
+        if (looked || (N > 4 && __ballot(left_in_list <= kRankAt))) {
+            rank(std::true_type{});
+            left_in_list = 4;
+        } else {
+            top = mine ? next : top;
+            next = mine ? third : next;
+            third = mine ? fourth : third;
+            fourth = mine ? none : fourth;
+            at = mine ? next_at : at;
+            next_at = mine ? third_at : next_at;
+            third_at = mine ? fourth_at : third_at;
+        }
     }
     float w = 0.0f;
     if (pick >= 0) {

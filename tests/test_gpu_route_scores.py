@@ -152,3 +152,18 @@ def test_same_bits_again():
     for n in (1, 3, 64):  # and a token's result does not depend on the others
         c = call(x[:n], F32, True, small_bias(1, 256), 8, 4, 2, 8, True, 2.5)
         assert np.array_equal(a[0][:n], c[0]) and np.array_equal(a[1][:n], c[1])
+
+
+@pytest.mark.parametrize("biased", [False, True])
+@pytest.mark.parametrize("n,n_group,k", [(256, 1, 16), (250, 1, 16), (512, 1, 16), (256, 8, 12), (256, 16, 16), (100, 1, 12)])
+def test_all_picks_among_neighbouring_experts(biased, n, n_group, k):
+    """the largest values stand next to each other, a step of 64 bits apart, equal and far ones among them"""
+    rng = np.random.default_rng(n + k)
+    x = rng.standard_normal((24, n)) * 0.1
+    for row in range(24):
+        at = rng.integers(0, n - 20)
+        x[row, at:at + 20] = 2.0 + rng.integers(0, 3, 20) * [2.0 ** -24, 2.0 ** -20, 0.01, 0.0][row % 4]
+    bias = np.where(rng.random(n) < 0.5, 0.25, 0.25 + 2.0 ** -25) if biased else None
+    for sigmoid in (False, True):
+        check(x, F32, sigmoid, bias, n_group, max(1, n_group // 2), 2, k, True, 1.0)
+        check(x, F16, sigmoid, bias, n_group, n_group, 1, k, True, 1.0)
