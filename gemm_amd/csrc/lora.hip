@@ -55,31 +55,27 @@ __device__ __forceinline__ void wave_meets() {
 /* addresses that come out of a table are global ones: without this the loads would ask LDS as well */
 template <class T> using Global = const T __attribute__((address_space(1))) *;
 
-/* N elements p[at..], zeros from `end` on; VEC: p + at on the vector's alignment, at and end multiples of N */
-template <class T, int N, bool VEC> __device__ __forceinline__ Vec<T, N> load(const T *p, int at, int end) {
-    Vec<T, N> e = {};
-    if constexpr (VEC) {
-        typedef uint32_t Words __attribute__((ext_vector_type(sizeof(T) * N / 4 < 4 ? sizeof(T) * N / 4 : 4)));
-        constexpr int kPieces = sizeof(T) * N / sizeof(Words);
-        struct { Words w[kPieces]; } raw = {};
-        if (at < end) {
+/* N elements p[at..], zeros from `end` on, at any element's address; WHOLE: at and end are multiples of N */
+template <class T, int N, bool WHOLE> __device__ __forceinline__ Vec<T, N> load(const T *p, int at, int end) {
+    typedef uint32_t Words __attribute__((ext_vector_type(sizeof(T) * N / 4 < 4 ? sizeof(T) * N / 4 : 4)));
+    typedef Words Anywhere __attribute__((aligned(sizeof(T))));
+    constexpr int kPieces = sizeof(T) * N / sizeof(Words);
+    struct { Words w[kPieces]; } raw = {};
+    if (WHOLE ? at < end : at + N <= end) {
 #pragma unroll
-            for (int i = 0; i < kPieces; i++) raw.w[i] = ((Global<Words>)(p + at))[i];
-        }
-        e = __builtin_bit_cast(Vec<T, N>, raw);
-    } else {
-        const Global<T> g = (Global<T>)p;
+        for (int i = 0; i < kPieces; i++) raw.w[i] = ((Global<Anywhere>)(p + at))[i];
+    }
+    Vec<T, N> e = __builtin_bit_cast(Vec<T, N>, raw);
+    if (!WHOLE && at < end && at + N > end) {
 #pragma unroll
-        for (int i = 0; i < N; i++)
+        for (int i = 0; i < N - 1; i++)
             if (at + i < end) {
                 if constexpr (Same<T, Bf16>::value) e.v[i].bits = ((Global<uint16_t>)p)[at + i];
-                else e.v[i] = g[at + i];
+                else e.v[i] = ((Global<T>)p)[at + i];
             }
     }
     return e;
 }
-
-__device__ __forceinline__ bool on(const void *p, size_t bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
 
 /* an adapter as the kernels take it: rank 0 where the table's entry cannot be used */
 struct Entry {
@@ -288,7 +284,7 @@ template <class T, int C> struct Rows16 {
 template <class W, class X, int RT, int NJ> constexpr int columns() { return native<W, X>() && RT + NJ <= 4 ? 64 : 32; }
 constexpr int kTurnBytes = 2 * 16 * 128; /* of a wave, for two of its operands in turn */
 
-/* a step on its way; WHOLE: all of its columns are there */
+/* a step on its way; WHOLE: all of its columns are there, else from where `from` stands some are not */
 template <class W, class X, int RT, int NJ> struct Step {
     static constexpr int C = columns<W, X, RT, NJ>();
     typedef Rows16<W, C> RowsW;
@@ -301,7 +297,7 @@ template <class W, class X, int RT, int NJ> struct Step {
     };
     template <bool WHOLE, class T, class R> static __device__ __forceinline__ void fetch_rows(R &r, const T *const (&from)[R::kLoads], int at, int n_cols) {
 #pragma unroll
-        for (int l = 0; l < R::kLoads; l++) r.v[l] = __builtin_bit_cast(typename R::Piece, load<T, 16 / sizeof(T), true>(from[l], at, WHOLE ? 0x7FFFFFFF : n_cols - R::column()));
+        for (int l = 0; l < R::kLoads; l++) r.v[l] = __builtin_bit_cast(typename R::Piece, load<T, 16 / sizeof(T), WHOLE>(from[l], at, WHOLE ? 0x7FFFFFFF : n_cols - R::column()));
     }
     template <bool WHOLE> __device__ __forceinline__ void fetch(const From &from, int step, int n_cols) {
 #pragma unroll
@@ -339,59 +335,43 @@ template <class W, class X, int RT, int NJ> struct Step {
 /* sums over columns [k0, k1) for RT groups of 16 ranks and NJ groups of 16 tokens, the n that list names; what comes of ranks and tokens that are not there is
  * not looked at */
 template <class W, class X, int RT, int NJ>
-__device__ __forceinline__ void shrink_sums(bool vec, const W *A, int rank0, int rank, const X *X0, int ldx, const uint8_t *list, int n, int n_cols, int k0, int k1,
+__device__ __forceinline__ void shrink_sums(const W *A, int rank0, int rank, const X *X0, int ldx, const uint8_t *list, int n, int n_cols, int k0, int k1,
                                             char *turn, f32x4 (&acc)[NJ][RT]) {
-    if (vec) { /* the next step is on its way while one is multiplied; behind the last one it is that once more */
-        typedef Step<W, X, RT, NJ> S;
-        typename S::From from;
+    /* the next step is on its way while one is multiplied; behind the last one it is that once more */
+    typedef Step<W, X, RT, NJ> S;
+    typename S::From from;
 #pragma unroll
-        for (int i = 0; i < RT; i++)
+    for (int i = 0; i < RT; i++)
 #pragma unroll
-            for (int l = 0; l < S::RowsW::kLoads; l++) {
-                const int r = rank0 + 16 * i + S::RowsW::row(l);
-                from.w[i][l] = A + (size_t)(r < rank ? r : rank - 1) * n_cols + S::RowsW::column();
-            }
-#pragma unroll
-        for (int j = 0; j < NJ; j++)
-#pragma unroll
-            for (int l = 0; l < S::RowsX::kLoads; l++) {
-                const int q = 16 * j + S::RowsX::row(l);
-                from.x[j][l] = X0 + (size_t)list[q < n ? q : 0] * ldx + S::RowsX::column();
-            }
-        const int whole = n_cols / S::C, last = (k1 + S::C - 1) / S::C, end = last < whole ? last : whole;
-        int k = k0 / S::C;
-        S s[2];
-        if (k < end) {
-            s[0].template fetch<true>(from, k, n_cols);
-            for (; k + 2 <= end; k += 2) {
-                s[1].template fetch<true>(from, k + 1, n_cols);
-                __builtin_amdgcn_sched_barrier(0); /* (the compiler would fetch where it multiplies) */
-                s[0].add_to(acc, turn);
-                s[0].template fetch<true>(from, k + 2 < end ? k + 2 : k + 1, n_cols);
-                __builtin_amdgcn_sched_barrier(0);
-                s[1].add_to(acc, turn);
-            }
-            if (k < end) s[0].add_to(acc, turn);
+        for (int l = 0; l < S::RowsW::kLoads; l++) {
+            const int r = rank0 + 16 * i + S::RowsW::row(l);
+            from.w[i][l] = A + (size_t)(r < rank ? r : rank - 1) * n_cols + S::RowsW::column();
         }
-        if (end < last && S::C * end < n_cols) {
-            s[0].template fetch<false>(from, end, n_cols);
+#pragma unroll
+    for (int j = 0; j < NJ; j++)
+#pragma unroll
+        for (int l = 0; l < S::RowsX::kLoads; l++) {
+            const int q = 16 * j + S::RowsX::row(l);
+            from.x[j][l] = X0 + (size_t)list[q < n ? q : 0] * ldx + S::RowsX::column();
+        }
+    const int whole = n_cols / S::C, last = (k1 + S::C - 1) / S::C, end = last < whole ? last : whole;
+    int k = k0 / S::C;
+    S s[2];
+    if (k < end) {
+        s[0].template fetch<true>(from, k, n_cols);
+        for (; k + 2 <= end; k += 2) {
+            s[1].template fetch<true>(from, k + 1, n_cols);
+            __builtin_amdgcn_sched_barrier(0); /* (the compiler would fetch where it multiplies) */
             s[0].add_to(acc, turn);
+            s[0].template fetch<true>(from, k + 2 < end ? k + 2 : k + 1, n_cols);
+            __builtin_amdgcn_sched_barrier(0);
+            s[1].add_to(acc, turn);
         }
-    } else { /* rows that do not lie on 16 bytes: element by element */
-        const int row = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4, end = k1 < n_cols ? k1 : n_cols;
-#pragma unroll 1
-        for (int at = k0 + 8 * g; at < end + 8 * g; at += 32) {
-            Vec<X, 8> b[NJ];
-#pragma unroll
-            for (int j = 0; j < NJ; j++) b[j] = load<X, 8, false>(X0 + (size_t)list[16 * j + row < n ? 16 * j + row : 0] * ldx, at, n_cols);
-#pragma unroll
-            for (int i = 0; i < RT; i++) {
-                const int r = rank0 + 16 * i + row;
-                const Vec<W, 8> w = load<W, 8, false>(A + (size_t)(r < rank ? r : rank - 1) * n_cols, at, n_cols);
-#pragma unroll
-                for (int j = 0; j < NJ; j++) acc[j][i] = multiply(w, b[j], acc[j][i]);
-            }
-        }
+        if (k < end) s[0].add_to(acc, turn);
+    }
+    if (end < last && S::C * end < n_cols) {
+        s[0].template fetch<false>(from, end, n_cols);
+        s[0].add_to(acc, turn);
     }
 }
 
@@ -415,7 +395,6 @@ lora_shrink_kernel(LoraCall c, LoraPlan p) {
     const int rank0 = block * 16 * RT;
     const int pieces = (c.n_cols + 63) / 64, share = part * kShrinkWaves + wv, shares = p.parts * kShrinkWaves;
     const int k0 = 64 * (int)((long long)pieces * share / shares), k1 = 64 * (int)((long long)pieces * (share + 1) / shares);
-    const bool x_vec = c.n_cols % 8 == 0 && on(c.X, 16) && (size_t)c.ldx * sizeof(X) % 16 == 0;
     Group *records = static_cast<Group *>(c.workspace) + (size_t)tile * p.groups;
     tokens.find(c, mat == 0 ? c.m[0].adapters : mat == 1 ? c.m[1].adapters : c.m[2].adapters, tile);
     for (int s = slot; s * NJ < p.groups; s += p.shrink_slots) {
@@ -443,7 +422,7 @@ lora_shrink_kernel(LoraCall c, LoraPlan p) {
         if (e.rank > rank0) { /* else no adapter, or none of its ranks here: nothing is read of h either */
             f32x4 acc[NJ][RT] = {};
             if (k0 < k1)
-                shrink_sums<W, X, RT, NJ>(x_vec && on(e.A, 16), static_cast<const W *>(e.A), rank0, e.rank, x0, c.ldx, list, n, c.n_cols, k0, k1, u.turn[wv], acc);
+                shrink_sums<W, X, RT, NJ>(static_cast<const W *>(e.A), rank0, e.rank, x0, c.ldx, list, n, c.n_cols, k0, k1, u.turn[wv], acc);
             /* the waves' sums, added in the waves' order */
             __syncthreads();
 #pragma unroll
@@ -489,40 +468,41 @@ lora_shrink_kernel(LoraCall c, LoraPlan p) {
 
 /* ------------------------------------------------------------------ Y + B h */
 
-/* four consecutive elements of a row, T float or the bits of a 16-bit type; WHOLE: all four are there, on the vector's alignment */
+/* four consecutive elements of a row at any element's address, of which `left` are there; T: float or the bits of a 16-bit type; WHOLE: all four are */
+template <class T> using Four = T __attribute__((ext_vector_type(4), aligned(sizeof(T))));
 template <class T, bool WHOLE> __device__ __forceinline__ f32x4 load4(const void *base, size_t at, int left, bool bf16) {
     const T *p = static_cast<const T *>(base) + at;
-    Vec<T, 4> v = {};
-    if constexpr (WHOLE) {
-        v = *reinterpret_cast<const Vec<T, 4> *>(p);
+    Four<T> v = {};
+    if (WHOLE || left > 3) {
+        v = *reinterpret_cast<const Four<T> *>(p);
     } else {
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (i < left) v.v[i] = p[i];
+        for (int i = 0; i < 3; i++)
+            if (i < left) v[i] = p[i];
     }
     f32x4 y;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        if constexpr (sizeof(T) == 4) y[i] = v.v[i];
-        else y[i] = bf16 ? to_f32(Bf16{v.v[i]}) : to_f32(__builtin_bit_cast(_Float16, v.v[i]));
+        if constexpr (sizeof(T) == 4) y[i] = v[i];
+        else y[i] = bf16 ? to_f32(Bf16{v[i]}) : to_f32(__builtin_bit_cast(_Float16, (uint16_t)v[i]));
     }
     return y;
 }
 /* the one rounding of a result in 16 bits: to the nearest, ties to even */
 template <class T, bool WHOLE> __device__ __forceinline__ void store4(void *base, size_t at, int left, bool bf16, f32x4 y) {
     T *p = static_cast<T *>(base) + at;
-    Vec<T, 4> v;
+    Four<T> v;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        if constexpr (sizeof(T) == 4) v.v[i] = y[i];
-        else v.v[i] = bf16 ? __builtin_bit_cast(uint16_t, (__bf16)y[i]) : __builtin_bit_cast(uint16_t, (_Float16)y[i]);
+        if constexpr (sizeof(T) == 4) v[i] = y[i];
+        else v[i] = bf16 ? __builtin_bit_cast(uint16_t, (__bf16)y[i]) : __builtin_bit_cast(uint16_t, (_Float16)y[i]);
     }
-    if constexpr (WHOLE) {
-        *reinterpret_cast<Vec<T, 4> *>(p) = v;
+    if (WHOLE || left > 3) {
+        *reinterpret_cast<Four<T> *>(p) = v;
     } else {
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (i < left) p[i] = v.v[i];
+        for (int i = 0; i < 3; i++)
+            if (i < left) p[i] = v[i];
     }
 }
 
@@ -614,7 +594,7 @@ lora_expand_kernel(LoraCall c, LoraPlan p) {
     const int row0 = (block * kExpandWaves + wv) * kRows;
     if (row0 >= m.n_rows) return;
     const bool y_bf16 = c.y_type == T_BF16, o_bf16 = c.out_type == T_BF16;
-    const bool whole = row0 + kRows <= m.n_rows && on(m.Y, 4 * sizeof(T)) && (!PAIR || on(c.m[1].Y, 4 * sizeof(T))) && m.ldy % 4 == 0 && on(m.out, 4 * sizeof(O)) && m.ldo % 4 == 0;
+    const bool whole = row0 + kRows <= m.n_rows;
     const size_t part = (size_t)c.n_mat * c.n_tok * p.rank_pad * sizeof(float);
     const int row = 4 * (lane % kLanes), left = m.n_rows - row0 - row; /* of the run */
     const int pieces = SPLIT ? (p.rank_pad + 31) / 32 * 12 : p.rank_pad / 4;
@@ -651,12 +631,12 @@ lora_expand_kernel(LoraCall c, LoraPlan p) {
                 f32x4 acc[MT] = {};
                 const char *h = hs + piece_at((size_t)(mat + a) * c.n_tok + first, pieces, lane >> 4, n, (lane & 15) < n ? lane & 15 : 0);
                 if constexpr (SPLIT) {
-                    if (e.rank % 8 == 0 && on(e.B, 16))
+                    if (e.rank % 8 == 0)
                         expand_split<MT, true>(e, row0, m.n_rows, h, n, acc);
                     else
                         expand_split<MT, false>(e, row0, m.n_rows, h, n, acc);
                 } else {
-                    if (e.rank % 4 == 0 && on(e.B, 4 * sizeof(W)))
+                    if (e.rank % 4 == 0)
                         expand_sums<W, MT, true>(e, row0, m.n_rows, h, n, part, p.parts, acc);
                     else
                         expand_sums<W, MT, false>(e, row0, m.n_rows, h, n, part, p.parts, acc);
@@ -713,13 +693,12 @@ lora_few_kernel(LoraCall c, LoraPlan p) {
     const int pieces = (c.n_cols + kFewPiece - 1) / kFewPiece, columns = NS > 1 || pieces > kWaves ? kWaves : pieces, shares = kWaves / columns;
     const int share = wv / columns, piece = wv % columns;
     const X *x0 = static_cast<const X *>(c.X) + token * c.ldx;
-    const bool x_vec = c.n_cols % 8 == 0 && on(c.X, 16) && (size_t)c.ldx * sizeof(X) % 16 == 0;
     int at[NS];
     float x[NS][8];
 #pragma unroll
     for (int s = 0; s < NS; s++) {
         at[s] = (piece + s * kWaves) * kFewPiece + 8 * lane;
-        const Vec<X, 8> v = x_vec ? load<X, 8, true>(x0, at[s], c.n_cols) : load<X, 8, false>(x0, at[s], c.n_cols);
+        const Vec<X, 8> v = load<X, 8, false>(x0, at[s], c.n_cols);
 #pragma unroll
         for (int i = 0; i < 8; i++) x[s][i] = to_f32(v.v[i]);
     }
@@ -749,7 +728,7 @@ lora_few_kernel(LoraCall c, LoraPlan p) {
 #pragma unroll
     for (int a = 0; a < MATS; a++) {
         const W *A = static_cast<const W *>(e[a].A);
-        const bool vec = c.n_cols % 8 == 0 && on(A, 16);
+        const bool whole = c.n_cols % 8 == 0;
         for (int r0 = share; r0 < e[a].rank && share < shares; r0 += 4 * shares) {
             Vec<W, 8> w[4][NS];
             float sum[4] = {};
@@ -757,7 +736,7 @@ lora_few_kernel(LoraCall c, LoraPlan p) {
             for (int q = 0; q < 4; q++) {
                 const int r = r0 + q * shares < e[a].rank ? r0 + q * shares : r0;
 #pragma unroll
-                for (int s = 0; s < NS; s++) w[q][s] = vec ? load<W, 8, true>(A + (size_t)r * c.n_cols, at[s], c.n_cols) : load<W, 8, false>(A + (size_t)r * c.n_cols, at[s], c.n_cols);
+                for (int s = 0; s < NS; s++) w[q][s] = whole ? load<W, 8, true>(A + (size_t)r * c.n_cols, at[s], c.n_cols) : load<W, 8, false>(A + (size_t)r * c.n_cols, at[s], c.n_cols);
             }
 #pragma unroll
             for (int q = 0; q < 4; q++) {
@@ -785,10 +764,10 @@ lora_few_kernel(LoraCall c, LoraPlan p) {
 #pragma unroll
     for (int a = 0; a < MATS; a++) {
         const W *B = static_cast<const W *>(e[a].B) + (size_t)row * e[a].rank;
-        const bool vec = e[a].rank % 8 == 0 && on(e[a].B, 16);
+        const bool whole = e[a].rank % 8 == 0;
         float sum = 0.0f;
         for (int r = 0; r < e[a].rank; r += 8) {
-            const Vec<W, 8> w = vec ? load<W, 8, true>(B, r, e[a].rank) : load<W, 8, false>(B, r, e[a].rank);
+            const Vec<W, 8> w = whole ? load<W, 8, true>(B, r, e[a].rank) : load<W, 8, false>(B, r, e[a].rank);
 #pragma unroll
             for (int i = 0; i < 8; i++) sum = r + i < e[a].rank ? fmaf(to_f32(w.v[i]), hs[a][r + i], sum) : sum;
         }
@@ -918,7 +897,7 @@ LoraPlan lora_plan(const LoraCall &c) {
     const long long fill = 256 / (bound * others); /* a workgroup on each compute unit: two do not find room */
     p.parts = (int)(fill < 1 ? 1 : fill < most ? fill : most);
     p.split = p.parts == 1 && c.lora_type == T_BF16;
-    const size_t a_bytes = c.max_rank * c.n_cols * element * (c.pair ? 2 : 1);
+    const size_t a_bytes = (size_t)c.max_rank * c.n_cols * element * (c.pair ? 2 : 1);
     p.few = c.n_tok <= kFewTokens && c.max_rank <= kFewMaxRank && c.n_cols <= 2 * kFewPiece * kLoraFewThreads / 64 && a_bytes <= kFewBytes;
     if (p.few) {
         long long blocks = 0;
