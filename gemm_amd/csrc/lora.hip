@@ -470,7 +470,7 @@ lora_shrink_kernel(LoraCall c, LoraPlan p) {
 
 /* four consecutive elements of a row at any element's address, of which `left` are there; T: float or the bits of a 16-bit type; WHOLE: all four are */
 template <class T> using Four = T __attribute__((ext_vector_type(4), aligned(sizeof(T))));
-template <class T, bool WHOLE> __device__ __forceinline__ f32x4 load4(const void *base, size_t at, int left, bool bf16) {
+template <class T, bool WHOLE> __device__ __forceinline__ Four<T> load4(const void *base, size_t at, int left) {
     const T *p = static_cast<const T *>(base) + at;
     Four<T> v = {};
     if (WHOLE || left > 3) {
@@ -480,6 +480,16 @@ template <class T, bool WHOLE> __device__ __forceinline__ f32x4 load4(const void
         for (int i = 0; i < 3; i++)
             if (i < left) v[i] = p[i];
     }
+    return v;
+}
+/* the same, not taken to registers of its own before the sums: its wait would be in front of theirs */
+template <class V> __device__ __forceinline__ V here(V v) {
+    typedef uint32_t Words __attribute__((ext_vector_type(sizeof(V) / 4)));
+    Words w = __builtin_bit_cast(Words, v);
+    asm volatile("" : "+v"(w));
+    return __builtin_bit_cast(V, w);
+}
+template <class T> __device__ __forceinline__ f32x4 values(Four<T> v, bool bf16) {
     f32x4 y;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
@@ -616,37 +626,42 @@ lora_expand_kernel(LoraCall c, LoraPlan p) {
             size_t run[kSteps]; /* the tokens of the lane's runs */
 #pragma unroll
             for (int s = 0; s < kSteps; s++) run[s] = token(s * kRuns + lane / kLanes);
-            f32x4 y[MATS][kSteps];
+            Four<T> raw[MATS][kSteps]; /* (on their way until the sums are there) */
 #pragma unroll
             for (int s = 0; s < kSteps; s++) {
-                y[0][s] = load4<T, WHOLE>(m.Y, run[s] * m.ldy + row0 + row, left, y_bf16);
-                if constexpr (PAIR) y[1][s] = load4<T, WHOLE>(c.m[1].Y, run[s] * m.ldy + row0 + row, left, y_bf16);
+                raw[0][s] = load4<T, WHOLE>(m.Y, run[s] * m.ldy + row0 + row, left);
+                if constexpr (PAIR) raw[1][s] = load4<T, WHOLE>(c.m[1].Y, run[s] * m.ldy + row0 + row, left);
             }
+            f32x4 y[MATS][kSteps];
 #pragma unroll
             for (int a = 0; a < MATS; a++) {
                 const int at = 8 + 4 * (mat + a);
                 const Entry e = {nullptr, (const void *)((uint64_t)__builtin_amdgcn_readlane(words, at + 1) << 32 | (uint32_t)__builtin_amdgcn_readlane(words, at)),
                                  (int)__builtin_amdgcn_readlane(words, at + 2), __uint_as_float(__builtin_amdgcn_readlane(words, at + 3))};
-                if (e.rank == 0) continue;
                 f32x4 acc[MT] = {};
-                const char *h = hs + piece_at((size_t)(mat + a) * c.n_tok + first, pieces, lane >> 4, n, (lane & 15) < n ? lane & 15 : 0);
-                if constexpr (SPLIT) {
-                    if (e.rank % 8 == 0)
-                        expand_split<MT, true>(e, row0, m.n_rows, h, n, acc);
-                    else
-                        expand_split<MT, false>(e, row0, m.n_rows, h, n, acc);
-                } else {
-                    if (e.rank % 4 == 0)
-                        expand_sums<W, MT, true>(e, row0, m.n_rows, h, n, part, p.parts, acc);
-                    else
-                        expand_sums<W, MT, false>(e, row0, m.n_rows, h, n, part, p.parts, acc);
+                if (e.rank != 0) {
+                    const char *h = hs + piece_at((size_t)(mat + a) * c.n_tok + first, pieces, lane >> 4, n, (lane & 15) < n ? lane & 15 : 0);
+                    if constexpr (SPLIT) {
+                        if (e.rank % 8 == 0)
+                            expand_split<MT, true>(e, row0, m.n_rows, h, n, acc);
+                        else
+                            expand_split<MT, false>(e, row0, m.n_rows, h, n, acc);
+                    } else {
+                        if (e.rank % 4 == 0)
+                            expand_sums<W, MT, true>(e, row0, m.n_rows, h, n, part, p.parts, acc);
+                        else
+                            expand_sums<W, MT, false>(e, row0, m.n_rows, h, n, part, p.parts, acc);
+                    }
+                    wave_meets();
+#pragma unroll
+                    for (int i = 0; i < MT; i++) *reinterpret_cast<f32x4 *>(&turn[wv][(lane & 15) * kStride + 16 * i + 4 * (lane >> 4)]) = acc[i];
+                    wave_meets();
                 }
-                wave_meets();
 #pragma unroll
-                for (int i = 0; i < MT; i++) *reinterpret_cast<f32x4 *>(&turn[wv][(lane & 15) * kStride + 16 * i + 4 * (lane >> 4)]) = acc[i];
-                wave_meets();
-#pragma unroll
-                for (int s = 0; s < kSteps; s++) y[a][s] += *reinterpret_cast<const f32x4 *>(&turn[wv][(s * kRuns + lane / kLanes) * kStride + row]);
+                for (int s = 0; s < kSteps; s++) {
+                    y[a][s] = values<T>(here(raw[a][s]), y_bf16);
+                    if (e.rank != 0) y[a][s] += *reinterpret_cast<const f32x4 *>(&turn[wv][(s * kRuns + lane / kLanes) * kStride + row]);
+                }
             }
             if constexpr (PAIR) {
 #pragma unroll
@@ -812,7 +827,7 @@ template <class W, class X, int RT> void launch_shrink(const LoraCall &c, const 
 template <class W, class X> void launch_shrink(const LoraCall &c, const LoraPlan &p) {
     if (p.rank_tiles == 1) launch_shrink<W, X, 1>(c, p);
     else if (p.rank_tiles == 2) launch_shrink<W, X, 2>(c, p);
-    else launch_shrink<W, X, 4>(c, p);
+    else if constexpr (!Same<W, float>::value) launch_shrink<W, X, 4>(c, p);
 }
 
 template <class W, class T, class O, bool PAIR> void launch_expand(const LoraCall &c, const LoraPlan &p) {
@@ -855,14 +870,15 @@ template <class W> hipError_t launch_both(const LoraCall &c, const LoraPlan &p) 
 
 }  // namespace
 
-/* 16 ranks, 32 or 64 to a workgroup */
-static int lora_rank_tiles(int max_rank) { return max_rank <= 16 ? 1 : max_rank <= 32 ? 2 : 4; }
+/* 16 ranks, 32 or, in 16 bits, 64 to a workgroup: the registers of 64 in fp32 do not fit, and the activations twice cost less than that (2048 tokens of 4096
+ * columns, rank 64, three tensors: 50 us for the first launch, 61 with 64 ranks) */
+static int lora_rank_tiles(int max_rank, uint32_t lora_type) { return max_rank <= 16 ? 1 : max_rank <= 32 || lora_type == T_F32 ? 2 : 4; }
 static int lora_token_groups(int n_tok) { return n_tok >= 1024 ? 2 : 1; }
 
 /* how many parts the columns are cut into at most: as far as a workgroup for each compute unit needs, and at least 64 columns for a wave; the second
  * launch reads every part of h again for each of its rows' workgroups */
 static int lora_most_parts(int n_mat, int max_rank, int n_cols, int n_tok) {
-    const int rt = lora_rank_tiles(max_rank);
+    const int rt = lora_rank_tiles(max_rank, T_F16);
     const long long tokens = 16ll * lora_token_groups(n_tok), groups = (n_tok + tokens - 1) / tokens * n_mat * ((max_rank + 16 * rt - 1) / (16 * rt));
     const long long want = groups >= 96 ? 1 : 256 / groups, most = n_cols / (64 * kShrinkWaves);
     const long long parts = want < most ? want : most;
@@ -884,7 +900,7 @@ LoraPlan lora_plan(const LoraCall &c) {
     p.tiles = (int)(((long long)c.n_tok + kTile - 1) / kTile);
     p.n_mat = c.n_mat;
     p.rank_pad = (c.max_rank + 15) / 16 * 16;
-    p.rank_tiles = lora_rank_tiles(c.max_rank);
+    p.rank_tiles = lora_rank_tiles(c.max_rank, c.lora_type);
     p.rank_blocks = (c.max_rank + 16 * p.rank_tiles - 1) / (16 * p.rank_tiles);
     p.token_groups = p.rank_tiles < 4 || native ? lora_token_groups(c.n_tok) : 1; /* (the registers) */
     /* the most groups that a tile can have */
@@ -904,20 +920,30 @@ LoraPlan lora_plan(const LoraCall &c) {
         for (int i = 0; i < (c.pair ? 1 : c.n_mat); i++) blocks += ((long long)c.m[i].n_rows + kLoraFewThreads - 1) / kLoraFewThreads;
         p.few = blocks * c.n_tok * a_bytes <= kFewBytesAll;
     }
-    p.row_tiles = c.n_tok <= 8 && !p.split ? 1 : 4;
-    p.row_blocks_all = 0;
-    for (int i = 0; i < 3; i++) {
-        const int rows = p.few ? kLoraFewThreads : 16 * kExpandWaves * p.row_tiles;
-        p.row_blocks[i] = i < c.n_mat && (i == 0 || !c.pair) ? (int)(((long long)c.m[i].n_rows + rows - 1) / rows) : 0;
-        p.row_blocks_all += p.row_blocks[i];
+    /* 64 rows to a wave of the second launch, which reads h once for them, or 16 where 64 make no more workgroups than there are compute units
+     * (10 tokens, rank 128, 719 rows: 13.7 us, 17.9 with 64) and for up to 8 tokens (8 tokens, gate and up of 14336 rows, rank 128: 21.4 us, 28.4 with 64); h in
+     * three bf16 numbers means many tokens */
+    auto row_blocks = [&](int rows) {
+        p.row_blocks_all = 0;
+        for (int i = 0; i < 3; i++) {
+            p.row_blocks[i] = i < c.n_mat && (i == 0 || !c.pair) ? (int)(((long long)c.m[i].n_rows + rows - 1) / rows) : 0;
+            p.row_blocks_all += p.row_blocks[i];
+        }
+    };
+    p.row_tiles = 4;
+    row_blocks(p.few ? kLoraFewThreads : 64 * kExpandWaves);
+    if (!p.few && !p.split && (c.n_tok <= 8 || (long long)p.row_blocks_all * p.groups * p.tiles <= 256)) {
+        p.row_tiles = 1;
+        row_blocks(16 * kExpandWaves);
     }
-    /* a workgroup for each group, unless that makes many more than the chip holds: then several groups to a workgroup, but in the first launch one for each
-     * that a prompt of one adapter has */
+    /* a workgroup for each group, unless that makes more than run at once: then several groups to a workgroup, in the first launch one for each that
+     * a prompt of one adapter has and a quarter more (2048 tokens in runs of 64 adapters, rank 16, three tensors: 15.4 us for the first launch with 256 workgroups, 31.3 with 1024,
+     * most of which have no group; 2048 tokens in runs of 6 adapters in fp32, rank 64: 36 us, 53 without the quarter more) */
     auto slots = [&](long long bound, long long least, long long others, long long many) {
         const long long want = others > 0 && many / others > least ? many / others : least;
         return (int)(want < bound ? want : bound);
     };
-    p.shrink_slots = slots(bound, full, others * p.parts, 1024);
+    p.shrink_slots = slots(bound, full + (full + 3) / 4, others * p.parts, 256);
     p.expand_slots = slots(p.groups, 1, (long long)p.tiles * p.row_blocks_all, 4096);
     return p;
 }
