@@ -6,14 +6,25 @@
  * for one to three tensors that share X, or, of two tensors (gate and up), out = silu(first) * second. A token whose id names no
  * adapter keeps its Y.
  *
- * Two launches: the first makes h (fp32, in the workspace, as partial sums over parts of the columns), the second adds the parts up
- * in their order and makes the results. Both go by tiles of 64 tokens. A wave holds one id per lane and finds the tile's classes,
- * tokens that share an adapter, by ballots; the tokens of a class are packed into groups of 16 columns of the matrix instruction, so
- * that an adapter is read once for all of them, whatever the order of the tokens. `slots` workgroups share a tile's classes: for a
- * decoding batch, in which nearly every token has its own adapter, one each.
+ * What has to move: X once, each adapter's A and B once, Y and the result once (2048 tokens, gate and up of 14336 rows, 322 MB: 63 us at the
+ * 5.12 TB/s of a copy). Multiplications are few, 4 max_rank to a result.
+ *
+ * A few tokens (lora_few_kernel): one launch. A workgroup takes 1024 results of a token and makes h for itself. Where the workgroups' reads of A add up to
+ * little that costs less than a second launch and h in memory: 1 token beside Q, K and V of 4096 columns, rank 16: 5.0 us, 7.4 + 4.1 in two launches; 24
+ * tokens: 8.3 us, 7.9 + 4.9; 48 tokens: 9.9, 9.0 + 4.9; 48 tokens of rank 32: 15.4, 9.8 + 6.3; 4 tokens beside gate and up of 14336 rows, rank 32: 20.3, 7.4 + 5.9.
+ *
+ * Any number of them: two launches, by tiles of 256 tokens.
+ *   lora_shrink_kernel makes h. A workgroup finds the tile's classes, tokens that share an adapter, packs the tokens of a class into groups of 16 (or
+ * 32), the columns of the matrix instruction, so that an adapter is read once for them whatever the order of the tokens, and takes one group of one tensor, or a
+ * few; its 16 waves share the columns and add their sums in order. It also writes a record of each group, from which the second launch knows all
+ * that it needs with one load. 2048 tokens, Q, K and V of 4096 columns, rank 64: 27 us; X comes three times, twice from L2.
+ *   lora_expand_kernel: a wave takes 64 rows of a tensor (or of gate and up) and a group, and writes results in runs of 128 to 256 bytes of a token. 2048
+ * tokens, gate and up of 14336 rows: 66 us, 95% of a copy's rate.
  *   Products: where the adapter and X are of one 16-bit type the first launch multiplies them on v_mfma_f32_16x16x32 of that type
  * (products exact, sums fp32); every other pair is widened to fp32 and goes through v_mfma_f32_16x16x4_f32, and so does h times B,
- * since h rounded to 16 bits would cost results in F32 their precision.
+ * since h rounded to 16 bits would cost results in F32 their precision. Of bf16 adapters and many tokens scale h is cut into three bf16 numbers, which hold its 24
+ * bits, and goes through the bf16 instruction three times, the products exact again: 23 us for the second launch of the case above, 29 with fp32.
+ *   No atomics: the same call gives the same bits.
  */
 #include "qlin_device.h"
 #include "qlin_internal.h"
@@ -101,7 +112,7 @@ struct alignas(16) Group {
     int32_t n;      /* 0: none */
     int32_t place;  /* of its first token among the tile's tokens sorted by id */
     uint8_t token[16];
-    int32_t unused[2];
+    int32_t to_16_bytes[2];
     struct {
         const void *B;
         int32_t rank;
@@ -375,6 +386,9 @@ __device__ __forceinline__ void shrink_sums(const W *A, int rank0, int rank, con
     }
 }
 
+/* the leading eight bits of a number */
+__device__ __forceinline__ float leading(float v) { return __uint_as_float(__float_as_uint(v) & 0xFFFF0000u); }
+
 template <class W, class X, int RT, int NJ>
 __global__ void __launch_bounds__(64 * kShrinkWaves)
 lora_shrink_kernel(LoraCall c, LoraPlan p) {
@@ -447,10 +461,11 @@ lora_shrink_kernel(LoraCall c, LoraPlan p) {
                     bf16x4 three[3];
 #pragma unroll
                     for (int d = 0; d < 4; d++) {
-                        three[0][d] = (__bf16)v[d];
-                        const float rest = v[d] - (float)three[0][d];
-                        three[1][d] = (__bf16)rest;
-                        three[2][d] = (__bf16)(rest - (float)three[1][d]);
+                        /* 24 bits are eight, eight and eight; an infinity leaves nothing, and the largest numbers do not become one */
+                        const float first = leading(v[d]), rest = fabsf(first) == INFINITY ? 0.0f : v[d] - first, second = leading(rest);
+                        three[0][d] = (__bf16)first;
+                        three[1][d] = (__bf16)second;
+                        three[2][d] = (__bf16)(rest - second);
                     }
                     const int pieces = (p.rank_pad + 31) / 32 * 12, piece = r / 32 * 12 + r % 32 / 8;
 #pragma unroll
@@ -873,13 +888,20 @@ template <class W> hipError_t launch_both(const LoraCall &c, const LoraPlan &p) 
 /* 16 ranks, 32 or, in 16 bits, 64 to a workgroup: the registers of 64 in fp32 do not fit, and the activations twice cost less than that (2048 tokens of 4096
  * columns, rank 64, three tensors: 50 us for the first launch, 61 with 64 ranks) */
 static int lora_rank_tiles(int max_rank, uint32_t lora_type) { return max_rank <= 16 ? 1 : max_rank <= 32 || lora_type == T_F32 ? 2 : 4; }
-static int lora_token_groups(int n_tok) { return n_tok >= 1024 ? 2 : 1; }
+static int lora_rank_blocks(int max_rank, uint32_t lora_type) {
+    const int ranks = 16 * lora_rank_tiles(max_rank, lora_type);
+    return (max_rank + ranks - 1) / ranks;
+}
+/* 16 tokens to a workgroup of the first launch or, where those would not all run at once, 32, which halves the reads of A (both launches, columns 4096: 2048
+ * tokens, three tensors of rank 64: 50 us, 59 with 16; 1300 tokens: 37 us, 34 with 16; 1024 tokens, gate and up of rank 32: 58 us, 51 with 16) */
+static int lora_token_groups(int n_mat, int max_rank, int n_tok) {
+    return ((long long)n_tok + 15) / 16 * n_mat * lora_rank_blocks(max_rank, T_F16) >= 256 ? 2 : 1;
+}
 
 /* how many parts the columns are cut into at most: as far as a workgroup for each compute unit needs, and at least 64 columns for a wave; the second
  * launch reads every part of h again for each of its rows' workgroups */
 static int lora_most_parts(int n_mat, int max_rank, int n_cols, int n_tok) {
-    const int rt = lora_rank_tiles(max_rank, T_F16);
-    const long long tokens = 16ll * lora_token_groups(n_tok), groups = (n_tok + tokens - 1) / tokens * n_mat * ((max_rank + 16 * rt - 1) / (16 * rt));
+    const long long tokens = 16ll * lora_token_groups(n_mat, max_rank, n_tok), groups = (n_tok + tokens - 1) / tokens * n_mat * lora_rank_blocks(max_rank, T_F16);
     const long long want = groups >= 96 ? 1 : 256 / groups, most = n_cols / (64 * kShrinkWaves);
     const long long parts = want < most ? want : most;
     return (int)(parts > 8 ? 8 : parts < 1 ? 1 : parts);
@@ -890,7 +912,7 @@ static int lora_most_parts(int n_mat, int max_rank, int n_cols, int n_tok) {
 static size_t lora_records(int n_tok, int groups) { return ((size_t)n_tok + kTile - 1) / kTile * groups * sizeof(Group); }
 size_t lora_workspace_bytes(int n_mat, int max_rank, int n_cols, int n_tok) {
     const size_t rank_pad = (max_rank + 15) / 16 * 16, split = (rank_pad + 31) / 32 * 192, sums = rank_pad * lora_most_parts(n_mat, max_rank, n_cols, n_tok) * sizeof(float);
-    return lora_records(n_tok, (n_tok < kTile ? n_tok : kTile) * lora_token_groups(n_tok)) + (size_t)n_mat * n_tok * (split > sums ? split : sums);
+    return lora_records(n_tok, (n_tok < kTile ? n_tok : kTile) * lora_token_groups(n_mat, max_rank, n_tok)) + (size_t)n_mat * n_tok * (split > sums ? split : sums);
 }
 
 LoraPlan lora_plan(const LoraCall &c) {
@@ -901,8 +923,8 @@ LoraPlan lora_plan(const LoraCall &c) {
     p.n_mat = c.n_mat;
     p.rank_pad = (c.max_rank + 15) / 16 * 16;
     p.rank_tiles = lora_rank_tiles(c.max_rank, c.lora_type);
-    p.rank_blocks = (c.max_rank + 16 * p.rank_tiles - 1) / (16 * p.rank_tiles);
-    p.token_groups = p.rank_tiles < 4 || native ? lora_token_groups(c.n_tok) : 1; /* (the registers) */
+    p.rank_blocks = lora_rank_blocks(c.max_rank, c.lora_type);
+    p.token_groups = p.rank_tiles < 4 || native ? lora_token_groups(c.n_mat, c.max_rank, c.n_tok) : 1; /* (the registers) */
     /* the most groups that a tile can have */
     const int tokens = c.n_tok < kTile ? c.n_tok : kTile, size = 16 * p.token_groups;
     const long long classes = c.n_adapter + 1ll < tokens ? c.n_adapter + 1ll : tokens, bound = (tokens - classes) / size + classes, full = (tokens + size - 1) / size;

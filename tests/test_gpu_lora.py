@@ -269,6 +269,22 @@ def test_what_is_not_finite_stays_with_its_tokens(pair, w, x, n_tok):
         assert not np.isfinite(b[mine]).any()
 
 
+@pytest.mark.parametrize("n_tok", [5, 80])
+def test_the_largest_numbers_and_infinities(n_tok):
+    """h is the activation itself and B 2^-100: an infinite h gives infinite results, the largest one results that are finite, off by the one rounding"""
+    c = Case(12, n_tok, [8], 64, [1], [0] * n_tok, BF16, F32)
+    a = c.adapters[0][0]
+    a.a_raw[:], a.b_raw[:], a.scale = 0, 0x0D80, np.float32(1.0)
+    a.a_raw[0, 5] = 0x3F80
+    most = np.finfo(np.float32).max
+    c.x_raw[:5, 5] = [1.0, np.inf, most, -most, -np.inf]
+    c.place()
+    got = c.run()[0]
+    assert (got[1] == np.inf).all() and (got[4] == -np.inf).all()
+    want = c.y_raw[0][2:4].astype(np.float64)[:, :8] + np.array([[1.0], [-1.0]]) * float(most) * 2.0 ** -100
+    assert (np.abs(got[2:4] - want) <= 2.0 ** -24 * np.abs(want)).all()
+
+
 def test_an_adapter_of_one_row_and_column_copies_what_it_should():
     """A picks column 5, B puts it into row 3, scale 2: exact"""
     c = Case(10, 3, [8], 64, [1], [0, -1, 0])
