@@ -940,7 +940,7 @@ LoraPlan lora_plan(const LoraCall &c) {
     if (p.few) {
         long long blocks = 0;
         for (int i = 0; i < (c.pair ? 1 : c.n_mat); i++) blocks += ((long long)c.m[i].n_rows + kLoraFewThreads - 1) / kLoraFewThreads;
-        p.few = blocks * c.n_tok * a_bytes <= kFewBytesAll;
+        p.few = blocks * c.n_tok * a_bytes <= kFewBytesAll && blocks * c.n_tok * kLoraFewThreads < 1ll << 32;
     }
     /* 64 rows to a wave of the second launch, which reads h once for them, or 16 where 64 make no more workgroups than there are compute units
      * (10 tokens, rank 128, 719 rows: 13.7 us, 17.9 with 64) and for up to 8 tokens (8 tokens, gate and up of 14336 rows, rank 128: 21.4 us, 28.4 with 64); h in

@@ -1575,6 +1575,7 @@ static int lora_call(LoraCall &c, void *workspace, size_t workspace_bytes) {
     for (int i = 0; i < c.n_mat; i++) {
         const LoraTensor &m = c.m[i];
         if (m.n_rows < 0 || m.ldy < m.n_rows || m.ldo < m.n_rows) return fail(QLIN_ERR_ARG, "negative size or a row pitch below the row");
+        if (m.n_rows > kLoraMaxRows) return fail(QLIN_ERR_ARG, "%d rows (up to %d)", m.n_rows, kLoraMaxRows);
         if (m.n_rows == 0 || c.n_tok == 0) continue;
         rows = true;
         if (!m.Y || (!m.out && (i == 0 || !c.pair)) || (!m.adapters && c.n_adapter)) return fail(QLIN_ERR_ARG, "null pointer");

@@ -404,8 +404,8 @@ int qlin_mxfp4_gemm_silu_mul_dev(const void *Wgate, const void *Wup, uint32_t x_
  * A tensor's adapters are a table in device memory, one entry each; A and B are packed rows, as the lora_a and lora_b tensors of an
  * adapter file are, all of one type (F32, F16 or BF16). The kernels read the table when they run: an engine changes an entry on the stream
  * between two calls, or between two replays of a graph. An entry with a null pointer, or whose rank is not in 1..max_rank, is no adapter,
- * nor is an id outside of 0..n_adapter-1 (-1 for a request without one): such a token's out is its Y. A and B need an element's
- * alignment; 16 bytes, and n_cols of a multiple of 8, X on 16 bytes and ldx of 16 bytes, are read faster, as are ranks of a multiple of 4. */
+ * nor is an id outside of 0..n_adapter-1 (-1 for a request without one): such a token's out is its Y. Everything needs an
+ * element's alignment, and n_cols, ranks and pitches are any; rows of A and X on 16 bytes and ranks of a multiple of 8 are read some 10% faster. */
 #define QLIN_LORA_MAX_RANK 256
 typedef struct qlin_lora {
     const void *A;  /* [rank, n_cols] */
@@ -425,7 +425,8 @@ typedef struct qlin_lora_tensor { /* one projection; in host memory, read before
  * stays with its tokens. workspace: device memory, 16-byte aligned, qlin_lora_workspace_bytes(n_mat, max_rank, n_cols, n_tok) bytes (0 for
  * sizes that are not positive), which holds nothing between calls; calls that share one must be ordered on one stream, and graphs that
  * share one must not run at the same time. What a call writes must not overlap with what it reads, but for an out that is its Y. n_cols
- * below 2^24, max_rank up to QLIN_LORA_MAX_RANK; what would take 2^32 threads or more is refused (64 tokens x 64 rows take 256). */
+ * below 2^24, n_rows up to 2^30, max_rank up to QLIN_LORA_MAX_RANK; what would take 2^32 threads or more is refused (256 tokens x 256 rows take at
+ * least 256). */
 size_t qlin_lora_workspace_bytes(int n_mat, int max_rank, int n_cols, int n_tok);
 int qlin_lora_add_dev(int n_mat, const qlin_lora_tensor *tensors, uint32_t lora_type, int n_adapter, int max_rank, const int32_t *ids,
                       uint32_t x_type, const void *X, uint32_t y_type, uint32_t out_type, int n_cols, int n_tok, int ldx, void *workspace,

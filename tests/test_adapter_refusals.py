@@ -67,6 +67,7 @@ def test_adapters_refuse(lib, call, code, change):
 @pytest.mark.parametrize("change,tensor", [
     ({}, dict(adapters=None)), ({}, dict(adapters=P + 4)), ({}, dict(Y=None)), ({}, dict(Y=P + 2)), ({}, dict(out=None)), ({}, dict(out=P + 2)), (dict(out_type=BF16), dict(out=P + 1)),
     ({}, dict(n_rows=-1)), ({}, dict(ldy=63)), ({}, dict(ldo=63)), (dict(n_tok=1 << 28, ws_bytes=1 << 60), dict(n_rows=1 << 28, ldy=1 << 28, ldo=1 << 28)),
+    (dict(n_tok=1, ws_bytes=1 << 60), dict(n_rows=2 ** 31 - 1, ldy=2 ** 31 - 1, ldo=2 ** 31 - 1)), ({}, dict(n_rows=2 ** 30 + 1, ldy=2 ** 30 + 1, ldo=2 ** 30 + 1)),
     (dict(n_tok=2 ** 31 - 1, ws_bytes=1 << 60), dict(n_rows=1 << 14, ldy=1 << 14, ldo=1 << 14)),
 ])
 def test_a_tensor_is_refused(lib, call, change, tensor):
