@@ -483,6 +483,13 @@ lora_shrink_kernel(LoraCall c, LoraPlan p) {
 
 /* ------------------------------------------------------------------ Y + B h */
 
+/* what was loaded, there at this place and not before or behind it */
+template <class V> __device__ __forceinline__ V here(V v) {
+    typedef uint32_t Words __attribute__((ext_vector_type(sizeof(V) / 4)));
+    Words w = __builtin_bit_cast(Words, v);
+    asm volatile("" : "+v"(w));
+    return __builtin_bit_cast(V, w);
+}
 /* four consecutive elements of a row at any element's address, of which `left` are there; T: float or the bits of a 16-bit type; WHOLE: all four are */
 template <class T> using Four = T __attribute__((ext_vector_type(4), aligned(sizeof(T))));
 template <class T, bool WHOLE> __device__ __forceinline__ Four<T> load4(const void *base, size_t at, int left) {
@@ -496,13 +503,6 @@ template <class T, bool WHOLE> __device__ __forceinline__ Four<T> load4(const vo
             if (i < left) v[i] = p[i];
     }
     return v;
-}
-/* the same, not taken to registers of its own before the sums: its wait would be in front of theirs */
-template <class V> __device__ __forceinline__ V here(V v) {
-    typedef uint32_t Words __attribute__((ext_vector_type(sizeof(V) / 4)));
-    Words w = __builtin_bit_cast(Words, v);
-    asm volatile("" : "+v"(w));
-    return __builtin_bit_cast(V, w);
 }
 template <class T> __device__ __forceinline__ f32x4 values(Four<T> v, bool bf16) {
     f32x4 y;
@@ -554,14 +554,19 @@ __device__ __forceinline__ void expand_sums(const Entry &e, int row0, int n_rows
 #pragma unroll
         for (int i = 0; i < MT; i++) w[i] = load<W, 4, VEC>(rows.b[i], r, e.rank);
         f32x4 v = *reinterpret_cast<const f32x4 *>(h);
-        for (int s = 1; s < parts; s += 4) { /* (four on their way at a time) */
-            f32x4 more[4];
+        auto others = [&](auto most) { /* all on their way at once */
+            f32x4 more[decltype(most)::value];
 #pragma unroll
-            for (int q = 0; q < 4; q++) more[q] = *reinterpret_cast<const f32x4 *>(h + (s + q < parts ? s + q : 0) * part);
+            for (int q = 0; q < most; q++) more[q] = *reinterpret_cast<const f32x4 *>(h + (q + 1 < parts ? q + 1 : 0) * part);
 #pragma unroll
-            for (int q = 0; q < 4; q++)
-                if (s + q < parts) v += more[q];
-        }
+            for (int q = 0; q < most; q++) {
+                const f32x4 one = here(more[q]); /* (the compiler would load where it adds, and wait for each) */
+                if (q + 1 < parts) v += one;
+            }
+        };
+        if (parts > 5) others(std::integral_constant<int, kLoraMostParts - 1>{});
+        else if (parts > 3) others(std::integral_constant<int, 4>{});
+        else if (parts > 1) others(std::integral_constant<int, 2>{});
         v *= e.scale;
 #pragma unroll
         for (int q = 0; q < 4; q++)
@@ -904,7 +909,7 @@ static int lora_most_parts(int n_mat, int max_rank, int n_cols, int n_tok) {
     const long long tokens = 16ll * lora_token_groups(n_mat, max_rank, n_tok), groups = (n_tok + tokens - 1) / tokens * n_mat * lora_rank_blocks(max_rank, T_F16);
     const long long want = groups >= 96 ? 1 : 256 / groups, most = n_cols / (64 * kShrinkWaves);
     const long long parts = want < most ? want : most;
-    return (int)(parts > 8 ? 8 : parts < 1 ? 1 : parts);
+    return (int)(parts > kLoraMostParts ? kLoraMostParts : parts < 1 ? 1 : parts);
 }
 
 /* the groups of every tile, of which there are at most as many as tokens, or half of them twice as many; then h in fp32 for each part, or, of
@@ -942,9 +947,9 @@ LoraPlan lora_plan(const LoraCall &c) {
         for (int i = 0; i < (c.pair ? 1 : c.n_mat); i++) blocks += ((long long)c.m[i].n_rows + kLoraFewThreads - 1) / kLoraFewThreads;
         p.few = blocks * c.n_tok * a_bytes <= kFewBytesAll && blocks * c.n_tok * kLoraFewThreads < 1ll << 32;
     }
-    /* 64 rows to a wave of the second launch, which reads h once for them, or 16 where 64 make no more workgroups than there are compute units
-     * (10 tokens, rank 128, 719 rows: 13.7 us, 17.9 with 64) and for up to 8 tokens (8 tokens, gate and up of 14336 rows, rank 128: 21.4 us, 28.4 with 64); h in
-     * three bf16 numbers means many tokens */
+    /* 64 rows to a wave of the second launch, which reads h once for them, or 16 where 64 make few workgroups, and for up to 8 tokens (10 tokens of 719 rows,
+     * rank 128: 7.1 us, 12.5 with 64; 16 beside Q, K and V of 6144 rows: 10.8, 15; 200 of 4096 rows, rank 32, 688 workgroups: 7.8, 6.6 with 64). h in three
+     * bf16 numbers means many tokens. */
     auto row_blocks = [&](int rows) {
         p.row_blocks_all = 0;
         for (int i = 0; i < 3; i++) {
@@ -954,7 +959,7 @@ LoraPlan lora_plan(const LoraCall &c) {
     };
     p.row_tiles = 4;
     row_blocks(p.few ? kLoraFewThreads : 64 * kExpandWaves);
-    if (!p.few && !p.split && (c.n_tok <= 8 || (long long)p.row_blocks_all * p.groups * p.tiles <= 256)) {
+    if (!p.few && !p.split && (c.n_tok <= 8 || (long long)p.row_blocks_all * p.groups * p.tiles <= 384)) {
         p.row_tiles = 1;
         row_blocks(16 * kExpandWaves);
     }

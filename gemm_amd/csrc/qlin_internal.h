@@ -297,6 +297,7 @@ struct LoraTensor {
     int32_t n_rows, ldy, ldo, unused;
 };
 constexpr int kLoraMaxRank = 256; /* = QLIN_LORA_MAX_RANK of the public header */
+constexpr int kLoraMostParts = 8; /* of the columns */
 constexpr int kLoraMaxRows = 1 << 30; /* (a row behind the last of a workgroup still is an int) */
 constexpr int kLoraTile = 256, kLoraGroupBytes = 80; /* tokens of a tile, bytes of a group's record */
 constexpr int kLoraShrinkThreads = 1024, kLoraExpandThreads = 256, kLoraFewThreads = 1024;
