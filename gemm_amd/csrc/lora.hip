@@ -19,7 +19,7 @@
  * few; its 16 waves share the columns and add their sums in order. It also writes a record of each group, from which the second launch knows all
  * that it needs with one load. 2048 tokens, Q, K and V of 4096 columns, rank 64: 27 us; X comes three times, twice from L2.
  *   lora_expand_kernel: a wave takes 64 rows of a tensor (or of gate and up) and a group, and writes results in runs of 128 to 256 bytes of a token. 2048
- * tokens, gate and up of 14336 rows: 66 us, 95% of a copy's rate.
+ * tokens, gate and up of 14336 rows, 305 MB: 66 us, 90% of a copy's rate.
  *   Products: where the adapter and X are of one 16-bit type the first launch multiplies them on v_mfma_f32_16x16x32 of that type
  * (products exact, sums fp32); every other pair is widened to fp32 and goes through v_mfma_f32_16x16x4_f32, and so does h times B,
  * since h rounded to 16 bits would cost results in F32 their precision. Of bf16 adapters and many tokens scale h is cut into three bf16 numbers, which hold its 24

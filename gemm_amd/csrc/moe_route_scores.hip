@@ -9,8 +9,8 @@
  *
  * The choice is the one of 64-bit values, also where two experts lie next to each other. Logits are read once and 8 top_k bytes a token written: 16384
  * tokens of 256 experts, 17.8 MB, would take 3.5 us at the 5.12 TB/s of a copy. What takes the time is the choice itself, one place after the other, each a
- * chain of some 15 dependent moves and comparisons: a wave of its own for a token takes 121 us there, 16 lanes for a token 18 us (sigmoid, a bias, 4 of 8
- * groups, 8 places; 24 us for 16 places). A single token takes 4.5 us, of which 2 are the launch.
+ * chain of some 15 dependent moves and comparisons: a wave of its own for a token takes 78 us there, 16 lanes for a token 18 us (sigmoid, a bias, 4 of 8
+ * groups, 8 places; 24 us for 16 places, 121 for 17 by a wave to a token). A single token takes 4.5 us, of which 2 are the launch.
  *   moe_route_row_kernel (16 lanes to a token) takes up to 512 experts and 16 places, where groups are 1, 2, 4 or 8 whole lanes: 37 us for 16384
  * tokens of 512 experts; moe_route_any_kernel (a wave to a token) all else: 105 us for 528 experts.
  */
