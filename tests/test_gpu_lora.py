@@ -315,3 +315,50 @@ def test_long_prompts(kind):
     ids = np.repeat([2, -1, 0, 1, 2], [300, 1, 499, 200, 100])
     c = Case(12, n_tok, [520, 520], 768, [64, 32, 16], ids, out=BF16 if kind == "gate_up" else F32, pair=kind == "gate_up")
     c.check()
+
+
+class Far:
+    """rows 2^27 elements apart in device memory: offsets that 32 bits do not hold, of bytes and of elements"""
+    PITCH = 1 << 27
+
+    def __init__(self, raw):
+        self.n, self.cols, self.dtype = raw.shape[0], raw.shape[1], raw.dtype
+        self.buf = qlinear.DevBuf(((self.n - 1) * self.PITCH + self.cols) * raw.itemsize)
+        self.ptr, self.nbytes = self.buf.ptr, self.buf.nbytes
+        for t in range(self.n):
+            row = np.ascontiguousarray(raw[t])
+            qlinear.check(qlinear.load().qlin_dev_upload(self.at(t), row.ctypes.data, row.nbytes))
+
+    def at(self, t):
+        return self.ptr + t * self.PITCH * self.dtype.itemsize
+
+    def rows(self):
+        out = np.empty((self.n, self.cols), self.dtype)
+        for t in range(self.n):
+            row = np.empty(self.cols, self.dtype)
+            qlinear.check(qlinear.load().qlin_dev_download(row.ctypes.data, self.at(t), row.nbytes))
+            out[t] = row
+        return out
+
+
+@pytest.mark.parametrize("rank", [8, 80])  # one launch, two
+def test_rows_far_apart(rank):
+    """the bits of the same rows next to each other"""
+    n_tok, n_rows, n_cols = 20, 70, 48
+    c = Case(13, n_tok, [n_rows, n_rows], n_cols, [rank, 5], mixed(n_tok, 2), pair=True)
+    want = c.run()[0]
+    x, gate, up = Far(c.x_raw), Far(c.y_raw[0]), Far(c.y_raw[1])
+    qlinear.lora_silu_mul_dev(c.tables[0], c.tables[1], BF16, 2, c.max_rank, c.dids, BF16, x, F32, gate, up, F32, gate, n_rows, n_cols, n_tok, Far.PITCH, Far.PITCH, Far.PITCH, c.ws)
+    qlinear.sync()
+    assert np.array_equal(gate.rows(), want) and np.array_equal(up.rows(), c.y_raw[1])
+
+
+@pytest.mark.parametrize("n_tok", [1, 3])
+def test_long_rows(n_tok):
+    Case(14, n_tok, [5], (1 << 21) + 5, [2, 1], mixed(n_tok, 2) if n_tok > 1 else [0]).check()
+
+
+def test_many_rows():
+    n_rows = (1 << 22) + 3
+    c = Case(15, 2, [n_rows], 16, [1, 2], [0, 1], y=BF16, out=BF16)
+    c.check()

@@ -167,3 +167,43 @@ def test_all_picks_among_neighbouring_experts(biased, n, n_group, k):
     for sigmoid in (False, True):
         check(x, F32, sigmoid, bias, n_group, max(1, n_group // 2), 2, k, True, 1.0)
         check(x, F16, sigmoid, bias, n_group, n_group, 1, k, True, 1.0)
+
+
+@pytest.mark.parametrize("n,k", [(60, 4), (60, 17)])  # 16 lanes to a token, a wave
+def test_rows_far_apart(n, k):
+    """rows 2^27 elements apart: offsets that 32 bits do not hold"""
+    n_tok, pitch = 20, 1 << 27
+    x = rows(5, n_tok, n).astype(np.float32)
+    want = call(x, F32, False, None, 1, 1, 1, k, True, 1.0)
+    far = qlinear.DevBuf(((n_tok - 1) * pitch + n) * 4)
+    for t in range(n_tok):
+        qlinear.check(qlinear.load().qlin_dev_upload(far.ptr + t * pitch * 4, x[t].ctypes.data, n * 4))
+    idx, w = qlinear.DevBuf(n_tok * k * 4), qlinear.DevBuf(n_tok * k * 4)
+    qlinear.moe_route_scores_dev(qlinear.ROUTE_SOFTMAX, F32, far, n_tok, n, pitch, None, 1, 1, 1, k, True, 1.0, idx, w)
+    qlinear.sync()
+    assert np.array_equal(idx.to_numpy(np.int32, (n_tok, k)), want[0]) and np.array_equal(w.to_numpy(np.float32, (n_tok, k)), want[1])
+
+
+@pytest.mark.parametrize("n,n_group,k", [(256, 8, 8), (60, 1, 17)])
+def test_in_a_graph(n, n_group, k):
+    """captured once, replayed on other logits, with eager calls between"""
+    import ctypes as C
+    hip = C.CDLL("libamdhip64.so")
+    n_tok, used = 33, max(1, n_group // 2)
+    bias = small_bias(3, n).astype(np.float32)
+    dx, db = qlinear.DevBuf(n_tok * n * 4), qlinear.DevBuf.from_numpy(bias)
+    idx, w = qlinear.DevBuf(n_tok * k * 4), qlinear.DevBuf(n_tok * k * 4)
+    stream, graph, gexec = C.c_void_p(), C.c_void_p(), C.c_void_p()
+    qlinear.check(qlinear.load().qlin_init(0))
+    assert hip.hipStreamCreate(C.byref(stream)) == 0
+    assert hip.hipStreamBeginCapture(stream, 0) == 0
+    qlinear.moe_route_scores_dev(qlinear.ROUTE_SIGMOID, F32, dx, n_tok, n, n, db, n_group, used, 2, k, True, 2.5, idx, w, stream)
+    assert hip.hipStreamEndCapture(stream, C.byref(graph)) == 0
+    assert hip.hipGraphInstantiate(C.byref(gexec), graph, None, None, C.c_size_t(0)) == 0
+    for replay in range(4):
+        x = np.ascontiguousarray(rows(replay, n_tok, n), np.float32)
+        qlinear.check(qlinear.load().qlin_dev_upload(dx.ptr, x.ctypes.data, x.nbytes))
+        assert hip.hipGraphLaunch(gexec, stream) == 0 and hip.hipStreamSynchronize(stream) == 0
+        want = call(x, F32, True, bias, n_group, used, 2, k, True, 2.5)
+        assert np.array_equal(idx.to_numpy(np.int32, (n_tok, k)), want[0]) and np.array_equal(w.to_numpy(np.float32, (n_tok, k)), want[1])
+    assert hip.hipGraphExecDestroy(gexec) == 0 and hip.hipGraphDestroy(graph) == 0 and hip.hipStreamDestroy(stream) == 0
