@@ -912,12 +912,16 @@ static int lora_most_parts(int n_mat, int max_rank, int n_cols, int n_tok) {
     return (int)(parts > kLoraMostParts ? kLoraMostParts : parts < 1 ? 1 : parts);
 }
 
-/* the groups of every tile, of which there are at most as many as tokens, or half of them twice as many; then h in fp32 for each part, or, of
- * one part, as three numbers in bf16 */
+/* The groups of every tile, of which there are at most as many as tokens, or half of them twice as many; then h in fp32 for each part, or, of one part, as three
+ * numbers in bf16. What fewer tokens, tensors, ranks or columns need is not more: tokens * parts is at most 256 * 16 / (n_mat * blocks of ranks) where there is more than one
+ * part, and a block has up to 64 ranks. */
 static size_t lora_records(int n_tok, int groups) { return ((size_t)n_tok + kTile - 1) / kTile * groups * sizeof(Group); }
 size_t lora_workspace_bytes(int n_mat, int max_rank, int n_cols, int n_tok) {
-    const size_t rank_pad = (max_rank + 15) / 16 * 16, split = (rank_pad + 31) / 32 * 192, sums = rank_pad * lora_most_parts(n_mat, max_rank, n_cols, n_tok) * sizeof(float);
-    return lora_records(n_tok, (n_tok < kTile ? n_tok : kTile) * lora_token_groups(n_mat, max_rank, n_tok)) + (size_t)n_mat * n_tok * (split > sums ? split : sums);
+    const size_t rank_pad = (max_rank + 15) / 16 * 16, tokens = n_tok, split = tokens * ((rank_pad + 31) / 32 * 192);
+    const size_t columns = n_cols / (64 * kShrinkWaves), parts = columns < 1 ? 1 : columns > kLoraMostParts ? kLoraMostParts : columns;
+    const size_t whole = tokens * rank_pad, cut = whole * parts, most = (rank_pad < 64 ? rank_pad : 64) * ((256 * 16 + n_mat - 1) / n_mat);
+    const size_t sums = (cut < most ? cut : most > whole ? most : whole) * sizeof(float);
+    return lora_records(n_tok, (n_tok < kTile ? n_tok : kTile) * lora_token_groups(n_mat, max_rank, n_tok)) + n_mat * (split > sums ? split : sums);
 }
 
 LoraPlan lora_plan(const LoraCall &c) {

@@ -423,7 +423,7 @@ typedef struct qlin_lora_tensor { /* one projection; in host memory, read before
  * order (neighbours that share an adapter share its loads). y_type and out_type: F32, F16 or BF16. The sums are fp32, the products of an
  * adapter and X exact, and a 16-bit result is rounded once; the same call gives the same bits. An infinity or a NaN in X or in an adapter
  * stays with its tokens. workspace: device memory, 16-byte aligned, qlin_lora_workspace_bytes(n_mat, max_rank, n_cols, n_tok) bytes (0 for
- * sizes that are not positive), which holds nothing between calls; calls that share one must be ordered on one stream, and graphs that
+ * sizes that are not positive; those of the largest call hold a smaller one's), which holds nothing between calls; calls that share one must be ordered on one stream, and graphs that
  * share one must not run at the same time. What a call writes must not overlap with what it reads, but for an out that is its Y. n_cols
  * below 2^24, n_rows up to 2^30, max_rank up to QLIN_LORA_MAX_RANK; what would take 2^32 threads or more is refused (256 tokens x 256 rows take at
  * least 256). */

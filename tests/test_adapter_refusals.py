@@ -2,6 +2,7 @@
 the workspace's size says."""
 import ctypes as C
 
+import numpy as np
 import pytest
 
 from gemm_amd import qlinear
@@ -106,3 +107,11 @@ def test_workspace(lib):
 
 def test_structures():
     assert qlinear.LORA_DTYPE.itemsize == 24 and C.sizeof(qlinear.LoraTensor) == 40
+
+
+def test_a_workspace_holds_what_smaller_calls_need(lib):
+    rng = np.random.default_rng(3)
+    for _ in range(3000):
+        large = [int(rng.integers(1, n + 1)) for n in (3, 256, 20000, rng.choice([64, 600, 5000]))]
+        small = [int(rng.integers(1, n + 1)) for n in large]
+        assert lib.qlin_lora_workspace_bytes(*small) <= lib.qlin_lora_workspace_bytes(*large), (small, large)

@@ -362,3 +362,18 @@ def test_many_rows():
     n_rows = (1 << 22) + 3
     c = Case(15, 2, [n_rows], 16, [1, 2], [0, 1], y=BF16, out=BF16)
     c.check()
+
+
+@pytest.mark.parametrize("n_tok,rows,n_cols,ranks", [(1, [70, 40, 40], 9000, [200]), (20, [300], 9000, [64, 80]), (70, [300], 4096, [16, 5, 16]), (300, [70, 40], 2100, [64, 3]), (2050, [70, 40], 64, [64, 20])])
+@pytest.mark.parametrize("w", [F32, BF16])
+def test_nothing_is_written_behind_the_workspace(n_tok, rows, n_cols, ranks, w):
+    c = Case(16, n_tok, rows, n_cols, ranks, mixed(n_tok, len(ranks)), w=w)
+    want, guard = c.run(), 4096
+    need = c.ws.nbytes
+    c.ws = qlinear.DevBuf.from_numpy(np.full(need + guard, 0xAB, np.uint8))
+    whole, c.ws.nbytes = c.ws.nbytes, need
+    c.fresh()
+    for a, b in zip(want, c.run()):
+        assert np.array_equal(a, b)
+    c.ws.nbytes = whole
+    assert (c.ws.to_numpy(np.uint8, (whole,))[need:] == 0xAB).all()
