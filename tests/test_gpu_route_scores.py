@@ -97,6 +97,27 @@ def test_what_is_not_there(sigmoid, biased, n, n_group):
     check(np.where(x < -1e38, -INF, x), BF16, sigmoid, bias, n_group, max(1, n_group // 2), 1, 6, True, 1.0)
 
 
+@pytest.mark.parametrize("sigmoid", [False, True])
+@pytest.mark.parametrize("low", [np.finfo(np.float32).min, -3.4e38, -1e38])
+@pytest.mark.parametrize("n,n_group,free,k", [(8, 1, 1, 4), (8, 1, 2, 8), (17, 1, 1, 9), (60, 1, 3, 4), (60, 4, 3, 12), (64, 1, 0, 8), (64, 8, 1, 8), (96, 1, 2, 6), (96, 8, 5, 12),
+                                              (160, 1, 4, 8), (160, 8, 9, 16), (160, 16, 2, 16), (256, 8, 6, 8), (256, 1, 1, 17), (257, 1, 1, 12), (512, 16, 3, 10)])
+def test_a_bias_of_the_lowest_value(sigmoid, low, n, n_group, free, k):
+    """the usual mask, a finite one: its experts come behind all others, by index, and none that is not there comes with them"""
+    x = rows(n + k, 6, n)
+    order = np.random.default_rng(n).permutation(n)
+    bias = small_bias(n, n)
+    bias[order[free:]] = low
+    x[1, ::3] = -INF
+    x[2, order[free:free + n // 2]] = NAN
+    x[3] = -INF
+    x[4, :n - 1] = -INF
+    x[5, order[:free]] = -INF
+    used = max(1, n_group // 2)
+    for group_top in (1, 2):
+        check(x, F32, sigmoid, bias, n_group, used, group_top, k, group_top == 1, 1.0)
+    check(x, BF16, sigmoid, bias, n_group, n_group, 1, k, True, 2.5)
+
+
 @pytest.mark.parametrize("t", [F32, BF16])
 @pytest.mark.parametrize("biased", [False, True])
 def test_equal_values_go_by_index(t, biased):
