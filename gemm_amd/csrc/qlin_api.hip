@@ -1573,9 +1573,10 @@ static int lora_call(LoraCall &c, void *workspace, size_t workspace_bytes) {
     if (int rc = check_float_rows("X", c.x_type, c.X, c.n_tok, c.n_cols, c.ldx)) return rc;
     bool rows = false;
     for (int i = 0; i < c.n_mat; i++) {
-        const LoraTensor &m = c.m[i];
+        LoraTensor &m = c.m[i];
         if (m.n_rows < 0 || m.ldy < m.n_rows || m.ldo < m.n_rows) return fail(QLIN_ERR_ARG, "negative size or a row pitch below the row");
         if (m.n_rows > kLoraMaxRows) return fail(QLIN_ERR_ARG, "%d rows (up to %d)", m.n_rows, kLoraMaxRows);
+        if (m.n_rows == 0) m.adapters = nullptr; /* not checked, so not read: the kernels take it for a tensor without adapters */
         if (m.n_rows == 0 || c.n_tok == 0) continue;
         rows = true;
         if (!m.Y || (!m.out && (i == 0 || !c.pair)) || (!m.adapters && c.n_adapter)) return fail(QLIN_ERR_ARG, "null pointer");

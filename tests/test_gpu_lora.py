@@ -248,6 +248,27 @@ def test_a_tensor_without_rows():
     assert (got[1] == -7).all()
 
 
+def test_a_tensor_without_rows_has_no_table():
+    """what a tensor without rows says of its adapters is not looked at: not a byte of the workspace depends on it"""
+    n_tok = 80  # two launches
+    c = Case(17, n_tok, [30, 30, 30], 64, [16, 8], mixed(n_tok, 2))
+    null = type("Null", (), {"ptr": None})()
+    seen = []
+    for table in (null, c.tables[1]):
+        c.ws = qlinear.DevBuf.from_numpy(np.full(c.ws.nbytes, 0xFF, np.uint8))
+        c.fresh()
+        tensors = qlinear.lora_tensors([(c.tables[0], c.dy[0], c.dout[0], 30, 30, 30), (table, null, null, 0, 0, 0), (c.tables[2], c.dy[2], c.dout[2], 30, 30, 30)])
+        qlinear.lora_add_dev(tensors, BF16, 2, 16, c.dids, BF16, c.dx, F32, F32, 64, n_tok, 64, c.ws)
+        qlinear.sync()
+        want, bound = c.want()
+        got = c.results()
+        for i in (0, 2):
+            assert (np.abs(got[i] - want[i]) <= bound[i]).all()
+        assert (got[1] == -7).all()
+        seen.append(c.ws.to_numpy(np.uint8, (c.ws.nbytes,)))
+    assert np.array_equal(*seen)
+
+
 @pytest.mark.parametrize("pair", [False, True])
 @pytest.mark.parametrize("w,x", [(BF16, BF16), (F16, F16), (BF16, F32)])
 @pytest.mark.parametrize("n_tok", [5, 80])
