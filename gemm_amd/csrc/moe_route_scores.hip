@@ -52,6 +52,19 @@ __device__ __forceinline__ double score_of(int kind, double x, double max, doubl
     const double e = exp(-fabs(x));
     return (x >= 0 ? 1.0 : e) / (1.0 + e);
 }
+/* What renormalised weights are made of: the chosen scores over exp(base), which the division takes out again. The base is the largest of the chosen logits, in a
+ * sigmoid only below 0, where a score is exp(x) / (1 + exp(x)): so one term is between 1/2 and 1 however small the scores themselves are (all
+ * of them below fp32 from logits of -104 down, or in a softmax whose largest logits a bias took out). Scores are 64-bit values: from e^-745.13 down they are 0,
+ * and a token all of whose chosen scores are has the weights 0, which an infinite base gives. max is the softmax's. */
+__device__ __forceinline__ float base_of(int kind, float largest, float max) {
+    if ((kind == 0 ? largest - max : largest) < -745.1332f) return INFINITY;
+    return kind == 0 ? largest : fminf(largest, 0.0f);
+}
+__device__ __forceinline__ double over_base(int kind, double x, double base) {
+    const double e = x == base ? 1.0 : exp(x - base); /* infinities share the weight */
+    if (kind == 0) return e;
+    return x >= 0 ? 1.0 / (1.0 + exp(-x)) : e / (1.0 + exp(x));
+}
 
 /* A token by one wave, its experts' 64-bit values in LDS: any number of experts, places and groups. Bound by the chain of a place: six moves of a
  * 64-bit value and an index between lanes (1 token of 128 experts, 17 places: 19 us). */
@@ -122,7 +135,7 @@ moe_route_any_kernel(RouteCall c) {
         }
         __syncthreads();
     }
-    double total = 0.0;
+    float largest = -INFINITY; /* of the chosen logits */
     for (int n = 0; n < c.top_k; n++) {
         double best = none;
         int at = 0x7FFFFFFF;
@@ -133,22 +146,30 @@ moe_route_any_kernel(RouteCall c) {
             }
         wave_best(best, at);
         const bool found = at != 0x7FFFFFFF;
-        double s = 0.0;
+        double w = 0.0;
         if (found) {
-            s = score_of(c.score, (double)to_f32(x[at]), max, sum);
+            const float logit = to_f32(x[at]);
+            largest = fmaxf(largest, logit);
+            if (!c.renorm) w = score_of(c.score, (double)logit, max, sum) * (double)c.scale;
             if ((at & 63) == lane) key[at] = none; /* its own to look at in the next round */
         }
-        total += s;
         if ((n & 63) == lane) {
             c.idx[out + n] = found ? at : -1;
-            c.w[out + n] = (float)(c.renorm ? s : s * (double)c.scale);
+            c.w[out + n] = (float)w;
         }
     }
-    if (c.renorm && total > 0.0) /* what a lane wrote, with the chosen scores once more in 64 bits */
+    if (!c.renorm) return;
+    const double base = base_of(c.score, largest, (float)max);
+    double total = 0.0;
+    auto places = [&](auto see) { /* the lane's own that hold an expert, which it wrote itself */
         for (int n = lane; n < c.top_k; n += 64) {
             const int at = c.idx[out + n];
-            if (at >= 0) c.w[out + n] = (float)(score_of(c.score, (double)to_f32(x[at]), max, sum) / total * (double)c.scale);
+            if (at >= 0) see(n, over_base(c.score, (double)to_f32(x[at]), base));
         }
+    };
+    places([&](int, double s) { total += s; });
+    total = wave_sum(total);
+    places([&](int n, double s) { c.w[out + n] = total > 0.0 ? (float)(s / total * (double)c.scale) : 0.0f; });
 }
 
 /* ------------------------------------------------------------------ up to 512 experts and 16 places */
@@ -453,13 +474,16 @@ moe_route_row_kernel(RouteCall c, int per, int group_lanes) {
         }
     }
     float w = 0.0f;
-    if (pick >= 0) {
-        const float p = to_f32(x[pick]);
+    const float p = pick >= 0 ? to_f32(x[pick]) : none;
+    const float base = c.renorm ? base_of(c.score, row_max(p), most) : c.score == 0 ? most : 0.0f;
+    if (pick >= 0) { /* as over_base, in fp32 */
+        const float e = expf(c.score != 0 ? -fabsf(p) : p == base ? 0.0f : p - base);
         if (c.score == 0) {
-            w = (p == most ? 1.0f : expf(p - most)) / sum;
+            w = c.renorm ? e : e / sum;
         } else {
-            const float e = expf(-fabsf(p));
-            w = (p >= 0.0f ? 1.0f : e) / (1.0f + e);
+            float over = p >= 0.0f ? 1.0f : e;
+            if (base != 0.0f) over = expf(p - base);
+            w = over / (1.0f + e);
         }
     }
     if (c.renorm) {

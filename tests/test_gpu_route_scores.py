@@ -154,6 +154,50 @@ def test_saturated_sigmoid():
     check(x, F32, False, np.zeros(64), 1, 1, 1, 5, True, 1.0)
 
 
+def shares(x, sigmoid, idx):
+    """the weights of the chosen experts, renormalised to 1, from the logarithms of their scores (up to what all have in common): right however small
+    the scores are; and how far fp32 may be off: the exponential's argument is the distance to the largest, rounded, besides as in route_bound"""
+    there = idx >= 0
+    v = np.where(there, x[np.maximum(idx, 0)], 0.0)
+    log = np.where(there, (np.minimum(v, 0.0) - np.log1p(np.exp(-np.abs(v)))) if sigmoid else v, -np.inf)
+    far = np.where(there, log.max() - log, 0.0)
+    w = np.where(there, np.exp(-far), 0.0)
+    w = w / w.sum()
+    return w, 2.0 ** -23 * (far + far.max() + 24.0) * w + 2.0 ** -126
+
+
+@pytest.mark.parametrize("k", [1, 5, 16, 17, 64])  # 16 lanes to a token, a wave
+@pytest.mark.parametrize("t", [F32, BF16])
+def test_renormalised_scores_below_fp32(k, t):
+    """all chosen scores denormal in fp32 or 0 there: the weights are those of the definition all the same; 0 where the scores are 0 in 64 bits too"""
+    rng = np.random.default_rng(k)
+    n, n_tok = 96, 9
+    x = rng.uniform(-104, -86, (n_tok, n))
+    x[1] = rng.uniform(-300, -90, n)
+    x[2] = rng.uniform(-130, -110, n)
+    x[3] = rng.uniform(-2000, -800, n)
+    x[4, :90] = -INF
+    x[5] = rng.uniform(-20, 3, n)
+    x[6] = rng.uniform(-100.0, -99.0, n)
+    x[7, 0] = 1.0
+    x[8] = -90.0
+    far = rng.standard_normal((n_tok, n))
+    far[:, 17] = np.linspace(60.0, 2000.0, n_tok)
+    far[8, 17] = INF
+    dominant = rng.permutation(n) / 8.0 + 1.0  # decides alone, in 64 bits too
+    without = dominant.copy()
+    without[17] = -INF
+    for x, sigmoid, bias in ((x, True, None), (x, True, dominant), (far, False, without)):
+        idx, w, v = call(x, t, sigmoid, bias, 1, 1, 1, k, True, 2.5)
+        for row in range(n_tok):
+            want_idx, _ = f.route(v[row], sigmoid, bias, 1, 1, 1, k, True, 2.5)
+            assert idx[row].tolist() == want_idx.tolist()
+            want, bound = shares(v[row], sigmoid, want_idx)
+            if not f.scores(v[row], sigmoid)[want_idx[want_idx >= 0]].any():
+                want = bound = 0.0 * want
+            assert (np.abs(w[row] - 2.5 * want) <= 2.5 * bound).all(), (row, w[row], 2.5 * want)
+
+
 def test_agrees_with_the_plain_router():
     """softmax over all, top_k, renormalised is what qlin_moe_route_dev does, but for its order among equal ones"""
     x = rows(8, 33, 128).astype(np.float32)
