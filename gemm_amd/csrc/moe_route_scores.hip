@@ -17,6 +17,7 @@
 #include "qlin_device.h"
 #include "qlin_internal.h"
 
+#include <cfloat>
 #include <type_traits>
 
 namespace qlin {
@@ -308,9 +309,8 @@ moe_route_row_kernel(RouteCall c, int per, int group_lanes) {
     /* how far an fp32 value may be from another to be taken for it: twice their error. A sigmoid's is below 4e-7 (argument, exponential and reciprocal), a
      * softmax's 2e-6 of itself (the sum's most of all), and no score is above 1 / sum; adding the bias rounds by 2^-24 */
     float away = 0.0f;
-    auto threshold = [&](float m) { return !BIAS || m == INFINITY ? m : m - (away + 2.4e-7f * fabsf(m)); };
-    /* (the type's lowest value less that is -infinity, which an expert that is not there has too) */
-    auto reaches = [&](float value, float least) { return value >= least && value > none; };
+    /* (and the lowest value that is one: experts that are not there have -infinity, which a lowest value less that would be) */
+    auto threshold = [&](float m) { return !BIAS || m == INFINITY ? m : fmaxf(m - (away + 2.4e-7f * fabsf(m)), -FLT_MAX); };
     if constexpr (BIAS) {
         const float inverse = __builtin_amdgcn_rcpf(sum);
         away = c.score == 0 ? 4e-6f * inverse : 8e-7f;
@@ -391,8 +391,8 @@ moe_route_row_kernel(RouteCall c, int per, int group_lanes) {
                 const float least = next > none ? threshold(next) : top > none ? threshold(top) : INFINITY;
 #pragma unroll
                 for (int j = 0; j < N; j++)
-                    if (__ballot(reaches(key[j], least))) {
-                        const double d = reaches(key[j], least) ? score64(here(v[j]), s64) + (double)c.bias[e0 + j] : (double)none;
+                    if (__ballot(key[j] >= least)) {
+                        const double d = key[j] >= least ? score64(here(v[j]), s64) + (double)c.bias[e0 + j] : (double)none;
                         b = fmax(b, fmin(a, d));
                         a = fmax(a, d);
                     }
@@ -432,14 +432,14 @@ moe_route_row_kernel(RouteCall c, int per, int group_lanes) {
         int which = at;
         if constexpr (BIAS) {
             const float least = threshold(m);
-            lanes = of_row(reaches(top, least));
-            looked = __ballot(reaches(next, least) || (lanes & (lanes - 1))); /* several that could be the largest */
+            lanes = of_row(top >= least);
+            looked = __ballot(next >= least || (lanes & (lanes - 1))); /* several that could be the largest */
             if (looked) {
                 double best = none;
                 const double s64 = sum64();
 #pragma unroll
                 for (int j = 0; j < N; j++) {
-                    const bool may = reaches(key[j], least) && !((gone >> j) & 1);
+                    const bool may = key[j] >= least && !((gone >> j) & 1);
                     if (__ballot(may)) {
                         const double d = may ? score64(here(v[j]), s64) + (double)c.bias[e0 + j] : (double)none;
                         which = d > best ? j : which;
