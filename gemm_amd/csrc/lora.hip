@@ -386,8 +386,10 @@ __device__ __forceinline__ void shrink_sums(const W *A, int rank0, int rank, con
     }
 }
 
-/* the leading eight bits of a number */
-__device__ __forceinline__ float leading(float v) { return __uint_as_float(__float_as_uint(v) & 0xFFFF0000u); }
+/* The leading eight bits of a number, or the eight-bit number next below where it has no more: something of its sign is left behind them in any case, and a
+ * number cut into three in bf16 (24 bits are eight, eight and eight) has none that is 0. An infinite element of B times each of the three is then the infinity that it is times the
+ * number, not the NaN of infinity times 0. The last of an infinity's three is one; 0 is 0 in all three; bf16 has no last one for numbers below 2^-110. */
+__device__ __forceinline__ float leading(float v) { return __uint_as_float((__float_as_uint(v) - (v != 0.0f ? 1 : 0)) & 0xFFFF0000u); }
 
 template <class W, class X, int RT, int NJ>
 __global__ void __launch_bounds__(64 * kShrinkWaves)
@@ -461,8 +463,7 @@ lora_shrink_kernel(LoraCall c, LoraPlan p) {
                     bf16x4 three[3];
 #pragma unroll
                     for (int d = 0; d < 4; d++) {
-                        /* 24 bits are eight, eight and eight; an infinity leaves nothing, and the largest numbers do not become one */
-                        const float first = leading(v[d]), rest = fabsf(first) == INFINITY ? 0.0f : v[d] - first, second = leading(rest);
+                        const float first = leading(v[d]), rest = v[d] - first, second = leading(rest);
                         three[0][d] = (__bf16)first;
                         three[1][d] = (__bf16)second;
                         three[2][d] = (__bf16)(rest - second);

@@ -306,6 +306,40 @@ def test_the_largest_numbers_and_infinities(n_tok):
     assert (np.abs(got[2:4] - want) <= 2.0 ** -24 * np.abs(want)).all()
 
 
+@pytest.mark.parametrize("pair", [False, True])
+@pytest.mark.parametrize("w", [BF16, F16, F32])
+@pytest.mark.parametrize("n_tok,n_cols,ranks", [(5, 64, [16, 3]), (20, 64, [80, 5]), (80, 64, [16, 3]), (80, 64, [33, 20]), (80, 2304, [16, 3]), (300, 64, [16, 64])])  # every way h goes
+def test_infinities_of_B(pair, w, n_tok, n_cols, ranks):
+    """an infinite element of B makes its results infinite, whatever bits h has: here the few of an element of A"""
+    ids = np.arange(n_tok) % 3 - 1
+    c = Case(18, n_tok, [70, 70], n_cols, ranks, ids, w, w, pair=pair)
+    one = f.as_type(np.ones(1), w)[0][0]
+    c.x_raw[:], c.x[:] = 0, 0.0
+    c.x_raw[:, 5], c.x[:, 5] = one, 1.0
+    c.place()
+    want, bound = c.want()
+    inf = f.as_type(np.array([np.inf, -np.inf]), w)[0]
+    for a in c.adapters[1]:  # (of gate and up: up)
+        for row, k, which in ((3, 0, 0), (5, 1, 1), (7, 0, 0), (7, a.rank - 1, 0), (69, 2, 1)):
+            a.b_raw[row, k], a.b[row, k] = inf[which], [np.inf, -np.inf][which]
+    c.place()
+    got = c.run()
+    g = [f.values(v, F32) for v in got]
+    if not pair:
+        assert (np.abs(g[0] - want[0]) <= bound[0]).all()
+    lost = np.zeros(want[-1].shape, bool)
+    lost[np.ix_(ids >= 0, [3, 5, 7, 69])] = True
+    assert (np.abs(g[-1] - want[-1])[~lost] <= bound[-1][~lost]).all()
+    for t in np.flatnonzero(ids >= 0):
+        a = c.adapters[1][ids[t]]
+        with np.errstate(invalid="ignore"):
+            expect = c.y[1][t] + float(a.scale) * (a.b @ a.a[:, 5])
+            if pair:
+                gate = c.adapters[0][ids[t]]
+                expect = f.silu(c.y[0][t] + float(gate.scale) * (gate.b @ gate.a[:, 5])) * expect
+        assert np.array_equal(g[-1][t][[3, 5, 7, 69]], expect[[3, 5, 7, 69]], equal_nan=True)
+
+
 def test_an_adapter_of_one_row_and_column_copies_what_it_should():
     """A picks column 5, B puts it into row 3, scale 2: exact"""
     c = Case(10, 3, [8], 64, [1], [0, -1, 0])
