@@ -11,7 +11,9 @@
  *
  * A few tokens (lora_few_kernel): one launch. A workgroup takes 1024 results of a token and makes h for itself. Where the workgroups' reads of A add up to
  * little that costs less than a second launch and h in memory: 1 token beside Q, K and V of 4096 columns, rank 16: 5.0 us, 7.4 + 4.1 in two launches; 24
- * tokens: 8.3 us, 7.9 + 4.9; 48 tokens: 9.9, 9.0 + 4.9; 48 tokens of rank 32: 15.4, 9.8 + 6.3; 4 tokens beside gate and up of 14336 rows, rank 32: 20.3, 7.4 + 5.9.
+ * tokens: 8.3 us, 7.9 + 4.9; 48 tokens: 9.9, 9.0 + 4.9; 4 tokens beside gate and up of 14336 rows, rank 32: 20.3, 7.4 + 5.9. The limits (kFewBytes) are no more than
+ * roughly where the two ways meet, and beyond them are calls that one launch would serve better: 48 tokens of rank 32: 15.4, taken are 9.8 + 6.3; 4 tokens of 14336
+ * columns, 4096 rows, rank 16: 9.6, taken 7.5 + 4.2; 1 token of rank 128: 10.3 (with twice the LDS), taken 10.9 + 4.4, where 22 tokens are better off with two, 19.7 and 10.5 + 6.0.
  *
  * Any number of them: two launches, by tiles of 256 tokens.
  *   lora_shrink_kernel makes h. A workgroup finds the tile's classes, tokens that share an adapter, packs the tokens of a class into groups of 16 (or
@@ -953,8 +955,9 @@ LoraPlan lora_plan(const LoraCall &c) {
         p.few = blocks * c.n_tok * a_bytes <= kFewBytesAll && blocks * c.n_tok * kLoraFewThreads < 1ll << 32;
     }
     /* 64 rows to a wave of the second launch, which reads h once for them, or 16 where 64 make few workgroups, and for up to 8 tokens (10 tokens of 719 rows,
-     * rank 128: 7.1 us, 12.5 with 64; 16 beside Q, K and V of 6144 rows: 10.8, 15; 200 of 4096 rows, rank 32, 688 workgroups: 7.8, 6.6 with 64). h in three
-     * bf16 numbers means many tokens. */
+     * rank 128: 7.1 us, 12.5 with 64; 16 beside Q, K and V of 6144 rows: 10.8, 15; 200 of 4096 rows, rank 32, 688 workgroups: 7.8, 6.6 with 64). Where h
+     * goes as three bf16 numbers it is always 64: many tokens, and any number of them where rows are narrower than 2048 columns (both launches, 1024 columns, 4096 rows, rank 128, 8 adapters: 1
+     * token 12.6 us, 12.2 with fp32 and 16 rows; 8 tokens 14.3, 14.4; 32 tokens 13.6, 14.4; 32 tokens and three tensors 18.7, 22.7). */
     auto row_blocks = [&](int rows) {
         p.row_blocks_all = 0;
         for (int i = 0; i < 3; i++) {

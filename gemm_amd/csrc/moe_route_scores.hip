@@ -9,10 +9,11 @@
  *
  * The choice is the one of 64-bit values, also where two experts lie next to each other. Logits are read once and 8 top_k bytes a token written: 16384
  * tokens of 256 experts, 17.8 MB, would take 3.5 us at the 5.12 TB/s of a copy. What takes the time is the choice itself, one place after the other, each a
- * chain of some 15 dependent moves and comparisons: a wave of its own for a token takes 78 us there, 16 lanes for a token 18 us (sigmoid, a bias, 4 of 8
- * groups, 8 places; 24 us for 16 places, 121 for 17 by a wave to a token). A single token takes 4.5 us, of which 2 are the launch.
- *   moe_route_row_kernel (16 lanes to a token) takes up to 512 experts and 16 places, where groups are 1, 2, 4 or 8 whole lanes: 37 us for 16384
- * tokens of 512 experts; moe_route_any_kernel (a wave to a token) all else: 105 us for 528 experts.
+ * chain of some 15 dependent moves and comparisons, and the order of a lane's experts: a wave of its own for a token took 78 us there, 16 lanes for a token take 18 us (sigmoid, a
+ * bias, 4 of 8 groups, 8 places; 24 us for 16 places, 106 for 17 by a wave to a token). Vector instructions are issued in 76% of the busy cycles there, 1470 by a wave (four
+ * tokens). A single token takes 4.8 us, of which 2 are the launch.
+ *   moe_route_row_kernel (16 lanes to a token) takes up to 512 experts and 16 places, where groups are 1, 2, 4 or 8 whole lanes: 35 us for 16384
+ * tokens of 512 experts; moe_route_any_kernel (a wave to a token) all else: 96 us for 528 experts.
  */
 #include "qlin_device.h"
 #include "qlin_internal.h"
@@ -68,7 +69,7 @@ __device__ __forceinline__ double over_base(int kind, double x, double base) {
 }
 
 /* A token by one wave, its experts' 64-bit values in LDS: any number of experts, places and groups. Bound by the chain of a place: six moves of a
- * 64-bit value and an index between lanes (1 token of 128 experts, 17 places: 19 us). */
+ * 64-bit value and an index between lanes (1 token of 128 experts, 17 places: 17 us). */
 template <class X>
 __global__ void __launch_bounds__(64)
 moe_route_any_kernel(RouteCall c) {
